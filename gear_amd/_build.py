@@ -10,7 +10,8 @@ CSRC = os.path.join(_PKG, "csrc")
 INCLUDE = os.path.join(_ROOT, "include")
 
 HIP_SOURCES = ["runtime.hip", "gather.hip", "scan.hip", "search.hip", "sort.hip", "topk.hip",
-               "scatter.hip"]
+               "scatter.hip", "ranges.hip", "norm_rotate.hip", "attention.hip", "attention_grad.hip",
+               "attention_step.hip"]
 LIBGEARHIP = os.path.join(_PKG, "libgearhip.so")
 
 # -packed-fp32-ops is switched off on purpose: hipcc -O3 otherwise forms v_pk_*_f32 from plain
@@ -98,8 +99,9 @@ def build_hostops():
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I", INCLUDE] + inc +
-         ["-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "torchops", "ops.cc"),
-          "-o", out, "-L", _PKG, "-lgearhip", "-Wl,-rpath,$ORIGIN"] + lib +
+         ["-isystem", sysconfig.get_paths()["include"]] +
+         [os.path.join(CSRC, "torchops", f) for f in ("ops.cc", "sequence.cc")] +
+         ["-o", out, "-L", _PKG, "-lgearhip", "-Wl,-rpath,$ORIGIN"] + lib +
          ["-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lamdhip64"])
     return out
 

@@ -26,6 +26,26 @@ class ColumnDesc(ctypes.Structure):
                 ("pad_head", ctypes.c_int32), ("zero_fill", ctypes.c_int32)]
 
 
+class NormRotateDesc(ctypes.Structure):
+    """struct gear_hip_norm_rotate_desc"""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3),
+                ("batch", c_i64), ("tokens", c_i64), ("q_heads", ctypes.c_int32),
+                ("k_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("pos", c_void_p), ("freqs", c_void_p), ("axes", ctypes.c_int32),
+                ("sections", ctypes.c_int32 * 4), ("weight_f32", ctypes.c_int32),
+                ("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", ctypes.c_float)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """struct gear_hip_attention_desc"""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_stride", c_i64 * 3),
+                ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("batch", c_i64), ("queries", c_i64),
+                ("keys", c_i64), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("lo", c_void_p),
+                ("hi", c_void_p), ("slopes", c_void_p), ("scale", ctypes.c_float),
+                ("cap", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); one entry per function of include/gear_hip.h
 SIGNATURES = {
     "gear_hip_abi_version": (c_int, []),
@@ -111,6 +131,26 @@ SIGNATURES = {
                                      c_size_t, c_void_p]),
     "gear_hip_scatter_i64": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_int, c_void_p,
                                      c_size_t, c_void_p]),
+    "gear_hip_token_ranges": (c_int, [c_void_p, c_void_p, c_i64, c_i64, c_i64, c_int, c_i64, c_i64,
+                                      c_i64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gear_hip_norm_rotate": (c_int, [ctypes.POINTER(NormRotateDesc), c_void_p, c_void_p, c_void_p]),
+    "gear_hip_norm_rotate_append": (c_int, [ctypes.POINTER(NormRotateDesc), c_void_p,
+                                            ctypes.POINTER(c_i64), c_void_p, c_void_p, c_i64, c_void_p,
+                                            ctypes.POINTER(c_i64), c_void_p, ctypes.POINTER(c_i64),
+                                            c_void_p]),
+    "gear_hip_norm_rotate_backward_workspace_bytes": (c_size_t, [c_i64]),
+    "gear_hip_norm_rotate_backward": (c_int, [ctypes.POINTER(NormRotateDesc), c_void_p,
+                                              ctypes.POINTER(c_i64), c_void_p, ctypes.POINTER(c_i64),
+                                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                              c_void_p]),
+    "gear_hip_attention": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_void_p, c_void_p]),
+    "gear_hip_attention_backward_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64]),
+    "gear_hip_attention_backward": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p,
+                                            ctypes.POINTER(c_i64), c_void_p, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_void_p, c_size_t, c_void_p]),
+    "gear_hip_attention_step_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "gear_hip_attention_step": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_void_p, c_size_t,
+                                        c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,221 @@
+// Attention of the newest tokens of rollouts over their caches (gear_hip_attention_step).
+//
+// Few queries, many keys: what counts is reading the caches once, at the rate of memory.  The queries of
+// all heads that share a key head are the rows of one matrix operand (32 at a time; most calls have fewer, the
+// unused rows cost nothing that memory would not), so every key is read once for all of them.  A rollout's
+// keys are split over `splits` workgroups and within one over its waves, 32 keys at a time; a wave takes K
+// straight into registers and V through a piece of LDS of its own (which turns it), so no wave waits
+// for another before the end.  What the parts of a split have -- maximum, sum, sums of p v -- is joined by a second
+// launch.
+#include <type_traits>
+
+#include "attention.hpp"
+
+namespace gearhip {
+namespace {
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kMaxSplits = 128;
+
+struct StepArgs {
+  AttentionArgs a;
+  int row_blocks, splits;
+  float *part_o;   // [batch][kv_heads][row_blocks][splits][32][dim]
+  float2 *part_ml; // [batch][kv_heads][row_blocks][splits][32]
+  void *out;
+};
+
+template <typename T, int D, bool SHAPED>
+__global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
+  __shared__ __attribute__((aligned(16))) float joined[kWaves][kRows][D];  // (V's tiles before that)
+  __shared__ float2 joined_ml[kWaves][kRows];
+  const AttentionArgs &a = g.a;
+  const int l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = l >> 5;
+  const int split = blockIdx.x % g.splits, unit = blockIdx.x / g.splits;
+  const int block = unit % g.row_blocks, kv_head = unit / g.row_blocks % a.kv_heads, b = unit / g.row_blocks / a.kv_heads;
+  const int shared = a.heads / a.kv_heads, rows = a.queries * shared;
+  const int r_own = block * kRows + (l & 31), i = r_own / shared, head = kv_head * shared + r_own % shared;
+  const bool row_there = r_own < rows;
+  T *v_tile = reinterpret_cast<T *>(joined[wave]);
+
+  Seen seen;
+  const int64_t row = (int64_t)b * a.queries + i;
+  seen.set(row_there ? a.lo[row] : 0, row_there ? a.hi[row] : 0, a.keys);
+  vec8<T> q[D / 16];
+  own_row_frags<T, D>(q, static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head, a.dim, !seen.empty());
+  const int length = seen.first < seen.end ? seen.end - seen.first : 0;
+  const int part = ((length + g.splits - 1) / g.splits + kRows - 1) / kRows * kRows;
+  const int64_t part_first = seen.first < seen.end ? seen.first + (int64_t)split * part : 0;
+  const int end = (int)min((int64_t)seen.end, part_first + part);
+
+  const Shape shape(a, row_there ? head : 0);
+  f32x16 o[D / 32] = {};
+  float m = -INFINITY, sum = 0;
+  const T *k_rows = static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head;
+  const T *v_rows = static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head;
+  vec8<T> k_next[D / 16];
+  TileLoad<T, D, kRows, kWave> v_next;
+  auto load = [&](int64_t k0) {
+    own_row_frags<T, D>(k_next, k_rows + (k0 + (l & 31)) * a.ks.token, a.dim, k0 + (l & 31) < end);
+    v_next.load(v_rows + k0 * a.vs.token, a.vs.token, l, a.dim, [&](int r) { return k0 + r < end; });
+  };
+  int64_t k0 = part_first + wave * kRows;
+  if (k0 < end) load(k0);
+  for (; k0 < end; k0 += kWaves * kRows) {
+    f32x16 s = {};
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) s = mfma(k_next[x], q[x], s);
+    wave_lds_sync();
+    v_next.store(v_tile, l);
+    wave_lds_sync();
+    if (k0 + kWaves * kRows < end) load(k0 + kWaves * kRows);
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = (int)k0 + result_row(r);
+      float shrink, y = SHAPED ? shape.score(s[r], seen.hi - 1 - key, shrink) : s[r] * a.scale_log2;
+      if (key >= end || (uint32_t)(key - seen.lo) >= (uint32_t)(seen.hi - seen.lo)) y = -INFINITY;
+      s[r] = y;
+      top = fmaxf(top, y);
+    }
+    top = fmaxf(m, fmaxf(top, other_half(top)));
+    const float from = top == -INFINITY ? 0.f : top;
+    const float rescale = exp2_fast(m - from);
+    m = top;
+    sum *= rescale;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = exp2_fast(s[r] - from);
+      sum += s[r];
+    }
+    const vec8<T> p0 = packed<T, 0>(s), p1 = packed<T, 1>(s);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      o[db] = mfma(columns_frag<T, D>(v_tile, 0, db), p0, o[db]);
+      o[db] = mfma(columns_frag<T, D>(v_tile, 16, db), p1, o[db]);
+    }
+  }
+  sum += other_half(sum);
+
+  // join the waves
+  __syncthreads();
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const f32x4 y = {o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
+      *reinterpret_cast<f32x4 *>(&joined[wave][l & 31][db * 32 + 8 * x + 4 * half]) = y;
+    }
+  if (half == 0) joined_ml[wave][l & 31] = make_float2(m, sum);
+  __syncthreads();
+  const int here = min(kRows, rows - block * kRows);
+  for (int x = threadIdx.x; x < here * a.dim; x += kThreads) {
+    const int r = x / a.dim, d = x - r * a.dim;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, joined_ml[w][r].x);
+    const float from = top == -INFINITY ? 0.f : top;
+    float total = 0, y = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float share = exp2_fast(joined_ml[w][r].x - from);
+      total += share * joined_ml[w][r].y;
+      y += share * joined[w][r][d];
+    }
+    if (g.splits == 1) {
+      const int at = block * kRows + r, t = at / shared, h = kv_head * shared + at % shared;
+      const int64_t q_row = (int64_t)b * a.queries + t;
+      const bool none = min(a.hi[q_row], a.keys) <= max(a.lo[q_row], 0);
+      static_cast<T *>(g.out)[(q_row * a.heads + h) * a.dim + d] = (T)(none ? 0.f : y / total);
+    } else {
+      const int64_t at = (int64_t)blockIdx.x * kRows + r;
+      g.part_o[at * a.dim + d] = y;
+      if (d == 0) g.part_ml[at] = make_float2(top, total);
+    }
+  }
+}
+
+// One workgroup a query and head: the parts of its split, joined.
+template <typename T>
+__global__ __launch_bounds__(128) void attention_join_kernel(StepArgs g) {
+  const AttentionArgs &a = g.a;
+  const int shared = a.heads / a.kv_heads;
+  const int64_t q_row = blockIdx.x / a.heads;
+  const int head = blockIdx.x % a.heads, kv_head = head / shared;
+  const int64_t b = q_row / a.queries;
+  const int r = (int)(q_row - b * a.queries) * shared + head % shared;
+  const int64_t unit = (b * a.kv_heads + kv_head) * g.row_blocks + r / kRows;
+  const int64_t first = unit * g.splits * kRows + r % kRows;  // part p: first + p * kRows
+  float top = -INFINITY;
+  for (int p = 0; p < g.splits; ++p) top = fmaxf(top, g.part_ml[first + (int64_t)p * kRows].x);
+  const float from = top == -INFINITY ? 0.f : top;
+  const int d = threadIdx.x;
+  if (d >= a.dim) return;
+  float total = 0, y = 0;
+  for (int p = 0; p < g.splits; ++p) {
+    const float2 ml = g.part_ml[first + (int64_t)p * kRows];
+    const float share = exp2_fast(ml.x - from);
+    total += share * ml.y;
+    y += share * g.part_o[(first + (int64_t)p * kRows) * a.dim + d];
+  }
+  const bool none = min(a.hi[q_row], a.keys) <= max(a.lo[q_row], 0);
+  static_cast<T *>(g.out)[(q_row * a.heads + head) * a.dim + d] = (T)(none ? 0.f : y / total);
+}
+
+int row_blocks_of(int64_t queries, int64_t heads, int64_t kv_heads) {
+  return (int)ceil_div64(queries * (heads / kv_heads), kRows);
+}
+
+// Parts of a rollout's keys: enough workgroups for the GPU, at least 256 keys each.
+int splits_of(int64_t units, int64_t keys) {
+  int64_t n = ceil_div64(1024, units < 1 ? 1 : units);
+  const int64_t most = ceil_div64(keys, 256);
+  if (n > most) n = most;
+  return (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
+}
+
+}  // namespace
+}  // namespace gearhip
+
+using namespace gearhip;
+
+extern "C" size_t gear_hip_attention_step_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                          int64_t kv_heads, int64_t head_dim) {
+  if (batch <= 0 || queries <= 0 || keys < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0) return 0;
+  const int64_t units = batch * kv_heads * row_blocks_of(queries, heads, kv_heads);
+  const int splits = splits_of(units, keys);
+  return splits == 1 ? 0 : (size_t)(units * splits * kRows) * (head_dim * sizeof(float) + sizeof(float2));
+}
+
+extern "C" int gear_hip_attention_step(const gear_hip_attention_desc *desc, void *out, void *workspace,
+                                       size_t workspace_bytes, void *stream) {
+  StepArgs g = {};
+  const int rc = attention_args(desc, g.a);
+  if (rc < 0) return rc;
+  const AttentionArgs &a = g.a;
+  if (rc == 1 || a.queries == 0) return 0;
+  if (out == nullptr) return GEAR_HIP_EINVAL;
+  if (a.queries > (1 << 20) || (int64_t)a.queries * a.heads * a.batch > INT_MAX) return GEAR_HIP_ERANGE;
+  const size_t want = gear_hip_attention_step_workspace_bytes(a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim);
+  if (want > 0 && (workspace == nullptr || workspace_bytes < want)) return GEAR_HIP_EWORKSPACE;
+  if (reinterpret_cast<uintptr_t>(out) % 16 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return GEAR_HIP_EALIGN;
+  g.row_blocks = row_blocks_of(a.queries, a.heads, a.kv_heads);
+  const int64_t units = (int64_t)a.batch * a.kv_heads * g.row_blocks;
+  g.splits = splits_of(units, a.keys);
+  if (units * g.splits > INT_MAX) return GEAR_HIP_ERANGE;
+  g.part_o = static_cast<float *>(workspace);
+  g.part_ml = reinterpret_cast<float2 *>(g.part_o + units * g.splits * kRows * a.dim);
+  g.out = out;
+  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto shaped) {
+    typedef decltype(type) T;
+    hipLaunchKernelGGL((attention_step_kernel<T, decltype(dim)::value, decltype(shaped)::value>),
+                       dim3((unsigned)(units * g.splits)), dim3(kThreads), 0, as_stream(stream), g);
+    if (g.splits > 1)
+      hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(128), 0,
+                         as_stream(stream), g);
+  });
+  GEARHIP_RETURN_IF_LAUNCH_FAILED();
+  return 0;
+}

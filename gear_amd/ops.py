@@ -396,3 +396,70 @@ class TopKState:
 def scatter(weights, idx, values, *, unique_indices=False):
     """weights[idx[j]] = values[j]; duplicates: last one wins.  fp32 or int64 tables."""
     return _hostops.scatter(weights, idx, values, bool(unique_indices), _ws)
+
+
+# ---- a batch of windows into a sequence model --------------------------------------------------
+# Rows of heads are [batch, tokens, heads, head_dim] tensors whose innermost dimension is contiguous and
+# whose rows lie at multiples of 16 bytes; other strides are free (a slice of one projection's output).
+
+def rotation_freqs(sections, base=10000.0, device="cuda"):
+    """The usual frequencies of norm_rotate: pair i of the n pairs of an axis turns by
+    base ** (-i / n) radians a position (float64 [sum of sections])."""
+    return torch.cat([float(base) ** (-torch.arange(n, dtype=torch.float64) / max(int(n), 1))
+                      for n in sections]).to(device)
+
+
+def token_ranges(mask=None, done=None, *, tokens_per_step=1, mode="causal", prefix=0, grid=None):
+    """The keys that each token of a batch of windows sees, and its positions.
+
+    mask, done: uint8 or bool [batch, steps]; the loader's validity mask (None: every step is valid)
+    and a column whose non-zero entries end an episode (None: none ends).  A document is a run of
+    valid steps without an end before its last step; a step is tokens_per_step tokens.
+    mode: a token sees its document up to itself ("causal"), up to its whole step ("step"), or all of
+    it ("document"); in the first `prefix` steps of a document tokens see each other in any case.
+    Returns int32 (lo, hi [batch, steps * tokens_per_step], pos [.., axes]): token i sees the keys
+    lo <= j < hi; tokens of invalid steps see nothing.  pos holds the step within the document, and
+    with grid=(rows, columns) also a token's row and column within its step."""
+    return _hostops.token_ranges(mask, done, int(tokens_per_step), mode, int(prefix), grid)
+
+
+def norm_rotate(q, k, pos, freqs, sections, q_weight=None, k_weight=None, *, eps=1e-6):
+    """Norm of every head's query and key, times a weight, and the rotation of its positions:
+    (q_out, k_out).  pos: int32 [batch, tokens, axes]; freqs: float64, radians a position;
+    sections: pairs (i, i + head_dim / 2) of each axis.  float32, float16, bfloat16."""
+    return _hostops.norm_rotate(q, k, pos, freqs, [int(n) for n in sections], q_weight, k_weight, float(eps))
+
+
+def norm_rotate_backward(dq_out, dk_out, q, k, pos, freqs, sections, q_weight=None, k_weight=None, *, eps=1e-6):
+    """Gradients of norm_rotate: (dq, dk, dq_weight, dk_weight); None where there is no weight."""
+    return _hostops.norm_rotate_backward(dq_out, dk_out, q, k, pos, freqs, [int(n) for n in sections], q_weight,
+                                         k_weight, float(eps), _ws)
+
+
+def norm_rotate_append(q, k, v, pos, freqs, sections, q_weight=None, k_weight=None, *, slots, k_cache, v_cache,
+                       eps=1e-6):
+    """norm_rotate for the newest tokens of rollouts: returns q_out; the result of k and the rows of v
+    are written to k_cache, v_cache [batch, cache tokens, heads, head_dim] at row slots[b, t] (int32;
+    a slot outside the cache writes nothing, the slots of one rollout must differ)."""
+    return _hostops.norm_rotate_append(q, k, v, pos, freqs, [int(n) for n in sections], q_weight, k_weight, slots,
+                                       k_cache, v_cache, float(eps))
+
+
+def range_attention(q, k, v, lo, hi, *, scale=None, cap=0.0, slopes=None):
+    """Softmax attention in which query i sees the keys lo[b, i] <= j < hi[b, i] (int32, as
+    token_ranges gives them): (out, lse float32 [batch, heads, queries]).
+    scale: of the products (None: head_dim ** -0.5); cap > 0: scores become cap * tanh(score / cap);
+    slopes (float32 [heads]): scores lose slopes[head] * |i + keys - queries - j|.  Queries that see
+    nothing get out 0 and lse -inf.  k, v may have fewer heads than q.  float16, bfloat16."""
+    return _hostops.range_attention(q, k, v, lo, hi, scale, float(cap), slopes)
+
+
+def range_attention_backward(dout, q, k, v, out, lse, lo, hi, *, scale=None, cap=0.0, slopes=None):
+    """Gradients (dq, dk, dv) of range_attention, whose out and lse it takes; bit-identical on every run."""
+    return _hostops.range_attention_backward(dout, q, k, v, out, lse, lo, hi, scale, float(cap), slopes, _ws)
+
+
+def range_attention_step(q, k_cache, v_cache, lo, hi, *, scale=None, cap=0.0, slopes=None):
+    """range_attention for the newest tokens of rollouts over their caches: out.  The distance that
+    slopes count is the one from the last key a query sees, |hi - 1 - j|."""
+    return _hostops.range_attention_step(q, k_cache, v_cache, lo, hi, scale, float(cap), slopes, _ws)

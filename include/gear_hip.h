@@ -442,6 +442,118 @@ int gear_hip_scatter_i64(int64_t *table, int64_t n, const int64_t *idx, const in
                          int64_t num, int unique_indices, void *workspace, size_t workspace_bytes,
                          void *stream);
 
+/* ---- a batch of windows into a sequence model ---------------------------------------------- */
+
+/* The calls of this part have no counterpart in the reference: they are what a sequence model of
+ * trajectories does with the batches of gear/loader/offline_loader.py:155-204. */
+
+/* element types of the calls below */
+#define GEAR_HIP_F32 0
+#define GEAR_HIP_F16 1
+#define GEAR_HIP_BF16 2
+
+/* Ranges of keys and positions of a batch of windows, from the loader's validity masks and a
+ * `done` column.  Step s of window b is valid where mask[b][s] != 0 (mask NULL: all are).  A
+ * document is a maximal run of valid steps without a done (done NULL: none) before its last step;
+ * it covers the steps [s0, s1).  A step is `tokens_per_step` tokens n; token i = s*n + u sees the
+ * keys lo[b][i] <= j < hi[b][i]:
+ *     lo = s0*n
+ *     hi = i+1 (GEAR_HIP_RANGE_CAUSAL), (s+1)*n (_STEP), s1*n (_DOCUMENT),
+ *          and max(hi, min(s0 + prefix, s1)*n) where prefix > 0 (the first steps see each other)
+ * Tokens of steps that are not valid get lo = hi = 0 and position 0.  pos is [batch][steps*n][axes]:
+ * s - s0 (axes = 1), or with grid_rows, grid_cols > 0 and n = grid_rows*grid_cols the three
+ * positions s - s0, u / grid_cols, u % grid_cols.  steps * n < 2^31, else GEAR_HIP_ERANGE. */
+#define GEAR_HIP_RANGE_CAUSAL 0
+#define GEAR_HIP_RANGE_STEP 1
+#define GEAR_HIP_RANGE_DOCUMENT 2
+int gear_hip_token_ranges(const uint8_t *mask, const uint8_t *done, int64_t batch, int64_t steps,
+                          int64_t tokens_per_step, int mode, int64_t prefix, int64_t grid_rows,
+                          int64_t grid_cols, int32_t *lo, int32_t *hi, int32_t *pos, void *stream);
+
+/* Norm of every head's query and key with the rotation of its positions, in one pass.  For a row x
+ * of head_dim D elements, y = x / sqrt(mean(x^2) + eps) * weight; the pair (y[i], y[i + D/2]) is
+ * turned by the angle pos[axis(i)] * freqs[i].  The first sections[0] pairs belong to axis 0, the
+ * next sections[1] to axis 1, ...; pairs beyond the sections are not turned.  All arithmetic is
+ * in 32 bits, the angles are reduced to a turn in 64, so that any int32 position is exact.
+ *   head_dim       a multiple of 16, at most 256
+ *   q, k           batch x tokens x heads x head_dim, the innermost contiguous; strides of batch,
+ *                  token and head in elements; bases and strides multiples of 16 bytes
+ *   q_weight, k_weight   head_dim elements of type f32 (weight_f32 != 0) or of the rows' type,
+ *                  or NULL: ones */
+typedef struct gear_hip_norm_rotate_desc {
+  const void *q, *k;
+  int64_t q_stride[3], k_stride[3];
+  int64_t batch, tokens;
+  int32_t q_heads, k_heads, head_dim, dtype;
+  const int32_t *pos;  /* [batch][tokens][axes] */
+  const double *freqs; /* [sum of sections], radians a position */
+  int32_t axes, sections[4];
+  int32_t weight_f32;
+  const void *q_weight, *k_weight;
+  float eps;
+} gear_hip_norm_rotate_desc;
+/* q_out, k_out: contiguous, of the inputs' type */
+int gear_hip_norm_rotate(const gear_hip_norm_rotate_desc *desc, void *q_out, void *k_out,
+                         void *stream);
+/* The same for the newest tokens of rollouts: the result of k and the rows of v (as k) go to row
+ * slots[b][t] of the caches [batch][cache_tokens][k_heads][head_dim] (strides of batch, token and
+ * head as above); a slot outside [0, cache_tokens) is not written. */
+int gear_hip_norm_rotate_append(const gear_hip_norm_rotate_desc *desc, const void *v,
+                                const int64_t *v_stride, void *q_out, const int32_t *slots,
+                                int64_t cache_tokens, void *k_cache, const int64_t *k_cache_stride,
+                                void *v_cache, const int64_t *v_cache_stride, void *stream);
+/* Gradients of gear_hip_norm_rotate: dq, dk (contiguous) from dq_out, dk_out (strides as above),
+ * and of the weights (of the weights' type, summed in 32 bits in a fixed order; NULL: not wanted).
+ * workspace: gear_hip_norm_rotate_backward_workspace_bytes(head_dim) bytes on the device. */
+size_t gear_hip_norm_rotate_backward_workspace_bytes(int64_t head_dim);
+int gear_hip_norm_rotate_backward(const gear_hip_norm_rotate_desc *desc, const void *dq_out,
+                                  const int64_t *dq_out_stride, const void *dk_out,
+                                  const int64_t *dk_out_stride, void *dq, void *dk,
+                                  void *dq_weight, void *dk_weight, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
+/* Attention in which query i sees the keys lo[b][i] <= j < hi[b][i] (as gear_hip_token_ranges
+ * gives them; ranges are cut to [0, keys)):
+ *     s_ij = scale * q_i . k_j;   cap > 0: s_ij = cap * tanh(s_ij / cap);
+ *     slopes != NULL: s_ij -= slopes[head] * |i + keys - queries - j|
+ *     p_ij = softmax of s_ij over the keys seen;  out_i = sum_j p_ij v_j;  lse_i = log sum_j exp s_ij
+ * A query that sees nothing gets out = 0, lse = -inf, and passes no gradient on; what its row of q
+ * (and of dout) holds is not looked at.  Head h reads key head h / (heads / kv_heads).
+ * Scores, statistics and sums are held in 32 bits; p (and its gradient) is rounded to the inputs'
+ * type where it is multiplied with rows of that type.
+ *   dtype     GEAR_HIP_F16 or GEAR_HIP_BF16; head_dim a multiple of 16, at most 128
+ *   q, k, v   batch x queries|keys x heads|kv_heads x head_dim, the innermost contiguous; strides
+ *             of batch, token and head in elements; bases and strides multiples of 16 bytes
+ *   queries, keys < 2^30;  scale > 0 */
+typedef struct gear_hip_attention_desc {
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t batch, queries, keys;
+  int32_t heads, kv_heads, head_dim, dtype;
+  const int32_t *lo, *hi; /* [batch][queries] */
+  const float *slopes;    /* [heads] or NULL */
+  float scale, cap;
+} gear_hip_attention_desc;
+/* out: [batch][queries][heads][head_dim] contiguous; lse: [batch][heads][queries] (NULL: not wanted) */
+int gear_hip_attention(const gear_hip_attention_desc *desc, void *out, float *lse, void *stream);
+/* Gradients dq, dk, dv (contiguous, laid out as q, k, v) from dout (strides as above) and the
+ * forward call's out and lse.  No atomics: the same bits on every run.
+ * workspace: gear_hip_attention_backward_workspace_bytes(batch, queries, heads) bytes, 256-byte aligned. */
+size_t gear_hip_attention_backward_workspace_bytes(int64_t batch, int64_t queries, int64_t heads);
+int gear_hip_attention_backward(const gear_hip_attention_desc *desc, const void *dout,
+                                const int64_t *dout_stride, const void *out, const float *lse,
+                                void *dq, void *dk, void *dv, void *workspace,
+                                size_t workspace_bytes, void *stream);
+/* The same attention for the newest tokens of rollouts over their caches (k, v: batch x keys =
+ * cache rows): few queries, each with the range of its own rollout.  The distance is counted from
+ * the last key that a query sees: |hi - 1 - j|.  The keys are split over workgroups and joined.
+ * workspace: gear_hip_attention_step_workspace_bytes(batch, queries, keys, heads, kv_heads,
+ * head_dim) bytes on the device, 256-byte aligned. */
+size_t gear_hip_attention_step_workspace_bytes(int64_t batch, int64_t queries, int64_t keys,
+                                               int64_t heads, int64_t kv_heads, int64_t head_dim);
+int gear_hip_attention_step(const gear_hip_attention_desc *desc, void *out, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -1,0 +1,232 @@
+"""Attention over ranges of keys, forward, backward and over caches, against 64 bits."""
+import itertools
+
+import pytest
+
+from conftest import announce
+from sequence_reference import Attention, worst
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _rows(g, B, T, H, D, dtype, scale=1.0):
+    return (torch.randn(B, T, H, D, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _masks(kind, B, T, S, g):
+    i = torch.arange(T, device="cuda").expand(B, T) + S - T
+    zero = torch.zeros_like(i)
+    if kind == "causal":
+        lo, hi = zero, i + 1
+    elif kind == "all":
+        lo, hi = zero, zero + S
+    elif kind == "documents":  # runs of 1 to 40 tokens, causal, empty rows between some
+        cut = torch.rand(B, T, generator=g, device="cuda") < 0.08
+        lo = torch.cummax(torch.where(cut, i, zero), 1).values
+        gone = torch.rand(B, T, generator=g, device="cuda") < 0.15
+        hi = torch.where(gone, lo, i + 1)
+    elif kind == "prefix":
+        lo, hi = zero, torch.maximum(i + 1, zero + S // 3)
+    elif kind == "band":
+        lo, hi = i - 20, i + 5  # reaches below 0 and beyond S
+    elif kind == "any":  # no order between rows at all
+        a, b = torch.randint(-5, S + 6, (2, B, T), generator=g, device="cuda")
+        lo, hi = a, b
+    else:  # nothing
+        lo, hi = zero + 3, zero + 3
+    return lo.int().contiguous(), hi.int().contiguous()
+
+
+def _check(B, T, S, H, HK, D, dtype, mask, cap=0.0, slopes=False, scale=None, seed=0, train=True):
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = _rows(g, B, T, H, D, dtype, 1.5)
+    k, v = _rows(g, B, S, 2 * HK, D, dtype, 1.5).split(HK, 2)  # side by side: not contiguous
+    lo, hi = _masks(mask, B, T, S, g)
+    form = dict(cap=cap, scale=scale, slopes=torch.rand(H, generator=g, device="cuda") if slopes else None)
+    announce("attention %s B=%d T=%d S=%d heads=%d/%d D=%d %s cap=%g slopes=%s" % (dtype, B, T, S, H, HK, D, mask, cap, slopes))
+    out, lse = ops.range_attention(q, k, v, lo, hi, **form)
+    dout = _rows(g, B, H, T, D, dtype).transpose(1, 2) if train else None
+    ref = Attention(q, k, v, lo, hi, dout=dout, **form)
+    assert out.is_contiguous() and worst(out, ref.out, ref.out_bound) <= 1
+    assert worst(lse, ref.lse, ref.lse_bound) <= 1
+    if not train:
+        return
+    dq, dk, dv = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi, **form)
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
+        assert got.dtype == dtype and got.is_contiguous()
+        assert worst(got, getattr(ref, name), getattr(ref, name + "_bound")) <= 1, name
+    again = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi, **form)
+    assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), again))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", ["causal", "all", "documents", "prefix", "band", "any", "nothing"])
+def test_masks(mask, dtype):
+    for (T, S), (cap, slopes) in itertools.product(((1, 1), (5, 70), (130, 130), (200, 333)), ((0.0, False), (4.0, True))):
+        _check(2, T, S, 4, 2, 64, dtype, mask, cap, slopes, seed=T + S)
+
+
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("heads", [(1, 1), (6, 2), (8, 1)])
+def test_sizes(D, heads):
+    for dtype in TYPES:
+        for T in (31, 32, 33, 63, 65, 128, 129):
+            _check(2, T, T, heads[0], heads[1], D, dtype, "documents", seed=D + T)
+
+
+def test_many_queries_and_keys():
+    _check(1, 1500, 1500, 2, 1, 128, torch.bfloat16, "causal", seed=1)
+    _check(1, 3000, 3000, 1, 1, 32, torch.float16, "documents", cap=10.0, seed=2)
+    _check(1, 4200, 70, 2, 2, 64, torch.float16, "all", seed=3)
+    _check(3, 90, 5000, 3, 3, 48, torch.bfloat16, "any", slopes=True, seed=4)
+    _check(70, 90, 90, 2, 2, 64, torch.bfloat16, "causal", seed=5)
+
+
+def test_scale_and_large_scores():
+    """Scores of hundreds: the maximum is taken off before the exponent."""
+    _check(2, 100, 100, 2, 2, 64, torch.float16, "causal", scale=3.0, seed=6)
+    _check(2, 100, 100, 2, 2, 64, torch.bfloat16, "causal", scale=1e-3, seed=7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_no_range_reaches_is_not_looked_at(dtype):
+    """Padding as torch.empty leaves it: NaN and infinities in keys nobody sees, in queries that see nothing and in
+    their gradients."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(8)
+    for T, pad in ((90, 30), (200, 64), (300, 131)):
+        q, k, v, dout = (_rows(g, 2, T, 4, 64, dtype) for _ in range(4))
+        i = torch.arange(T, device="cuda").expand(2, T)
+        lo = torch.full_like(i, pad).int()
+        hi = torch.where(i < pad, 0, i + 1).int()
+        clean = [x.clone() for x in (q, k, v, dout)]
+        for x in clean:
+            x[:, :pad] = 0
+        for bad in (float("nan"), float("inf"), torch.finfo(dtype).min):
+            for x in (q, k, v, dout):
+                x[:, :pad] = bad
+            announce("padding of %s, T=%d, %s" % (bad, T, dtype))
+            out, lse = ops.range_attention(q, k, v, lo, hi)
+            want, want_lse = ops.range_attention(*clean[:3], lo, hi)
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
+            assert not out[:, :pad].any() and bool((lse[..., :pad] == -float("inf")).all())
+            got = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi)
+            for a, b in zip(got, ops.range_attention_backward(clean[3], *clean[:3], want, want_lse, lo, hi)):
+                assert torch.equal(a, b)
+
+
+def test_gradient_against_differences():
+    """f16 inputs, a step of 2^-4: the value is a sum of B*T*H*D products of out (rounded: 2^-11 of its size)."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(9)
+    q, k, v, dout = (_rows(g, 1, 6, 2, 16, torch.float16) for _ in range(4))
+    lo, hi = _masks("causal", 1, 6, 6, g)
+    form = dict(cap=3.0, slopes=torch.tensor([0.1, 0.4], device="cuda"))
+    announce("attention: differences")
+    out, lse = ops.range_attention(q, k, v, lo, hi, **form)
+    grads = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi, **form)
+    h = 2.0 ** -4
+    for i, grad in enumerate(grads):
+        for at in (0, 40, 100, 191):
+            values = []
+            for sign in (1, -1):
+                args = [x.clone() for x in (q, k, v)]
+                args[i].view(-1)[at] += sign * h
+                step = float(args[i].view(-1)[at]) - float((q, k, v)[i].view(-1)[at])
+                values.append((step, Attention(*args, lo, hi, **form).out.flatten() @ dout.double().flatten()))
+            slope = float((values[0][1] - values[1][1]) / (values[0][0] - values[1][0]))
+            # the difference's own error: h^2/6 of the third derivative (scores of O(1): below 4 a term); the gradient's: its bound
+            ref = Attention(q, k, v, lo, hi, dout=dout, **form)
+            name = ("dq", "dk", "dv")[i]
+            bound = float(getattr(ref, name + "_bound").flatten()[at])
+            assert abs(float(grad.view(-1)[at]) - slope) <= bound + h * h / 6 * 4 * float(dout.abs().sum()) / 6
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_step_over_caches(dtype):
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(10)
+    for B, T, L, H, HK, D in ((1, 1, 1, 1, 1, 16), (3, 1, 33, 4, 4, 64), (2, 3, 700, 6, 2, 80), (5, 2, 257, 32, 2, 128),
+                              (2, 1, 40000, 16, 2, 64), (1, 70, 300, 4, 4, 32), (300, 4, 90, 3, 3, 48)):
+        q, k, v = _rows(g, B, T, H, D, dtype, 1.5), _rows(g, B, L, HK, D, dtype, 1.5), _rows(g, B, L, HK, D, dtype, 1.5)
+        hi = torch.randint(0, L + 1, (B, 1), generator=g, device="cuda") - torch.arange(T, device="cuda").flip(0)
+        lo = (torch.rand(B, 1, generator=g, device="cuda") * 0.5 * hi.clamp(min=0)).long().expand(B, T).clone()
+        lo[0] = -3
+        hi[0, -1] = L + 9
+        lo, hi = lo.int().contiguous(), hi.int().contiguous()
+        # beyond what is filled a cache holds anything
+        at = torch.arange(L, device="cuda")
+        free = (at[None] >= hi.amax(1, keepdim=True))[:, :, None, None]
+        k, v = torch.where(free, float("nan"), k), torch.where(free, float("inf"), v)
+        for cap, slopes in ((0.0, False), (5.0, True)):
+            form = dict(cap=cap, slopes=torch.rand(H, generator=g, device="cuda") * 0.1 if slopes else None)
+            announce("step %s B=%d T=%d L=%d heads=%d/%d D=%d cap=%g" % (dtype, B, T, L, H, HK, D, cap))
+            out = ops.range_attention_step(q, k, v, lo, hi, **form)
+            ref = Attention(q, k, v, lo, hi, place=hi - 1, **form)
+            assert worst(out, ref.out, ref.out_bound) <= 1
+
+
+def test_no_keys_no_queries_no_batch():
+    from gear_amd import ops
+    announce("attention: empty sizes")
+    for B, T, S in ((0, 4, 4), (2, 0, 4), (2, 4, 0), (2, 0, 0)):
+        q, k, v = (torch.empty(B, n, 2, 32, dtype=torch.float16, device="cuda") for n in (T, S, S))
+        lo, hi = torch.zeros(B, T, dtype=torch.int32, device="cuda"), torch.full((B, T), 9, dtype=torch.int32, device="cuda")
+        out, lse = ops.range_attention(q, k, v, lo, hi)
+        assert out.shape == q.shape and not out.any() and bool((lse == -float("inf")).all())
+        dq, dk, dv = ops.range_attention_backward(q, q, k, v, out, lse, lo, hi)
+        assert not dq.any() and not dk.any() and not dv.any()
+        assert not ops.range_attention_step(q, k, v, lo, hi).any()
+
+
+def test_rows_beyond_32_bit_offsets():
+    """A cache whose last rows lie more than 2^32 elements from its first."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(12)
+    announce("rows beyond 2^32 elements")
+    L, stride = 70, (1 << 26) + 8
+    store = torch.empty((L - 1) * stride + 64, dtype=torch.float16, device="cuda")
+    far = store.as_strided((1, L, 2, 32), (0, stride, 32, 1))
+    near = _rows(g, 1, L, 2, 32, torch.float16)
+    far.copy_(near)
+    q = _rows(g, 1, L, 2, 32, torch.float16)
+    lo, hi = _masks("causal", 1, L, L, g)
+    out, lse = ops.range_attention(q, near, near, lo, hi)
+    got, got_lse = ops.range_attention(q, far, far, lo, hi)
+    assert torch.equal(out, got) and torch.equal(lse, got_lse)
+    for a, b in zip(ops.range_attention_backward(q, q, near, near, out, lse, lo, hi),
+                    ops.range_attention_backward(q, q, far, far, out, lse, lo, hi)):
+        assert torch.equal(a, b)
+    assert torch.equal(ops.range_attention_step(q[:, -1:], near, near, lo[:, -1:].contiguous(), hi[:, -1:].contiguous()),
+                       ops.range_attention_step(q[:, -1:], far, far, lo[:, -1:].contiguous(), hi[:, -1:].contiguous()))
+
+
+def test_calls_on_two_streams():
+    """Scratch of its own for each stream: calls in flight on two do not meet."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(13)
+    announce("attention on two streams")
+    sets = []
+    for _ in range(2):
+        q, k, v, dout = (_rows(g, 4, 300, 4, 64, torch.bfloat16) for _ in range(4))
+        sets.append((q, k, v, dout) + _masks("causal", 4, 300, 300, g))
+    want = []
+    for q, k, v, dout, lo, hi in sets:
+        out, lse = ops.range_attention(q, k, v, lo, hi)
+        want.append(ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi) + (ops.range_attention_step(q[:, :1].contiguous(), k, v, lo[:, -1:].contiguous(), hi[:, -1:].contiguous()),))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(10):
+        for x, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                q, k, v, dout, lo, hi = sets[x]
+                out, lse = ops.range_attention(q, k, v, lo, hi)
+                got[x] = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi) + (ops.range_attention_step(q[:, :1].contiguous(), k, v, lo[:, -1:].contiguous(), hi[:, -1:].contiguous()),)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
