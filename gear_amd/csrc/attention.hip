@@ -41,19 +41,20 @@ int attention_args(const gear_hip_attention_desc *d, AttentionArgs &a) {
 
 namespace {
 
-constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kMostWaves = 4;
 constexpr int kTile = 64;  // keys of a tile
 
-template <typename T, int D, bool SHAPED>
-__global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a, T *__restrict__ out,
-                                                             float *__restrict__ lse, int blocks) {
-  __shared__ __attribute__((aligned(16))) T k_tile[kTile * D];
-  __shared__ __attribute__((aligned(16))) T v_tile[kTile * D];
-  __shared__ int ranges[kWaves][2];
+template <typename T, int D, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArgs a, T *__restrict__ out,
+                                                                    float *__restrict__ lse, int blocks) {
+  __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * D];  // (at the end: the rows of the output)
+  __shared__ __attribute__((aligned(16))) T v_tile[2][kTile * D];
+  __shared__ int ranges[WAVES][2];
   const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
-  const int block = blockIdx.x % blocks, bh = blockIdx.x / blocks, head = bh % a.heads, b = bh / a.heads;
+  // a head's workgroups share its keys: next to each other on one die; the last first, where causal rows see most
+  const int at = same_die_index(), block = blocks - 1 - at % blocks, bh = at / blocks, head = bh % a.heads, b = bh / a.heads;
   const int kv_head = head / (a.heads / a.kv_heads);
-  const int i = block * (kWaves * kRows) + wave * kRows + (l & 31);
+  const int i = (block * WAVES + wave) * kRows + (l & 31);
   const bool row_there = i < a.queries;
 
   Seen seen;
@@ -65,62 +66,68 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a, T 
   __syncthreads();
   int first = INT_MAX, end = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) first = min(first, ranges[w][0]), end = max(end, ranges[w][1]);
+  for (int w = 0; w < WAVES; ++w) first = min(first, ranges[w][0]), end = max(end, ranges[w][1]);
+  first = __builtin_amdgcn_readfirstlane(first), end = __builtin_amdgcn_readfirstlane(end);
 
-  const Shape shape(a, head);
+  const Scores<MODE> scores(a, head);
   const int place = i + a.keys - a.queries;
   f32x16 o[D / 32] = {};
-  float m = -INFINITY, sum = 0;
+  float m = -INFINITY, sum = 0;  // m: of z
 
-  const T *k_rows = static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head;
-  const T *v_rows = static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head;
-  TileLoad<T, D, kTile, kThreads> k_load, v_load;
-  auto load = [&](int k0) {
-    auto there = [&](int r) { return k0 + r >= first && k0 + r < end; };
-    k_load.load(k_rows + k0 * a.ks.token, a.ks.token, tid, a.dim, there);
-    v_load.load(v_rows + k0 * a.vs.token, a.vs.token, tid, a.dim, there);
+  const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+  const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
+  auto load = [&](int k0, T *k_to, T *v_to) {
+    k_rows.template ask<WAVES>(k_to, k0, wave);
+    v_rows.template ask<WAVES>(v_to, k0, wave);
   };
-  int k0 = first < end ? first / kTile * kTile : 0;
-  if (k0 < end) load(k0);
-  for (; k0 < end; k0 += kTile) {
-    __syncthreads();
-    k_load.store(k_tile, tid);
-    v_load.store(v_tile, tid);
-    __syncthreads();
-    if (k0 + kTile < end) load(k0 + kTile);
-    if (!seen.touches(k0, k0 + kTile)) continue;
+  auto tile = [&](int k0, const T *k_here, const T *v_here) {
+    if (!seen.touches(k0, k0 + kTile)) return;
     const bool whole = seen.covers(k0, k0 + kTile);
-
     f32x16 s[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = f32x16{};
 #pragma unroll
-      for (int x = 0; x < D / 16; ++x) s[kb] = mfma(rows_frag<T, D>(k_tile, kb * 32, x), q[x], s[kb]);
+      for (int x = 0; x < D / 16; ++x) s[kb] = mfma(rows_frag<T, D>(k_here, kb * 32, x), q[x], s[kb]);
     }
+    const float ahead = (float)(place - k0 - 4 * half);
     float top = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int key = k0 + kb * 32 + result_row(r);
-        float shrink, y = SHAPED ? shape.score(s[kb][r], place - key, shrink) : s[kb][r] * a.scale_log2;
-        if (!whole && (uint32_t)(key - seen.lo) >= (uint32_t)(seen.hi - seen.lo)) y = -INFINITY;
-        s[kb][r] = y;
-        top = fmaxf(top, y);
+        const int offset = kb * 32 + 8 * (r >> 2) + (r & 3);
+        s[kb][r] = scores.z(s[kb][r], ahead - (float)offset);
       }
-    top = fmaxf(m, fmaxf(top, other_half(top)));
-    const float from = top == -INFINITY ? 0.f : top;  // (no key seen yet)
-    const float rescale = exp2_fast(m - from);
-    m = top;
-    sum *= rescale;
+    if (__builtin_expect(!whole, 0)) {
+      const uint32_t from_lo = (uint32_t)(k0 + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (from_lo + (uint32_t)(kb * 32 + 8 * (r >> 2) + (r & 3)) >= count) s[kb][r] = -INFINITY;
+      asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    top = max_of_halves(top);
+    // the sums are rescaled only where a maximum grows by more than 2^8: p stays below that
+    if (wave_ballot((top - m) * scores.factor > 8.f) != 0) {
+      const float grown = fmaxf(m, top);
+      const float rescale = grown == -INFINITY ? 1.f : exp2_fast((m - grown) * scores.factor);
+      m = grown;
+      sum *= rescale;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
+    }
+    const float from = m == -INFINITY ? 0.f : -m * scores.factor;  // (no key seen yet)
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[kb][r] = exp2_fast(s[kb][r] - from);
+        s[kb][r] = exp2_fast(fmaf(s[kb][r], scores.factor, from));
         sum += s[kb][r];
       }
 #pragma unroll
@@ -128,29 +135,35 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(AttentionArgs a, T 
       const vec8<T> p0 = packed<T, 0>(s[kb]), p1 = packed<T, 1>(s[kb]);
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) {
-        o[db] = mfma(columns_frag<T, D>(v_tile, kb * 32, db), p0, o[db]);
-        o[db] = mfma(columns_frag<T, D>(v_tile, kb * 32 + 16, db), p1, o[db]);
+        o[db] = mfma(columns_frag<T, D>(v_here, kb * 32, db), p0, o[db]);
+        o[db] = mfma(columns_frag<T, D>(v_here, kb * 32 + 16, db), p1, o[db]);
       }
     }
+  };
+  int k0 = first < end ? first / kTile * kTile : 0;
+  if (k0 < end) load(k0, k_tile[0], v_tile[0]);
+  for (; k0 < end; k0 += 2 * kTile) {
+    staged_wait();
+    __syncthreads();
+    if (k0 + kTile < end) load(k0 + kTile, k_tile[1], v_tile[1]);
+    tile(k0, k_tile[0], v_tile[0]);
+    if (k0 + kTile >= end) break;
+    staged_wait();
+    __syncthreads();
+    if (k0 + 2 * kTile < end) load(k0 + 2 * kTile, k_tile[0], v_tile[0]);
+    tile(k0 + kTile, k_tile[1], v_tile[1]);
   }
 
-  sum += other_half(sum);
-  if (!row_there) return;
+  sum = sum_of_halves(sum);
   const bool empty = seen.empty();
-  const float over = 1.f / sum;
-  if (lse != nullptr && half == 0)
-    lse[((int64_t)b * a.heads + head) * a.queries + i] = empty ? -INFINITY : (m + __builtin_log2f(sum)) * kLn2;
-  T *to = out + (row * a.heads + head) * a.dim;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + 8 * g + 4 * half;
-      vec4<T> x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (T)(empty ? 0.f : o[db][4 * g + e] * over);
-      if (d < a.dim) *reinterpret_cast<vec4<T> *>(to + d) = x;
-    }
+  if (lse != nullptr && half == 0 && row_there)
+    lse[((int64_t)b * a.heads + head) * a.queries + i] =
+        empty ? -INFINITY : (m * scores.factor + scores.offset + __builtin_log2f(sum)) * kLn2;
+  __syncthreads();  // the tiles are free
+  const int i0 = (block * WAVES + wave) * kRows;
+  store_rows<T, D>(k_tile[0] + wave * kRows * D, o, 1.f / sum, empty, a.dim, [&](int r) {
+    return i0 + r < a.queries ? out + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
+  });
 }
 
 }  // namespace
@@ -165,12 +178,17 @@ extern "C" int gear_hip_attention(const gear_hip_attention_desc *desc, void *out
   if (rc == 1 || a.queries == 0) return 0;
   if (out == nullptr) return GEAR_HIP_EINVAL;
   if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return GEAR_HIP_EALIGN;
-  const int blocks = (int)ceil_div64(a.queries, kWaves * kRows);
-  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto shaped) {
+  // as few workgroups as hold all rows, and in each no more waves than the rows need
+  const int groups = (int)ceil_div64(a.queries, kRows), blocks = (groups + kMostWaves - 1) / kMostWaves;
+  const int waves = (groups + blocks - 1) / blocks;
+  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
-    hipLaunchKernelGGL((attention_kernel<T, decltype(dim)::value, decltype(shaped)::value>),
-                       dim3((unsigned)blocks * a.heads * a.batch), dim3(kThreads), 0, as_stream(stream), a,
-                       static_cast<T *>(out), lse, blocks);
+    by_waves(waves, [&](auto w) {
+      constexpr int kWaves = decltype(w)::value;
+      hipLaunchKernelGGL((attention_kernel<T, decltype(dim)::value, decltype(mode)::value, kWaves>),
+                         dim3((unsigned)blocks * a.heads * a.batch), dim3(kWaves * kWave), 0, as_stream(stream), a,
+                         static_cast<T *>(out), lse, blocks);
+    });
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
   return 0;

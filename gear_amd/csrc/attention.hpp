@@ -81,12 +81,18 @@ __device__ __forceinline__ vec8<T> columns_frag(const T *tile, int first, int bl
   return __builtin_bit_cast(vec8<T>, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// 8 neighbouring results as an operand of the next product
+// 8 neighbouring results as an operand of the next product (in pairs: one instruction rounds two)
 template <typename T, int U>
 __device__ __forceinline__ vec8<T> packed(const f32x16 &x) {
-  const f32x8 y = U == 0 ? __builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7)
-                         : __builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15);
-  return __builtin_convertvector(y, vec8<T>);
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef T pair __attribute__((ext_vector_type(2)));
+  vec8<T> y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const pair z = __builtin_convertvector((f32x2){x[8 * U + 2 * e], x[8 * U + 2 * e + 1]}, pair);
+    y[2 * e] = z[0], y[2 * e + 1] = z[1];
+  }
+  return y;
 }
 
 // row of the result that element r of this lane holds
@@ -132,8 +138,74 @@ struct TileLoad {
   }
 };
 
-// The value of the lane 32 further (or before): the other half of the same result column.
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// Rows of a tile of ROWS rows straight from memory into LDS, 64 pieces an instruction, the instructions dealt
+// out to the waves of a workgroup.  Rows outside [first, end) are replaced by the nearest inside, pieces
+// beyond `dim` by the last: what a tile holds there is finite wherever the rows in range are, and multiplied
+// by zeros only.  A tile is complete after staged_wait() in every wave and a barrier.
+// The instruction is written out because the compiler, which cannot tell the tile that is asked for from
+// the one that is read meanwhile, has every read of LDS behind its builtin wait for the memory.
+template <typename T, int D, int ROWS>
+struct Stage {
+  static constexpr int kPieces = D / 8, kRowsEach = kWave / kPieces, kCount = ROWS / kRowsEach;
+  const T *base;
+  int64_t stride;
+  int first, end, dim;
+  int64_t offset[2];  // of the lane's piece within an even and an odd instruction's rows
+
+  __device__ __forceinline__ Stage(const T *base, int64_t stride, int first, int end, int dim)
+      : base(base), stride(stride), first(first), end(end), dim(dim) {
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) offset[odd] = (lane_id() / kPieces) * stride + piece(odd) * 8;
+  }
+  // (rows of an instruction differ from those of the next but one by a multiple of 8: the same swizzle)
+  __device__ __forceinline__ int piece(int x) const {
+    const int l = lane_id();
+    return min((l % kPieces) ^ swizzle<D>(x * kRowsEach + l / kPieces), dim / 8 - 1);
+  }
+  __device__ __forceinline__ void one(const T *from, T *to) const {
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T *)to;
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(from), "s"(__builtin_amdgcn_readfirstlane(at))
+                 : "memory", "m0");
+  }
+  // the share of wave `wave` of WAVES
+  template <int WAVES>
+  __device__ __forceinline__ void ask(T *tile, int row0, int wave) const {
+    if (row0 >= first && row0 + ROWS <= end) {
+#pragma unroll
+      for (int y = 0; y < (kCount + WAVES - 1) / WAVES; ++y) {
+        const int x = wave + y * WAVES;
+        if ((y + 1) * WAVES > kCount && x >= kCount) break;
+        one(base + (int64_t)(row0 + x * kRowsEach) * stride + ((x & 1) ? offset[1] : offset[0]), tile + x * kWave * 8);
+      }
+    } else {
+#pragma unroll 1
+      for (int x = wave; x < kCount; x += WAVES) {
+        const int row = row0 + x * kRowsEach + lane_id() / kPieces;
+        one(base + (int64_t)min(max(row, first), end - 1) * stride + piece(x) * 8, tile + x * kWave * 8);
+      }
+    }
+  }
+};
+// (the builtin: the compiler then knows that its own loads have arrived too, and waits for none of them, and with
+// them for what is asked for next, inside the loop)
+__device__ __forceinline__ void staged_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// The maximum and the sum of a lane's value and that of the lane 32 further (or before): the other half of the
+// same result column.
+__device__ __forceinline__ float max_of_halves(float x) {
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float x) {
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
 
 template <typename F>
 __device__ __forceinline__ int wave_reduce(int x, const F &f) {
@@ -163,38 +235,85 @@ struct Seen {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh by 1 - 2 / (1 + e^2x): within 2e-7 of 1, which the cap scales like its scores
-__device__ __forceinline__ float tanh_of(float x) {
-  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + exp2_fast(x * (2 * kLog2e)));
-}
-
-// A score as an exponent of 2, from the product of the rows; `shrink`: the cap's derivative there.
-struct Shape {
-  float scale_log2, over_cap, cap_log2, slope_log2;
-  bool capped;
-  __device__ __forceinline__ Shape(const AttentionArgs &a, int head)
-      : scale_log2(a.scale_log2), over_cap(a.cap > 0 ? a.scale / a.cap : 0), cap_log2(a.cap * kLog2e),
-        slope_log2(a.slopes ? a.slopes[head] * kLog2e : 0), capped(a.cap > 0) {}
-  __device__ __forceinline__ float score(float x, int distance, float &shrink) const {
-    float y = x * scale_log2;
+// Scores as exponents of 2: factor * z + offset, where z comes from the product x of the rows.
+//   plain       z = x
+//   kCap        cap tanh(u) = cap (1 - 2 / (1 + e^2u)): z = -1 / (1 + e^2u), in [-1, 0]
+//   kBias       z = x scale log2(e) - slope |distance|, and with the cap the same of the capped score
+// so that a plain or capped score costs no instruction for its scale: it is part of the exponent's
+// multiply-add.  The cap is within 2^-23 cap of the exact one, as 32-bit scores of that size are.
+constexpr int kCap = 1, kBias = 2;
+template <int MODE>
+struct Scores {
+  float factor, offset, inner, outer, slope;
+  __device__ __forceinline__ Scores(const AttentionArgs &a, int head) {
+    const float cap_log2 = a.cap * kLog2e;
+    inner = MODE & kCap ? a.scale / a.cap * (2 * kLog2e) : a.scale_log2;
+    outer = 2 * cap_log2;
+    slope = MODE & kBias && a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    factor = MODE == 0 ? a.scale_log2 : MODE == kCap ? outer : 1.f;
+    offset = MODE & kCap ? cap_log2 : 0.f;
+  }
+  // -1 / (1 + e^2u)
+  __device__ __forceinline__ float capped(float x) const { return __builtin_amdgcn_rcpf(-1.f - exp2_fast(x * inner)); }
+  __device__ __forceinline__ float z(float x, float distance) const {
+    if (MODE == 0) return x;
+    if (MODE == kCap) return capped(x);
+    const float off = -slope * fabsf(distance);
+    return MODE == kBias ? fmaf(x, inner, off) : fmaf(capped(x), outer, off);
+  }
+  // the same, and the derivative of the cap: 1 - tanh^2 = -4 z (1 + z)
+  __device__ __forceinline__ float z(float x, float distance, float &shrink) const {
     shrink = 1.f;
-    if (capped) {
-      const float t = tanh_of(x * over_cap);
-      y = t * cap_log2;
-      shrink = 1.f - t * t;
-    }
-    return y - slope_log2 * (float)abs(distance);
+    if (!(MODE & kCap)) return z(x, distance);
+    const float c = capped(x);
+    shrink = -4.f * fmaf(c, c, c);
+    return MODE == kCap ? c : fmaf(c, outer, -slope * fabsf(distance));
   }
 };
 
-// f(std::integral_constant<int, D>(), element, std::bool_constant<shaped>()) for the call's type and sizes
+// Workgroups go round the 8 dies: neighbours in this numbering share a die, and its cache.
+__device__ __forceinline__ int same_die_index() {
+  const int n = gridDim.x, per = n / 8, rest = n % 8, die = blockIdx.x % 8;
+  return die * per + min(die, rest) + blockIdx.x / 8;
+}
+
+// The 32 rows of 32 * (D / 32) results that a wave holds by columns (column l%32: row l%32 of the output), times
+// `factor` of the column, to memory through a piece of LDS of 32 * D elements of the wave's own, 16 bytes a lane.
+// to(row): where a row begins, or null.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void store_rows(T *piece, const f32x16 *x, float factor, bool zero, int dim, const F &to) {
+  const int l = lane_id(), half = l >> 5;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      vec4<T> y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (T)(zero ? 0.f : x[db][4 * g + e] * factor);
+      *reinterpret_cast<vec4<T> *>(piece + piece_at<D>(l & 31, db * 4 + g) + 4 * half) = y;
+    }
+  wave_lds_sync();
+#pragma unroll
+  for (int y = 0; y < D / 16; ++y) {
+    const int at = y * kWave + l, row = at / (D / 8), c = at % (D / 8);
+    T *p = to(row);
+    if (p != nullptr && c * 8 < dim)
+      *reinterpret_cast<vec8<T> *>(p + c * 8) = *reinterpret_cast<const vec8<T> *>(piece + piece_at<D>(row, c));
+  }
+}
+
+// f(std::integral_constant<int, D>(), element, std::integral_constant<int, MODE>()) for the call's type and sizes
 template <typename F>
 void by_attention_type(const AttentionArgs &a, int dtype, const F &f) {
   auto shape = [&](auto dim, auto type) {
-    if (a.cap > 0 || a.slopes != nullptr)
-      f(dim, type, std::true_type());
+    if (a.slopes == nullptr && !(a.cap > 0))
+      f(dim, type, std::integral_constant<int, 0>());
+    else if (a.slopes == nullptr)
+      f(dim, type, std::integral_constant<int, kCap>());
+    else if (!(a.cap > 0))
+      f(dim, type, std::integral_constant<int, kBias>());
     else
-      f(dim, type, std::false_type());
+      f(dim, type, std::integral_constant<int, kCap | kBias>());
   };
   auto dims = [&](auto type) {
     if (a.dim <= 32)
@@ -208,6 +327,19 @@ void by_attention_type(const AttentionArgs &a, int dtype, const F &f) {
     dims(f16());
   else
     dims(bf16());
+}
+
+// f(std::integral_constant<int, waves>()), 1 to 4 waves
+template <typename F>
+void by_waves(int waves, const F &f) {
+  if (waves == 1)
+    f(std::integral_constant<int, 1>());
+  else if (waves == 2)
+    f(std::integral_constant<int, 2>());
+  else if (waves == 3)
+    f(std::integral_constant<int, 3>());
+  else
+    f(std::integral_constant<int, 4>());
 }
 
 // Checks of what every attention call takes.  0: go on; 1: no queries; else the error.

@@ -28,7 +28,7 @@ struct GradArgs {
   int blocks;      // workgroups of a head
 };
 
-template <typename T, int D, bool SHAPED>
+template <typename T, int D, int MODE>
 __global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
   __shared__ __attribute__((aligned(16))) T k_tile[kTile * D];
   __shared__ __attribute__((aligned(16))) T v_tile[kTile * D];
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
     for (int x = 0; x < D / 16; ++x)
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)dout[x][e] * (float)out[x][e];
-    delta += other_half(delta);
+    delta = sum_of_halves(delta);
   }
   float lse_log2 = INFINITY;  // a row that sees nothing: p = 0
   if (row_there) {
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) first = min(first, ranges[w][0]), end = max(end, ranges[w][1]);
 
-  const Shape shape(a, head);
+  const Scores<MODE> scores(a, head);
   const int place = i + a.keys - a.queries;
   f32x16 dq[D / 32] = {};
   const T *k_rows = static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head;
@@ -105,9 +105,10 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = kk + result_row(r);
-        float shrink = 1.f, y = SHAPED ? shape.score(s[r], place - key, shrink) : s[r] * a.scale_log2;
-        float ds = exp2_fast(y - lse_log2) * (dp[r] - delta);
-        if (SHAPED) ds *= shrink;
+        float shrink;
+        const float z = scores.z(s[r], (float)(place - key), shrink);
+        float ds = exp2_fast(fmaf(z, scores.factor, scores.offset - lse_log2)) * (dp[r] - delta);
+        if (MODE & kCap) ds *= shrink;
         if (!whole && (uint32_t)(key - seen.lo) >= (uint32_t)(seen.hi - seen.lo)) ds = 0;
         s[r] = ds;
       }
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
 template <typename T>
 constexpr float kRaise = std::is_same<T, f16>::value ? 10.f : 0.f;
 
-template <typename T, int D, bool SHAPED>
+template <typename T, int D, int MODE>
 __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(GradArgs g) {
   __shared__ __attribute__((aligned(16))) T q_tile[kTile * D];
   __shared__ __attribute__((aligned(16))) T g_tile[kTile * D];
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(GradArgs g) {
 
   for (int x = 0; x < shared; ++x) {
     const int head = kv_head * shared + x;
-    const Shape shape(a, head);
+    const Scores<MODE> scores(a, head);
     const T *q_rows = static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head;
     const T *g_rows = static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head;
     const int64_t stats = ((int64_t)b * a.heads + head) * a.queries;
@@ -215,11 +216,11 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(GradArgs g) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = 4 * z + e;
-              float shrink = 1.f;
-              const float y = SHAPED ? shape.score(s[r], i0 + r0 + e + a.keys - a.queries - key, shrink) : s[r] * a.scale_log2;
-              float p = exp2_fast(y - (lse[e] - kRaise<T>));
+              float shrink;
+              const float z = scores.z(s[r], (float)(i0 + r0 + e + a.keys - a.queries - key), shrink);
+              float p = exp2_fast(fmaf(z, scores.factor, scores.offset + kRaise<T> - lse[e]));
               float ds = p * (lower * dp[r] - lower * delta[e]);
-              if (SHAPED) ds *= shrink;
+              if (MODE & kCap) ds *= shrink;
               if (!whole && (uint32_t)(key - lo[e]) >= (uint32_t)(hi[e] - lo[e])) p = ds = 0;
               s[r] = p, dp[r] = ds;
             }
@@ -294,17 +295,17 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
   g.delta = static_cast<float *>(workspace);
   g.bounds = reinterpret_cast<i32x4 *>(static_cast<char *>(workspace) + delta_bytes(a.batch, a.queries, a.heads));
   g.dq = dq, g.dk = dk, g.dv = dv;
-  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto shaped) {
+  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
     constexpr int D = decltype(dim)::value;
-    constexpr bool kShaped = decltype(shaped)::value;
+    constexpr int kMode = decltype(mode)::value;
     g.blocks = (int)ceil_div64(a.queries, kWaves * kRows);
     if (g.blocks > 0)
-      hipLaunchKernelGGL((attention_dq_kernel<T, D, kShaped>), dim3((unsigned)g.blocks * a.heads * a.batch),
+      hipLaunchKernelGGL((attention_dq_kernel<T, D, kMode>), dim3((unsigned)g.blocks * a.heads * a.batch),
                          dim3(kThreads), 0, as_stream(stream), g);
     g.blocks = (int)ceil_div64(a.keys, kWaves * kRows);
     if (g.blocks > 0)
-      hipLaunchKernelGGL((attention_dkv_kernel<T, D, kShaped>), dim3((unsigned)g.blocks * a.kv_heads * a.batch),
+      hipLaunchKernelGGL((attention_dkv_kernel<T, D, kMode>), dim3((unsigned)g.blocks * a.kv_heads * a.batch),
                          dim3(kThreads), 0, as_stream(stream), g);
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();

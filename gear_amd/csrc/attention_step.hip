@@ -25,7 +25,7 @@ struct StepArgs {
   void *out;
 };
 
-template <typename T, int D, bool SHAPED>
+template <typename T, int D, int MODE>
 __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
   __shared__ __attribute__((aligned(16))) float joined[kWaves][kRows][D];  // (V's tiles before that)
   __shared__ float2 joined_ml[kWaves][kRows];
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
   const int64_t part_first = seen.first < seen.end ? seen.first + (int64_t)split * part : 0;
   const int end = (int)min((int64_t)seen.end, part_first + part);
 
-  const Shape shape(a, row_there ? head : 0);
+  const Scores<MODE> scores(a, row_there ? head : 0);
   f32x16 o[D / 32] = {};
   float m = -INFINITY, sum = 0;
   const T *k_rows = static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head;
@@ -73,12 +73,12 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int key = (int)k0 + result_row(r);
-      float shrink, y = SHAPED ? shape.score(s[r], seen.hi - 1 - key, shrink) : s[r] * a.scale_log2;
+      float y = fmaf(scores.z(s[r], (float)(seen.hi - 1 - key)), scores.factor, scores.offset);
       if (key >= end || (uint32_t)(key - seen.lo) >= (uint32_t)(seen.hi - seen.lo)) y = -INFINITY;
       s[r] = y;
       top = fmaxf(top, y);
     }
-    top = fmaxf(m, fmaxf(top, other_half(top)));
+    top = fmaxf(m, max_of_halves(top));
     const float from = top == -INFINITY ? 0.f : top;
     const float rescale = exp2_fast(m - from);
     m = top;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
       o[db] = mfma(columns_frag<T, D>(v_tile, 16, db), p1, o[db]);
     }
   }
-  sum += other_half(sum);
+  sum = sum_of_halves(sum);
 
   // join the waves
   __syncthreads();
@@ -208,9 +208,9 @@ extern "C" int gear_hip_attention_step(const gear_hip_attention_desc *desc, void
   g.part_o = static_cast<float *>(workspace);
   g.part_ml = reinterpret_cast<float2 *>(g.part_o + units * g.splits * kRows * a.dim);
   g.out = out;
-  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto shaped) {
+  by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
-    hipLaunchKernelGGL((attention_step_kernel<T, decltype(dim)::value, decltype(shaped)::value>),
+    hipLaunchKernelGGL((attention_step_kernel<T, decltype(dim)::value, decltype(mode)::value>),
                        dim3((unsigned)(units * g.splits)), dim3(kThreads), 0, as_stream(stream), g);
     if (g.splits > 1)
       hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(128), 0,
