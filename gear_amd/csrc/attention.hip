@@ -70,6 +70,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
   first = __builtin_amdgcn_readfirstlane(first), end = __builtin_amdgcn_readfirstlane(end);
 
   const Scores<MODE> scores(a, head);
+  const TileReader<T, D> reader;
   const int place = i + a.keys - a.queries;
   f32x16 o[D / 32] = {};
   float m = -INFINITY, sum = 0;  // m: of z
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = f32x16{};
 #pragma unroll
-      for (int x = 0; x < D / 16; ++x) s[kb] = mfma(rows_frag<T, D>(k_here, kb * 32, x), q[x], s[kb]);
+      for (int x = 0; x < D / 16; ++x) s[kb] = mfma(reader.rows(k_here, kb * 32, x), q[x], s[kb]);
     }
     const float ahead = (float)(place - k0 - 4 * half);
     float top = -INFINITY;
@@ -135,8 +136,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
       const vec8<T> p0 = packed<T, 0>(s[kb]), p1 = packed<T, 1>(s[kb]);
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) {
-        o[db] = mfma(columns_frag<T, D>(v_here, kb * 32, db), p0, o[db]);
-        o[db] = mfma(columns_frag<T, D>(v_here, kb * 32 + 16, db), p1, o[db]);
+        o[db] = mfma(reader.columns(v_here, kb * 32, db), p0, o[db]);
+        o[db] = mfma(reader.columns(v_here, kb * 32 + 16, db), p1, o[db]);
       }
     }
   };

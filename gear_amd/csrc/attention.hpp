@@ -81,6 +81,38 @@ __device__ __forceinline__ vec8<T> columns_frag(const T *tile, int first, int bl
   return __builtin_bit_cast(vec8<T>, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The same two operands by offsets that a lane works out once: what remains of an address is a constant of the
+// instruction.  (swizzle() of a row is the same for rows a multiple of 8 apart, and changes the lower 3 bits of a
+// piece only.)
+template <typename T, int D>
+struct TileReader {
+  static constexpr int kRowOffsets = D / 16 < 4 ? D / 16 : 4, kColumnOffsets = D / 32 < 2 ? 1 : 2;
+  int row[kRowOffsets], column[kColumnOffsets];  // elements
+  __device__ __forceinline__ TileReader() {
+    const int l = lane_id(), half = l >> 5, t = l & 15;
+#pragma unroll
+    for (int s = 0; s < kRowOffsets; ++s) row[s] = piece_at<D>(l & 31, 2 * s + half);
+#pragma unroll
+    for (int b = 0; b < kColumnOffsets; ++b)
+      column[b] = piece_at<D>(4 * half + (t >> 2), 4 * b + 2 * ((l >> 4) & 1) + ((t & 3) >> 1)) + 4 * (t & 1);
+  }
+  // rows first.. (a multiple of 8) as rows_frag
+  __device__ __forceinline__ vec8<T> rows(const T *tile, int first, int s) const {
+    return *reinterpret_cast<const vec8<T> *>(tile + row[s % kRowOffsets] + first * D + s / kRowOffsets * 64);
+  }
+  // rows first.. (a multiple of 16) as columns_frag
+  __device__ __forceinline__ vec8<T> columns(const T *tile, int first, int block) const {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    auto read = [&](int r) {
+      const T *p = tile + column[block % kColumnOffsets] + r * D + block / kColumnOffsets * 64;
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(const_cast<T *>(p)));
+    };
+    const s16x4 a = read(first), b = read(first + 8);
+    return __builtin_bit_cast(vec8<T>, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
 // 8 neighbouring results as an operand of the next product (in pairs: one instruction rounds two)
 template <typename T, int U>
 __device__ __forceinline__ vec8<T> packed(const f32x16 &x) {
@@ -162,8 +194,7 @@ struct Stage {
     const int l = lane_id();
     return min((l % kPieces) ^ swizzle<D>(x * kRowsEach + l / kPieces), dim / 8 - 1);
   }
-  __device__ __forceinline__ void one(const T *from, T *to) const {
-    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T *)to;
+  __device__ __forceinline__ void one(const T *from, uint32_t at) const {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :
                  : "v"(from), "s"(__builtin_amdgcn_readfirstlane(at))
@@ -172,18 +203,20 @@ struct Stage {
   // the share of wave `wave` of WAVES
   template <int WAVES>
   __device__ __forceinline__ void ask(T *tile, int row0, int wave) const {
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T *)tile + wave * 1024;
+    constexpr int kNext = WAVES * 1024;  // bytes of LDS that the waves' instructions fill together
     if (row0 >= first && row0 + ROWS <= end) {
 #pragma unroll
       for (int y = 0; y < (kCount + WAVES - 1) / WAVES; ++y) {
         const int x = wave + y * WAVES;
         if ((y + 1) * WAVES > kCount && x >= kCount) break;
-        one(base + (int64_t)(row0 + x * kRowsEach) * stride + ((x & 1) ? offset[1] : offset[0]), tile + x * kWave * 8);
+        one(base + (int64_t)(row0 + x * kRowsEach) * stride + ((x & 1) ? offset[1] : offset[0]), at + y * kNext);
       }
     } else {
 #pragma unroll 1
-      for (int x = wave; x < kCount; x += WAVES) {
+      for (int x = wave, to = at; x < kCount; x += WAVES, to += kNext) {
         const int row = row0 + x * kRowsEach + lane_id() / kPieces;
-        one(base + (int64_t)min(max(row, first), end - 1) * stride + piece(x) * 8, tile + x * kWave * 8);
+        one(base + (int64_t)min(max(row, first), end - 1) * stride + piece(x) * 8, to);
       }
     }
   }
