@@ -23,30 +23,133 @@ struct GradArgs {
   Strides gs;
   const float *lse;
   float *delta;    // [batch][heads][queries]
-  i32x4 *bounds;   // [batch][ceil(queries/32)]: first, end, all_from, all_to
+  i32x4 *bounds;   // [batch][ceil(queries/32)]: first, end, all_from, all_to (0 where a row sees nothing, or is none)
   void *dq, *dk, *dv;
   int blocks;      // workgroups of a head
 };
 
-template <typename T, int D, int MODE>
-__global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
-  __shared__ __attribute__((aligned(16))) T k_tile[kTile * D];
-  __shared__ __attribute__((aligned(16))) T v_tile[kTile * D];
-  __shared__ int ranges[kWaves][2];
+// 32 keys (rows `row0`.. of the tiles, kk.. in memory) by the wave's 32 queries, a lane a query: the gradients of the scores, or,
+// for delta alone, the lane's share of sum p dp.
+template <bool DELTA, typename T, int D, int MODE>
+__device__ __forceinline__ f32x16 grads_by_query(const T *k_tile, const T *v_tile, int row0, int kk, const vec8<T> (&q)[D / 16],
+                                                 const vec8<T> (&dout)[D / 16], const TileReader<T, D> &reader,
+                                                 const Scores<MODE> &scores, const Seen &seen, int place, float less,
+                                                 float &delta) {
+  const int half = lane_id() >> 5;
+  f32x16 s = {}, dp = {};
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_tile, row0, x), q[x], s);
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x) dp = mfma(reader.rows(v_tile, row0, x), dout[x], dp);
+  const float ahead = (float)(place - kk - 4 * half);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float shrink;
+    const float z = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)), shrink);
+    const float p = exp2_fast(fmaf(z, scores.factor, less));
+    s[r] = DELTA ? p * dp[r] : p * (dp[r] - delta) * ((MODE & kCap) ? shrink : 1.f);
+  }
+  if (__builtin_expect(!seen.covers(kk, kk + 32), 0)) {
+    const uint32_t from_lo = (uint32_t)(kk + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) >= count) s[r] = 0;
+    asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
+  }
+  if (DELTA) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) delta += s[r];
+  }
+  return s;
+}
+
+// x += (rows row0.. of the tile, transposed) times the 32 x 32 block y
+template <typename T, int D>
+__device__ __forceinline__ void add_columns(f32x16 (&x)[D / 32], const T *tile, int row0, const f32x16 &y, const TileReader<T, D> &reader) {
+  const vec8<T> y0 = packed<T, 0>(y), y1 = packed<T, 1>(y);
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) {
+    x[db] = mfma(reader.columns(tile, row0, db), y0, x[db]);
+    x[db] = mfma(reader.columns(tile, row0 + 16, db), y1, x[db]);
+  }
+}
+
+// p is at most 1 and often far below the smallest normal f16, so it is multiplied with dout 2^10 times as large.
+template <typename T>
+constexpr float kRaise = std::is_same<T, f16>::value ? 10.f : 0.f;
+
+// What the keys' side needs of `N` queries, in LDS.
+template <int N>
+struct __attribute__((aligned(16))) QueryRows {
+  float lse[N], delta[N];  // lse in exponents of 2, infinite where a row sees nothing
+  int lo[N], hi[N];        // 0, 0 there
+};
+
+// 32 queries (rows `row0`.. of the tiles and of `rows`, i0.. in memory) by the wave's 32 keys, a lane a key: dv += p^T dout,
+// dk += ds^T q.
+template <typename T, int D, int MODE, int N>
+__device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], const T *q_tile, const T *g_tile, int row0,
+                                           const QueryRows<N> &rows, const vec8<T> (&k)[D / 16], const vec8<T> (&v)[D / 16],
+                                           const TileReader<T, D> &reader, const Scores<MODE> &scores, int ahead, int key,
+                                           bool whole) {
+  const int half = lane_id() >> 5;
+  f32x16 s = {}, dp = {};
+#pragma unroll
+  for (int y = 0; y < D / 16; ++y) s = mfma(reader.rows(q_tile, row0, y), k[y], s);
+#pragma unroll
+  for (int y = 0; y < D / 16; ++y) dp = mfma(reader.rows(g_tile, row0, y), v[y], dp);
+  constexpr float lower = 1.f / (1 << (int)kRaise<T>);
+  const float distance = (float)(ahead + 4 * half - key);
+#pragma unroll
+  for (int z = 0; z < 4; ++z) {
+    const int r0 = row0 + 8 * z + 4 * half;
+    const f32x4 lse = *reinterpret_cast<const f32x4 *>(rows.lse + r0), delta = *reinterpret_cast<const f32x4 *>(rows.delta + r0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 4 * z + e;
+      float shrink;
+      const float y = scores.z(s[r], distance + (float)(8 * z + e), shrink);
+      const float p = exp2_fast(fmaf(y, scores.factor, scores.offset + kRaise<T> - lse[e]));
+      float ds = p * (kRaise<T> > 0 ? fmaf(lower, dp[r], -lower * delta[e]) : dp[r] - delta[e]);
+      if (MODE & kCap) ds *= shrink;
+      s[r] = p, dp[r] = ds;
+    }
+  }
+  if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const int r0 = row0 + 8 * z + 4 * half;
+      const i32x4 lo = *reinterpret_cast<const i32x4 *>(rows.lo + r0), hi = *reinterpret_cast<const i32x4 *>(rows.hi + r0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((uint32_t)(key - lo[e]) >= (uint32_t)(hi[e] - lo[e])) s[4 * z + e] = dp[4 * z + e] = 0;
+    }
+    asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
+  }
+  add_columns<T, D>(dv, g_tile, row0, s, reader);
+  add_columns<T, D>(dk, q_tile, row0, dp, reader);
+}
+
+template <typename T, int D, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs g) {
+  __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * D];  // (at the end: the rows of dq)
+  __shared__ __attribute__((aligned(16))) T v_tile[2][kTile * D];
+  __shared__ int ranges[WAVES][2];
   const AttentionArgs &a = g.a;
   const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
-  const int block = blockIdx.x % g.blocks, bh = blockIdx.x / g.blocks, head = bh % a.heads, b = bh / a.heads;
+  const int at = same_die_index(), block = g.blocks - 1 - at % g.blocks, bh = at / g.blocks, head = bh % a.heads, b = bh / a.heads;
   const int kv_head = head / (a.heads / a.kv_heads);
-  const int i = block * (kWaves * kRows) + wave * kRows + (l & 31);
+  const int i0 = (block * WAVES + wave) * kRows, i = i0 + (l & 31);
   const bool row_there = i < a.queries;
 
   Seen seen;
   const int64_t row = (int64_t)b * a.queries + i;
   seen.set(row_there ? a.lo[row] : 0, row_there ? a.hi[row] : 0, a.keys);
   if (l == 0) ranges[wave][0] = seen.first, ranges[wave][1] = seen.end;
-  const int group = block * kWaves + wave, groups = (a.queries + kRows - 1) / kRows;
-  if (head == 0 && l == 0 && group < groups)
-    g.bounds[(int64_t)b * groups + group] = i32x4{seen.first, seen.end, seen.all_from, seen.all_to};
+  const bool some_empty = wave_ballot(seen.empty()) != 0;
+  if (head == 0 && l == 0 && i0 < a.queries)
+    g.bounds[(int64_t)b * ((a.queries + kRows - 1) / kRows) + i0 / kRows] =
+        i32x4{seen.first, seen.end, seen.all_from, some_empty ? 0 : seen.all_to};
 
   vec8<T> q[D / 16], dout[D / 16];
   own_row_frags<T, D>(q, static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head, a.dim, !seen.empty());
@@ -64,89 +167,56 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(GradArgs g) {
   }
   float lse_log2 = INFINITY;  // a row that sees nothing: p = 0
   if (row_there) {
-    const int64_t at = ((int64_t)b * a.heads + head) * a.queries + i;
-    if (half == 0) g.delta[at] = delta;
-    if (!seen.empty()) lse_log2 = g.lse[at] * kLog2e;
+    const int64_t stats = ((int64_t)b * a.heads + head) * a.queries + i;
+    if (half == 0) g.delta[stats] = delta;
+    if (!seen.empty()) lse_log2 = g.lse[stats] * kLog2e;
   }
   __syncthreads();
   int first = INT_MAX, end = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) first = min(first, ranges[w][0]), end = max(end, ranges[w][1]);
+  for (int w = 0; w < WAVES; ++w) first = min(first, ranges[w][0]), end = max(end, ranges[w][1]);
+  first = __builtin_amdgcn_readfirstlane(first), end = __builtin_amdgcn_readfirstlane(end);
 
   const Scores<MODE> scores(a, head);
+  const TileReader<T, D> reader;
+  const float less = scores.offset - lse_log2;
   const int place = i + a.keys - a.queries;
   f32x16 dq[D / 32] = {};
-  const T *k_rows = static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head;
-  const T *v_rows = static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head;
-  TileLoad<T, D, kTile, kThreads> k_load, v_load;
-  auto load = [&](int k0) {
-    auto there = [&](int r) { return k0 + r >= first && k0 + r < end; };
-    k_load.load(k_rows + k0 * a.ks.token, a.ks.token, tid, a.dim, there);
-    v_load.load(v_rows + k0 * a.vs.token, a.vs.token, tid, a.dim, there);
+  const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+  const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
+  auto load = [&](int k0, int to) __attribute__((always_inline)) {
+    k_rows.template ask<WAVES>(k_tile[to], k0, wave);
+    v_rows.template ask<WAVES>(v_tile[to], k0, wave);
   };
-  int k0 = first < end ? first / kTile * kTile : 0;
-  if (k0 < end) load(k0);
-  for (; k0 < end; k0 += kTile) {
+  int k0 = first < end ? first / kTile * kTile : 0, buffer = 0;
+  if (k0 < end) load(k0, 0);
+  for (; k0 < end; k0 += kTile, buffer ^= 1) {
+    staged_wait();
     __syncthreads();
-    k_load.store(k_tile, tid);
-    v_load.store(v_tile, tid);
-    __syncthreads();
-    if (k0 + kTile < end) load(k0 + kTile);
-#pragma unroll
+    if (k0 + kTile < end) load(k0 + kTile, buffer ^ 1);
+    const T *k_here = k_tile[buffer], *v_here = v_tile[buffer];
+#pragma unroll 1
     for (int kb = 0; kb < 2; ++kb) {
       const int kk = k0 + kb * 32;
       if (!seen.touches(kk, kk + 32)) continue;
-      const bool whole = seen.covers(kk, kk + 32);
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) s = mfma(rows_frag<T, D>(k_tile, kb * 32, x), q[x], s);
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) dp = mfma(rows_frag<T, D>(v_tile, kb * 32, x), dout[x], dp);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = kk + result_row(r);
-        float shrink;
-        const float z = scores.z(s[r], (float)(place - key), shrink);
-        float ds = exp2_fast(fmaf(z, scores.factor, scores.offset - lse_log2)) * (dp[r] - delta);
-        if (MODE & kCap) ds *= shrink;
-        if (!whole && (uint32_t)(key - seen.lo) >= (uint32_t)(seen.hi - seen.lo)) ds = 0;
-        s[r] = ds;
-      }
-      const vec8<T> d0 = packed<T, 0>(s), d1 = packed<T, 1>(s);
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-        dq[db] = mfma(columns_frag<T, D>(k_tile, kb * 32, db), d0, dq[db]);
-        dq[db] = mfma(columns_frag<T, D>(k_tile, kb * 32 + 16, db), d1, dq[db]);
-      }
+      const f32x16 ds = grads_by_query<false, T, D, MODE>(k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less, delta);
+      add_columns<T, D>(dq, k_here, kb * 32, ds, reader);
     }
   }
-  if (!row_there) return;
-  T *to = static_cast<T *>(g.dq) + (row * a.heads + head) * a.dim;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int d = db * 32 + 8 * x + 4 * half;
-      vec4<T> y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(seen.empty() ? 0.f : dq[db][4 * x + e] * a.scale);
-      if (d < a.dim) *reinterpret_cast<vec4<T> *>(to + d) = y;
-    }
+  __syncthreads();
+  store_rows<T, D>(k_tile[0] + wave * kRows * D, dq, a.scale, seen.empty(), a.dim, [&](int r) {
+    return i0 + r < a.queries ? static_cast<T *>(g.dq) + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
+  });
 }
 
-// p is at most 1 and often far below the smallest normal f16, so it is multiplied with dout 2^10 times as large.
-template <typename T>
-constexpr float kRaise = std::is_same<T, f16>::value ? 10.f : 0.f;
-
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(kThreads) void attention_dkv_kernel(GradArgs g) {
-  __shared__ __attribute__((aligned(16))) T q_tile[kTile * D];
-  __shared__ __attribute__((aligned(16))) T g_tile[kTile * D];
-  __shared__ __attribute__((aligned(16))) float row_lse[kTile], row_delta[kTile];
-  __shared__ __attribute__((aligned(16))) int row_lo[kTile], row_hi[kTile];
+__global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) {
+  __shared__ __attribute__((aligned(16))) T q_tile[2][kTile * D];  // (at the end: the rows of dk and dv)
+  __shared__ __attribute__((aligned(16))) T g_tile[2][kTile * D];
+  __shared__ QueryRows<kTile> rows[2];
   const AttentionArgs &a = g.a;
   const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
-  const int block = blockIdx.x % g.blocks, bh = blockIdx.x / g.blocks, kv_head = bh % a.kv_heads, b = bh / a.kv_heads;
+  const int at = same_die_index(), block = at % g.blocks, bh = at / g.blocks, kv_head = bh % a.kv_heads, b = bh / a.kv_heads;
   const int shared = a.heads / a.kv_heads;
   const int block_key = block * (kWaves * kRows), wave_key = block_key + wave * kRows, key = wave_key + (l & 31);
   const bool key_there = key < a.keys;
@@ -158,104 +228,201 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(GradArgs g) {
   const int groups = (a.queries + kRows - 1) / kRows, tiles = (a.queries + kTile - 1) / kTile;
   const i32x4 *bounds = g.bounds + (int64_t)b * groups;
   const i32x4 nothing = {INT_MAX, 0, 0, 0};
+  const TileReader<T, D> reader;
 
-  for (int x = 0; x < shared; ++x) {
-    const int head = kv_head * shared + x;
-    const Scores<MODE> scores(a, head);
-    const T *q_rows = static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head;
-    const T *g_rows = static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head;
-    const int64_t stats = ((int64_t)b * a.heads + head) * a.queries;
-    for (int tile_base = 0; tile_base < tiles; tile_base += kWave) {
-      // which of the next 64 tiles of queries see any of the workgroup's keys
+  // The tiles of queries that see any of the workgroup's keys, head after head: 64 are looked at at a time.
+  int head = kv_head * shared, base = -kWave;
+  uint64_t left = 0;
+  auto next_tile = [&]() __attribute__((always_inline)) -> int {  // or -1
+    while (left == 0) {
+      base += kWave;
+      if (base >= tiles) {
+        base = 0;
+        if (++head == (kv_head + 1) * shared || tiles == 0) return -1;
+      }
       bool reaches = false;
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int group = 2 * (tile_base + l) + y;
+        const int group = 2 * (base + l) + y;
         if (group < groups) reaches |= bounds[group][0] < block_key + kWaves * kRows && bounds[group][1] > block_key;
       }
-      for (uint64_t left = wave_ballot(reaches); left != 0; left &= left - 1) {
-        const int tile = tile_base + (int)__builtin_ctzll(left), i0 = tile * kTile;
-        __syncthreads();
-        {
-          auto there = [&](int r) {
-            const int64_t row = (int64_t)b * a.queries + i0 + r;
-            return i0 + r < a.queries && min(a.hi[row], a.keys) > max(a.lo[row], 0);
-          };
-          TileLoad<T, D, kTile, kThreads> q_load, g_load;
-          q_load.load(q_rows + i0 * a.qs.token, a.qs.token, tid, a.dim, there);
-          g_load.load(g_rows + i0 * g.gs.token, g.gs.token, tid, a.dim, there);
-          if (tid < kTile) {
-            const bool ok = there(tid);
-            const int64_t row = (int64_t)b * a.queries + i0 + tid;
-            row_lse[tid] = ok ? g.lse[stats + i0 + tid] * kLog2e : INFINITY;
-            row_delta[tid] = ok ? g.delta[stats + i0 + tid] : 0;
-            row_lo[tid] = ok ? max(a.lo[row], 0) : 0;
-            row_hi[tid] = ok ? min(a.hi[row], a.keys) : 0;
-          }
-          q_load.store(q_tile, tid);
-          g_load.store(g_tile, tid);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          const i32x4 reach = 2 * tile + qb < groups ? bounds[2 * tile + qb] : nothing;
-          if (reach[0] >= wave_key + kRows || reach[1] <= wave_key) continue;
-          const bool whole = reach[2] <= wave_key && reach[3] >= wave_key + kRows;
-          f32x16 s = {}, dp = {};
-#pragma unroll
-          for (int y = 0; y < D / 16; ++y) s = mfma(rows_frag<T, D>(q_tile, qb * 32, y), k[y], s);
-#pragma unroll
-          for (int y = 0; y < D / 16; ++y) dp = mfma(rows_frag<T, D>(g_tile, qb * 32, y), v[y], dp);
-          constexpr float lower = 1.f / (1 << (int)kRaise<T>);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const int r0 = qb * 32 + 8 * z + 4 * half;
-            const f32x4 lse = *reinterpret_cast<const f32x4 *>(row_lse + r0), delta = *reinterpret_cast<const f32x4 *>(row_delta + r0);
-            i32x4 lo = {}, hi = {};
-            if (!whole) lo = *reinterpret_cast<const i32x4 *>(row_lo + r0), hi = *reinterpret_cast<const i32x4 *>(row_hi + r0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = 4 * z + e;
-              float shrink;
-              const float z = scores.z(s[r], (float)(i0 + r0 + e + a.keys - a.queries - key), shrink);
-              float p = exp2_fast(fmaf(z, scores.factor, scores.offset + kRaise<T> - lse[e]));
-              float ds = p * (lower * dp[r] - lower * delta[e]);
-              if (MODE & kCap) ds *= shrink;
-              if (!whole && (uint32_t)(key - lo[e]) >= (uint32_t)(hi[e] - lo[e])) p = ds = 0;
-              s[r] = p, dp[r] = ds;
-            }
-          }
-          const vec8<T> p0 = packed<T, 0>(s), p1 = packed<T, 1>(s), d0 = packed<T, 0>(dp), d1 = packed<T, 1>(dp);
-#pragma unroll
-          for (int db = 0; db < D / 32; ++db) {
-            dv[db] = mfma(columns_frag<T, D>(g_tile, qb * 32, db), p0, dv[db]);
-            dv[db] = mfma(columns_frag<T, D>(g_tile, qb * 32 + 16, db), p1, dv[db]);
-            dk[db] = mfma(columns_frag<T, D>(q_tile, qb * 32, db), d0, dk[db]);
-            dk[db] = mfma(columns_frag<T, D>(q_tile, qb * 32 + 16, db), d1, dk[db]);
-          }
+      left = wave_ballot(reaches);
+    }
+    const int tile = base + (int)__builtin_ctzll(left);
+    left &= left - 1;
+    return tile;
+  };
+  float next_lse = 0, next_delta = 0;
+  int next_lo = 0, next_hi = 0;
+  auto ask = [&](int tile, int to) __attribute__((always_inline)) {
+    const int i0 = tile * kTile;
+    const Stage<T, D, kTile> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
+    const Stage<T, D, kTile> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
+    q_rows.template ask<kWaves>(q_tile[to], i0, wave);
+    g_rows.template ask<kWaves>(g_tile[to], i0, wave);
+    if (tid < kTile) {
+      const int i = i0 + tid;
+      const int64_t row = (int64_t)b * a.queries + i;
+      next_lo = i < a.queries ? max(a.lo[row], 0) : 0, next_hi = i < a.queries ? min(a.hi[row], a.keys) : 0;
+      const bool sees = next_hi > next_lo;
+      const int64_t stats = ((int64_t)b * a.heads + head) * a.queries + i;
+      next_lse = sees ? g.lse[stats] * kLog2e : INFINITY;
+      next_delta = sees ? g.delta[stats] : 0;
+      if (!sees) next_lo = next_hi = 0;
+    }
+  };
+  auto keep = [&](int to) __attribute__((always_inline)) {
+    if (tid < kTile) rows[to].lse[tid] = next_lse, rows[to].delta[tid] = next_delta, rows[to].lo[tid] = next_lo, rows[to].hi[tid] = next_hi;
+  };
+
+  int tile = tiles > 0 ? next_tile() : -1, tile_head = head, buffer = 0;
+  if (tile >= 0) ask(tile, 0);
+  for (; tile >= 0; buffer ^= 1) {
+    staged_wait();
+    keep(buffer);
+    __syncthreads();
+    const i32x4 reach0 = bounds[2 * tile], reach1 = 2 * tile + 1 < groups ? bounds[2 * tile + 1] : nothing;
+    if (reach0[3] == 0 || reach1[3] == 0) {  // rows that see nothing may hold anything: zeros in their place
+      for (int x = tid; x < kTile * D / 8; x += kThreads) {
+        const int r = x / (D / 8);
+        if (rows[buffer].hi[r] == 0) {
+          *reinterpret_cast<vec8<T> *>(q_tile[buffer] + x * 8) = vec8<T>{};
+          *reinterpret_cast<vec8<T> *>(g_tile[buffer] + x * 8) = vec8<T>{};
         }
       }
+      __syncthreads();
+    }
+    const int i0 = tile * kTile;
+    const Scores<MODE> scores(a, tile_head);
+    tile = next_tile();
+    tile_head = head;
+    if (tile >= 0) ask(tile, buffer ^ 1);
+#pragma unroll 1
+    for (int qb = 0; qb < 2; ++qb) {
+      const i32x4 reach = qb ? reach1 : reach0;
+      if (reach[0] >= wave_key + kRows || reach[1] <= wave_key) continue;
+      add_by_key<T, D, MODE>(dk, dv, q_tile[buffer], g_tile[buffer], qb * 32, rows[buffer], k, v, reader, scores,
+                             i0 + qb * 32 + a.keys - a.queries, key, reach[2] <= wave_key && reach[3] >= wave_key + kRows);
     }
   }
-  if (!key_there) return;
-  const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kv_head) * a.dim;
-  constexpr float lower = 1.f / (1 << (int)kRaise<T>);
+  __syncthreads();
+  const auto to = [&](void *p) {
+    return [=](int r) {
+      return wave_key + r < a.keys ? static_cast<T *>(p) + (((int64_t)b * a.keys + wave_key + r) * a.kv_heads + kv_head) * a.dim : nullptr;
+    };
+  };
+  store_rows<T, D>(q_tile[0] + wave * kRows * D, dk, a.scale, false, a.dim, to(g.dk));
+  store_rows<T, D>(g_tile[0] + wave * kRows * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
+}
+
+// ---- short windows: one launch ----------------------------------------------------------------------------
+// Where all queries and all keys of a window are at most 128 (and a row at most 64 elements), a workgroup holds queries,
+// keys, values and dout of a window and key head in LDS: each is read once, out not at all, because delta
+// can be summed from the probabilities themselves -- in 32 bits, where dout . out begins from the rounded out.
+// A wave is responsible for 32 queries (delta, dq) and for 32 keys (dk, dv) in turn.
+template <typename T, int D, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(GradArgs g) {
+  constexpr int kMost = WAVES * kRows;
+  __shared__ __attribute__((aligned(16))) T q_tile[kMost * D], g_tile[kMost * D], k_tile[kMost * D], v_tile[kMost * D];
+  __shared__ QueryRows<kMost> rows;
+  __shared__ i32x4 bounds[WAVES];
+  const AttentionArgs &a = g.a;
+  const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
+  const int unit = same_die_index(), kv_head = unit % a.kv_heads, b = unit / a.kv_heads;
+  const int shared = a.heads / a.kv_heads, own = wave * kRows, mine = own + (l & 31);
+  const int64_t row = (int64_t)b * a.queries + mine;
+  const bool row_there = mine < a.queries;
+  const TileReader<T, D> reader;
+
+  Seen seen;
+  seen.set(row_there ? a.lo[row] : 0, row_there ? a.hi[row] : 0, a.keys);
+  const uint64_t empties = wave_ballot(seen.empty());
+  if (half == 0) rows.lo[mine] = seen.lo, rows.hi[mine] = seen.hi;
+  if (l == 0) bounds[wave] = i32x4{seen.first, seen.end, seen.all_from, empties != 0 ? 0 : seen.all_to};
+  __syncthreads();
+  int first = INT_MAX, end = 0;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int d = db * 32 + 8 * x + 4 * half;
-      vec4<T> y, z;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = (T)(dk[db][4 * x + e] * a.scale);
-        z[e] = (T)(dv[db][4 * x + e] * lower);
-      }
-      if (d < a.dim) {
-        *reinterpret_cast<vec4<T> *>(static_cast<T *>(g.dk) + to + d) = y;
-        *reinterpret_cast<vec4<T> *>(static_cast<T *>(g.dv) + to + d) = z;
-      }
+  for (int w = 0; w < WAVES; ++w) first = min(first, bounds[w][0]), end = max(end, bounds[w][1]);
+  first = __builtin_amdgcn_readfirstlane(first), end = __builtin_amdgcn_readfirstlane(end);
+  if (first < end) {
+    const Stage<T, D, kRows> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+    const Stage<T, D, kRows> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
+    k_rows.template ask<1>(k_tile + own * D, own, 0);
+    v_rows.template ask<1>(v_tile + own * D, own, 0);
+  }
+  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  for (int x = 0; x < shared; ++x) {
+    const int head = kv_head * shared + x;
+    const int64_t stats = ((int64_t)b * a.heads + head) * a.queries + mine;
+    if (first < end) {
+      const Stage<T, D, kRows> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
+      const Stage<T, D, kRows> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
+      q_rows.template ask<1>(q_tile + own * D, own, 0);
+      g_rows.template ask<1>(g_tile + own * D, own, 0);
     }
+    const float lse_log2 = seen.empty() ? INFINITY : g.lse[stats] * kLog2e;
+    if (half == 0) rows.lse[mine] = lse_log2;
+    staged_wait();
+    if (empties != 0) {  // rows that see nothing may hold anything: zeros in their place
+      wave_lds_sync();
+      for (int y = l; y < kRows * D / 8; y += kWave)
+        if ((empties >> (y / (D / 8))) & 1) {
+          *reinterpret_cast<vec8<T> *>(q_tile + own * D + y * 8) = vec8<T>{};
+          *reinterpret_cast<vec8<T> *>(g_tile + own * D + y * 8) = vec8<T>{};
+        }
+    }
+    __syncthreads();
+    const Scores<MODE> scores(a, head);
+    const float less = scores.offset - lse_log2;
+    const int place = mine + a.keys - a.queries;
+    vec8<T> u[D / 16], w[D / 16];  // rows of the wave: of q and dout, then of k and v, then of q and dout
+    auto take = [&](const T *p, const T *r) __attribute__((always_inline)) {
+#pragma unroll
+      for (int y = 0; y < D / 16; ++y) {
+        u[y] = reader.rows(p, own, y), w[y] = reader.rows(r, own, y);
+        if ((2 * y + half) * 8 >= a.dim) u[y] = w[y] = vec8<T>{};  // (the tiles repeat a piece there)
+      }
+    };
+    float delta = 0;
+    take(q_tile, g_tile);
+#pragma unroll 1
+    for (int kk = 0; kk < kMost; kk += kRows)
+      if (seen.touches(kk, kk + kRows))
+        grads_by_query<true, T, D, MODE>(k_tile, v_tile, kk, kk, u, w, reader, scores, seen, place, less, delta);
+    delta = sum_of_halves(delta);
+    if (half == 0) rows.delta[mine] = delta;
+    __syncthreads();
+    take(k_tile, v_tile);
+#pragma unroll 1
+    for (int qb = 0; qb < WAVES; ++qb) {
+      const i32x4 reach = bounds[qb];
+      if (__builtin_amdgcn_readfirstlane(reach[0]) >= own + kRows || __builtin_amdgcn_readfirstlane(reach[1]) <= own) continue;
+      const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
+      add_by_key<T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
+    }
+    __syncthreads();
+    take(q_tile, g_tile);
+    f32x16 dq[D / 32] = {};
+#pragma unroll 1
+    for (int kk = 0; kk < kMost; kk += kRows)
+      if (seen.touches(kk, kk + kRows)) {
+        const f32x16 ds = grads_by_query<false, T, D, MODE>(k_tile, v_tile, kk, kk, u, w, reader, scores, seen, place, less, delta);
+        add_columns<T, D>(dq, k_tile, kk, ds, reader);
+      }
+    wave_lds_sync();
+    store_rows<T, D>(q_tile + own * D, dq, a.scale, seen.empty(), a.dim, [&](int r) {
+      return own + r < a.queries ? static_cast<T *>(g.dq) + (((int64_t)b * a.queries + own + r) * a.heads + head) * a.dim : nullptr;
+    });
+    wave_lds_sync();
+  }
+  __syncthreads();
+  const auto to = [&](void *p) {
+    return [=](int r) {
+      return own + r < a.keys ? static_cast<T *>(p) + (((int64_t)b * a.keys + own + r) * a.kv_heads + kv_head) * a.dim : nullptr;
+    };
+  };
+  store_rows<T, D>(k_tile + own * D, dk, a.scale, false, a.dim, to(g.dk));
+  store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
 }
 
 size_t delta_bytes(int64_t batch, int64_t queries, int64_t heads) {
@@ -295,14 +462,31 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
   g.delta = static_cast<float *>(workspace);
   g.bounds = reinterpret_cast<i32x4 *>(static_cast<char *>(workspace) + delta_bytes(a.batch, a.queries, a.heads));
   g.dq = dq, g.dk = dk, g.dv = dv;
+  const int longest = a.queries > a.keys ? a.queries : a.keys;
+  if (longest <= 4 * kRows && a.dim <= 64) {
+    by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
+      if constexpr (decltype(dim)::value <= 64)
+        by_waves((longest + kRows - 1) / kRows, [&](auto w) {
+          hipLaunchKernelGGL((attention_window_grad_kernel<decltype(type), decltype(dim)::value, decltype(mode)::value, decltype(w)::value>),
+                             dim3((unsigned)a.kv_heads * a.batch), dim3(decltype(w)::value * kWave), 0, as_stream(stream), g);
+        });
+    });
+    GEARHIP_RETURN_IF_LAUNCH_FAILED();
+    return 0;
+  }
   by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
     constexpr int D = decltype(dim)::value;
     constexpr int kMode = decltype(mode)::value;
-    g.blocks = (int)ceil_div64(a.queries, kWaves * kRows);
-    if (g.blocks > 0)
-      hipLaunchKernelGGL((attention_dq_kernel<T, D, kMode>), dim3((unsigned)g.blocks * a.heads * a.batch),
-                         dim3(kThreads), 0, as_stream(stream), g);
+    if (a.queries > 0) {
+      const int groups = (int)ceil_div64(a.queries, kRows);
+      g.blocks = (groups + kWaves - 1) / kWaves;
+      by_waves((groups + g.blocks - 1) / g.blocks, [&](auto w) {
+        hipLaunchKernelGGL((attention_dq_kernel<T, D, kMode, decltype(w)::value>),
+                           dim3((unsigned)g.blocks * a.heads * a.batch), dim3(decltype(w)::value * kWave), 0,
+                           as_stream(stream), g);
+      });
+    }
     g.blocks = (int)ceil_div64(a.keys, kWaves * kRows);
     if (g.blocks > 0)
       hipLaunchKernelGGL((attention_dkv_kernel<T, D, kMode>), dim3((unsigned)g.blocks * a.kv_heads * a.batch),
