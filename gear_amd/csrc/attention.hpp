@@ -58,32 +58,12 @@ __device__ __forceinline__ int piece_at(int row, int c) {
   return row * D + ((c ^ swizzle<D>(row)) << 3);
 }
 
-// The operand whose row (or column) l%32 is row `first` + l%32 of the tile, contracted elements 16*s...
-template <typename T, int D>
-__device__ __forceinline__ vec8<T> rows_frag(const T *tile, int first, int s) {
-  const int l = lane_id();
-  return *reinterpret_cast<const vec8<T> *>(tile + piece_at<D>(first + (l & 31), 2 * s + (l >> 5)));
-}
-
-// The operand whose row l%32 is column 32*block + l%32 of the tile, contracted over the rows first..first+15
-// in the order above.
-template <typename T, int D>
-__device__ __forceinline__ vec8<T> columns_frag(const T *tile, int first, int block) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef short s16x8 __attribute__((ext_vector_type(8)));
-  const int l = lane_id(), t = l & 15;
-  const int row = first + 4 * (l >> 5) + (t >> 2), column = 32 * block + 16 * ((l >> 4) & 1) + 4 * (t & 3);
-  auto read = [&](int r) {
-    const T *p = tile + piece_at<D>(r, column >> 3) + (column & 7);
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(const_cast<T *>(p)));
-  };
-  const s16x4 a = read(row), b = read(row + 8);
-  return __builtin_bit_cast(vec8<T>, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// The same two operands by offsets that a lane works out once: what remains of an address is a constant of the
+// Operands out of a tile, by offsets that a lane works out once: what remains of an address is a constant of the
 // instruction.  (swizzle() of a row is the same for rows a multiple of 8 apart, and changes the lower 3 bits of a
 // piece only.)
+//   rows     the operand whose row (or column) l%32 is row first + l%32 of the tile, contracted over the elements 16 s..
+//   columns  the operand whose row l%32 is column 32 block + l%32, contracted over the rows first..first + 15 in the
+//            order above
 template <typename T, int D>
 struct TileReader {
   static constexpr int kRowOffsets = D / 16 < 4 ? D / 16 : 4, kColumnOffsets = D / 32 < 2 ? 1 : 2;
@@ -96,11 +76,11 @@ struct TileReader {
     for (int b = 0; b < kColumnOffsets; ++b)
       column[b] = piece_at<D>(4 * half + (t >> 2), 4 * b + 2 * ((l >> 4) & 1) + ((t & 3) >> 1)) + 4 * (t & 1);
   }
-  // rows first.. (a multiple of 8) as rows_frag
+  // (first: a multiple of 8)
   __device__ __forceinline__ vec8<T> rows(const T *tile, int first, int s) const {
     return *reinterpret_cast<const vec8<T> *>(tile + row[s % kRowOffsets] + first * D + s / kRowOffsets * 64);
   }
-  // rows first.. (a multiple of 16) as columns_frag
+  // (first: a multiple of 16)
   __device__ __forceinline__ vec8<T> columns(const T *tile, int first, int block) const {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -145,30 +125,6 @@ __device__ __forceinline__ void own_row_frags(vec8<T> (&f)[D / 16], const T *row
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) f[s] = piece_or_zero(row, 2 * s + h, there && (2 * s + h) * 8 < dim);
 }
-
-// Rows first.. of a tile of ROWS rows on their way from memory to LDS through the registers of a
-// workgroup of THREADS threads.
-template <typename T, int D, int ROWS, int THREADS>
-struct TileLoad {
-  static constexpr int kPieces = ROWS * D / 8 / THREADS;
-  vec8<T> x[kPieces];
-  // there(row): whether the row is read
-  template <typename F>
-  __device__ __forceinline__ void load(const T *base, int64_t stride, int thread, int dim, const F &there) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int at = thread + i * THREADS, row = at / (D / 8), c = at % (D / 8);
-      x[i] = piece_or_zero(base + row * stride, c, c * 8 < dim && there(row));
-    }
-  }
-  __device__ __forceinline__ void store(T *tile, int thread) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int at = thread + i * THREADS, row = at / (D / 8), c = at % (D / 8);
-      *reinterpret_cast<vec8<T> *>(tile + piece_at<D>(row, c)) = x[i];
-    }
-  }
-};
 
 // Rows of a tile of ROWS rows straight from memory into LDS, 64 pieces an instruction, the instructions dealt
 // out to the waves of a workgroup.  Rows outside [first, end) are replaced by the nearest inside, pieces
@@ -221,11 +177,14 @@ struct Stage {
     }
   }
 };
+// All but the last `LEFT` instructions of the wave (of this kind, and the compiler's own loads and stores) are complete.
 // (the builtin: the compiler then knows that its own loads have arrived too, and waits for none of them, and with
 // them for what is asked for next, inside the loop)
+template <int LEFT = 0>
 __device__ __forceinline__ void staged_wait() {
+  static_assert(LEFT < 64, "");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (LEFT & 15) | (LEFT >> 4 << 14));  // vmcnt
   asm volatile("" ::: "memory");
 }
 
@@ -310,20 +269,18 @@ __device__ __forceinline__ int same_die_index() {
   return die * per + min(die, rest) + blockIdx.x / 8;
 }
 
-// The 32 rows of 32 * (D / 32) results that a wave holds by columns (column l%32: row l%32 of the output), times
-// `factor` of the column, to memory through a piece of LDS of 32 * D elements of the wave's own, 16 bytes a lane.
-// to(row): where a row begins, or null.
+// The 32 rows of 32 * (D / 32) results that a wave holds by columns (column l%32: row l%32 of the output), rounded, to
+// memory through a piece of LDS of 32 * D elements of the wave's own, 16 bytes a lane.  to(row): where a row begins, or null.
 template <typename T, int D, typename F>
-__device__ __forceinline__ void store_rows(T *piece, const f32x16 *x, float factor, bool zero, int dim, const F &to) {
+__device__ __forceinline__ void store_packed(T *piece, const vec8<T> (&x)[D / 32][2], int dim, const F &to) {
   const int l = lane_id(), half = l >> 5;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      vec4<T> y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(zero ? 0.f : x[db][4 * g + e] * factor);
-      *reinterpret_cast<vec4<T> *>(piece + piece_at<D>(l & 31, db * 4 + g) + 4 * half) = y;
+      const vec8<T> &y = x[db][g >> 1];
+      *reinterpret_cast<vec4<T> *>(piece + piece_at<D>(l & 31, db * 4 + g) + 4 * half) =
+          (g & 1) ? __builtin_shufflevector(y, y, 4, 5, 6, 7) : __builtin_shufflevector(y, y, 0, 1, 2, 3);
     }
   wave_lds_sync();
 #pragma unroll
@@ -333,6 +290,18 @@ __device__ __forceinline__ void store_rows(T *piece, const f32x16 *x, float fact
     if (p != nullptr && c * 8 < dim)
       *reinterpret_cast<vec8<T> *>(p + c * 8) = *reinterpret_cast<const vec8<T> *>(piece + piece_at<D>(row, c));
   }
+}
+// The same from sums, times `factor` of the column; zeros where `zero`.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void store_rows(T *piece, f32x16 (&x)[D / 32], float factor, bool zero, int dim, const F &to) {
+  vec8<T> y[D / 32][2];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[db][r] = zero ? 0.f : x[db][r] * factor;
+    y[db][0] = packed<T, 0>(x[db]), y[db][1] = packed<T, 1>(x[db]);
+  }
+  store_packed<T, D>(piece, y, dim, to);
 }
 
 // f(std::integral_constant<int, D>(), element, std::integral_constant<int, MODE>()) for the call's type and sizes

@@ -316,8 +316,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
 }
 
 // ---- short windows: one launch ----------------------------------------------------------------------------
-// Where all queries and all keys of a window are at most 128 (and a row at most 64 elements), a workgroup holds queries,
-// keys, values and dout of a window and key head in LDS: each is read once, out not at all, because delta
+// Where all queries and all keys of a window are at most 128 (and a row at most 64 elements, and no heads share keys),
+// a workgroup holds queries, keys, values and dout of a window and head in LDS: each is read once, out not at all, because delta
 // can be summed from the probabilities themselves -- in 32 bits, where dout . out begins from the rounded out.
 // A wave is responsible for 32 queries (delta, dq) and for 32 keys (dk, dv) in turn.
 template <typename T, int D, int MODE, int WAVES>
@@ -328,16 +328,24 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
   __shared__ i32x4 bounds[WAVES];
   const AttentionArgs &a = g.a;
   const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
-  const int unit = same_die_index(), kv_head = unit % a.kv_heads, b = unit / a.kv_heads;
-  const int shared = a.heads / a.kv_heads, own = wave * kRows, mine = own + (l & 31);
-  const int64_t row = (int64_t)b * a.queries + mine;
+  const int unit = same_die_index(), head = unit % a.heads, b = unit / a.heads;
+  const int own = wave * kRows, mine = own + (l & 31);
+  const int64_t row = (int64_t)b * a.queries + mine, stats = ((int64_t)b * a.heads + head) * a.queries + mine;
   const bool row_there = mine < a.queries;
   const TileReader<T, D> reader;
 
+  // (asked for before anything is known of the ranges; rows beyond the last are copies of it)
+  const Stage<T, D, kRows> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
+  const Stage<T, D, kRows> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
+  const int lo = row_there ? a.lo[row] : 0, hi = row_there ? a.hi[row] : 0;
+  const float lse = row_there ? g.lse[stats] : 0;
+  q_rows.template ask<1>(q_tile + own * D, own, 0);
+  g_rows.template ask<1>(g_tile + own * D, own, 0);
   Seen seen;
-  seen.set(row_there ? a.lo[row] : 0, row_there ? a.hi[row] : 0, a.keys);
+  seen.set(lo, hi, a.keys);
+  const float lse_log2 = seen.empty() ? INFINITY : lse * kLog2e;
   const uint64_t empties = wave_ballot(seen.empty());
-  if (half == 0) rows.lo[mine] = seen.lo, rows.hi[mine] = seen.hi;
+  if (half == 0) rows.lo[mine] = seen.lo, rows.hi[mine] = seen.hi, rows.lse[mine] = lse_log2;
   if (l == 0) bounds[wave] = i32x4{seen.first, seen.end, seen.all_from, empties != 0 ? 0 : seen.all_to};
   __syncthreads();
   int first = INT_MAX, end = 0;
@@ -345,44 +353,37 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
   for (int w = 0; w < WAVES; ++w) first = min(first, bounds[w][0]), end = max(end, bounds[w][1]);
   first = __builtin_amdgcn_readfirstlane(first), end = __builtin_amdgcn_readfirstlane(end);
   if (first < end) {
-    const Stage<T, D, kRows> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
-    const Stage<T, D, kRows> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
+    const Stage<T, D, kRows> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + head * a.ks.head, a.ks.token, first, end, a.dim);
+    const Stage<T, D, kRows> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + head * a.vs.head, a.vs.token, first, end, a.dim);
     k_rows.template ask<1>(k_tile + own * D, own, 0);
     v_rows.template ask<1>(v_tile + own * D, own, 0);
   }
-  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
-  for (int x = 0; x < shared; ++x) {
-    const int head = kv_head * shared + x;
-    const int64_t stats = ((int64_t)b * a.heads + head) * a.queries + mine;
-    if (first < end) {
-      const Stage<T, D, kRows> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
-      const Stage<T, D, kRows> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
-      q_rows.template ask<1>(q_tile + own * D, own, 0);
-      g_rows.template ask<1>(g_tile + own * D, own, 0);
+  staged_wait();
+  if (empties != 0) {  // rows that see nothing may hold anything: zeros in their place
+    wave_lds_sync();
+    for (int y = l; y < kRows * D / 8; y += kWave)
+      if ((empties >> (y / (D / 8))) & 1) {
+        *reinterpret_cast<vec8<T> *>(q_tile + own * D + y * 8) = vec8<T>{};
+        *reinterpret_cast<vec8<T> *>(g_tile + own * D + y * 8) = vec8<T>{};
+      }
+  }
+  __syncthreads();
+  const Scores<MODE> scores(a, head);
+  vec8<T> u[D / 16], w[D / 16];  // rows of the wave: of q and dout, then of k and v
+  auto take = [&](const T *p, const T *r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < D / 16; ++y) u[y] = reader.rows(p, own, y), w[y] = reader.rows(r, own, y);
+    if (a.dim < D) {  // the tiles repeat a piece there
+#pragma unroll
+      for (int y = 0; y < D / 16; ++y)
+        if ((2 * y + half) * 8 >= a.dim) u[y] = w[y] = vec8<T>{};
+      asm volatile("");
     }
-    const float lse_log2 = seen.empty() ? INFINITY : g.lse[stats] * kLog2e;
-    if (half == 0) rows.lse[mine] = lse_log2;
-    staged_wait();
-    if (empties != 0) {  // rows that see nothing may hold anything: zeros in their place
-      wave_lds_sync();
-      for (int y = l; y < kRows * D / 8; y += kWave)
-        if ((empties >> (y / (D / 8))) & 1) {
-          *reinterpret_cast<vec8<T> *>(q_tile + own * D + y * 8) = vec8<T>{};
-          *reinterpret_cast<vec8<T> *>(g_tile + own * D + y * 8) = vec8<T>{};
-        }
-    }
-    __syncthreads();
-    const Scores<MODE> scores(a, head);
+  };
+  vec8<T> dq_kept[D / 32][2];
+  {
     const float less = scores.offset - lse_log2;
     const int place = mine + a.keys - a.queries;
-    vec8<T> u[D / 16], w[D / 16];  // rows of the wave: of q and dout, then of k and v, then of q and dout
-    auto take = [&](const T *p, const T *r) __attribute__((always_inline)) {
-#pragma unroll
-      for (int y = 0; y < D / 16; ++y) {
-        u[y] = reader.rows(p, own, y), w[y] = reader.rows(r, own, y);
-        if ((2 * y + half) * 8 >= a.dim) u[y] = w[y] = vec8<T>{};  // (the tiles repeat a piece there)
-      }
-    };
     float delta = 0;
     take(q_tile, g_tile);
 #pragma unroll 1
@@ -391,17 +392,6 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
         grads_by_query<true, T, D, MODE>(k_tile, v_tile, kk, kk, u, w, reader, scores, seen, place, less, delta);
     delta = sum_of_halves(delta);
     if (half == 0) rows.delta[mine] = delta;
-    __syncthreads();
-    take(k_tile, v_tile);
-#pragma unroll 1
-    for (int qb = 0; qb < WAVES; ++qb) {
-      const i32x4 reach = bounds[qb];
-      if (__builtin_amdgcn_readfirstlane(reach[0]) >= own + kRows || __builtin_amdgcn_readfirstlane(reach[1]) <= own) continue;
-      const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
-      add_by_key<T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
-    }
-    __syncthreads();
-    take(q_tile, g_tile);
     f32x16 dq[D / 32] = {};
 #pragma unroll 1
     for (int kk = 0; kk < kMost; kk += kRows)
@@ -409,20 +399,31 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
         const f32x16 ds = grads_by_query<false, T, D, MODE>(k_tile, v_tile, kk, kk, u, w, reader, scores, seen, place, less, delta);
         add_columns<T, D>(dq, k_tile, kk, ds, reader);
       }
-    wave_lds_sync();
-    store_rows<T, D>(q_tile + own * D, dq, a.scale, seen.empty(), a.dim, [&](int r) {
-      return own + r < a.queries ? static_cast<T *>(g.dq) + (((int64_t)b * a.queries + own + r) * a.heads + head) * a.dim : nullptr;
-    });
-    wave_lds_sync();
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      dq[db] *= a.scale;
+      dq_kept[db][0] = packed<T, 0>(dq[db]), dq_kept[db][1] = packed<T, 1>(dq[db]);
+    }
   }
   __syncthreads();
-  const auto to = [&](void *p) {
+  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  take(k_tile, v_tile);
+#pragma unroll 1
+  for (int qb = 0; qb < WAVES; ++qb) {
+    const i32x4 reach = bounds[qb];
+    if (__builtin_amdgcn_readfirstlane(reach[0]) >= own + kRows || __builtin_amdgcn_readfirstlane(reach[1]) <= own) continue;
+    const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
+    add_by_key<T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
+  }
+  __syncthreads();
+  const auto to = [&](void *p, int count) {
     return [=](int r) {
-      return own + r < a.keys ? static_cast<T *>(p) + (((int64_t)b * a.keys + own + r) * a.kv_heads + kv_head) * a.dim : nullptr;
+      return own + r < count ? static_cast<T *>(p) + (((int64_t)b * count + own + r) * a.heads + head) * a.dim : nullptr;
     };
   };
-  store_rows<T, D>(k_tile + own * D, dk, a.scale, false, a.dim, to(g.dk));
-  store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
+  store_packed<T, D>(q_tile + own * D, dq_kept, a.dim, to(g.dq, a.queries));
+  store_rows<T, D>(k_tile + own * D, dk, a.scale, false, a.dim, to(g.dk, a.keys));
+  store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv, a.keys));
 }
 
 size_t delta_bytes(int64_t batch, int64_t queries, int64_t heads) {
@@ -463,12 +464,12 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
   g.bounds = reinterpret_cast<i32x4 *>(static_cast<char *>(workspace) + delta_bytes(a.batch, a.queries, a.heads));
   g.dq = dq, g.dk = dk, g.dv = dv;
   const int longest = a.queries > a.keys ? a.queries : a.keys;
-  if (longest <= 4 * kRows && a.dim <= 64) {
+  if (longest <= 4 * kRows && a.dim <= 64 && a.heads == a.kv_heads && a.queries > 0) {
     by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
       if constexpr (decltype(dim)::value <= 64)
         by_waves((longest + kRows - 1) / kRows, [&](auto w) {
           hipLaunchKernelGGL((attention_window_grad_kernel<decltype(type), decltype(dim)::value, decltype(mode)::value, decltype(w)::value>),
-                             dim3((unsigned)a.kv_heads * a.batch), dim3(decltype(w)::value * kWave), 0, as_stream(stream), g);
+                             dim3((unsigned)a.heads * a.batch), dim3(decltype(w)::value * kWave), 0, as_stream(stream), g);
         });
     });
     GEARHIP_RETURN_IF_LAUNCH_FAILED();

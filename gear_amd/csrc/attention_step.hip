@@ -26,8 +26,11 @@ struct StepArgs {
 };
 
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
-  __shared__ __attribute__((aligned(16))) float joined[kWaves][kRows][D];  // (V's tiles before that)
+__global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g) {
+  constexpr int kAsks = D / 8;  // instructions that ask for a tile of K and V
+  constexpr size_t kTileBytes = sizeof(T) * kRows * D, kJoinBytes = sizeof(float) * kRows * D;
+  constexpr size_t kOwnBytes = 4 * kTileBytes > kJoinBytes ? 4 * kTileBytes : kJoinBytes;
+  __shared__ __attribute__((aligned(16))) char memory[kWaves][kOwnBytes];  // two tiles of K and V a wave; its sums
   __shared__ float2 joined_ml[kWaves][kRows];
   const AttentionArgs &a = g.a;
   const int l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = l >> 5;
@@ -36,78 +39,98 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
   const int shared = a.heads / a.kv_heads, rows = a.queries * shared;
   const int r_own = block * kRows + (l & 31), i = r_own / shared, head = kv_head * shared + r_own % shared;
   const bool row_there = r_own < rows;
-  T *v_tile = reinterpret_cast<T *>(joined[wave]);
+  T *k_tile[2], *v_tile[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    k_tile[x] = reinterpret_cast<T *>(memory[wave] + x * 2 * kTileBytes);
+    v_tile[x] = reinterpret_cast<T *>(memory[wave] + (x * 2 + 1) * kTileBytes);
+  }
 
   Seen seen;
   const int64_t row = (int64_t)b * a.queries + i;
   seen.set(row_there ? a.lo[row] : 0, row_there ? a.hi[row] : 0, a.keys);
   vec8<T> q[D / 16];
   own_row_frags<T, D>(q, static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head, a.dim, !seen.empty());
+  // this workgroup's part of the keys that the rows see, [first, end)
   const int length = seen.first < seen.end ? seen.end - seen.first : 0;
   const int part = ((length + g.splits - 1) / g.splits + kRows - 1) / kRows * kRows;
-  const int64_t part_first = seen.first < seen.end ? seen.first + (int64_t)split * part : 0;
-  const int end = (int)min((int64_t)seen.end, part_first + part);
+  const int first = (int)min((int64_t)seen.end, (length > 0 ? seen.first : 0) + (int64_t)split * part);
+  const int end = (int)min((int64_t)seen.end, (int64_t)first + part);
 
   const Scores<MODE> scores(a, row_there ? head : 0);
+  const TileReader<T, D> reader;
   f32x16 o[D / 32] = {};
-  float m = -INFINITY, sum = 0;
-  const T *k_rows = static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head;
-  const T *v_rows = static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head;
-  vec8<T> k_next[D / 16];
-  TileLoad<T, D, kRows, kWave> v_next;
-  auto load = [&](int64_t k0) {
-    own_row_frags<T, D>(k_next, k_rows + (k0 + (l & 31)) * a.ks.token, a.dim, k0 + (l & 31) < end);
-    v_next.load(v_rows + k0 * a.vs.token, a.vs.token, l, a.dim, [&](int r) { return k0 + r < end; });
+  float m = -INFINITY, sum = 0;  // m: of z
+  const Stage<T, D, kRows> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+  const Stage<T, D, kRows> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
+  constexpr int kStep = kWaves * kRows;
+  auto ask = [&](int k0, int to) __attribute__((always_inline)) {
+    k_rows.template ask<1>(k_tile[to], k0, 0);
+    v_rows.template ask<1>(v_tile[to], k0, 0);
   };
-  int64_t k0 = part_first + wave * kRows;
-  if (k0 < end) load(k0);
-  for (; k0 < end; k0 += kWaves * kRows) {
+  auto tile = [&](int k0, int from_buffer) __attribute__((always_inline)) {
     f32x16 s = {};
 #pragma unroll
-    for (int x = 0; x < D / 16; ++x) s = mfma(k_next[x], q[x], s);
-    wave_lds_sync();
-    v_next.store(v_tile, l);
-    wave_lds_sync();
-    if (k0 + kWaves * kRows < end) load(k0 + kWaves * kRows);
+    for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_tile[from_buffer], 0, x), q[x], s);
+    const float ahead = (float)(seen.hi - 1 - k0 - 4 * half);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)));
+    if (__builtin_expect(k0 + kRows > end || !seen.covers(k0, k0 + kRows), 0)) {
+      const uint32_t from_lo = (uint32_t)(k0 + 4 * half - seen.lo), count = (uint32_t)(min(seen.hi, end) - seen.lo);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) >= count || seen.lo >= end) s[r] = -INFINITY;
+      asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
+    }
     float top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int key = (int)k0 + result_row(r);
-      float y = fmaf(scores.z(s[r], (float)(seen.hi - 1 - key)), scores.factor, scores.offset);
-      if (key >= end || (uint32_t)(key - seen.lo) >= (uint32_t)(seen.hi - seen.lo)) y = -INFINITY;
-      s[r] = y;
-      top = fmaxf(top, y);
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = max_of_halves(top);
+    // the sums are rescaled only where a maximum grows by more than 2^8: p stays below that
+    if (wave_ballot((top - m) * scores.factor > 8.f) != 0) {
+      const float grown = fmaxf(m, top);
+      const float rescale = grown == -INFINITY ? 1.f : exp2_fast((m - grown) * scores.factor);
+      m = grown;
+      sum *= rescale;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
     }
-    top = fmaxf(m, max_of_halves(top));
-    const float from = top == -INFINITY ? 0.f : top;
-    const float rescale = exp2_fast(m - from);
-    m = top;
-    sum *= rescale;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
+    const float from = m == -INFINITY ? 0.f : -m * scores.factor;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[r] = exp2_fast(s[r] - from);
+      s[r] = exp2_fast(fmaf(s[r], scores.factor, from));
       sum += s[r];
     }
     const vec8<T> p0 = packed<T, 0>(s), p1 = packed<T, 1>(s);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
-      o[db] = mfma(columns_frag<T, D>(v_tile, 0, db), p0, o[db]);
-      o[db] = mfma(columns_frag<T, D>(v_tile, 16, db), p1, o[db]);
+      o[db] = mfma(reader.columns(v_tile[from_buffer], 0, db), p0, o[db]);
+      o[db] = mfma(reader.columns(v_tile[from_buffer], 16, db), p1, o[db]);
     }
+  };
+  int k0 = first + wave * kRows;
+  if (k0 < end) ask(k0, 0);
+  if (k0 + kStep < end) ask(k0 + kStep, 1);
+  for (int buffer = 0; k0 < end; k0 += kStep, buffer ^= 1) {
+    if (k0 + kStep < end)
+      staged_wait<kAsks>();  // the next tile may still be on its way
+    else
+      staged_wait<0>();
+    tile(k0, buffer);
+    if (k0 + 2 * kStep < end) ask(k0 + 2 * kStep, buffer);
   }
   sum = sum_of_halves(sum);
 
-  // join the waves
-  __syncthreads();
+  // join the waves (each reads and writes its own memory until here)
+  m = m == -INFINITY ? m : m * scores.factor;
+  float *own_sums = reinterpret_cast<float *>(memory[wave]);
+  wave_lds_sync();
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const f32x4 y = {o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
-      *reinterpret_cast<f32x4 *>(&joined[wave][l & 31][db * 32 + 8 * x + 4 * half]) = y;
-    }
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<f32x4 *>(own_sums + (l & 31) * D + db * 32 + 8 * x + 4 * half) =
+          f32x4{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
   if (half == 0) joined_ml[wave][l & 31] = make_float2(m, sum);
   __syncthreads();
   const int here = min(kRows, rows - block * kRows);
@@ -122,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
     for (int w = 0; w < kWaves; ++w) {
       const float share = exp2_fast(joined_ml[w][r].x - from);
       total += share * joined_ml[w][r].y;
-      y += share * joined[w][r][d];
+      y += share * reinterpret_cast<const float *>(memory[w])[r * D + d];
     }
     if (g.splits == 1) {
       const int at = block * kRows + r, t = at / shared, h = kv_head * shared + at % shared;
@@ -137,9 +160,12 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs g) {
   }
 }
 
-// One workgroup a query and head: the parts of its split, joined.
+// One workgroup a query and head: the parts of its split, joined.  Every thread takes 4 elements of each eighth part (or
+// more often, with shorter rows), so that the loads of a row's parts are in flight together.
 template <typename T>
-__global__ __launch_bounds__(128) void attention_join_kernel(StepArgs g) {
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(StepArgs g) {
+  __shared__ float share[kMaxSplits];
+  __shared__ f32x4 sums[kThreads];
   const AttentionArgs &a = g.a;
   const int shared = a.heads / a.kv_heads;
   const int64_t q_row = blockIdx.x / a.heads;
@@ -148,20 +174,37 @@ __global__ __launch_bounds__(128) void attention_join_kernel(StepArgs g) {
   const int r = (int)(q_row - b * a.queries) * shared + head % shared;
   const int64_t unit = (b * a.kv_heads + kv_head) * g.row_blocks + r / kRows;
   const int64_t first = unit * g.splits * kRows + r % kRows;  // part p: first + p * kRows
-  float top = -INFINITY;
-  for (int p = 0; p < g.splits; ++p) top = fmaxf(top, g.part_ml[first + (int64_t)p * kRows].x);
+  // (every wave works the shares out for itself)
+  const int l = lane_id();
+  float top = -INFINITY, total = 0;
+  for (int p = l; p < g.splits; p += kWave) top = fmaxf(top, g.part_ml[first + (int64_t)p * kRows].x);
+#pragma unroll
+  for (int x = 1; x < kWave; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
   const float from = top == -INFINITY ? 0.f : top;
-  const int d = threadIdx.x;
-  if (d >= a.dim) return;
-  float total = 0, y = 0;
-  for (int p = 0; p < g.splits; ++p) {
+  for (int p = l; p < g.splits; p += kWave) {
     const float2 ml = g.part_ml[first + (int64_t)p * kRows];
-    const float share = exp2_fast(ml.x - from);
-    total += share * ml.y;
-    y += share * g.part_o[(first + (int64_t)p * kRows) * a.dim + d];
+    const float s = exp2_fast(ml.x - from);
+    total += s * ml.y;
+    share[p] = s;
   }
+#pragma unroll
+  for (int x = 1; x < kWave; x *= 2) total += __shfl_xor(total, x);
+  __syncthreads();
+  const int lanes = a.dim / 4, groups = kThreads / lanes, group = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
+  f32x4 y = {};
+  if (group < groups)
+#pragma unroll 4
+    for (int p = group; p < g.splits; p += groups)
+      y += share[p] * *reinterpret_cast<const f32x4 *>(g.part_o + (first + (int64_t)p * kRows) * a.dim + d);
+  sums[threadIdx.x] = y;
+  __syncthreads();
+  if (group != 0) return;
+  for (int x = 1; x < groups; ++x) y += sums[x * lanes + threadIdx.x];
   const bool none = min(a.hi[q_row], a.keys) <= max(a.lo[q_row], 0);
-  static_cast<T *>(g.out)[(q_row * a.heads + head) * a.dim + d] = (T)(none ? 0.f : y / total);
+  vec4<T> z;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = (T)(none ? 0.f : y[e] / total);
+  *reinterpret_cast<vec4<T> *>(static_cast<T *>(g.out) + (q_row * a.heads + head) * a.dim + d) = z;
 }
 
 int row_blocks_of(int64_t queries, int64_t heads, int64_t kv_heads) {
@@ -213,7 +256,7 @@ extern "C" int gear_hip_attention_step(const gear_hip_attention_desc *desc, void
     hipLaunchKernelGGL((attention_step_kernel<T, decltype(dim)::value, decltype(mode)::value>),
                        dim3((unsigned)(units * g.splits)), dim3(kThreads), 0, as_stream(stream), g);
     if (g.splits > 1)
-      hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(128), 0,
+      hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(kThreads), 0,
                          as_stream(stream), g);
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
