@@ -130,9 +130,10 @@ __device__ __forceinline__ void own_row_frags(vec8<T> (&f)[D / 16], const T *row
 // out to the waves of a workgroup.  Rows outside [first, end) are replaced by the nearest inside, pieces
 // beyond `dim` by the last: what a tile holds there is finite wherever the rows in range are, and multiplied
 // by zeros only.  A tile is complete after staged_wait() in every wave and a barrier.
+// ONCE: what nobody reads again is loaded past the caches.
 // The instruction is written out because the compiler, which cannot tell the tile that is asked for from
 // the one that is read meanwhile, has every read of LDS behind its builtin wait for the memory.
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool ONCE = false>
 struct Stage {
   static constexpr int kPieces = D / 8, kRowsEach = kWave / kPieces, kCount = ROWS / kRowsEach;
   const T *base;
@@ -151,10 +152,11 @@ struct Stage {
     return min((l % kPieces) ^ swizzle<D>(x * kRowsEach + l / kPieces), dim / 8 - 1);
   }
   __device__ __forceinline__ void one(const T *from, uint32_t at) const {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                 :
-                 : "v"(from), "s"(__builtin_amdgcn_readfirstlane(at))
-                 : "memory", "m0");
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(at);
+    if (ONCE)
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(m0) : "memory", "m0");
+    else
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
   }
   // the share of wave `wave` of WAVES
   template <int WAVES>
@@ -199,11 +201,16 @@ __device__ __forceinline__ float sum_of_halves(float x) {
   return __uint_as_float(y[0]) + __uint_as_float(y[1]);
 }
 
+// f over the 64 lanes, for an f with f(x, x) == x (lanes without a partner are given their own value)
 template <typename F>
 __device__ __forceinline__ int wave_reduce(int x, const F &f) {
-#pragma unroll
-  for (int m = 1; m < kWave; m *= 2) x = f(x, __shfl_xor(x, m));
-  return __builtin_amdgcn_readfirstlane(x);
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, kDppRowShr1, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, kDppRowShr2, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, kDppRowShr4, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, kDppRowShr8, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, kDppRowBcast15, 0xa, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, kDppRowBcast31, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, kWave - 1);
 }
 
 // The keys that the rows of a wave see: row `lane%32` those in [lo, hi).
