@@ -5,10 +5,10 @@
 // angle_i = pos[axis(i)] * freqs[i].  Backwards, g = the gradient turned back, dw = sum of g n over rows,
 // h = g w and dx = r (h - n mean(h n)).  Only x is read again: r and n are cheaper to work out than to load.
 //
-// Bound by memory: 4 bytes a 16-bit element forward, 6 backward.  A row takes D/16 lanes (rounded up to a
-// power of two), each with the same 8 elements of both halves, so that a pair is in one lane, loads are 16
-// bytes and the sums over a row are a few lane exchanges.  A workgroup takes kTokens tokens with all
-// their heads: a token's sines serve all of them, and are worked out once, into LDS.  The angle is
+// Bound by memory: 4 bytes a 16-bit element forward, 6 backward.  A lane holds 16 bytes of each half of a row, the same
+// elements of both, so that a pair is in one lane; the lanes of a row (rounded up to a power of two) sum by a few
+// exchanges in registers.  A workgroup takes
+// kTokens tokens with all their heads: a token's sines serve all of them, and are worked out once, into LDS.  The angle is
 // reduced in 64 bits -- position times frequency in turns, less the whole turns -- because 32 bits
 // leave 6e-5 radians of the fastest pair at position 1000 and nothing at all at 10^7; it costs one
 // 64-bit product a pair and token.
@@ -20,7 +20,8 @@ namespace gearhip {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kTokens = 8;       // a workgroup's tokens, where there are enough of them
+constexpr int kTurns = 1024;       // sines and cosines of a workgroup's tokens, 8 KB of LDS
+constexpr int kTokens = 16;        // its tokens, where there are enough of them
 constexpr int kMaxDim = 256;
 constexpr int kGradBlocks = 1024;  // workgroups of the backward pass: each leaves one row of weight sums
 
@@ -57,7 +58,7 @@ __device__ __forceinline__ const T *row_at(const void *p, const Strides &s, int6
 }
 
 // cos and sin of `count` tokens from `first` on, dim/2 pairs each
-__device__ __forceinline__ void turns(const NormArgs &a, int64_t first, int count, float2 (*cs)[kMaxDim / 2]) {
+__device__ __forceinline__ void turns(const NormArgs &a, int64_t first, int count, float2 *cs) {
   const int half = a.dim / 2, pairs = a.upto[a.axes - 1];
   for (int x = threadIdx.x; x < count * half; x += kBlock) {
     const int token = x / half, i = x - token * half;
@@ -68,56 +69,69 @@ __device__ __forceinline__ void turns(const NormArgs &a, int64_t first, int coun
       turn -= rint(turn);
       sincospif((float)(2 * turn), &v.y, &v.x);
     }
-    cs[token][i] = v;
+    cs[x] = v;
   }
 }
 
+// Sum over the LPR lanes of a row, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-  for (int m = 1; m < LPR; m *= 2) x += __shfl_xor(x, m);
+  x = dpp_add<0xB1>(x);                  // lanes 1 apart
+  if (LPR > 2) x = dpp_add<0x4E>(x);     // 2 apart
+  if (LPR > 4) x = dpp_add<0x141>(x);    // the other half of 8
+  if (LPR > 8) x = dpp_add<0x140>(x);    // the other half of 16
+  if (LPR > 16) x += __shfl_xor(x, 16);
   return x;
 }
 
-__device__ __forceinline__ float sum8(f32x8 x) {
+__device__ __forceinline__ float sum_of(f32x4 x) { return (x[0] + x[1]) + (x[2] + x[3]); }
+__device__ __forceinline__ float sum_of(f32x8 x) {
   return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 }
 
+// The elements of a half that a lane holds: 16 bytes of them.
 template <typename T>
-__device__ __forceinline__ f32x8 weights8(const void *w, int f32, int at) {
-  f32x8 x = {1, 1, 1, 1, 1, 1, 1, 1};
-  if (w == nullptr) return x;
+constexpr int kEach = 16 / sizeof(T);
+template <typename T>
+using Part = float __attribute__((ext_vector_type(16 / sizeof(T))));
+
+template <typename T>
+__device__ __forceinline__ Part<T> weights_at(const void *w, int f32, int at) {
+  Part<T> x;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    x[e] = f32 ? static_cast<const float *>(w)[at + e] : (float)static_cast<const T *>(w)[at + e];
+  for (int e = 0; e < kEach<T>; ++e)
+    x[e] = w == nullptr ? 1.f : f32 ? static_cast<const float *>(w)[at + e] : (float)static_cast<const T *>(w)[at + e];
   return x;
 }
 
+template <typename T>
 struct Halves {
-  f32x8 lo, hi;
+  Part<T> lo, hi;
 };
 
 template <typename T>
-__device__ __forceinline__ Halves load_halves(const T *row, int at, int half) {
-  Row8<T> a, b;
-  a.load(row + at);
-  b.load(row + half + at);
-  return Halves{a.floats(), b.floats()};
+__device__ __forceinline__ Halves<T> load_halves(const T *row, int at, int half) {
+  typedef T raw __attribute__((ext_vector_type(16 / sizeof(T))));
+  return Halves<T>{__builtin_convertvector(*reinterpret_cast<const raw *>(row + at), Part<T>),
+                   __builtin_convertvector(*reinterpret_cast<const raw *>(row + half + at), Part<T>)};
 }
 template <typename T>
-__device__ __forceinline__ void store_halves(T *row, int at, int half, const Halves &x) {
-  Row8<T> a, b;
-  a.set(x.lo);
-  b.set(x.hi);
-  a.store(row + at);
-  b.store(row + half + at);
+__device__ __forceinline__ void store_halves(T *row, int at, int half, const Halves<T> &x) {
+  typedef T raw __attribute__((ext_vector_type(16 / sizeof(T))));
+  *reinterpret_cast<raw *>(row + at) = __builtin_convertvector(x.lo, raw);
+  *reinterpret_cast<raw *>(row + half + at) = __builtin_convertvector(x.hi, raw);
 }
 
 // (y0, y1) turned by the angle of (c, s), or back
-__device__ __forceinline__ Halves turned(const Halves &y, const float2 *cs, float sign) {
-  Halves z;
+template <typename T>
+__device__ __forceinline__ Halves<T> turned(const Halves<T> &y, const float2 *cs, float sign) {
+  Halves<T> z;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kEach<T>; ++e) {
     const float c = cs[e].x, s = sign * cs[e].y;
     z.lo[e] = y.lo[e] * c - y.hi[e] * s;
     z.hi[e] = y.hi[e] * c + y.lo[e] * s;
@@ -125,107 +139,143 @@ __device__ __forceinline__ Halves turned(const Halves &y, const float2 *cs, floa
   return z;
 }
 
-template <int LPR>
-__device__ __forceinline__ float inverse_norm(const Halves &x, int dim, float eps) {
-  return 1.f / sqrtf(row_sum<LPR>(sum8(x.lo * x.lo) + sum8(x.hi * x.hi)) / dim + eps);
+template <int LPR, typename T>
+__device__ __forceinline__ float inverse_norm(const Halves<T> &x, float over_dim, float eps) {
+  return __builtin_amdgcn_rsqf(fmaf(row_sum<LPR>(sum_of(x.lo * x.lo) + sum_of(x.hi * x.hi)), over_dim, eps));
 }
+
+// What a workgroup needs of its tokens.
+struct Tokens {
+  int64_t batch[kTokens], token[kTokens];
+};
+__device__ __forceinline__ void tokens_of(const NormArgs &a, int64_t first, int count, Tokens &at) {
+  if ((int)threadIdx.x < count) {
+    const int64_t n = first + threadIdx.x, b = n / a.tokens;
+    at.batch[threadIdx.x] = b, at.token[threadIdx.x] = n - b * a.tokens;
+  }
+}
+
+// The rows (token, head) that a lane's group goes through, kBlock / LPR apart.
+struct RowWalk {
+  int token, head;
+  __device__ __forceinline__ RowWalk(int r, int heads) : token(r / heads), head(r - token * heads) {}
+  __device__ __forceinline__ void on(int by, int heads) {
+    head += by;
+    while (head >= heads) head -= heads, ++token;
+  }
+};
 
 template <typename T, int LPR>
 __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormArgs a, int per_block) {
-  __shared__ float2 cs[kTokens][kMaxDim / 2];
+  __shared__ __attribute__((aligned(16))) float2 cs[kTurns];  // [token][dim / 2]
+  __shared__ Tokens tokens;
   const int64_t all = a.batch * a.tokens, first = (int64_t)blockIdx.x * per_block;
   const int count = (int)min((int64_t)per_block, all - first), half = a.dim / 2;
-  turns(a, first, count, cs);
-  __syncthreads();
-  const int at = (threadIdx.x % LPR) * 8;
+  const int at = (threadIdx.x % LPR) * kEach<T>;
   const bool active = at < half;
   const int heads = a.q_heads + a.k_heads + (a.v_out ? a.k_heads : 0);
-  f32x8 w[2][2] = {};
+  const float over_dim = 1.f / a.dim;
+  tokens_of(a, first, count, tokens);
+  __syncthreads();
+  auto load = [&](const RowWalk &r) __attribute__((always_inline)) {
+    Halves<T> x = {};
+    if (!active || r.token >= count) return x;
+    const int64_t b = tokens.batch[r.token], t = tokens.token[r.token];
+    const int kh = r.head - a.q_heads;
+    return load_halves(r.head < a.q_heads   ? row_at<T>(a.q, a.qs, b, t, r.head)
+                       : kh < a.k_heads     ? row_at<T>(a.k, a.ks, b, t, kh)
+                                            : row_at<T>(a.v, a.vs, b, t, kh - a.k_heads),
+                       at, half);
+  };
+  // (a row is asked for before the one before it is worked on, the first before the sines)
+  RowWalk walk(threadIdx.x / LPR, heads), ahead = walk;
+  Halves<T> next = load(ahead);
+  Part<T> w[2][2] = {};
   if (active) {
-    w[0][0] = weights8<T>(a.q_weight, a.weight_f32, at);
-    w[0][1] = weights8<T>(a.q_weight, a.weight_f32, half + at);
-    w[1][0] = weights8<T>(a.k_weight, a.weight_f32, at);
-    w[1][1] = weights8<T>(a.k_weight, a.weight_f32, half + at);
+    w[0][0] = weights_at<T>(a.q_weight, a.weight_f32, at);
+    w[0][1] = weights_at<T>(a.q_weight, a.weight_f32, half + at);
+    w[1][0] = weights_at<T>(a.k_weight, a.weight_f32, at);
+    w[1][1] = weights_at<T>(a.k_weight, a.weight_f32, half + at);
   }
+  turns(a, first, count, cs);
+  __syncthreads();
   // (all lanes of a wave go round alike: the sums exchange lanes)
-  for (int base = 0; base < count * heads; base += kBlock / LPR) {
-    const int r = base + threadIdx.x / LPR;
-    const bool here = active && r < count * heads;
-    const int token = here ? r / heads : 0, h = here ? r - token * heads : 0;
-    const int64_t n = first + token, b = n / a.tokens, t = n - b * a.tokens;
-    const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.k_heads;
-    const int64_t kh = is_v ? h - a.q_heads - a.k_heads : h - a.q_heads;
-    Halves x = {};
-    if (here)
-      x = is_q ? load_halves(row_at<T>(a.q, a.qs, b, t, h), at, half)
-               : load_halves(is_v ? row_at<T>(a.v, a.vs, b, t, kh) : row_at<T>(a.k, a.ks, b, t, kh), at, half);
-    const float r_norm = inverse_norm<LPR>(x, a.dim, a.eps);
-    if (!here) continue;
+  for (int base = 0; base < count * heads; base += kBlock / LPR, walk = ahead) {
+    Halves<T> x = base == 0 ? next : load(walk);
+    ahead.on(kBlock / LPR, heads);
+    const float r_norm = inverse_norm<LPR>(x, over_dim, a.eps);
+    if (!active || walk.token >= count) continue;
+    const bool is_q = walk.head < a.q_heads, is_v = walk.head >= a.q_heads + a.k_heads;
     if (!is_v) {
-      const f32x8 w0 = is_q ? w[0][0] : w[1][0], w1 = is_q ? w[0][1] : w[1][1];
-      x = turned(Halves{x.lo * r_norm * w0, x.hi * r_norm * w1}, &cs[token][at], 1.f);
+      const Part<T> w0 = is_q ? w[0][0] : w[1][0], w1 = is_q ? w[0][1] : w[1][1];
+      x = turned(Halves<T>{x.lo * r_norm * w0, x.hi * r_norm * w1}, cs + walk.token * half + at, 1.f);
     }
+    const int64_t n = first + walk.token;
+    const int kh = walk.head - a.q_heads - (is_v ? a.k_heads : 0);
     T *to;
     if (is_q) {
-      to = static_cast<T *>(a.q_out) + (n * a.q_heads + h) * a.dim;
+      to = static_cast<T *>(a.q_out) + (n * a.q_heads + walk.head) * a.dim;
     } else if (a.slots == nullptr) {
       to = static_cast<T *>(a.k_out) + (n * a.k_heads + kh) * a.dim;
     } else {
-      const int64_t slot = a.slots[n];
+      const int64_t slot = a.slots[n], b = tokens.batch[walk.token];
       if (slot < 0 || slot >= a.cache_tokens) continue;
       to = is_v ? static_cast<T *>(a.v_out) + b * a.vcs.batch + slot * a.vcs.token + kh * a.vcs.head
                 : static_cast<T *>(a.k_out) + b * a.kcs.batch + slot * a.kcs.token + kh * a.kcs.head;
     }
-    store_halves(to, at, half, x);
+    store_halves<T>(to, at, half, x);
   }
 }
 
 template <typename T, int LPR>
 __global__ __launch_bounds__(kBlock) void norm_rotate_grad_kernel(NormArgs a, int per_block) {
-  __shared__ float2 cs[kTokens][kMaxDim / 2];
-  __shared__ float sums[kBlock / LPR][LPR * 16];
+  __shared__ __attribute__((aligned(16))) float2 cs[kTurns];  // [token][dim / 2]
+  __shared__ Tokens tokens;
+  __shared__ __attribute__((aligned(32))) float sums[kBlock / LPR][2 * LPR * kEach<T>];
   const int64_t all = a.batch * a.tokens;
-  const int half = a.dim / 2, at = (threadIdx.x % LPR) * 8;
+  const int half = a.dim / 2, at = (threadIdx.x % LPR) * kEach<T>;
   const bool active = at < half;
+  const float over_dim = 1.f / a.dim;
+#pragma unroll 1
   for (int side = 0; side < 2; ++side) {  // queries, then keys: one set of weights and sums at a time
     const void *px = side ? a.k : a.q, *pg = side ? a.gk : a.gq, *pw = side ? a.k_weight : a.q_weight;
     const Strides &sx = side ? a.ks : a.qs, &sg = side ? a.gks : a.gqs;
     const int heads = side ? a.k_heads : a.q_heads;
     T *to = static_cast<T *>(side ? a.k_out : a.q_out);
-    f32x8 w0 = {}, w1 = {}, d0 = {}, d1 = {};
-    if (active) w0 = weights8<T>(pw, a.weight_f32, at), w1 = weights8<T>(pw, a.weight_f32, half + at);
-    for (int64_t first = (int64_t)blockIdx.x * per_block; first < all; first += (int64_t)gridDim.x * per_block) {
+    Part<T> w0 = {}, w1 = {}, d0 = {}, d1 = {};
+    if (active) w0 = weights_at<T>(pw, a.weight_f32, at), w1 = weights_at<T>(pw, a.weight_f32, half + at);
+    for (int64_t first = (int64_t)blockIdx.x * per_block; first < all && heads > 0; first += (int64_t)gridDim.x * per_block) {
       const int count = (int)min((int64_t)per_block, all - first);
       __syncthreads();
+      tokens_of(a, first, count, tokens);
       turns(a, first, count, cs);
       __syncthreads();
-      for (int base = 0; base < count * heads; base += kBlock / LPR) {
-        const int r = base + threadIdx.x / LPR;
-        const bool here = active && r < count * heads;
-        const int token = here ? r / heads : 0, h = here ? r - token * heads : 0;
-        const int64_t n = first + token, b = n / a.tokens, t = n - b * a.tokens;
-        Halves x = {}, g = {};
+      RowWalk walk(threadIdx.x / LPR, heads);
+      for (int base = 0; base < count * heads; base += kBlock / LPR, walk.on(kBlock / LPR, heads)) {
+        const bool here = active && walk.token < count;
+        Halves<T> x = {}, g = {};
         if (here) {
-          x = load_halves(row_at<T>(px, sx, b, t, h), at, half);
-          g = turned(load_halves(row_at<T>(pg, sg, b, t, h), at, half), &cs[token][at], -1.f);
+          const int64_t b = tokens.batch[walk.token], t = tokens.token[walk.token];
+          x = load_halves(row_at<T>(px, sx, b, t, walk.head), at, half);
+          g = turned(load_halves(row_at<T>(pg, sg, b, t, walk.head), at, half), cs + walk.token * half + at, -1.f);
         }
-        const float r_norm = inverse_norm<LPR>(x, a.dim, a.eps);
+        const float r_norm = inverse_norm<LPR>(x, over_dim, a.eps);
         x.lo *= r_norm, x.hi *= r_norm;
         d0 += g.lo * x.lo, d1 += g.hi * x.hi;
         g.lo *= w0, g.hi *= w1;
-        const float mean = row_sum<LPR>(sum8(g.lo * x.lo) + sum8(g.hi * x.hi)) / a.dim;
+        const float mean = row_sum<LPR>(sum_of(g.lo * x.lo) + sum_of(g.hi * x.hi)) * over_dim;
         if (here)
-          store_halves(to + (n * heads + h) * a.dim, at, half,
-                       Halves{r_norm * (g.lo - x.lo * mean), r_norm * (g.hi - x.hi * mean)});
+          store_halves<T>(to + ((first + walk.token) * heads + walk.head) * a.dim, at, half,
+                       Halves<T>{r_norm * (g.lo - x.lo * mean), r_norm * (g.hi - x.hi * mean)});
       }
     }
     if (!a.want_weights) continue;
     __syncthreads();
-    *reinterpret_cast<f32x8 *>(&sums[threadIdx.x / LPR][at]) = d0;
-    *reinterpret_cast<f32x8 *>(&sums[threadIdx.x / LPR][LPR * 8 + at]) = d1;
+    *reinterpret_cast<Part<T> *>(&sums[threadIdx.x / LPR][at]) = d0;
+    *reinterpret_cast<Part<T> *>(&sums[threadIdx.x / LPR][LPR * kEach<T> + at]) = d1;
     __syncthreads();
     for (int i = threadIdx.x; i < a.dim; i += kBlock) {
-      const int column = i < half ? i : LPR * 8 + i - half;
+      const int column = i < half ? i : LPR * kEach<T> + i - half;
       float s = 0;
       for (int r = 0; r < kBlock / LPR; ++r) s += sums[r][column];
       a.sums[((int64_t)blockIdx.x * 2 + side) * a.dim + i] = s;
@@ -233,16 +283,23 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_grad_kernel(NormArgs a, in
   }
 }
 
-// The sums of all workgroups, a column a wave.
+// The sums of all workgroups: 16 of the 2 * dim columns a workgroup, 16 threads a column.
+constexpr int kColumns = 16;
 template <typename T>
-__global__ __launch_bounds__(kWave) void norm_rotate_weights_kernel(const float *sums, int blocks, int dim, int f32,
-                                                                    void *gq, void *gk) {
-  const int side = blockIdx.x >= (unsigned)dim, i = blockIdx.x - side * dim;
+__global__ __launch_bounds__(kBlock) void norm_rotate_weights_kernel(const float *sums, int blocks, int dim, int f32,
+                                                                     void *gq, void *gk) {
+  __shared__ float part[kBlock / kColumns][kColumns];
+  const int c = threadIdx.x % kColumns, group = threadIdx.x / kColumns, column = blockIdx.x * kColumns + c;
   float s = 0;
-  for (int r = lane_id(); r < blocks; r += kWave) s += sums[((int64_t)r * 2 + side) * dim + i];
-  s = row_sum<kWave>(s);
+#pragma unroll 8
+  for (int r = group; r < blocks; r += kBlock / kColumns) s += sums[(int64_t)r * 2 * dim + column];
+  part[group][c] = s;
+  __syncthreads();
+  if (group != 0) return;
+  for (int x = 1; x < kBlock / kColumns; ++x) s += part[x][c];
+  const int side = column >= dim, i = column - side * dim;
   void *to = side ? gk : gq;
-  if (lane_id() != 0 || to == nullptr) return;
+  if (to == nullptr) return;
   if (f32)
     static_cast<float *>(to)[i] = s;
   else
@@ -298,14 +355,17 @@ int prepare(const gear_hip_norm_rotate_desc *d, NormArgs &a) {
 template <typename F>
 void by_type_and_lanes(int dtype, int dim, const F &f) {
   auto lanes = [&](auto type) {
-    if (dim <= 32)
+    const int n = dim / 2 / kEach<decltype(type)>;
+    if (n <= 2)
       f(type, std::integral_constant<int, 2>());
-    else if (dim <= 64)
+    else if (n <= 4)
       f(type, std::integral_constant<int, 4>());
-    else if (dim <= 128)
+    else if (n <= 8)
       f(type, std::integral_constant<int, 8>());
-    else
+    else if (n <= 16)
       f(type, std::integral_constant<int, 16>());
+    else if constexpr (sizeof(type) == 4)
+      f(type, std::integral_constant<int, 32>());
   };
   if (dtype == GEAR_HIP_F32)
     lanes(float());
@@ -315,16 +375,19 @@ void by_type_and_lanes(int dtype, int dim, const F &f) {
     lanes(bf16());
 }
 
-// Tokens a workgroup: the sines of kTokens serve all their heads, but few tokens are spread over the GPU.
-int tokens_per_block(int64_t tokens) {
-  int n = kTokens;
+// Tokens a workgroup: the sines of a token serve all its heads, and what is done once a workgroup has to be spread over
+// its rows (forward, 94080 tokens of 20 heads of 128: 2 tokens 436 us, 4 296, 8 241, 16 216, 32 224), but few tokens are
+// spread over the GPU, two workgroups for each of 256 CUs.
+int tokens_per_block(int64_t tokens, int dim) {
+  int n = kTurns / (dim / 2);
+  if (n > kTokens) n = kTokens;
   while (n > 1 && ceil_div64(tokens, n) < 512) n /= 2;
   return n;
 }
 
 int forward(const NormArgs &a, int dtype, void *stream) {
   const int64_t all = a.batch * a.tokens;
-  const int n = tokens_per_block(all);
+  const int n = tokens_per_block(all, a.dim);
   by_type_and_lanes(dtype, a.dim, [&](auto type, auto lanes) {
     hipLaunchKernelGGL((norm_rotate_kernel<decltype(type), decltype(lanes)::value>), dim3((unsigned)ceil_div64(all, n)),
                        dim3(kBlock), 0, as_stream(stream), a, n);
@@ -400,7 +463,7 @@ extern "C" int gear_hip_norm_rotate_backward(const gear_hip_norm_rotate_desc *de
     a.q_out = dq, a.k_out = dk;
     a.sums = static_cast<float *>(workspace);
     const int64_t all = a.batch * a.tokens;
-    const int n = tokens_per_block(all);
+    const int n = tokens_per_block(all, a.dim);
     blocks = (int)min(ceil_div64(all, n), (int64_t)kGradBlocks);
     by_type_and_lanes(desc->dtype, a.dim, [&](auto type, auto lanes) {
       hipLaunchKernelGGL((norm_rotate_grad_kernel<decltype(type), decltype(lanes)::value>), dim3(blocks), dim3(kBlock), 0,
@@ -410,7 +473,7 @@ extern "C" int gear_hip_norm_rotate_backward(const gear_hip_norm_rotate_desc *de
   }
   if (!a.want_weights) return 0;
   by_type_and_lanes(desc->dtype, 16, [&](auto type, auto) {
-    hipLaunchKernelGGL((norm_rotate_weights_kernel<decltype(type)>), dim3(2 * desc->head_dim), dim3(kWave), 0,
+    hipLaunchKernelGGL((norm_rotate_weights_kernel<decltype(type)>), dim3(2 * desc->head_dim / kColumns), dim3(kBlock), 0,
                        as_stream(stream), static_cast<const float *>(workspace), blocks, desc->head_dim,
                        desc->weight_f32 != 0, dq_weight, dk_weight);
   });
