@@ -4,7 +4,9 @@
 // needs is the nearest start at or below its step and, for documents and prefixes, the nearest end.
 // A wave takes 64 steps of one window: both are ballots and bit scans of a 64-bit word.  A document
 // that began before the wave's steps (or ends behind them) is looked for there, 1024 steps a look;
-// nothing passes between waves, so any number of windows and any length is one launch.
+// nothing passes between waves, so any number of windows and any length is one launch.  Where 64 steps are many
+// tokens, several waves find the same ranges and each writes kWrite tokens of them (8 x 1000 steps of 49 tokens: 22 us by
+// one wave, 7 by several).
 // Two bytes a step are read, 12 (20 with a grid) a token written: launch-bound for the sizes of a batch.
 #include "wave.hpp"
 
@@ -12,10 +14,12 @@ namespace gearhip {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kWrite = 256;  // tokens a wave writes
 
 struct RangesArgs {
   const uint8_t *mask, *done;
-  int64_t batch, steps, chunks;
+  int64_t batch, steps;
+  uint32_t chunks, slices;  // of 64 steps of a window; of a chunk's tokens
   int tokens, mode, cols;
   int64_t prefix;
   int32_t *lo, *hi, *pos;
@@ -30,43 +34,55 @@ struct Steps {
   __device__ __forceinline__ bool breaks(int64_t s) const { return !valid(s) || ends(s); }
 };
 
+// Which of the 16 steps from s on break, a bit each; steps outside the window do not.
+__device__ __forceinline__ uint32_t breaks16(const Steps &w, int64_t s) {
+  if (s <= -16 || s >= w.steps) return 0;
+  uint32_t found = 0;
+  if (w.steps < 16) {
+    for (int e = 0; e < 16; ++e)
+      if (s + e >= 0 && s + e < w.steps && w.breaks(s + e)) found |= 1u << e;
+    return found;
+  }
+  const int64_t at = min(max(s, (int64_t)0), w.steps - 16);  // the nearest 16 inside, shifted into place
+  u32x4 m = {~0u, ~0u, ~0u, ~0u}, d = {};
+  if (w.mask != nullptr) m = reinterpret_cast<const u32x4_any *>(w.mask + at)->v;
+  if (w.done != nullptr) d = reinterpret_cast<const u32x4_any *>(w.done + at)->v;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (((m[e / 4] >> (e % 4 * 8)) & 0xff) == 0 || ((d[e / 4] >> (e % 4 * 8)) & 0xff) != 0) found |= 1u << e;
+  return s < at ? (found << (int)(at - s)) & 0xffff : found >> (int)(s - at);
+}
+
 // The largest step below `top` that breaks, or -1.  All lanes of the wave, `top` the same in all.
 __device__ __forceinline__ int64_t last_break_below(const Steps &w, int64_t top) {
-  constexpr int kEach = 16;
   const int lane = lane_id();
-  for (; top > 0; top -= kWave * kEach) {
-    const int64_t mine = top - (int64_t)(lane + 1) * kEach;  // this lane looks at [mine, mine + kEach)
-    int64_t found = -1;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (mine + e >= 0 && w.breaks(mine + e)) found = mine + e;
-    const uint64_t any = wave_ballot(found >= 0);
-    if (any) return wave_read_lane(found, (int)__builtin_ctzll(any));
+  for (; top > 0; top -= kWave * 16) {
+    const int64_t mine = top - (int64_t)(lane + 1) * 16;
+    const uint32_t found = breaks16(w, mine);
+    const uint64_t any = wave_ballot(found != 0);
+    if (any) return wave_read_lane(mine + 31 - __builtin_clz(found | 1), (int)__builtin_ctzll(any));
   }
   return -1;
 }
 
 // The smallest step from `from` on that breaks, or steps.
 __device__ __forceinline__ int64_t first_break_from(const Steps &w, int64_t from) {
-  constexpr int kEach = 16;
   const int lane = lane_id();
-  for (; from < w.steps; from += kWave * kEach) {
-    const int64_t mine = from + (int64_t)lane * kEach;
-    int64_t found = -1;
-#pragma unroll
-    for (int e = kEach - 1; e >= 0; --e)
-      if (mine + e < w.steps && w.breaks(mine + e)) found = mine + e;
-    const uint64_t any = wave_ballot(found >= 0);
-    if (any) return wave_read_lane(found, (int)__builtin_ctzll(any));
+  for (; from < w.steps; from += kWave * 16) {
+    const int64_t mine = from + (int64_t)lane * 16;
+    const uint32_t found = breaks16(w, mine);
+    const uint64_t any = wave_ballot(found != 0);
+    if (any) return wave_read_lane(mine + __builtin_ctz(found | 1u << 31), (int)__builtin_ctzll(any));
   }
   return w.steps;
 }
 
 __global__ __launch_bounds__(kWaves *kWave) void token_ranges_kernel(RangesArgs a) {
-  const int64_t unit = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (unit >= a.batch * a.chunks) return;
+  const uint32_t unit = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t chunk = unit / a.slices, slice = unit - chunk * a.slices, window = chunk / a.chunks;
+  if (window >= a.batch) return;
   const int lane = lane_id();
-  const int64_t b = unit / a.chunks, base = (unit % a.chunks) * kWave, s = base + lane;
+  const int64_t b = window, base = (int64_t)(chunk - window * a.chunks) * kWave, s = base + lane;
   const Steps w{a.mask ? a.mask + b * a.steps : nullptr, a.done ? a.done + b * a.steps : nullptr, a.steps};
 
   const bool valid = w.valid(s), ends = w.ends(s);
@@ -95,14 +111,15 @@ __global__ __launch_bounds__(kWaves *kWave) void token_ranges_kernel(RangesArgs 
     if (a.mode == GEAR_HIP_RANGE_DOCUMENT) hi = (int)(s1 * n);
     if (a.prefix > 0) hi = max(hi, (int)(min(s0 + a.prefix, s1) * n));
   }
-  const int here = (int)min((int64_t)kWave, a.steps - base) * n;
+  const uint32_t here = (uint32_t)min((int64_t)kWave, a.steps - base) * n;
+  const uint32_t from_token = slice * kWrite, to_token = min(here, from_token + kWrite);
   const int64_t first = (b * a.steps + base) * n;
-  for (uint32_t x = 0; x < (uint32_t)here; x += kWave) {  // (all lanes go round alike: the shuffles need them all)
+  for (uint32_t x = from_token; x < to_token; x += kWave) {  // (all lanes go round alike: the shuffles need them all)
     const uint32_t i = x + lane;
     const int step = i / (uint32_t)n, u = i - (uint32_t)step * n;
     const int t_lo = __shfl(lo, step & 63), t_hi = __shfl(hi, step & 63), t_time = __shfl(time, step & 63);
     const bool ok = (valids >> (step & 63)) & 1;
-    if (i >= (uint32_t)here) continue;
+    if (i >= to_token) continue;
     a.lo[first + i] = t_lo;
     const int own = (int)(base * n) + (int)i + 1;
     a.hi[first + i] = ok && a.mode == GEAR_HIP_RANGE_CAUSAL ? max(t_hi, own) : t_hi;
@@ -137,10 +154,11 @@ extern "C" int gear_hip_token_ranges(const uint8_t *mask, const uint8_t *done, i
     return GEAR_HIP_EINVAL;
   if (batch == 0 || steps == 0) return 0;
   if (lo == nullptr || hi == nullptr || pos == nullptr) return GEAR_HIP_EINVAL;
-  RangesArgs a{mask, done, batch, steps, ceil_div64(steps, kWave), (int)tokens_per_step, mode, (int)grid_cols,
+  const int64_t longest = steps < kWave ? steps : kWave;
+  RangesArgs a{mask, done, batch, steps, (uint32_t)ceil_div64(steps, kWave), (uint32_t)ceil_div64(longest * tokens_per_step, kWrite), (int)tokens_per_step, mode, (int)grid_cols,
                prefix < steps ? prefix : steps, lo, hi, pos};
-  if (batch > ((int64_t)kMost * kWaves) / a.chunks) return GEAR_HIP_ERANGE;
-  const int64_t blocks = ceil_div64(batch * a.chunks, kWaves);
+  if (batch > kMost / a.chunks / a.slices) return GEAR_HIP_ERANGE;
+  const int64_t blocks = ceil_div64(batch * a.chunks * a.slices, kWaves);
   hipLaunchKernelGGL(token_ranges_kernel, dim3((unsigned)blocks), dim3(kWaves * kWave), 0, as_stream(stream), a);
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
   return 0;
