@@ -62,11 +62,16 @@ __device__ __forceinline__ int piece_at(int row, int c) {
 // instruction.  (swizzle() of a row is the same for rows a multiple of 8 apart, and changes the lower 3 bits of a
 // piece only.)
 //   rows     the operand whose row (or column) l%32 is row first + l%32 of the tile, contracted over the elements 16 s..
-//   columns  the operand whose row l%32 is column 32 block + l%32, contracted over the rows first..first + 15 in the
-//            order above
+//   columns  the operand whose row l%32 is column `column_of<D>(block, l%32)`, contracted over the rows
+//            first..first + 15 in the order above.  With rows of 128 elements a block is two runs of 16 columns 64 apart:
+//            32 next to each other lie in half of the banks.
+template <int D>
+constexpr int column_of(int block, int r) {
+  return D == 128 ? 16 * block + r % 16 + 64 * (r / 16) : 32 * block + r;
+}
 template <typename T, int D>
 struct TileReader {
-  static constexpr int kRowOffsets = D / 16 < 4 ? D / 16 : 4, kColumnOffsets = D / 32 < 2 ? 1 : 2;
+  static constexpr int kRowOffsets = D / 16 < 4 ? D / 16 : 4, kColumnOffsets = D / 32, kColumnPieces = D == 128 ? 2 : 4;
   int row[kRowOffsets], column[kColumnOffsets];  // elements
   __device__ __forceinline__ TileReader() {
     const int l = lane_id(), half = l >> 5, t = l & 15;
@@ -74,7 +79,7 @@ struct TileReader {
     for (int s = 0; s < kRowOffsets; ++s) row[s] = piece_at<D>(l & 31, 2 * s + half);
 #pragma unroll
     for (int b = 0; b < kColumnOffsets; ++b)
-      column[b] = piece_at<D>(4 * half + (t >> 2), 4 * b + 2 * ((l >> 4) & 1) + ((t & 3) >> 1)) + 4 * (t & 1);
+      column[b] = piece_at<D>(4 * half + (t >> 2), kColumnPieces * b + (D == 128 ? 8 : 2) * ((l >> 4) & 1) + ((t & 3) >> 1)) + 4 * (t & 1);
   }
   // (first: a multiple of 8)
   __device__ __forceinline__ vec8<T> rows(const T *tile, int first, int s) const {
@@ -85,7 +90,7 @@ struct TileReader {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     auto read = [&](int r) {
-      const T *p = tile + column[block % kColumnOffsets] + r * D + block / kColumnOffsets * 64;
+      const T *p = tile + column[block] + r * D;
       return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(const_cast<T *>(p)));
     };
     const s16x4 a = read(first), b = read(first + 8);
@@ -286,7 +291,7 @@ __device__ __forceinline__ void store_packed(T *piece, const vec8<T> (&x)[D / 32
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const vec8<T> &y = x[db][g >> 1];
-      *reinterpret_cast<vec4<T> *>(piece + piece_at<D>(l & 31, db * 4 + g) + 4 * half) =
+      *reinterpret_cast<vec4<T> *>(piece + piece_at<D>(l & 31, column_of<D>(db, 8 * g) / 8) + 4 * half) =
           (g & 1) ? __builtin_shufflevector(y, y, 4, 5, 6, 7) : __builtin_shufflevector(y, y, 0, 1, 2, 3);
     }
   wave_lds_sync();

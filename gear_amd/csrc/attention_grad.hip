@@ -252,36 +252,42 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
     left &= left - 1;
     return tile;
   };
+  // What a tile needs is asked for while the one before it is worked on, and not looked at until then.
   float next_lse = 0, next_delta = 0;
   int next_lo = 0, next_hi = 0;
+  i32x4 next_reach0 = nothing, next_reach1 = nothing;
   auto ask = [&](int tile, int to) __attribute__((always_inline)) {
     const int i0 = tile * kTile;
     const Stage<T, D, kTile> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
     const Stage<T, D, kTile> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
     q_rows.template ask<kWaves>(q_tile[to], i0, wave);
     g_rows.template ask<kWaves>(g_tile[to], i0, wave);
+    next_reach0 = bounds[2 * tile], next_reach1 = bounds[min(2 * tile + 1, groups - 1)];
     if (tid < kTile) {
-      const int i = i0 + tid;
-      const int64_t row = (int64_t)b * a.queries + i;
-      next_lo = i < a.queries ? max(a.lo[row], 0) : 0, next_hi = i < a.queries ? min(a.hi[row], a.keys) : 0;
-      const bool sees = next_hi > next_lo;
-      const int64_t stats = ((int64_t)b * a.heads + head) * a.queries + i;
-      next_lse = sees ? g.lse[stats] * kLog2e : INFINITY;
-      next_delta = sees ? g.delta[stats] : 0;
-      if (!sees) next_lo = next_hi = 0;
+      const int i = min(i0 + tid, a.queries - 1);
+      const int64_t row = (int64_t)b * a.queries + i, stats = ((int64_t)b * a.heads + head) * a.queries + i;
+      next_lo = a.lo[row], next_hi = a.hi[row], next_lse = g.lse[stats], next_delta = g.delta[stats];
     }
   };
-  auto keep = [&](int to) __attribute__((always_inline)) {
-    if (tid < kTile) rows[to].lse[tid] = next_lse, rows[to].delta[tid] = next_delta, rows[to].lo[tid] = next_lo, rows[to].hi[tid] = next_hi;
+  auto keep = [&](int i0, int to) __attribute__((always_inline)) {
+    if (tid < kTile) {
+      const int lo = max(next_lo, 0), hi = min(next_hi, a.keys);
+      const bool sees = i0 + tid < a.queries && hi > lo;
+      rows[to].lse[tid] = sees ? next_lse * kLog2e : INFINITY, rows[to].delta[tid] = sees ? next_delta : 0;
+      rows[to].lo[tid] = sees ? lo : 0, rows[to].hi[tid] = sees ? hi : 0;
+    }
   };
 
-  int tile = tiles > 0 ? next_tile() : -1, tile_head = head, buffer = 0;
+  int tile = tiles > 0 ? next_tile() : -1, tile_head = -1, buffer = 0;
+  Scores<MODE> scores(a, head < a.heads ? head : 0);
   if (tile >= 0) ask(tile, 0);
   for (; tile >= 0; buffer ^= 1) {
+    const int i0 = tile * kTile;
     staged_wait();
-    keep(buffer);
+    keep(i0, buffer);
+    if (head != tile_head) scores = Scores<MODE>(a, head), tile_head = head;
+    const i32x4 reach0 = next_reach0, reach1 = 2 * tile + 1 < groups ? next_reach1 : nothing;
     __syncthreads();
-    const i32x4 reach0 = bounds[2 * tile], reach1 = 2 * tile + 1 < groups ? bounds[2 * tile + 1] : nothing;
     if (reach0[3] == 0 || reach1[3] == 0) {  // rows that see nothing may hold anything: zeros in their place
       for (int x = tid; x < kTile * D / 8; x += kThreads) {
         const int r = x / (D / 8);
@@ -292,10 +298,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
       }
       __syncthreads();
     }
-    const int i0 = tile * kTile;
-    const Scores<MODE> scores(a, tile_head);
     tile = next_tile();
-    tile_head = head;
     if (tile >= 0) ask(tile, buffer ^ 1);
 #pragma unroll 1
     for (int qb = 0; qb < 2; ++qb) {

@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      *reinterpret_cast<f32x4 *>(own_sums + (l & 31) * D + db * 32 + 8 * x + 4 * half) =
+      *reinterpret_cast<f32x4 *>(own_sums + (l & 31) * D + column_of<D>(db, 8 * x) + 4 * half) =
           f32x4{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
   if (half == 0) joined_ml[wave][l & 31] = make_float2(m, sum);
   __syncthreads();
