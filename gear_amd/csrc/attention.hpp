@@ -163,6 +163,12 @@ struct Stage {
     else
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
   }
+  // pieces beyond dim, which repeat the last, made zeros: for the operand that has to be (once complete)
+  __device__ __forceinline__ void clear_beyond(T *tile) const {
+    const int extra = kPieces - dim / 8;
+    for (int x = lane_id(); x < ROWS * extra; x += kWave)
+      *reinterpret_cast<vec8<T> *>(tile + piece_at<D>(x / extra, dim / 8 + x % extra)) = vec8<T>{};
+  }
   // the share of wave `wave` of WAVES
   template <int WAVES>
   __device__ __forceinline__ void ask(T *tile, int row0, int wave) const {
@@ -184,6 +190,12 @@ struct Stage {
     }
   }
 };
+// 4 bytes a lane into LDS, in the same way: lane l's to `to` + 4 l.
+__device__ __forceinline__ void stage_words(const void *from, const void *to) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)const_cast<void *>(to));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
+}
+
 // All but the last `LEFT` instructions of the wave (of this kind, and the compiler's own loads and stores) are complete.
 // (the builtin: the compiler then knows that its own loads have arrived too, and waits for none of them, and with
 // them for what is asked for next, inside the loop)

@@ -22,8 +22,11 @@ struct GradArgs {
   const void *dout, *out;
   Strides gs;
   const float *lse;
-  float *delta;    // [batch][heads][queries]
-  i32x4 *bounds;   // [batch][ceil(queries/32)]: first, end, all_from, all_to (0 where a row sees nothing, or is none)
+  // left by the first launch for the second, padded to `padded` queries (those see nothing):
+  float *lse_log2, *delta;  // [batch][heads][padded]; infinite and 0 where a row sees nothing
+  int *lo, *hi;             // [batch][padded]; 0, 0 there
+  i32x4 *bounds;            // [batch][padded / 32]: first, end, all_from, all_to (0 where a row sees nothing)
+  int padded;
   void *dq, *dk, *dv;
   int blocks;      // workgroups of a head
 };
@@ -87,17 +90,18 @@ struct __attribute__((aligned(16))) QueryRows {
 
 // 32 queries (rows `row0`.. of the tiles and of `rows`, i0.. in memory) by the wave's 32 keys, a lane a key: dv += p^T dout,
 // dk += ds^T q.
-template <typename T, int D, int MODE, int N>
+// KEEP_V: V's operands are in v, else in LDS, the wave's 32 rows at own_v.
+template <bool KEEP_V, typename T, int D, int MODE, int N>
 __device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], const T *q_tile, const T *g_tile, int row0,
                                            const QueryRows<N> &rows, const vec8<T> (&k)[D / 16], const vec8<T> (&v)[D / 16],
-                                           const TileReader<T, D> &reader, const Scores<MODE> &scores, int ahead, int key,
+                                           const T *own_v, const TileReader<T, D> &reader, const Scores<MODE> &scores, int ahead, int key,
                                            bool whole) {
   const int half = lane_id() >> 5;
   f32x16 s = {}, dp = {};
 #pragma unroll
   for (int y = 0; y < D / 16; ++y) s = mfma(reader.rows(q_tile, row0, y), k[y], s);
 #pragma unroll
-  for (int y = 0; y < D / 16; ++y) dp = mfma(reader.rows(g_tile, row0, y), v[y], dp);
+  for (int y = 0; y < D / 16; ++y) dp = mfma(reader.rows(g_tile, row0, y), KEEP_V ? v[y] : reader.rows(own_v, 0, y), dp);
   constexpr float lower = 1.f / (1 << (int)kRaise<T>);
   const float distance = (float)(ahead + 4 * half - key);
 #pragma unroll
@@ -147,9 +151,11 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   seen.set(row_there ? a.lo[row] : 0, row_there ? a.hi[row] : 0, a.keys);
   if (l == 0) ranges[wave][0] = seen.first, ranges[wave][1] = seen.end;
   const bool some_empty = wave_ballot(seen.empty()) != 0;
-  if (head == 0 && l == 0 && i0 < a.queries)
-    g.bounds[(int64_t)b * ((a.queries + kRows - 1) / kRows) + i0 / kRows] =
-        i32x4{seen.first, seen.end, seen.all_from, some_empty ? 0 : seen.all_to};
+  if (head == 0 && i < g.padded) {
+    if (half == 0) g.lo[(int64_t)b * g.padded + i] = seen.lo, g.hi[(int64_t)b * g.padded + i] = seen.hi;
+    if (l == 0)
+      g.bounds[((int64_t)b * g.padded + i0) / kRows] = i32x4{seen.first, seen.end, seen.all_from, some_empty ? 0 : seen.all_to};
+  }
 
   vec8<T> q[D / 16], dout[D / 16];
   own_row_frags<T, D>(q, static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head, a.dim, !seen.empty());
@@ -166,10 +172,10 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
     delta = sum_of_halves(delta);
   }
   float lse_log2 = INFINITY;  // a row that sees nothing: p = 0
-  if (row_there) {
-    const int64_t stats = ((int64_t)b * a.heads + head) * a.queries + i;
-    if (half == 0) g.delta[stats] = delta;
-    if (!seen.empty()) lse_log2 = g.lse[stats] * kLog2e;
+  if (!seen.empty()) lse_log2 = g.lse[((int64_t)b * a.heads + head) * a.queries + i] * kLog2e;
+  if (half == 0 && i < g.padded) {
+    const int64_t stats = ((int64_t)b * a.heads + head) * g.padded + i;
+    g.lse_log2[stats] = lse_log2, g.delta[stats] = delta;
   }
   __syncthreads();
   int first = INT_MAX, end = 0;
@@ -209,13 +215,18 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   });
 }
 
+// Rows of 128 elements leave no registers for V beside K, dk and dv at two waves a SIMD (spilled, they would be waited for
+// together with the tiles to come): V stays in LDS, and to make room for it a tile is 32 queries.
 template <typename T, int D, int MODE>
 __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) {
+  constexpr bool kKeepV = D < 128;  // in registers
+  constexpr int kTile = kKeepV ? 64 : 32, kSides = kTile / kRows;
   __shared__ __attribute__((aligned(16))) T q_tile[2][kTile * D];  // (at the end: the rows of dk and dv)
   __shared__ __attribute__((aligned(16))) T g_tile[2][kTile * D];
+  __shared__ __attribute__((aligned(16))) T v_rows[kKeepV ? 8 : kWaves * kRows * D];
   __shared__ QueryRows<kTile> rows[2];
   const AttentionArgs &a = g.a;
-  const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
+  const int l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int at = same_die_index(), block = at % g.blocks, bh = at / g.blocks, kv_head = bh % a.kv_heads, b = bh / a.kv_heads;
   const int shared = a.heads / a.kv_heads;
   const int block_key = block * (kWaves * kRows), wave_key = block_key + wave * kRows, key = wave_key + (l & 31);
@@ -223,11 +234,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
 
   vec8<T> k[D / 16], v[D / 16];
   own_row_frags<T, D>(k, static_cast<const T *>(a.k) + b * a.ks.batch + key * a.ks.token + kv_head * a.ks.head, a.dim, key_there);
-  own_row_frags<T, D>(v, static_cast<const T *>(a.v) + b * a.vs.batch + key * a.vs.token + kv_head * a.vs.head, a.dim, key_there);
+  T *own_v = v_rows + wave * kRows * D;
+  const T *v_base = static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head;
+  if (kKeepV) {
+    own_row_frags<T, D>(v, v_base + key * a.vs.token, a.dim, key_there);
+  } else {
+    const Stage<T, D, kRows> v_stage(v_base, a.vs.token, 0, a.keys, a.dim);
+    v_stage.template ask<1>(own_v, wave_key, 0);
+    staged_wait();
+    v_stage.clear_beyond(own_v);
+    wave_lds_sync();
+  }
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
-  const int groups = (a.queries + kRows - 1) / kRows, tiles = (a.queries + kTile - 1) / kTile;
-  const i32x4 *bounds = g.bounds + (int64_t)b * groups;
-  const i32x4 nothing = {INT_MAX, 0, 0, 0};
+  const int groups = g.padded / kRows, tiles = (a.queries + kTile - 1) / kTile;
+  // (read through the scalar cache: the launch before wrote them)
+  typedef const __attribute__((address_space(4))) i32x4 *Bounds;
+  const Bounds bounds = (Bounds)(uintptr_t)(g.bounds + (int64_t)b * groups);
   const TileReader<T, D> reader;
 
   // The tiles of queries that see any of the workgroup's keys, head after head: 64 are looked at at a time.
@@ -241,10 +263,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
         if (++head == (kv_head + 1) * shared || tiles == 0) return -1;
       }
       bool reaches = false;
+      if (base + l < tiles) {
+        const i32x4 *mine = g.bounds + (int64_t)b * groups + (base + l) * kSides;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int group = 2 * (base + l) + y;
-        if (group < groups) reaches |= bounds[group][0] < block_key + kWaves * kRows && bounds[group][1] > block_key;
+        for (int y = 0; y < kSides; ++y) reaches |= mine[y][0] < block_key + kWaves * kRows && mine[y][1] > block_key;
       }
       left = wave_ballot(reaches);
     }
@@ -252,60 +274,47 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
     left &= left - 1;
     return tile;
   };
-  // What a tile needs is asked for while the one before it is worked on, and not looked at until then.
-  float next_lse = 0, next_delta = 0;
-  int next_lo = 0, next_hi = 0;
-  i32x4 next_reach0 = nothing, next_reach1 = nothing;
+  // A tile is asked for while the one before it is worked on: rows of q and dout, and (an array a wave) what is known of them.
   auto ask = [&](int tile, int to) __attribute__((always_inline)) {
     const int i0 = tile * kTile;
     const Stage<T, D, kTile> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
     const Stage<T, D, kTile> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
     q_rows.template ask<kWaves>(q_tile[to], i0, wave);
     g_rows.template ask<kWaves>(g_tile[to], i0, wave);
-    next_reach0 = bounds[2 * tile], next_reach1 = bounds[min(2 * tile + 1, groups - 1)];
-    if (tid < kTile) {
-      const int i = min(i0 + tid, a.queries - 1);
-      const int64_t row = (int64_t)b * a.queries + i, stats = ((int64_t)b * a.heads + head) * a.queries + i;
-      next_lo = a.lo[row], next_hi = a.hi[row], next_lse = g.lse[stats], next_delta = g.delta[stats];
-    }
-  };
-  auto keep = [&](int i0, int to) __attribute__((always_inline)) {
-    if (tid < kTile) {
-      const int lo = max(next_lo, 0), hi = min(next_hi, a.keys);
-      const bool sees = i0 + tid < a.queries && hi > lo;
-      rows[to].lse[tid] = sees ? next_lse * kLog2e : INFINITY, rows[to].delta[tid] = sees ? next_delta : 0;
-      rows[to].lo[tid] = sees ? lo : 0, rows[to].hi[tid] = sees ? hi : 0;
-    }
+    static_assert(kWaves == 4, "");
+    const int64_t stats = ((int64_t)b * a.heads + head) * g.padded + i0, of_batch = (int64_t)b * g.padded + i0;
+    const void *from = wave == 0 ? (const void *)(g.lse_log2 + stats) : wave == 1 ? (const void *)(g.delta + stats)
+                       : wave == 2 ? (const void *)(g.lo + of_batch) : (const void *)(g.hi + of_batch);
+    if (l < kTile) stage_words(static_cast<const int *>(from) + l, reinterpret_cast<const int *>(&rows[to]) + wave * kTile);
   };
 
   int tile = tiles > 0 ? next_tile() : -1, tile_head = -1, buffer = 0;
-  Scores<MODE> scores(a, head < a.heads ? head : 0);
+  Scores<MODE> scores(a, kv_head * shared);
   if (tile >= 0) ask(tile, 0);
   for (; tile >= 0; buffer ^= 1) {
     const int i0 = tile * kTile;
+    i32x4 reach[kSides];
+#pragma unroll
+    for (int y = 0; y < kSides; ++y) reach[y] = bounds[tile * kSides + y];
+    if (MODE & kBias && head != tile_head) scores = Scores<MODE>(a, head), tile_head = head;
     staged_wait();
-    keep(i0, buffer);
-    if (head != tile_head) scores = Scores<MODE>(a, head), tile_head = head;
-    const i32x4 reach0 = next_reach0, reach1 = 2 * tile + 1 < groups ? next_reach1 : nothing;
     __syncthreads();
-    if (reach0[3] == 0 || reach1[3] == 0) {  // rows that see nothing may hold anything: zeros in their place
-      for (int x = tid; x < kTile * D / 8; x += kThreads) {
-        const int r = x / (D / 8);
-        if (rows[buffer].hi[r] == 0) {
+    if (reach[0][3] == 0 || reach[kSides - 1][3] == 0) {  // rows that see nothing may hold anything: zeros in their place
+      for (int x = threadIdx.x; x < kTile * D / 8; x += kThreads)
+        if (rows[buffer].hi[x / (D / 8)] == 0) {
           *reinterpret_cast<vec8<T> *>(q_tile[buffer] + x * 8) = vec8<T>{};
           *reinterpret_cast<vec8<T> *>(g_tile[buffer] + x * 8) = vec8<T>{};
         }
-      }
       __syncthreads();
     }
     tile = next_tile();
     if (tile >= 0) ask(tile, buffer ^ 1);
-#pragma unroll 1
-    for (int qb = 0; qb < 2; ++qb) {
-      const i32x4 reach = qb ? reach1 : reach0;
-      if (reach[0] >= wave_key + kRows || reach[1] <= wave_key) continue;
-      add_by_key<T, D, MODE>(dk, dv, q_tile[buffer], g_tile[buffer], qb * 32, rows[buffer], k, v, reader, scores,
-                             i0 + qb * 32 + a.keys - a.queries, key, reach[2] <= wave_key && reach[3] >= wave_key + kRows);
+#pragma unroll
+    for (int y = 0; y < kSides; ++y) {
+      if (reach[y][0] >= wave_key + kRows || reach[y][1] <= wave_key) continue;
+      add_by_key<kKeepV, T, D, MODE>(dk, dv, q_tile[buffer], g_tile[buffer], y * kRows, rows[buffer], k, v, own_v, reader, scores,
+                                     i0 + y * kRows + a.keys - a.queries, key,
+                                     reach[y][2] <= wave_key && reach[y][3] >= wave_key + kRows);
     }
   }
   __syncthreads();
@@ -314,8 +323,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
       return wave_key + r < a.keys ? static_cast<T *>(p) + (((int64_t)b * a.keys + wave_key + r) * a.kv_heads + kv_head) * a.dim : nullptr;
     };
   };
-  store_rows<T, D>(q_tile[0] + wave * kRows * D, dk, a.scale, false, a.dim, to(g.dk));
-  store_rows<T, D>(g_tile[0] + wave * kRows * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
+  // (the 4 x 32 rows of dk fill both tiles of q, those of dv the tiles of dout or what was V)
+  store_rows<T, D>(kKeepV ? q_tile[0] + wave * kRows * D : own_v, dk, a.scale, false, a.dim, to(g.dk));
+  wave_lds_sync();
+  store_rows<T, D>(kKeepV ? g_tile[0] + wave * kRows * D : own_v, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
 }
 
 // ---- short windows: one launch ----------------------------------------------------------------------------
@@ -416,7 +427,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     const i32x4 reach = bounds[qb];
     if (__builtin_amdgcn_readfirstlane(reach[0]) >= own + kRows || __builtin_amdgcn_readfirstlane(reach[1]) <= own) continue;
     const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
-    add_by_key<T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
+    add_by_key<true, T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, nullptr, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
   }
   __syncthreads();
   const auto to = [&](void *p, int count) {
@@ -429,9 +440,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
   store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv, a.keys));
 }
 
-size_t delta_bytes(int64_t batch, int64_t queries, int64_t heads) {
-  return align_up((size_t)(batch * heads * queries) * sizeof(float), 256);
-}
+// Queries in the statistics: whole tiles.
+int64_t padded(int64_t queries) { return ceil_div64(queries, 64) * 64; }
 
 }  // namespace
 }  // namespace gearhip
@@ -440,7 +450,8 @@ using namespace gearhip;
 
 extern "C" size_t gear_hip_attention_backward_workspace_bytes(int64_t batch, int64_t queries, int64_t heads) {
   if (batch <= 0 || queries <= 0 || heads <= 0) return 0;
-  return delta_bytes(batch, queries, heads) + (size_t)(batch * ceil_div64(queries, kRows)) * sizeof(i32x4);
+  const size_t rows = (size_t)(batch * padded(queries));
+  return rows * heads * 2 * sizeof(float) + rows * 2 * sizeof(int) + rows / kRows * sizeof(i32x4);
 }
 
 extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, const void *dout,
@@ -463,8 +474,13 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
     g.gs = Strides{dout_stride[0], dout_stride[1], dout_stride[2]};
   }
   g.dout = dout, g.out = out, g.lse = lse;
-  g.delta = static_cast<float *>(workspace);
-  g.bounds = reinterpret_cast<i32x4 *>(static_cast<char *>(workspace) + delta_bytes(a.batch, a.queries, a.heads));
+  g.padded = (int)padded(a.queries);
+  const int64_t rows = (int64_t)a.batch * g.padded;
+  g.bounds = static_cast<i32x4 *>(workspace);
+  g.lse_log2 = reinterpret_cast<float *>(g.bounds + rows / kRows);
+  g.delta = g.lse_log2 + rows * a.heads;
+  g.lo = reinterpret_cast<int *>(g.delta + rows * a.heads);
+  g.hi = g.lo + rows;
   g.dq = dq, g.dk = dk, g.dv = dv;
   const int longest = a.queries > a.keys ? a.queries : a.keys;
   if (longest <= 4 * kRows && a.dim <= 64 && a.heads == a.kv_heads && a.queries > 0) {
@@ -483,7 +499,7 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
     constexpr int D = decltype(dim)::value;
     constexpr int kMode = decltype(mode)::value;
     if (a.queries > 0) {
-      const int groups = (int)ceil_div64(a.queries, kRows);
+      const int groups = g.padded / kRows;  // (padding included: its statistics are written too)
       g.blocks = (groups + kWaves - 1) / kWaves;
       by_waves((groups + g.blocks - 1) / g.blocks, [&](auto w) {
         hipLaunchKernelGGL((attention_dq_kernel<T, D, kMode, decltype(w)::value>),
