@@ -31,39 +31,39 @@ struct GradArgs {
   int blocks;      // workgroups of a head
 };
 
-// 32 keys (rows `row0`.. of the tiles, kk.. in memory) by the wave's 32 queries, a lane a query: the gradients of the scores, or,
-// for delta alone, the lane's share of sum p dp.
-template <bool DELTA, typename T, int D, int MODE>
-__device__ __forceinline__ f32x16 grads_by_query(const T *k_tile, const T *v_tile, int row0, int kk, const vec8<T> (&q)[D / 16],
-                                                 const vec8<T> (&dout)[D / 16], const TileReader<T, D> &reader,
-                                                 const Scores<MODE> &scores, const Seen &seen, int place, float less,
-                                                 float &delta) {
+// 32 keys (rows `row0`.. of the tiles, kk.. in memory) by the wave's 32 queries, a lane a query: s, the probabilities times
+// the cap's derivative, and dp; `delta` gains the lane's share of sum p dp.
+template <typename T, int D, int MODE>
+__device__ __forceinline__ void by_query(f32x16 &s, f32x16 &dp, float &delta, const T *k_tile, const T *v_tile, int row0, int kk,
+                                         const vec8<T> (&q)[D / 16], const vec8<T> (&dout)[D / 16], const TileReader<T, D> &reader,
+                                         const Scores<MODE> &scores, const Seen &seen, int place, float less) {
   const int half = lane_id() >> 5;
-  f32x16 s = {}, dp = {};
+  s = dp = f32x16{};
 #pragma unroll
   for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_tile, row0, x), q[x], s);
 #pragma unroll
   for (int x = 0; x < D / 16; ++x) dp = mfma(reader.rows(v_tile, row0, x), dout[x], dp);
   const float ahead = (float)(place - kk - 4 * half);
+  f32x16 shrink;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    float shrink;
-    const float z = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)), shrink);
-    const float p = exp2_fast(fmaf(z, scores.factor, less));
-    s[r] = DELTA ? p * dp[r] : p * (dp[r] - delta) * ((MODE & kCap) ? shrink : 1.f);
+    float of_cap;
+    const float z = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)), of_cap);
+    s[r] = exp2_fast(fmaf(z, scores.factor, less));
+    shrink[r] = of_cap;
   }
   if (__builtin_expect(!seen.covers(kk, kk + 32), 0)) {
     const uint32_t from_lo = (uint32_t)(kk + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      if (from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) >= count) s[r] = 0;
+      if (from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) >= count) s[r] = dp[r] = shrink[r] = 0;
     asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
   }
-  if (DELTA) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) delta += s[r];
+  for (int r = 0; r < 16; ++r) {
+    delta += s[r] * dp[r];
+    if (MODE & kCap) s[r] *= shrink[r];
   }
-  return s;
 }
 
 // x += (rows row0.. of the tile, transposed) times the 32 x 32 block y
@@ -205,8 +205,12 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
     for (int kb = 0; kb < 2; ++kb) {
       const int kk = k0 + kb * 32;
       if (!seen.touches(kk, kk + 32)) continue;
-      const f32x16 ds = grads_by_query<false, T, D, MODE>(k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less, delta);
-      add_columns<T, D>(dq, k_here, kb * 32, ds, reader);
+      f32x16 s, dp;
+      float unused = 0;
+      by_query<T, D, MODE>(s, dp, unused, k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+      add_columns<T, D>(dq, k_here, kb * 32, s, reader);
     }
   }
   __syncthreads();
@@ -399,19 +403,21 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     const float less = scores.offset - lse_log2;
     const int place = mine + a.keys - a.queries;
     float delta = 0;
+    f32x16 s[WAVES], dp[WAVES];
     take(q_tile, g_tile);
-#pragma unroll 1
-    for (int kk = 0; kk < kMost; kk += kRows)
-      if (seen.touches(kk, kk + kRows))
-        grads_by_query<true, T, D, MODE>(k_tile, v_tile, kk, kk, u, w, reader, scores, seen, place, less, delta);
+#pragma unroll
+    for (int x = 0; x < WAVES; ++x)
+      if (seen.touches(x * kRows, x * kRows + kRows))
+        by_query<T, D, MODE>(s[x], dp[x], delta, k_tile, v_tile, x * kRows, x * kRows, u, w, reader, scores, seen, place, less);
     delta = sum_of_halves(delta);
     if (half == 0) rows.delta[mine] = delta;
     f32x16 dq[D / 32] = {};
-#pragma unroll 1
-    for (int kk = 0; kk < kMost; kk += kRows)
-      if (seen.touches(kk, kk + kRows)) {
-        const f32x16 ds = grads_by_query<false, T, D, MODE>(k_tile, v_tile, kk, kk, u, w, reader, scores, seen, place, less, delta);
-        add_columns<T, D>(dq, k_tile, kk, ds, reader);
+#pragma unroll
+    for (int x = 0; x < WAVES; ++x)
+      if (seen.touches(x * kRows, x * kRows + kRows)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[x][r] *= dp[x][r] - delta;
+        add_columns<T, D>(dq, k_tile, x * kRows, s[x], reader);
       }
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
@@ -420,8 +426,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     }
   }
   __syncthreads();
-  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  const auto to = [&](void *p, int count) {
+    return [=](int r) {
+      return own + r < count ? static_cast<T *>(p) + (((int64_t)b * count + own + r) * a.heads + head) * a.dim : nullptr;
+    };
+  };
   take(k_tile, v_tile);
+  wave_lds_sync();  // nobody reads the wave's rows of K any more
+  store_packed<T, D>(k_tile + own * D, dq_kept, a.dim, to(g.dq, a.queries));
+  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
 #pragma unroll 1
   for (int qb = 0; qb < WAVES; ++qb) {
     const i32x4 reach = bounds[qb];
@@ -429,13 +442,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
     add_by_key<true, T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, nullptr, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
   }
-  __syncthreads();
-  const auto to = [&](void *p, int count) {
-    return [=](int r) {
-      return own + r < count ? static_cast<T *>(p) + (((int64_t)b * count + own + r) * a.heads + head) * a.dim : nullptr;
-    };
-  };
-  store_packed<T, D>(q_tile + own * D, dq_kept, a.dim, to(g.dq, a.queries));
+  wave_lds_sync();
   store_rows<T, D>(k_tile + own * D, dk, a.scale, false, a.dim, to(g.dk, a.keys));
   store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv, a.keys));
 }
