@@ -6,7 +6,7 @@
 // in full need no comparison.
 #include <type_traits>
 
-#include "attention.hpp"
+#include "attention_exact.hpp"
 
 namespace gearhip {
 
@@ -157,14 +157,25 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
 
   sum = sum_of_halves(sum);
   const bool empty = seen.empty();
+  const float lse_log2 = m * scores.factor + scores.offset + __builtin_log2f(sum);
   if (lse != nullptr && half == 0 && row_there)
-    lse[((int64_t)b * a.heads + head) * a.queries + i] =
-        empty ? -INFINITY : (m * scores.factor + scores.offset + __builtin_log2f(sum)) * kLn2;
+    lse[((int64_t)b * a.heads + head) * a.queries + i] = empty ? -INFINITY : lse_log2 * kLn2;
+  uint32_t bad = columns_not_finite(o, !empty);
   __syncthreads();  // the tiles are free
   const int i0 = (block * WAVES + wave) * kRows;
   store_rows<T, D>(k_tile[0] + wave * kRows * D, o, 1.f / sum, empty, a.dim, [&](int r) {
     return i0 + r < a.queries ? out + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
   });
+  if (__builtin_expect(bad == 0, 1)) return;
+  staged_wait();  // (what is stored above, before it is stored again)
+  for (; bad != 0; bad &= bad - 1) {
+    const int r = __builtin_ctz(bad), at_row = i0 + r;
+    Pair x;
+    if (exact_out<T, MODE>(x, static_cast<const T *>(a.q) + b * a.qs.batch + at_row * a.qs.token + head * a.qs.head, k_rows.base,
+                           a.ks.token, v_rows.base, a.vs.token, wave_read_lane(seen.lo, r), wave_read_lane(seen.hi, r), a.dim,
+                           at_row + a.keys - a.queries, lane_value(lse_log2, r), scores))
+      store_pair(out + (((int64_t)b * a.queries + at_row) * a.heads + head) * a.dim, x, a.dim);
+  }
 }
 
 }  // namespace

@@ -9,7 +9,7 @@
 //      reach them; scores are not transposed here, a lane holds one key
 #include <type_traits>
 
-#include "attention.hpp"
+#include "attention_exact.hpp"
 
 namespace gearhip {
 namespace {
@@ -30,6 +30,64 @@ struct GradArgs {
   void *dq, *dk, *dv;
   int blocks;      // workgroups of a head
 };
+
+// Rows i0 + r of dq, r a bit of `bad`, worked out alone (lse and delta: of the lane's row).
+template <typename T, int MODE>
+__device__ __forceinline__ void mend_dq(const GradArgs &g, uint32_t bad, int b, int head, int kv_head, int i0, const Seen &seen,
+                                        float lse_log2, float delta, const Scores<MODE> &scores) {
+  const AttentionArgs &a = g.a;
+  staged_wait();  // (what was stored, before it is stored again)
+  for (; bad != 0; bad &= bad - 1) {
+    const int r = __builtin_ctz(bad), i = i0 + r;
+    Pair x;
+    if (exact_dq<T, MODE>(x, static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head,
+                          static_cast<const T *>(g.dout) + b * g.gs.batch + i * g.gs.token + head * g.gs.head,
+                          static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token,
+                          static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, wave_read_lane(seen.lo, r),
+                          wave_read_lane(seen.hi, r), a.dim, i + a.keys - a.queries, lane_value(lse_log2, r), lane_value(delta, r), scores))
+      store_pair(static_cast<T *>(g.dq) + (((int64_t)b * a.queries + i) * a.heads + head) * a.dim, Pair{x.x * a.scale, x.y * a.scale}, a.dim);
+  }
+}
+
+// Keys first_key + c of dk and dv, c a bit of `bad`, worked out alone, over all heads that share them.  known(head, i, lse, delta,
+// lo, hi): what is known of a query.
+template <typename T, int MODE, typename F>
+__device__ __forceinline__ void mend_dkv(const GradArgs &g, uint32_t bad, int b, int kv_head, int first_key, const F &known) {
+  const AttentionArgs &a = g.a;
+  const int shared = a.heads / a.kv_heads;
+  staged_wait();
+  for (; bad != 0; bad &= bad - 1) {
+    const int key = first_key + __builtin_ctz(bad);
+    if (key >= a.keys) break;
+    const Pair k = load_pair(static_cast<const T *>(a.k) + b * a.ks.batch + key * a.ks.token + kv_head * a.ks.head, a.dim);
+    const Pair v = load_pair(static_cast<const T *>(a.v) + b * a.vs.batch + key * a.vs.token + kv_head * a.vs.head, a.dim);
+    bool fine = finite_pair(k) && finite_pair(v);
+    Pair dk = {0.f, 0.f}, dv = {0.f, 0.f};
+    for (int pass = 0; pass < 2; ++pass)  // whether all that sees the key is finite; then the sums
+      for (int head = kv_head * shared; head < (kv_head + 1) * shared && fine; ++head) {
+        const Scores<MODE> scores(a, head);
+        for (int i = 0; i < a.queries && fine; ++i) {
+          float lse_log2, delta;
+          int lo, hi;
+          known(head, i, lse_log2, delta, lo, hi);
+          if (key < lo || key >= hi) continue;
+          const Pair q = load_pair(static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head, a.dim);
+          const Pair d = load_pair(static_cast<const T *>(g.dout) + b * g.gs.batch + i * g.gs.token + head * g.gs.head, a.dim);
+          if (pass == 0) {
+            fine = finite_pair(q) && finite_pair(d) && fabsf(lse_log2) < INFINITY && fabsf(delta) < INFINITY;
+          } else {
+            const float2 y = exact_pair(dot(q, k), dot(d, v), i + a.keys - a.queries - key, lse_log2, delta, scores);
+            dv.x += y.x * d.x, dv.y += y.x * d.y;
+            dk.x += y.y * q.x, dk.y += y.y * q.y;
+          }
+        }
+      }
+    if (!fine) continue;
+    const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kv_head) * a.dim;
+    store_pair(static_cast<T *>(g.dk) + to, Pair{dk.x * a.scale, dk.y * a.scale}, a.dim);
+    store_pair(static_cast<T *>(g.dv) + to, dv, a.dim);
+  }
+}
 
 // 32 keys (rows `row0`.. of the tiles, kk.. in memory) by the wave's 32 queries, a lane a query: s, the probabilities times
 // the cap's derivative, and dp; `delta` gains the lane's share of sum p dp.
@@ -214,9 +272,11 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
     }
   }
   __syncthreads();
+  const uint32_t bad = columns_not_finite(dq, !seen.empty());
   store_rows<T, D>(k_tile[0] + wave * kRows * D, dq, a.scale, seen.empty(), a.dim, [&](int r) {
     return i0 + r < a.queries ? static_cast<T *>(g.dq) + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
   });
+  if (__builtin_expect(bad != 0, 0)) mend_dq<T, MODE>(g, bad, b, head, kv_head, i0, seen, lse_log2, delta, scores);
 }
 
 // Rows of 128 elements leave no registers for V beside K, dk and dv at two waves a SIMD (spilled, they would be waited for
@@ -327,10 +387,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
       return wave_key + r < a.keys ? static_cast<T *>(p) + (((int64_t)b * a.keys + wave_key + r) * a.kv_heads + kv_head) * a.dim : nullptr;
     };
   };
+  const uint32_t bad = columns_not_finite(dk, key_there) | columns_not_finite(dv, key_there);
   // (the 4 x 32 rows of dk fill both tiles of q, those of dv the tiles of dout or what was V)
   store_rows<T, D>(kKeepV ? q_tile[0] + wave * kRows * D : own_v, dk, a.scale, false, a.dim, to(g.dk));
   wave_lds_sync();
   store_rows<T, D>(kKeepV ? g_tile[0] + wave * kRows * D : own_v, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
+  if (__builtin_expect(bad != 0, 0))
+    mend_dkv<T, MODE>(g, bad, b, kv_head, wave_key, [&](int of_head, int i, float &lse_log2, float &delta, int &lo, int &hi) {
+      const int64_t stats = ((int64_t)b * a.heads + of_head) * g.padded + i, of_batch = (int64_t)b * g.padded + i;
+      lse_log2 = g.lse_log2[stats], delta = g.delta[stats], lo = g.lo[of_batch], hi = g.hi[of_batch];
+    });
 }
 
 // ---- short windows: one launch ----------------------------------------------------------------------------
@@ -399,6 +465,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     }
   };
   vec8<T> dq_kept[D / 32][2];
+  uint32_t bad_dq;
+  float own_delta;
   {
     const float less = scores.offset - lse_log2;
     const int place = mine + a.keys - a.queries;
@@ -419,6 +487,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
         for (int r = 0; r < 16; ++r) s[x][r] *= dp[x][r] - delta;
         add_columns<T, D>(dq, k_tile, x * kRows, s[x], reader);
       }
+    bad_dq = columns_not_finite(dq, !seen.empty()), own_delta = delta;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
       dq[db] *= a.scale;
@@ -442,9 +511,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
     add_by_key<true, T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, nullptr, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
   }
+  const uint32_t bad = columns_not_finite(dk, mine < a.keys) | columns_not_finite(dv, mine < a.keys);
   wave_lds_sync();
   store_rows<T, D>(k_tile + own * D, dk, a.scale, false, a.dim, to(g.dk, a.keys));
   store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv, a.keys));
+  if (__builtin_expect(bad_dq != 0, 0)) mend_dq<T, MODE>(g, bad_dq, b, head, head, own, seen, lse_log2, own_delta, scores);
+  if (__builtin_expect(bad != 0, 0))
+    mend_dkv<T, MODE>(g, bad, b, head, own, [&](int, int i, float &lse_of, float &delta, int &lo_of, int &hi_of) {
+      lse_of = rows.lse[i], delta = rows.delta[i], lo_of = rows.lo[i], hi_of = rows.hi[i];
+    });
 }
 
 // Queries in the statistics: whole tiles.

@@ -9,7 +9,7 @@
 // launch.
 #include <type_traits>
 
-#include "attention.hpp"
+#include "attention_exact.hpp"
 
 namespace gearhip {
 namespace {
@@ -24,6 +24,22 @@ struct StepArgs {
   float2 *part_ml; // [batch][kv_heads][row_blocks][splits][32]
   void *out;
 };
+
+// Row r of a key head's rows, worked out alone (max_log2: maximum and sum of its scores, without the offset).
+template <typename T, int MODE>
+__device__ __forceinline__ void mend_row(const StepArgs &g, int64_t b, int r, int kv_head, float max_log2) {
+  const AttentionArgs &a = g.a;
+  const int shared = a.heads / a.kv_heads, t = r / shared, head = kv_head * shared + r % shared;
+  const int64_t row = b * a.queries + t;
+  const int lo = max(a.lo[row], 0), hi = min(a.hi[row], a.keys);
+  const Scores<MODE> scores(a, head);
+  Pair x;
+  if (hi > lo && exact_out<T, MODE>(x, static_cast<const T *>(a.q) + b * a.qs.batch + t * a.qs.token + head * a.qs.head,
+                                    static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token,
+                                    static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, lo, hi, a.dim,
+                                    a.hi[row] - 1, max_log2 + scores.offset, scores))
+    store_pair(static_cast<T *>(g.out) + (row * a.heads + head) * a.dim, x, a.dim);
+}
 
 template <typename T, int D, int MODE>
 __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g) {
@@ -138,6 +154,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
   if (half == 0) joined_ml[wave][l & 31] = make_float2(m, sum);
   __syncthreads();
   const int here = min(kRows, rows - block * kRows);
+  bool bad = false;
   for (int x = threadIdx.x; x < here * a.dim; x += kThreads) {
     const int r = x / a.dim, d = x - r * a.dim;
     float top = -INFINITY;
@@ -156,17 +173,28 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
       const int64_t q_row = (int64_t)b * a.queries + t;
       const bool none = min(a.hi[q_row], a.keys) <= max(a.lo[q_row], 0);
       static_cast<T *>(g.out)[(q_row * a.heads + h) * a.dim + d] = (T)(none ? 0.f : y / total);
+      bad = bad || (!none && !(fabsf(y) < INFINITY));
     } else {
       const int64_t at = ((((int64_t)b * a.kv_heads + kv_head) * g.row_blocks + block) * g.splits + split) * kRows + r;
       g.part_o[at * a.dim + d] = y;
       if (d == 0) g.part_ml[at] = make_float2(top, total);
     }
   }
+  if (g.splits > 1 || __builtin_expect(!__syncthreads_or(bad), 1)) return;
+  for (int r = wave; r < here; r += kWaves) {  // (which rows it is was not kept: all of them are looked at)
+    float top = -INFINITY, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, joined_ml[w][r].x);
+    const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += exp2_fast(joined_ml[w][r].x - from) * joined_ml[w][r].y;
+    mend_row<T, MODE>(g, b, block * kRows + r, kv_head, top + __builtin_log2f(total));
+  }
 }
 
 // One workgroup a query and head: the parts of its split, joined.  Every thread takes 4 elements of each eighth part (or
 // more often, with shorter rows), so that the loads of a row's parts are in flight together.
-template <typename T>
+template <typename T, int MODE>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(StepArgs g) {
   __shared__ float share[kMaxSplits];
   __shared__ f32x4 sums[kThreads];
@@ -202,13 +230,17 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(StepArgs g) {
       y += share[p] * *reinterpret_cast<const f32x4 *>(g.part_o + (first + (int64_t)p * kRows) * a.dim + d);
   sums[threadIdx.x] = y;
   __syncthreads();
-  if (group != 0) return;
-  for (int x = 1; x < groups; ++x) y += sums[x * lanes + threadIdx.x];
-  const bool none = min(a.hi[q_row], a.keys) <= max(a.lo[q_row], 0);
-  vec4<T> z;
+  bool bad = false;
+  if (group == 0) {
+    for (int x = 1; x < groups; ++x) y += sums[x * lanes + threadIdx.x];
+    const bool none = min(a.hi[q_row], a.keys) <= max(a.lo[q_row], 0);
+    vec4<T> z;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) z[e] = (T)(none ? 0.f : y[e] / total);
-  *reinterpret_cast<vec4<T> *>(static_cast<T *>(g.out) + (q_row * a.heads + head) * a.dim + d) = z;
+    for (int e = 0; e < 4; ++e) z[e] = (T)(none ? 0.f : y[e] / total), bad = bad || (!none && !(fabsf(y[e]) < INFINITY));
+    *reinterpret_cast<vec4<T> *>(static_cast<T *>(g.out) + (q_row * a.heads + head) * a.dim + d) = z;
+  }
+  if (__builtin_expect(__syncthreads_or(bad), 0) && threadIdx.x < kWave)
+    mend_row<T, MODE>(g, b, r, kv_head, top + __builtin_log2f(total));
 }
 
 int row_blocks_of(int64_t queries, int64_t heads, int64_t kv_heads) {
@@ -261,7 +293,7 @@ extern "C" int gear_hip_attention_step(const gear_hip_attention_desc *desc, void
     hipLaunchKernelGGL((attention_step_kernel<T, decltype(dim)::value, decltype(mode)::value>),
                        dim3((unsigned)workgroups), dim3(kThreads), 0, as_stream(stream), g);
     if (g.splits > 1)
-      hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(kThreads), 0,
+      hipLaunchKernelGGL((attention_join_kernel<T, decltype(mode)::value>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(kThreads), 0,
                          as_stream(stream), g);
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();

@@ -119,6 +119,55 @@ def test_what_no_range_reaches_is_not_looked_at(dtype):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_some_rows_see_does_not_reach_the_others(dtype, bad):
+    """A key (or a query and its gradient) that is not finite: rows that see it are NaN or infinite, the others as if it
+    were not there."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(14)
+    for T, H, HK, D, cap in ((90, 2, 2, 64, 0.0), (90, 4, 2, 48, 6.0), (300, 2, 1, 128, 0.0), (200, 2, 2, 32, 6.0)):
+        q, k, v, dout = (_rows(g, 2, T, h, D, dtype) for h in (H, HK, HK, H))
+        form = dict(cap=cap, slopes=torch.rand(H, generator=g, device="cuda") * 0.1 if cap else None)
+        lo, hi = _masks("causal", 2, T, T, g)
+        ref = Attention(q, k, v, lo, hi, dout=dout, **form)
+        at = 2 * T // 3 + 5
+        announce("%s at %d of %d, %s, D=%d" % (bad, at, T, dtype, D))
+        # a key: queries before it do not see it
+        k2, v2 = k.clone(), v.clone()
+        k2[0, at, :, 3] = bad
+        v2[0, at] = bad
+        out, lse = ops.range_attention(q, k2, v2, lo, hi, **form)
+        same = torch.ones(2, T, dtype=torch.bool, device="cuda")
+        same[0, at:] = False
+        pick = lambda x: x[same]  # noqa: E731
+        assert worst(pick(out), pick(ref.out), pick(ref.out_bound)) <= 1
+        assert worst(lse.transpose(1, 2)[same], ref.lse.transpose(1, 2)[same], ref.lse_bound.transpose(1, 2)[same]) <= 1
+        assert not torch.isfinite(out[0, at:]).all(-1).any()
+        dq = ops.range_attention_backward(dout, q, k2, v2, out, lse, lo, hi, **form)[0]
+        assert worst(pick(dq), pick(ref.dq), pick(ref.dq_bound)) <= 1
+        # a query and its gradient: keys behind it are not seen by it
+        q2, dout2 = q.clone(), dout.clone()
+        q2[1, at], dout2[1, at] = bad, bad
+        out, lse = ops.range_attention(q2, k, v, lo, hi, **form)
+        dq, dk, dv = ops.range_attention_backward(dout2, q2, k, v, out, lse, lo, hi, **form)
+        same[:] = True
+        same[1, at] = False
+        assert worst(pick(out), pick(ref.out), pick(ref.out_bound)) <= 1
+        assert worst(pick(dq), pick(ref.dq), pick(ref.dq_bound)) <= 1
+        same[:] = True
+        same[1, :at + 1] = False
+        assert worst(pick(dk), pick(ref.dk), pick(ref.dk_bound)) <= 1
+        assert worst(pick(dv), pick(ref.dv), pick(ref.dv_bound)) <= 1
+        assert not torch.isfinite(dv[1, :at + 1]).any()
+        # over caches: the newest of three tokens sees one key more
+        new = hi[:, at - 2:at + 1].contiguous()
+        out = ops.range_attention_step(q[:, at - 2:at + 1], k2, v2, lo[:, :3].contiguous(), new, **form)
+        assert worst(out[0, :2], ref.out[0, at - 2:at], ref.out_bound[0, at - 2:at]) <= 1
+        assert not torch.isfinite(out[0, 2]).all(-1).any()
+        assert worst(out[1], ref.out[1, at - 2:at + 1], ref.out_bound[1, at - 2:at + 1]) <= 1
+
+
 def test_gradient_against_differences():
     """f16 inputs, a step of 2^-4: the value is a sum of B*T*H*D products of out (rounded: 2^-11 of its size)."""
     from gear_amd import ops
