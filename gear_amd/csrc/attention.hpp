@@ -143,18 +143,17 @@ struct Stage {
   static constexpr int kPieces = D / 8, kRowsEach = kWave / kPieces, kCount = ROWS / kRowsEach;
   const T *base;
   int64_t stride;
-  int first, end, dim;
+  int first, end, dim, lane;
   int64_t offset[2];  // of the lane's piece within an even and an odd instruction's rows
 
-  __device__ __forceinline__ Stage(const T *base, int64_t stride, int first, int end, int dim)
-      : base(base), stride(stride), first(first), end(end), dim(dim) {
+  __device__ __forceinline__ Stage(const T *base, int64_t stride, int first, int end, int dim, int lane = lane_id())
+      : base(base), stride(stride), first(first), end(end), dim(dim), lane(lane) {
 #pragma unroll
-    for (int odd = 0; odd < 2; ++odd) offset[odd] = (lane_id() / kPieces) * stride + piece(odd) * 8;
+    for (int odd = 0; odd < 2; ++odd) offset[odd] = (lane / kPieces) * stride + piece(odd) * 8;
   }
   // (rows of an instruction differ from those of the next but one by a multiple of 8: the same swizzle)
   __device__ __forceinline__ int piece(int x) const {
-    const int l = lane_id();
-    return min((l % kPieces) ^ swizzle<D>(x * kRowsEach + l / kPieces), dim / 8 - 1);
+    return min((lane % kPieces) ^ swizzle<D>(x * kRowsEach + lane / kPieces), dim / 8 - 1);
   }
   __device__ __forceinline__ void one(const T *from, uint32_t at) const {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane(at);
@@ -184,7 +183,7 @@ struct Stage {
     } else {
 #pragma unroll 1
       for (int x = wave, to = at; x < kCount; x += WAVES, to += kNext) {
-        const int row = row0 + x * kRowsEach + lane_id() / kPieces;
+        const int row = row0 + x * kRowsEach + lane / kPieces;
         one(base + (int64_t)min(max(row, first), end - 1) * stride + piece(x) * 8, to);
       }
     }
@@ -261,11 +260,14 @@ constexpr int kCap = 1, kBias = 2;
 template <int MODE>
 struct Scores {
   float factor, offset, inner, outer, slope;
-  __device__ __forceinline__ Scores(const AttentionArgs &a, int head) {
+  // (UNIFORM: one head for the whole wave, its slope in a scalar register)
+  template <bool UNIFORM = true>
+  __device__ __forceinline__ Scores(const AttentionArgs &a, int head, std::bool_constant<UNIFORM> = {}) {
     const float cap_log2 = a.cap * kLog2e;
     inner = MODE & kCap ? a.scale / a.cap * (2 * kLog2e) : a.scale_log2;
     outer = 2 * cap_log2;
     slope = MODE & kBias && a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    if (MODE & kBias && UNIFORM) slope = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(slope)));
     factor = MODE == 0 ? a.scale_log2 : MODE == kCap ? outer : 1.f;
     offset = MODE & kCap ? cap_log2 : 0.f;
   }

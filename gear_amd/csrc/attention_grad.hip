@@ -341,8 +341,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
   // A tile is asked for while the one before it is worked on: rows of q and dout, and (an array a wave) what is known of them.
   auto ask = [&](int tile, int to) __attribute__((always_inline)) {
     const int i0 = tile * kTile;
-    const Stage<T, D, kTile> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim);
-    const Stage<T, D, kTile> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim);
+    int lane = l;
+    // with a bias there are too few registers to keep what Stage works out between the tiles (2 x 8193: 725 us spilled, 675
+    // worked out again; without, 961 kept, 1028 worked out again)
+    if (MODE & kBias) asm volatile("" : "+v"(lane));
+    const Stage<T, D, kTile> q_rows(static_cast<const T *>(a.q) + b * a.qs.batch + head * a.qs.head, a.qs.token, 0, a.queries, a.dim, lane);
+    const Stage<T, D, kTile> g_rows(static_cast<const T *>(g.dout) + b * g.gs.batch + head * g.gs.head, g.gs.token, 0, a.queries, a.dim, lane);
     q_rows.template ask<kWaves>(q_tile[to], i0, wave);
     g_rows.template ask<kWaves>(g_tile[to], i0, wave);
     static_assert(kWaves == 4, "");

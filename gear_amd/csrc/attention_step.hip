@@ -77,7 +77,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
   const int first = (int)min((int64_t)seen.end, (length > 0 ? seen.first : 0) + (int64_t)split * part);
   const int end = (int)min((int64_t)seen.end, (int64_t)first + part);
 
-  const Scores<MODE> scores(a, row_there ? head : 0);
+  const Scores<MODE> scores(a, row_there ? head : 0, std::false_type());
   const TileReader<T, D> reader;
   f32x16 o[D / 32] = {};
   float m = -INFINITY, sum = 0;  // m: of z
