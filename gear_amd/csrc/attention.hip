@@ -1,9 +1,14 @@
 // Attention over ranges of keys, forward (gear_hip_attention).
 //
-// A workgroup takes 128 queries of one head, 32 a wave; tiles of 64 keys pass through LDS.  The softmax runs
-// along: a lane holds its query's maximum m and sum l so far, in exponents of 2, and the sums of p v are
-// rescaled when m grows.  Tiles outside a wave's ranges are passed over, tiles that all its rows see
-// in full need no comparison.
+//   out_i = sum_j p_ij v_j,  p_ij = exp(z_ij - lse_i),  lse_i = log sum_j exp z_ij,  j in [lo_i, hi_i)
+// A workgroup takes up to 128 queries of one head, 32 a wave; tiles of 32 keys pass through LDS, two deep, the next asked for
+// while one is worked on.  The softmax runs along: a lane holds its query's maximum m and sum l so far, in exponents of 2,
+// and the sums of p v are rescaled when m grows.  Tiles outside a wave's ranges are passed over, tiles that all its rows
+// see in full need no comparison.  p is rounded to the type for its product (the matrix unit takes nothing wider at this
+// rate), its sum is of the values before that.
+// bf16: 2048 windows of 90, 8 heads of 64, causal: 133 us, bound by memory (755 MB, 5.7 TB/s).  2 x 8193, 16 heads of 128 over 8,
+// packed, a bias: 334 us, 720 TFLOP/s of the pairs that are seen; 32 x 1470, 16 over 4, frames, a cap: 429 us, 410 TFLOP/s.  There the
+// exponentials (and the tanh of the cap) and the matrix unit take about the same time and do not overlap in full.
 #include <type_traits>
 
 #include "attention_exact.hpp"
@@ -42,12 +47,15 @@ int attention_args(const gear_hip_attention_desc *d, AttentionArgs &a) {
 namespace {
 
 constexpr int kMostWaves = 4;
-constexpr int kTile = 64;  // keys of a tile
+// Keys of a tile.  With 32, three waves a SIMD have the registers and the LDS they need with rows of 128, and less is passed
+// over at the edges of ranges: us with 32 / 64, 2048 windows of 90 (64) 133 / 150, 32 x 1470 with a cap (128) 429 / 487,
+// 2 x 8193 with a bias 334 / 326.
+constexpr int kTile = 32;
 
 template <typename T, int D, int MODE, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArgs a, T *__restrict__ out,
                                                                     float *__restrict__ lse, int blocks) {
-  __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * D];  // (at the end: the rows of the output)
+  __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * D];  // (at the end, with those of V: the rows of the output)
   __shared__ __attribute__((aligned(16))) T v_tile[2][kTile * D];
   __shared__ int ranges[WAVES][2];
   const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
@@ -81,38 +89,24 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
     k_rows.template ask<WAVES>(k_to, k0, wave);
     v_rows.template ask<WAVES>(v_to, k0, wave);
   };
-  auto tile = [&](int k0, const T *k_here, const T *v_here) {
+  auto tile = [&](int k0, const T *k_here, const T *v_here) __attribute__((always_inline)) {
     if (!seen.touches(k0, k0 + kTile)) return;
-    const bool whole = seen.covers(k0, k0 + kTile);
-    f32x16 s[2];
+    f32x16 s = {};
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      s[kb] = f32x16{};
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) s[kb] = mfma(reader.rows(k_here, kb * 32, x), q[x], s[kb]);
-    }
+    for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_here, 0, x), q[x], s);
     const float ahead = (float)(place - k0 - 4 * half);
-    float top = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int offset = kb * 32 + 8 * (r >> 2) + (r & 3);
-        s[kb][r] = scores.z(s[kb][r], ahead - (float)offset);
-      }
-    if (__builtin_expect(!whole, 0)) {
+    for (int r = 0; r < 16; ++r) s[r] = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)));
+    if (__builtin_expect(!seen.covers(k0, k0 + kTile), 0)) {
       const uint32_t from_lo = (uint32_t)(k0 + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (from_lo + (uint32_t)(kb * 32 + 8 * (r >> 2) + (r & 3)) >= count) s[kb][r] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) >= count) s[r] = -INFINITY;
       asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
     }
+    float top = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     top = max_of_halves(top);
     // the sums are rescaled only where a maximum grows by more than 2^8: p stays below that
     if (wave_ballot((top - m) * scores.factor > 8.f) != 0) {
@@ -125,20 +119,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
     }
     const float from = m == -INFINITY ? 0.f : -m * scores.factor;  // (no key seen yet)
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int r = 0; r < 16; ++r) {
+      s[r] = exp2_fast(fmaf(s[r], scores.factor, from));
+      sum += s[r];
+    }
+    const vec8<T> p0 = packed<T, 0>(s), p1 = packed<T, 1>(s);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[kb][r] = exp2_fast(fmaf(s[kb][r], scores.factor, from));
-        sum += s[kb][r];
-      }
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const vec8<T> p0 = packed<T, 0>(s[kb]), p1 = packed<T, 1>(s[kb]);
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-        o[db] = mfma(reader.columns(v_here, kb * 32, db), p0, o[db]);
-        o[db] = mfma(reader.columns(v_here, kb * 32 + 16, db), p1, o[db]);
-      }
+    for (int db = 0; db < D / 32; ++db) {
+      o[db] = mfma(reader.columns(v_here, 0, db), p0, o[db]);
+      o[db] = mfma(reader.columns(v_here, 16, db), p1, o[db]);
     }
   };
   int k0 = first < end ? first / kTile * kTile : 0;
@@ -163,7 +152,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
   uint32_t bad = columns_not_finite(o, !empty);
   __syncthreads();  // the tiles are free
   const int i0 = (block * WAVES + wave) * kRows;
-  store_rows<T, D>(k_tile[0] + wave * kRows * D, o, 1.f / sum, empty, a.dim, [&](int r) {
+  T *piece = (wave < 2 ? k_tile[wave] : v_tile[wave - 2]);
+  store_rows<T, D>(piece, o, 1.f / sum, empty, a.dim, [&](int r) {
     return i0 + r < a.queries ? out + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
   });
   if (__builtin_expect(bad == 0, 1)) return;
