@@ -59,11 +59,18 @@ __device__ __forceinline__ uint32_t columns_not_finite(const f32x16 (&x)[N], boo
   return (uint32_t)bad | (uint32_t)(bad >> 32);
 }
 
-// Whether rows [lo, hi) are finite.
+// Whether rows [lo, hi) are finite, 16 loads at a time.
 template <typename T>
 __device__ __forceinline__ bool rows_finite(const T *rows, int64_t stride, int lo, int hi, int dim) {
-  for (int j = lo; j < hi; ++j)
-    if (!finite_pair(load_pair(rows + j * stride, dim))) return false;
+  for (int j = lo; j < hi; j += 16) {
+    Pair sum = {0.f, 0.f};
+#pragma unroll
+    for (int y = 0; y < 16; ++y) {
+      const Pair x = load_pair(rows + min(j + y, hi - 1) * stride, dim);
+      sum.x = fmaf(x.x, 0.f, sum.x), sum.y = fmaf(x.y, 0.f, sum.y);
+    }
+    if (!finite_pair(sum)) return false;
+  }
   return true;
 }
 

@@ -62,6 +62,14 @@ __device__ __forceinline__ void mend_dkv(const GradArgs &g, uint32_t bad, int b,
     const Pair k = load_pair(static_cast<const T *>(a.k) + b * a.ks.batch + key * a.ks.token + kv_head * a.ks.head, a.dim);
     const Pair v = load_pair(static_cast<const T *>(a.v) + b * a.vs.batch + key * a.vs.token + kv_head * a.vs.head, a.dim);
     bool fine = finite_pair(k) && finite_pair(v);
+    // (64 queries at a time by what is known of them: a gradient or a score that is not finite shows there)
+    for (int head = kv_head * shared; head < (kv_head + 1) * shared && fine; ++head)
+      for (int i0 = 0; i0 < a.queries && fine; i0 += kWave) {
+        float lse_log2, delta;
+        int lo, hi;
+        known(head, min(i0 + lane_id(), a.queries - 1), lse_log2, delta, lo, hi);
+        fine = wave_ballot(key >= lo && key < hi && !(fabsf(lse_log2) < INFINITY && fabsf(delta) < INFINITY)) == 0;
+      }
     Pair dk = {0.f, 0.f}, dv = {0.f, 0.f};
     for (int pass = 0; pass < 2; ++pass)  // whether all that sees the key is finite; then the sums
       for (int head = kv_head * shared; head < (kv_head + 1) * shared && fine; ++head) {
@@ -74,7 +82,7 @@ __device__ __forceinline__ void mend_dkv(const GradArgs &g, uint32_t bad, int b,
           const Pair q = load_pair(static_cast<const T *>(a.q) + b * a.qs.batch + i * a.qs.token + head * a.qs.head, a.dim);
           const Pair d = load_pair(static_cast<const T *>(g.dout) + b * g.gs.batch + i * g.gs.token + head * g.gs.head, a.dim);
           if (pass == 0) {
-            fine = finite_pair(q) && finite_pair(d) && fabsf(lse_log2) < INFINITY && fabsf(delta) < INFINITY;
+            fine = finite_pair(q) && finite_pair(d);
           } else {
             const float2 y = exact_pair(dot(q, k), dot(d, v), i + a.keys - a.queries - key, lse_log2, delta, scores);
             dv.x += y.x * d.x, dv.y += y.x * d.y;
