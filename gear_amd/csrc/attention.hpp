@@ -12,8 +12,8 @@
 // operand, rows of V by key, comes from LDS through the transposing read: a group of 16 lanes reads 4 rows of
 // 16 elements and each lane gets a column.
 //
-// Rows lie in LDS as 16-byte pieces; piece c of row r at c ^ swizzle(r), so that both the reads of a
-// piece of 8 consecutive rows and the transposing read of 2 pieces of 4 rows touch every bank once.
+// Rows lie in LDS as 16-byte pieces; piece c of row r at c ^ swizzle(r), so that the pieces of 8 consecutive rows, and
+// the transposing read of 2 pieces of 4 rows, lie in different banks (rows of 128 elements: in half of all banks).
 #pragma once
 #include <limits.h>
 
@@ -58,17 +58,18 @@ __device__ __forceinline__ int piece_at(int row, int c) {
   return row * D + ((c ^ swizzle<D>(row)) << 3);
 }
 
+// Which column of a tile the row r of operand `block` is.  With rows of 128 elements a block is two runs of 16 columns 64 apart: 32
+// next to each other lie in half of the banks.
+template <int D>
+constexpr int column_of(int block, int r) {
+  return D == 128 ? 16 * block + r % 16 + 64 * (r / 16) : 32 * block + r;
+}
 // Operands out of a tile, by offsets that a lane works out once: what remains of an address is a constant of the
 // instruction.  (swizzle() of a row is the same for rows a multiple of 8 apart, and changes the lower 3 bits of a
 // piece only.)
 //   rows     the operand whose row (or column) l%32 is row first + l%32 of the tile, contracted over the elements 16 s..
 //   columns  the operand whose row l%32 is column `column_of<D>(block, l%32)`, contracted over the rows
-//            first..first + 15 in the order above.  With rows of 128 elements a block is two runs of 16 columns 64 apart:
-//            32 next to each other lie in half of the banks.
-template <int D>
-constexpr int column_of(int block, int r) {
-  return D == 128 ? 16 * block + r % 16 + 64 * (r / 16) : 32 * block + r;
-}
+//            first..first + 15 in the order above
 template <typename T, int D>
 struct TileReader {
   static constexpr int kRowOffsets = D / 16 < 4 ? D / 16 : 4, kColumnOffsets = D / 32, kColumnPieces = D == 128 ? 2 : 4;

@@ -3,10 +3,13 @@
 // Few queries, many keys: what counts is reading the caches once, at the rate of memory.  The queries of
 // all heads that share a key head are the rows of one matrix operand (32 at a time; most calls have fewer, the
 // unused rows cost nothing that memory would not), so every key is read once for all of them.  A rollout's
-// keys are split over `splits` workgroups and within one over its waves, 32 keys at a time; a wave takes K
-// straight into registers and V through a piece of LDS of its own (which turns it), so no wave waits
-// for another before the end.  What the parts of a split have -- maximum, sum, sums of p v -- is joined by a second
-// launch.
+// keys are split over `splits` workgroups and within one over its waves, 32 keys at a time.  A wave has two tiles of K and
+// V in a piece of LDS of its own, filled past the caches (nobody reads a key again) while the one before is worked on, so no
+// wave waits for another before the end.  What the parts of a split have -- maximum, sum, sums of p v -- is joined by a second
+// launch, in a fixed order.
+// Bound by memory.  bf16: 256 rollouts of up to 3000 keys, 8 heads of 64: 142 us, 5.3 TB/s of the keys that are seen; 3 of up to 131071,
+// 16 heads of 128 over 2: 60 us (3.2 TB/s), of which the join is 6 and starting and ending workgroups that fill a CU's LDS
+// alone most of the rest.  Tried there: two waves a workgroup 63, 64 or 256 parts 62 and 84, parts of one size 75.
 #include <type_traits>
 
 #include "attention_exact.hpp"

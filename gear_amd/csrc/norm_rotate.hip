@@ -12,6 +12,8 @@
 // reduced in 64 bits -- position times frequency in turns, less the whole turns -- because 32 bits
 // leave 6e-5 radians of the fastest pair at position 1000 and nothing at all at 10^7; it costs one
 // 64-bit product a pair and token.
+// Measured, forward and backward (with the sums of dw): 1024 x 60 tokens, 8 + 8 heads of 32, 32 bits: 58 and 78 us (4.3 and 4.8
+// TB/s); 64 x 1470, 16 + 4 of 128, bf16, three axes: 212 and 302 us (4.5 and 4.8 TB/s), where a plain copy of as much reaches 4.8.
 #include <type_traits>
 
 #include "half.hpp"
