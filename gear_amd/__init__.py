@@ -5,6 +5,7 @@ Layers (bottom up):
   gear_amd/libgearhip.so   that C ABI (built by gear_amd._build / __graft_entry__.build)
   gear_amd._cabi           ctypes binding of the C ABI
   gear_amd.ops             tensor-level calls (torch tensors only carry device memory + stream)
+  gear_amd.sequence        autograd operators and a causal model over batches of windows
   gear_amd/csrc/host       host C++ (specs, table layout, patterns, handler, index set, memory)
   gear_amd.libgear         pybind11 module with the reference's `libgear.core` names
   gear_amd.{specs,dtypes,sampler,loader,dataset,mpu}   the reference's `gear` Python API

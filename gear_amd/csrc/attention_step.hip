@@ -8,8 +8,9 @@
 // wave waits for another before the end.  What the parts of a split have -- maximum, sum, sums of p v -- is joined by a second
 // launch, in a fixed order.
 // Bound by memory.  bf16: 256 rollouts of up to 3000 keys, 8 heads of 64: 142 us, 5.3 TB/s of the keys that are seen; 3 of up to 131071,
-// 16 heads of 128 over 2: 60 us (3.2 TB/s), of which the join is 6 and starting and ending workgroups that fill a CU's LDS
-// alone most of the rest.  Tried there: two waves a workgroup 63, 64 or 256 parts 62 and 84, parts of one size 75.
+// 16 heads of 128 over 2: 64 us (3.1 TB/s; 49 at best) and 6 for the join.  There a workgroup fills a CU's LDS alone, and its start
+// and end are time in which the CU asks for little: two waves a workgroup 63 us, 64 parts 62, 256 parts 84, parts of
+// one size 75.
 #include <type_traits>
 
 #include "attention_exact.hpp"
