@@ -247,10 +247,6 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   }
   float lse_log2 = INFINITY;  // a row that sees nothing: p = 0
   if (!seen.empty()) lse_log2 = g.lse[((int64_t)b * a.heads + head) * a.queries + i] * kLog2e;
-  if (half == 0 && i < g.padded) {
-    const int64_t stats = ((int64_t)b * a.heads + head) * g.padded + i;
-    g.lse_log2[stats] = lse_log2, g.delta[stats] = delta;
-  }
   __syncthreads();
   int first = INT_MAX, end = 0;
 #pragma unroll
@@ -262,6 +258,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   const float less = scores.offset - lse_log2;
   const int place = i + a.keys - a.queries;
   f32x16 dq[D / 32] = {};
+  float summed = 0;  // sum p dp: what delta is, without the rounding of out
   const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
   auto load = [&](int k0, int to) __attribute__((always_inline)) {
@@ -280,12 +277,16 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
       const int kk = k0 + kb * 32;
       if (!seen.touches(kk, kk + 32)) continue;
       f32x16 s, dp;
-      float unused = 0;
-      by_query<T, D, MODE>(s, dp, unused, k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less);
+      by_query<T, D, MODE>(s, dp, summed, k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
       add_columns<T, D>(dq, k_here, kb * 32, s, reader);
     }
+  }
+  summed = sum_of_halves(summed);
+  if (half == 0 && i < g.padded) {
+    const int64_t stats = ((int64_t)b * a.heads + head) * g.padded + i;
+    g.lse_log2[stats] = lse_log2, g.delta[stats] = summed;
   }
   __syncthreads();
   const uint32_t bad = columns_not_finite(dq, !seen.empty());
