@@ -7,13 +7,14 @@
 //   1. by queries (the layout of the forward pass): delta, dq, and the range that each 32 queries see
 //   2. by keys: a wave holds 32 keys and passes over all queries (of all heads that share them) whose ranges
 //      reach them; scores are not transposed here, a lane holds one key
-// delta starts from out as it was stored, rounded: dq and dk are then within 0.0025..0.0034 of the exact ones in bf16 (norm of
-// the difference over the norm), where the rounding of p and ds to the type alone leaves 0.0017.  A delta of sum_j p_ij dp_ij in
-// 32 bits takes a third pass over the keys with two products, 2/7 more work.  Short windows, whose probabilities
-// stay in registers, have it for nothing: one launch (below).
+// dq's delta is dout . out, which starts from out as it was stored, rounded; on the way sum_j p_ij dp_ij is summed in 32 bits for the
+// second launch, which costs it next to nothing.  In bf16 dk is then within 0.0024 of the exact one (norm of the difference over
+// the norm; 0.0034 with dout . out), dq within 0.0025..0.0029, where the rounding of the results alone leaves 0.0017.  The exact
+// delta for dq too takes a third pass over the keys with two products, 2/7 more work.  Short windows, whose
+// probabilities stay in registers, have it for nothing: one launch (below).
 // p and ds are rounded to the type for their products, the sums are held in 32 bits.
-// Bound by the matrix unit, the exponentials and LDS together: 2 x 8193, 16 heads of 128 over 8, packed, with a bias: 1. 400 us (three
-// products, 900 TFLOP/s), 2. 676 us (four products of twice the loads, 710); 32 x 1470, 16 over 4, frames, a cap: 668 and 946 us.
+// Bound by the matrix unit, the exponentials and LDS together: 2 x 8193, 16 heads of 128 over 8, packed, with a bias: 1. 411 us (three
+// products, 880 TFLOP/s), 2. 678 us (four products of twice the loads, 710); 32 x 1470, 16 over 4, frames, a cap: 674 and 950 us.
 // Tiles of 32 keys in 1., which the forward pass gains by, change nothing here: 404 against 407, 697 against 686 us.
 #include <type_traits>
 
