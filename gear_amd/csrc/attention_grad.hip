@@ -287,7 +287,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   summed = sum_of_halves(summed);
   if (half == 0 && i < g.padded) {
     const int64_t stats = ((int64_t)b * a.heads + head) * g.padded + i;
-    g.lse_log2[stats] = lse_log2, g.delta[stats] = summed;
+    g.lse_log2[stats] = lse_log2, g.delta[stats] = seen.empty() ? 0.f : summed;
   }
   __syncthreads();
   const uint32_t bad = columns_not_finite(dq, !seen.empty());
