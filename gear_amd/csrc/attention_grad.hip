@@ -502,7 +502,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
     for (int x = 0; x < WAVES; ++x)
       if (seen.touches(x * kRows, x * kRows + kRows))
         by_query<T, D, MODE>(s[x], dp[x], delta, k_tile, v_tile, x * kRows, x * kRows, u, w, reader, scores, seen, place, less);
-    delta = sum_of_halves(delta);
+    delta = seen.empty() ? 0.f : sum_of_halves(delta);
     if (half == 0) rows.delta[mine] = delta;
     f32x16 dq[D / 32] = {};
 #pragma unroll
@@ -516,6 +516,11 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
       dq[db] *= a.scale;
+      if (empties != 0) {  // (p = 0 is not enough where a key that others see is not finite)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[db][r] = seen.empty() ? 0.f : dq[db][r];
+        asm volatile("");
+      }
       dq_kept[db][0] = packed<T, 0>(dq[db]), dq_kept[db][1] = packed<T, 1>(dq[db]);
     }
   }

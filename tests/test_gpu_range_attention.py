@@ -279,3 +279,36 @@ def test_calls_on_two_streams():
     torch.cuda.synchronize()
     for a, b in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_that_see_nothing_get_nothing_beside_rows_that_see_what_is_not_finite(dtype, bad):
+    """Padding at the head of a window, and a key (its K, or its V) that is not finite and that every other row sees, or
+    those behind it: padding gets gradients of 0 and passes none on, in one launch (T <= 128, a key head a head) and in two."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(15)
+    for T, H, HK, D, cap in ((60, 2, 2, 64, 0.0), (128, 2, 2, 48, 5.0), (60, 4, 2, 64, 0.0), (200, 2, 2, 128, 0.0)):
+        q, k, v, dout = (_rows(g, 2, T, h, D, dtype) for h in (H, HK, HK, H))
+        pad, at = 10, 2 * T // 3
+        i = torch.arange(T, device="cuda").expand(2, T)
+        for sees in ("all", "causal"):
+            lo = torch.where(i < pad, 0, pad).int()
+            hi = torch.where(i < pad, 0, T if sees == "all" else i + 1).int()
+            ref = Attention(q, k, v, lo, hi, cap=cap, dout=dout)
+            for where in ("K", "V"):
+                k2, v2 = k.clone(), v.clone()
+                (k2 if where == "K" else v2)[0, at] = bad
+                announce("padding beside %s of %s, T=%d D=%d %s %s" % (where, bad, T, D, sees, dtype))
+                out, lse = ops.range_attention(q, k2, v2, lo, hi, cap=cap)
+                dq, dk, dv = ops.range_attention_backward(dout, q, k2, v2, out, lse, lo, hi, cap=cap)
+                assert not out[:, :pad].any() and bool((lse[..., :pad] == -float("inf")).all())
+                assert torch.equal(dq[:, :pad], torch.zeros_like(dq[:, :pad]))
+                assert not dk[:, :pad].any() and not dv[:, :pad].any()  # keys of padding, which nobody sees
+                # rows before the key, and the other window, as if it were not there
+                before = slice(0, at if sees == "causal" else pad)
+                for name, got in (("out", out), ("dq", dq)):
+                    want, bound = getattr(ref, name), getattr(ref, name + "_bound")
+                    assert worst(got[0, before], want[0, before], bound[0, before]) <= 1
+                for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+                    assert worst(got[1], getattr(ref, name)[1], getattr(ref, name + "_bound")[1]) <= 1
