@@ -41,7 +41,7 @@ __device__ __forceinline__ void mend_row(const StepArgs &g, int64_t b, int r, in
   if (hi > lo && exact_out<T, MODE>(x, static_cast<const T *>(a.q) + b * a.qs.batch + t * a.qs.token + head * a.qs.head,
                                     static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token,
                                     static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, lo, hi, a.dim,
-                                    a.hi[row] - 1, max_log2 + scores.offset, scores))
+                                    hi - 1, max_log2 + scores.offset, scores))
     store_pair(static_cast<T *>(g.out) + (row * a.heads + head) * a.dim, x, a.dim);
 }
 

@@ -312,3 +312,26 @@ def test_rows_that_see_nothing_get_nothing_beside_rows_that_see_what_is_not_fini
                     assert worst(got[0, before], want[0, before], bound[0, before]) <= 1
                 for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
                     assert worst(got[1], getattr(ref, name)[1], getattr(ref, name + "_bound")[1]) <= 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L", [90, 3000])
+def test_step_whose_ranges_reach_beyond_the_cache_beside_a_key_that_is_not_finite(dtype, L):
+    """Two tokens, of which the second sees a key that is not finite: the first is worked out alone, and its distances count from
+    the last key there is.  (In one part and in several.)"""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(16)
+    B, T, H, HK, D = 2, 2, 4, 2, 64
+    q, k, v = _rows(g, B, T, H, D, dtype), _rows(g, B, L, HK, D, dtype), _rows(g, B, L, HK, D, dtype)
+    slopes = torch.rand(H, generator=g, device="cuda") * 0.5
+    lo = torch.tensor([[50, 0], [50, 50]], dtype=torch.int32, device="cuda")
+    hi = torch.tensor([[L + 7, L + 9], [L + 30, L]], dtype=torch.int32, device="cuda")
+    for cap in (0.0, 5.0):
+        ref = Attention(q, k, v, lo, hi, cap=cap, slopes=slopes, place=hi.clamp(max=L) - 1)
+        v2 = v.clone()
+        v2[0, 40:50] = float("inf")
+        announce("step beyond the cache %s L=%d cap=%g" % (dtype, L, cap))
+        out = ops.range_attention_step(q, k, v2, lo, hi, cap=cap, slopes=slopes)
+        assert worst(out[0, 0], ref.out[0, 0], ref.out_bound[0, 0]) <= 1
+        assert worst(out[1], ref.out[1], ref.out_bound[1]) <= 1
+        assert not torch.isfinite(out[0, 1]).any()
