@@ -26,7 +26,9 @@ int attention_args(const gear_hip_attention_desc *d, AttentionArgs &a) {
   if (d == nullptr || d->batch < 0 || d->queries < 0 || d->keys < 0 || d->heads < 1 || d->kv_heads < 1) return GEAR_HIP_EINVAL;
   if (d->dtype != GEAR_HIP_F16 && d->dtype != GEAR_HIP_BF16) return GEAR_HIP_EINVAL;
   if (d->heads % d->kv_heads != 0 || d->head_dim < 16 || d->head_dim % 16 != 0) return GEAR_HIP_EINVAL;
-  if (!(d->scale > 0) || !(d->scale < 1e30f) || !(d->cap >= 0) || !(d->cap < 1e30f)) return GEAR_HIP_EINVAL;
+  if (!(d->scale > 0) || !(d->scale < 1e30f) || !(d->cap >= 0) || !(d->cap < 1e30f) ||
+      (d->cap > 0 && !(d->scale / d->cap < 1e30f)))
+    return GEAR_HIP_EINVAL;
   if (d->head_dim > 128 || d->queries >= (1 << 30) || d->keys >= (1 << 30) || d->batch >= (1 << 30)) return GEAR_HIP_ERANGE;
   // workgroups of a launch, and rows of the statistics
   if (d->batch * ceil_div64(d->queries, kRows) > INT_MAX / d->heads || d->batch * ceil_div64(d->keys, kRows) > INT_MAX / d->heads)
@@ -95,8 +97,9 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_here, 0, x), q[x], s);
     const float ahead = (float)(place - k0 - 4 * half);
+    scores.cap_far(s);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)));
+    for (int r = 0; r < 16; ++r) s[r] = scores.z(scores.in_tile(s[r]), ahead - (float)(8 * (r >> 2) + (r & 3)));
     if (__builtin_expect(!seen.covers(k0, k0 + kTile), 0)) {
       const uint32_t from_lo = (uint32_t)(k0 + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
 #pragma unroll

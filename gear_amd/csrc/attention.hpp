@@ -253,40 +253,73 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // Scores as exponents of 2: factor * z + offset, where z comes from the product x of the rows.
 //   plain       z = x
-//   kCap        cap tanh(u) = cap (1 - 2 / (1 + e^2u)): z = -1 / (1 + e^2u), in [-1, 0]
+//   kCap        cap tanh(u), u = x scale / cap: z = -1 / (1 + e^2u), in [-1, 0], from tanh(u) = 1 - 2 / (1 + e^2u)
+//   with kFar   z = tanh(u)
 //   kBias       z = x scale log2(e) - slope |distance|, and with the cap the same of the capped score
 // so that a plain or capped score costs no instruction for its scale: it is part of the exponent's
-// multiply-add.  The cap is within 2^-23 cap of the exact one, as 32-bit scores of that size are.
-constexpr int kCap = 1, kBias = 2;
+// multiply-add.
+// The first form of the cap is off by up to 2^-22 cap however small the score is, so it is for caps up to kNearCap: 1.6e-5 at
+// most, which moves p by a thirtieth of its own rounding to fp16.  kFar, for larger caps, takes tanh up to |u| = kSmall
+// as u + u^3 P(u^2), with P fitted to be least off relative to tanh (0.7 units of 2^-24 at most): a score is within a few units of
+// itself whatever the cap.  A tile whose arguments are all that small, as they are where the cap is far above the scores, takes
+// only that.  At a cap of 30 kFar would take 457 / 684 / 1035 us in the three kernels of 32 x 1470 against 432 / 690 / 970, at
+// one of 5, whose tiles hold both kinds of arguments, 580 forward against 431.
+constexpr int kCap = 1, kBias = 2, kFar = 4;
+constexpr float kNearCap = 64.f;
 template <int MODE>
 struct Scores {
+  static constexpr float kSmall = 0.35f;
   float factor, offset, inner, outer, slope;
   // (UNIFORM: one head for the whole wave, its slope in a scalar register)
   template <bool UNIFORM = true>
   __device__ __forceinline__ Scores(const AttentionArgs &a, int head, std::bool_constant<UNIFORM> = {}) {
     const float cap_log2 = a.cap * kLog2e;
-    inner = MODE & kCap ? a.scale / a.cap * (2 * kLog2e) : a.scale_log2;
-    outer = 2 * cap_log2;
+    inner = MODE & kFar ? a.scale / a.cap : MODE & kCap ? a.scale / a.cap * (2 * kLog2e) : a.scale_log2;
+    outer = MODE & kFar ? cap_log2 : 2 * cap_log2;
     slope = MODE & kBias && a.slopes ? a.slopes[head] * kLog2e : 0.f;
     if (MODE & kBias && UNIFORM) slope = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(slope)));
-    factor = MODE == 0 ? a.scale_log2 : MODE == kCap ? outer : 1.f;
-    offset = MODE & kCap ? cap_log2 : 0.f;
+    factor = !(MODE & kCap) ? a.scale_log2 : outer;
+    if (MODE & kBias) factor = 1.f;
+    offset = MODE & kCap && !(MODE & kFar) ? cap_log2 : 0.f;
   }
-  // -1 / (1 + e^2u)
-  __device__ __forceinline__ float capped(float x) const { return __builtin_amdgcn_rcpf(-1.f - exp2_fast(x * inner)); }
-  __device__ __forceinline__ float z(float x, float distance) const {
-    if (MODE == 0) return x;
-    if (MODE == kCap) return capped(x);
-    const float off = -slope * fabsf(distance);
-    return MODE == kBias ? fmaf(x, inner, off) : fmaf(capped(x), outer, off);
+  static __device__ __forceinline__ float tanh_small(float u) {
+    const float w = u * u;
+    return fmaf(u * w, fmaf(fmaf(w, -0.0491485037f, 0.132998258f), w, -0.333326638f), u);
   }
-  // the same, and the derivative of the cap: 1 - tanh^2 = -4 z (1 + z)
-  __device__ __forceinline__ float z(float x, float distance, float &shrink) const {
-    shrink = 1.f;
-    if (!(MODE & kCap)) return z(x, distance);
-    const float c = capped(x);
-    shrink = -4.f * fmaf(c, c, c);
-    return MODE == kCap ? c : fmaf(c, outer, -slope * fabsf(distance));
+  static __device__ __forceinline__ float tanh_any(float u) {
+    const float large = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_fast(u * (2 * kLog2e))), 1.f);
+    return fabsf(u) <= kSmall ? tanh_small(u) : large;
+  }
+  // a product made what z() and shrink() take; with kFar those of a tile before all else
+  __device__ __forceinline__ float capped(float x) const {
+    if (!(MODE & kCap)) return x;
+    return MODE & kFar ? tanh_any(x * inner) : __builtin_amdgcn_rcpf(-1.f - exp2_fast(x * inner));
+  }
+  __device__ __forceinline__ void cap_far(f32x16 &x) const {
+    if (!(MODE & kFar)) return;
+    float most = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] *= inner;
+      most = fmaxf(most, fabsf(x[r]));
+    }
+    if (__builtin_expect(wave_ballot(most > kSmall) == 0, 1)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = tanh_small(x[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = tanh_any(x[r]);
+    }
+  }
+  // (of an element of a tile)
+  __device__ __forceinline__ float in_tile(float x) const { return MODE & kFar ? x : capped(x); }
+  __device__ __forceinline__ float z(float c, float distance) const {
+    if (!(MODE & kBias)) return c;
+    return fmaf(c, MODE & kCap ? outer : inner, -slope * fabsf(distance));
+  }
+  // the derivative of the cap: 1 - tanh^2 = -4 z (1 + z)
+  __device__ __forceinline__ float shrink(float c) const {
+    return !(MODE & kCap) ? 1.f : MODE & kFar ? fmaf(-c, c, 1.f) : -4.f * fmaf(c, c, c);
   }
 };
 
@@ -335,14 +368,19 @@ __device__ __forceinline__ void store_rows(T *piece, f32x16 (&x)[D / 32], float 
 template <typename F>
 void by_attention_type(const AttentionArgs &a, int dtype, const F &f) {
   auto shape = [&](auto dim, auto type) {
-    if (a.slopes == nullptr && !(a.cap > 0))
-      f(dim, type, std::integral_constant<int, 0>());
-    else if (a.slopes == nullptr)
-      f(dim, type, std::integral_constant<int, kCap>());
-    else if (!(a.cap > 0))
-      f(dim, type, std::integral_constant<int, kBias>());
+    auto with = [&](auto bias) {
+      constexpr int kWith = decltype(bias)::value;
+      if (!(a.cap > 0))
+        f(dim, type, std::integral_constant<int, kWith>());
+      else if (a.cap <= kNearCap)
+        f(dim, type, std::integral_constant<int, kWith | kCap>());
+      else
+        f(dim, type, std::integral_constant<int, kWith | kCap | kFar>());
+    };
+    if (a.slopes == nullptr)
+      with(std::integral_constant<int, 0>());
     else
-      f(dim, type, std::integral_constant<int, kCap | kBias>());
+      with(std::integral_constant<int, kBias>());
   };
   auto dims = [&](auto type) {
     if (a.dim <= 32)

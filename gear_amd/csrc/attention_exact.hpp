@@ -82,7 +82,7 @@ __device__ __forceinline__ bool exact_out(Pair &out, const T *q, const T *k, int
   const Pair own = load_pair(q, dim);
   out = Pair{0.f, 0.f};
   for (int j = lo; j < hi; ++j) {
-    const float z = scores.z(dot(own, load_pair(k + j * k_stride, dim)), (float)(place - j));
+    const float z = scores.z(scores.capped(dot(own, load_pair(k + j * k_stride, dim))), (float)(place - j));
     const float p = exp2_fast(fmaf(z, scores.factor, scores.offset - lse_log2));
     const Pair x = load_pair(v + j * v_stride, dim);
     out.x += p * x.x, out.y += p * x.y;
@@ -93,10 +93,9 @@ __device__ __forceinline__ bool exact_out(Pair &out, const T *q, const T *k, int
 // p and the gradient of the score of one pair
 template <int MODE>
 __device__ __forceinline__ float2 exact_pair(float product, float dp, int distance, float lse_log2, float delta, const Scores<MODE> &scores) {
-  float shrink;
-  const float z = scores.z(product, (float)distance, shrink);
-  const float p = exp2_fast(fmaf(z, scores.factor, scores.offset - lse_log2));
-  return make_float2(p, p * (dp - delta) * shrink);
+  const float x = scores.capped(product);
+  const float p = exp2_fast(fmaf(scores.z(x, (float)distance), scores.factor, scores.offset - lse_log2));
+  return make_float2(p, p * (dp - delta) * scores.shrink(x));
 }
 
 // One row of dq, without the scale.

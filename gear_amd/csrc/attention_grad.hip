@@ -120,12 +120,12 @@ __device__ __forceinline__ void by_query(f32x16 &s, f32x16 &dp, float &delta, co
   for (int x = 0; x < D / 16; ++x) dp = mfma(reader.rows(v_tile, row0, x), dout[x], dp);
   const float ahead = (float)(place - kk - 4 * half);
   f32x16 shrink;
+  scores.cap_far(s);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    float of_cap;
-    const float z = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)), of_cap);
+    const float c = scores.in_tile(s[r]), z = scores.z(c, ahead - (float)(8 * (r >> 2) + (r & 3)));
+    shrink[r] = scores.shrink(c);
     s[r] = exp2_fast(fmaf(z, scores.factor, less));
-    shrink[r] = of_cap;
   }
   if (__builtin_expect(!seen.covers(kk, kk + 32), 0)) {
     const uint32_t from_lo = (uint32_t)(kk + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
@@ -179,6 +179,7 @@ __device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D 
   for (int y = 0; y < D / 16; ++y) dp = mfma(reader.rows(g_tile, row0, y), KEEP_V ? v[y] : reader.rows(own_v, 0, y), dp);
   constexpr float lower = 1.f / (1 << (int)kRaise<T>);
   const float distance = (float)(ahead + 4 * half - key);
+  scores.cap_far(s);
 #pragma unroll
   for (int z = 0; z < 4; ++z) {
     const int r0 = row0 + 8 * z + 4 * half;
@@ -186,8 +187,7 @@ __device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = 4 * z + e;
-      float shrink;
-      const float y = scores.z(s[r], distance + (float)(8 * z + e), shrink);
+      const float c = scores.in_tile(s[r]), y = scores.z(c, distance + (float)(8 * z + e)), shrink = scores.shrink(c);
       const float p = exp2_fast(fmaf(y, scores.factor, scores.offset + kRaise<T> - lse[e]));
       float ds = p * (kRaise<T> > 0 ? fmaf(lower, dp[r], -lower * delta[e]) : dp[r] - delta[e]);
       if (MODE & kCap) ds *= shrink;

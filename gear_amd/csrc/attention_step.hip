@@ -97,8 +97,9 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_tile[from_buffer], 0, x), q[x], s);
     const float ahead = (float)(seen.hi - 1 - k0 - 4 * half);
+    scores.cap_far(s);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = scores.z(s[r], ahead - (float)(8 * (r >> 2) + (r & 3)));
+    for (int r = 0; r < 16; ++r) s[r] = scores.z(scores.in_tile(s[r]), ahead - (float)(8 * (r >> 2) + (r & 3)));
     if (__builtin_expect(k0 + kRows > end || !seen.covers(k0, k0 + kRows), 0)) {
       const uint32_t from_lo = (uint32_t)(k0 + 4 * half - seen.lo), count = (uint32_t)(min(seen.hi, end) - seen.lo);
 #pragma unroll

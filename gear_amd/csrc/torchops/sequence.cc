@@ -254,8 +254,9 @@ struct Attention {
     keep[1] = need_like(hi, at::kInt, "hi", device, {batch, queries});
     if (!slopes.is_none()) keep[2] = need_like(slopes, at::kFloat, "slopes", device, {heads});
     const double s = scale.is_none() ? 1.0 / std::sqrt((double)dim) : scale.cast<double>();
-    if (!(s > 0) || !std::isfinite(s)) bad_value("scale must be a number above 0");
-    if (!(cap >= 0) || !std::isfinite(cap)) bad_value("cap must be a number of at least 0 (0: no cap)");
+    if (!((float)s > 0) || !(s < 1e30)) bad_value("scale must be a number above 0 (of 32 bits, below 1e30)");
+    if (!(cap >= 0) || !(cap < 1e30) || (cap > 0 && !(s / cap < 1e30)))
+      bad_value("cap must be a number of at least 0 (0: no cap), below 1e30 and above 1e-30 times the scale");
     d.q = q.ptr(), d.k = k.ptr(), d.v = v.ptr();
     std::copy(q.stride, q.stride + 3, d.q_stride);
     std::copy(k.stride, k.stride + 3, d.k_stride);

@@ -448,7 +448,7 @@ def norm_rotate_append(q, k, v, pos, freqs, sections, q_weight=None, k_weight=No
 def range_attention(q, k, v, lo, hi, *, scale=None, cap=0.0, slopes=None):
     """Softmax attention in which query i sees the keys lo[b, i] <= j < hi[b, i] (int32, as
     token_ranges gives them): (out, lse float32 [batch, heads, queries]).
-    scale: of the products (None: head_dim ** -0.5); cap > 0: scores become cap * tanh(score / cap);
+    scale: of the products (None: head_dim ** -0.5); cap > 0 (below 1e30): scores become cap * tanh(score / cap);
     slopes (float32 [heads]): scores lose slopes[head] * |i + keys - queries - j|.  Queries that see
     nothing get out 0 and lse -inf.  k, v may have fewer heads than q.  float16, bfloat16."""
     return _hostops.range_attention(q, k, v, lo, hi, scale, float(cap), slopes)

@@ -335,3 +335,58 @@ def test_step_whose_ranges_reach_beyond_the_cache_beside_a_key_that_is_not_finit
         assert worst(out[0, 0], ref.out[0, 0], ref.out_bound[0, 0]) <= 1
         assert worst(out[1], ref.out[1], ref.out_bound[1]) <= 1
         assert not torch.isfinite(out[0, 1]).any()
+
+
+@pytest.mark.parametrize("cap", [0.5, 30.0, 64.0, 65.0, 1e3, 1e5, 1e8, 1e29])
+def test_capped_scores_are_as_exact_as_scores(cap):
+    """A query that sees one key: its lse is its score.  q . k has one product, so that what is seen is the scale, the cap
+    and the logarithm's units: a score is off by at most 16 units of 32 bits of ITSELF (its scale 1, the argument and the
+    tanh 8, the exponent's factor 2, the way to base 2 and back 2; the logarithm of a sum of 1: 2e-7).  Caps up to 64 may be
+    off by 2^-22 of the cap on top, 1.6e-5 at most."""
+    from gear_amd import ops
+    T, D = 500, 64
+    announce("capped scores one by one, cap %g" % cap)
+    x = torch.logspace(-4, 4, T, dtype=torch.float64, device="cuda")
+    x = torch.where(torch.arange(T, device="cuda") % 2 == 0, x, -x).bfloat16()
+    q, k = (torch.zeros(1, T, 1, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q[0, :, 0, 5], k[0, :, 0, 5] = x, 1.0
+    lo = torch.arange(T, dtype=torch.int32, device="cuda")[None].contiguous()
+    scale = 0.125
+    for slopes in (None, torch.zeros(1, device="cuda")):
+        _, lse = ops.range_attention(q, k, k, lo, lo + 1, cap=cap, scale=scale, slopes=slopes)
+        want = cap * torch.tanh(x.double() * scale / cap)
+        near = 2.0 ** -22 * cap if cap <= 64 else 0
+        assert bool(((lse[0, 0].double() - want).abs() <= 16 * 2.0 ** -24 * want.abs() + 2e-7 + near).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [30.0, 1e4, 1e6, 1e8, 1e29])
+def test_large_caps(cap, dtype):
+    """A cap far above the scores leaves them as they are: forward, gradients (in one launch and in two) and a step, within
+    the bounds of scores without a cap (whose size is the scores', not the cap's)."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(17)
+    for T, H, HK, D, slopes in ((100, 2, 2, 64, False), (300, 4, 2, 80, True)):
+        q, k, v, dout = (_rows(g, 2, T, h, D, dtype, 1.5) for h in (H, HK, HK, H))
+        lo, hi = _masks("documents", 2, T, T, g)
+        form = dict(slopes=torch.rand(H, generator=g, device="cuda") * 0.1 if slopes else None)
+        announce("cap %g, %s, T=%d" % (cap, dtype, T))
+        ref, free = Attention(q, k, v, lo, hi, cap=cap, dout=dout, **form), Attention(q, k, v, lo, hi, dout=dout, **form)
+        out, lse = ops.range_attention(q, k, v, lo, hi, cap=cap, **form)
+        grads = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi, cap=cap, **form)
+        assert worst(lse, ref.lse, free.lse_bound) <= 1
+        if cap >= 1e4:  # (at 30 the probabilities, and with them the bounds, differ from those without a cap)
+            for name, got in zip(("out", "dq", "dk", "dv"), (out,) + tuple(grads)):
+                assert worst(got, getattr(ref, name), getattr(free, name + "_bound")) <= 1, name
+        place = hi - 1
+        ref, free = Attention(q, k, v, lo, hi, cap=cap, place=place, **form), Attention(q, k, v, lo, hi, place=place, **form)
+        out = ops.range_attention_step(q, k, v, lo, hi, cap=cap, **form)
+        assert worst(out, ref.out, ref.out_bound if cap < 1e4 else free.out_bound) <= 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_caps_that_scores_reach(dtype):
+    """Scores of up to hundreds under caps of their size: tiles hold small arguments of the tanh and large ones."""
+    for cap in (65.0, 200.0):
+        _check(2, 100, 100, 2, 2, 64, dtype, "causal", cap, scale=3.0, seed=20)
+        _check(1, 300, 300, 4, 2, 80, dtype, "documents", cap, True, scale=3.0, seed=21)

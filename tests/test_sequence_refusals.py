@@ -148,3 +148,27 @@ def test_codes_without_a_gpu():
     assert lib.gear_hip_attention_backward_workspace_bytes(2, 100, 4) >= 4 * 2 * 100 * 4 + 2 * 4 * 16
     assert lib.gear_hip_attention_step_workspace_bytes(1, 1, 100, 8, 8, 64) == 0
     assert lib.gear_hip_attention_step_workspace_bytes(1, 1, 100_000, 8, 1, 64) > 0
+
+
+def test_scales_and_caps_that_32_bits_do_not_hold():
+    """By code before the device is touched: a scale and a cap below 1e30, and a scale below 1e30 times the cap."""
+    from gear_amd import _cabi
+    lib = _cabi.load()
+    for scale, cap, code in ((1e30, 0.0, -1), (1.0, 1e30, -1), (1.0, 1e-30, -1), (1e10, 1e-25, -1), (1.0, 1e-29, 0), (1.0, 1e29, 0),
+                             (1e29, 1e29, 0)):
+        att = _cabi.AttentionDesc(batch=0, queries=3, keys=3, heads=2, kv_heads=1, head_dim=32, dtype=1, scale=scale, cap=cap)
+        assert lib.gear_hip_attention(ctypes.byref(att), None, None, None) == code, (scale, cap)
+
+
+@pytest.mark.gpu
+def test_attention_refuses_caps_and_scales_by_name():
+    from gear_amd import ops
+    q, lo = torch.zeros(2, 3, 4, 32, device="cuda").half(), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    for call in (ops.range_attention, ops.range_attention_step):
+        for cap in (1e30, 1e300, 1e-31, 1e-300):
+            with pytest.raises(ValueError, match="cap must be"):
+                call(q, q, q, lo, lo, cap=cap)
+        with pytest.raises(ValueError, match="scale must be"):
+            call(q, q, q, lo, lo, scale=1e30)
+        with pytest.raises(ValueError, match="scale must be"):
+            call(q, q, q, lo, lo, scale=1e-300)
