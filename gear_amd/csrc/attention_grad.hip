@@ -106,10 +106,60 @@ __device__ __forceinline__ void mend_dkv(const GradArgs &g, uint32_t bad, int b,
   }
 }
 
+// ds = p (dp - delta) is as large as the gradients that come in, and those may be anywhere: below 2^-24, where fp16 ends, or beyond
+// 2^16.  So each column of sums (a lane's query, or its key) has ds rounded to fp16 times a power of two of its own, by which
+// |dp - delta| lies below 2^15 and its largest began at 2^8..2^9 (p is at most 1): where a later tile goes beyond that, the power
+// is lowered and the sums with it.  A ds is off by 2^-33 of the largest |dp - delta| at most, which does not depend on the
+// gradients' size.  fp16, 2 x 8193 with a bias: 429 + 725 us, 416 + 704 without; 2048 windows of 90: 369, 366.  bf16 has the
+// exponents of 32 bits: there this is nothing.
+template <typename T>
+struct Lift {
+  static constexpr bool kOn = std::is_same<T, f16>::value;
+  int e = 0;          // the power is 2^e
+  float limit = 0.f;  // of |dp - delta|
+  __device__ __forceinline__ float power() const { return kOn ? __builtin_ldexpf(1.f, e) : 1.f; }
+  __device__ __forceinline__ float back() const { return kOn ? __builtin_ldexpf(1.f, -e) : 1.f; }
+  static __device__ __forceinline__ int power_of(float top) { return min(9 - __builtin_amdgcn_frexp_expf(top), 100); }
+  // top: the largest of a tile's that the lane has
+  __device__ __forceinline__ bool beyond(float top) const { return kOn && wave_ballot(top > limit) != 0; }
+  template <int N>
+  __device__ __forceinline__ void lower(float top, f32x16 (&sums)[N]) {
+    top = max_of_halves(top);
+    const bool beyond = top > limit && top < INFINITY;
+    const int to = beyond ? power_of(top) : e;
+    const float by = __builtin_ldexpf(1.f, to - e);
+    limit = beyond ? __builtin_ldexpf(1.f, 15 - to) : limit;
+    e = to;
+#pragma unroll
+    for (int x = 0; x < N; ++x) sums[x] *= by;
+  }
+};
+__device__ __forceinline__ float largest(const f32x16 &x) {
+  float top = 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+  return top;
+}
+
+// What by_query() does with the largest |dp| that a row sees of a tile: has the row's sums follow it, or keeps it.
+template <typename T, int N>
+struct Follow {
+  Lift<T> &lift;
+  f32x16 (&sums)[N];
+  float delta;  // its size
+  __device__ __forceinline__ void saw(float top) const {
+    if (__builtin_expect(lift.beyond(top + delta), 0)) lift.lower(top + delta, sums);
+  }
+};
+struct Keep {
+  float &most;
+  __device__ __forceinline__ void saw(float top) const { most = fmaxf(most, top); }
+};
+
 // 32 keys (rows `row0`.. of the tiles, kk.. in memory) by the wave's 32 queries, a lane a query: s, the probabilities times
 // the cap's derivative, and dp; `delta` gains the lane's share of sum p dp.
-template <typename T, int D, int MODE>
-__device__ __forceinline__ void by_query(f32x16 &s, f32x16 &dp, float &delta, const T *k_tile, const T *v_tile, int row0, int kk,
+template <typename T, int D, int MODE, typename F>
+__device__ __forceinline__ void by_query(f32x16 &s, f32x16 &dp, float &delta, const F &of_row, const T *k_tile, const T *v_tile, int row0, int kk,
                                          const vec8<T> (&q)[D / 16], const vec8<T> (&dout)[D / 16], const TileReader<T, D> &reader,
                                          const Scores<MODE> &scores, const Seen &seen, int place, float less) {
   const int half = lane_id() >> 5;
@@ -127,13 +177,16 @@ __device__ __forceinline__ void by_query(f32x16 &s, f32x16 &dp, float &delta, co
     shrink[r] = scores.shrink(c);
     s[r] = exp2_fast(fmaf(z, scores.factor, less));
   }
+  float top = Lift<T>::kOn ? largest(dp) : 0;
   if (__builtin_expect(!seen.covers(kk, kk + 32), 0)) {
     const uint32_t from_lo = (uint32_t)(kk + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
 #pragma unroll
     for (int r = 0; r < 16; ++r)
       if (from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) >= count) s[r] = dp[r] = shrink[r] = 0;
+    if (Lift<T>::kOn) top = largest(dp);
     asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
   }
+  of_row.saw(top);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     delta += s[r] * dp[r];
@@ -167,7 +220,7 @@ struct __attribute__((aligned(16))) QueryRows {
 // dk += ds^T q.
 // KEEP_V: V's operands are in v, else in LDS, the wave's 32 rows at own_v.
 template <bool KEEP_V, typename T, int D, int MODE, int N>
-__device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], const T *q_tile, const T *g_tile, int row0,
+__device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], Lift<T> &lift, const T *q_tile, const T *g_tile, int row0,
                                            const QueryRows<N> &rows, const vec8<T> (&k)[D / 16], const vec8<T> (&v)[D / 16],
                                            const T *own_v, const TileReader<T, D> &reader, const Scores<MODE> &scores, int ahead, int key,
                                            bool whole) {
@@ -177,7 +230,6 @@ __device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D 
   for (int y = 0; y < D / 16; ++y) s = mfma(reader.rows(q_tile, row0, y), k[y], s);
 #pragma unroll
   for (int y = 0; y < D / 16; ++y) dp = mfma(reader.rows(g_tile, row0, y), KEEP_V ? v[y] : reader.rows(own_v, 0, y), dp);
-  constexpr float lower = 1.f / (1 << (int)kRaise<T>);
   const float distance = (float)(ahead + 4 * half - key);
   scores.cap_far(s);
 #pragma unroll
@@ -189,11 +241,13 @@ __device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D 
       const int r = 4 * z + e;
       const float c = scores.in_tile(s[r]), y = scores.z(c, distance + (float)(8 * z + e)), shrink = scores.shrink(c);
       const float p = exp2_fast(fmaf(y, scores.factor, scores.offset + kRaise<T> - lse[e]));
-      float ds = p * (kRaise<T> > 0 ? fmaf(lower, dp[r], -lower * delta[e]) : dp[r] - delta[e]);
+      float ds = dp[r] - delta[e];
+      if (!Lift<T>::kOn) ds *= p;
       if (MODE & kCap) ds *= shrink;
       s[r] = p, dp[r] = ds;
     }
   }
+  float top = Lift<T>::kOn ? largest(dp) : 0;
   if (__builtin_expect(!whole, 0)) {
 #pragma unroll
     for (int z = 0; z < 4; ++z) {
@@ -203,7 +257,14 @@ __device__ __forceinline__ void add_by_key(f32x16 (&dk)[D / 32], f32x16 (&dv)[D 
       for (int e = 0; e < 4; ++e)
         if ((uint32_t)(key - lo[e]) >= (uint32_t)(hi[e] - lo[e])) s[4 * z + e] = dp[4 * z + e] = 0;
     }
+    if (Lift<T>::kOn) top = largest(dp);
     asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
+  }
+  if (__builtin_expect(lift.beyond(top), 0)) lift.lower(top, dk);
+  if (Lift<T>::kOn) {
+    const float power = __builtin_ldexpf(1.f, lift.e - (int)kRaise<T>);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] *= power * s[r];
   }
   add_columns<T, D>(dv, g_tile, row0, s, reader);
   add_columns<T, D>(dk, q_tile, row0, dp, reader);
@@ -259,6 +320,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   const float less = scores.offset - lse_log2;
   const int place = i + a.keys - a.queries;
   f32x16 dq[D / 32] = {};
+  Lift<T> lift;
   float summed = 0;  // sum p dp: what delta is, without the rounding of out
   const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
@@ -278,9 +340,9 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
       const int kk = k0 + kb * 32;
       if (!seen.touches(kk, kk + 32)) continue;
       f32x16 s, dp;
-      by_query<T, D, MODE>(s, dp, summed, k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less);
+      by_query<T, D, MODE>(s, dp, summed, Follow<T, D / 32>{lift, dq, fabsf(delta)}, k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+      for (int r = 0; r < 16; ++r) s[r] *= Lift<T>::kOn ? fmaf(dp[r], lift.power(), -delta * lift.power()) : dp[r] - delta;
       add_columns<T, D>(dq, k_here, kb * 32, s, reader);
     }
   }
@@ -291,7 +353,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   }
   __syncthreads();
   const uint32_t bad = columns_not_finite(dq, !seen.empty());
-  store_rows<T, D>(k_tile[0] + wave * kRows * D, dq, a.scale, seen.empty(), a.dim, [&](int r) {
+  store_rows<T, D>(k_tile[0] + wave * kRows * D, dq, a.scale * lift.back(), seen.empty(), a.dim, [&](int r) {
     return i0 + r < a.queries ? static_cast<T *>(g.dq) + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
   });
   if (__builtin_expect(bad != 0, 0)) mend_dq<T, MODE>(g, bad, b, head, kv_head, i0, seen, lse_log2, delta, scores);
@@ -328,6 +390,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
     wave_lds_sync();
   }
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  Lift<T> lift;
   const int groups = g.padded / kRows, tiles = (a.queries + kTile - 1) / kTile;
   // (read through the scalar cache: the launch before wrote them)
   typedef const __attribute__((address_space(4))) i32x4 *Bounds;
@@ -398,7 +461,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
 #pragma unroll
     for (int y = 0; y < kSides; ++y) {
       if (reach[y][0] >= wave_key + kRows || reach[y][1] <= wave_key) continue;
-      add_by_key<kKeepV, T, D, MODE>(dk, dv, q_tile[buffer], g_tile[buffer], y * kRows, rows[buffer], k, v, own_v, reader, scores,
+      add_by_key<kKeepV, T, D, MODE>(dk, dv, lift, q_tile[buffer], g_tile[buffer], y * kRows, rows[buffer], k, v, own_v, reader, scores,
                                      i0 + y * kRows + a.keys - a.queries, key,
                                      reach[y][2] <= wave_key && reach[y][3] >= wave_key + kRows);
     }
@@ -411,7 +474,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(GradArgs g) 
   };
   const uint32_t bad = columns_not_finite(dk, key_there) | columns_not_finite(dv, key_there);
   // (the 4 x 32 rows of dk fill both tiles of q, those of dv the tiles of dout or what was V)
-  store_rows<T, D>(kKeepV ? q_tile[0] + wave * kRows * D : own_v, dk, a.scale, false, a.dim, to(g.dk));
+  store_rows<T, D>(kKeepV ? q_tile[0] + wave * kRows * D : own_v, dk, a.scale * lift.back(), false, a.dim, to(g.dk));
   wave_lds_sync();
   store_rows<T, D>(kKeepV ? g_tile[0] + wave * kRows * D : own_v, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv));
   if (__builtin_expect(bad != 0, 0))
@@ -495,27 +558,30 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
   {
     const float less = scores.offset - lse_log2;
     const int place = mine + a.keys - a.queries;
-    float delta = 0;
+    float delta = 0, most = 0;
     f32x16 s[WAVES], dp[WAVES];
     take(q_tile, g_tile);
 #pragma unroll
     for (int x = 0; x < WAVES; ++x)
       if (seen.touches(x * kRows, x * kRows + kRows))
-        by_query<T, D, MODE>(s[x], dp[x], delta, k_tile, v_tile, x * kRows, x * kRows, u, w, reader, scores, seen, place, less);
+        by_query<T, D, MODE>(s[x], dp[x], delta, Keep{most}, k_tile, v_tile, x * kRows, x * kRows, u, w, reader, scores, seen, place, less);
     delta = seen.empty() ? 0.f : sum_of_halves(delta);
     if (half == 0) rows.delta[mine] = delta;
     f32x16 dq[D / 32] = {};
+    Lift<T> lift;  // (all of the row's dp are known)
+    lift.e = Lift<T>::power_of(max_of_halves(most) + fabsf(delta));
 #pragma unroll
     for (int x = 0; x < WAVES; ++x)
       if (seen.touches(x * kRows, x * kRows + kRows)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[x][r] *= dp[x][r] - delta;
+        for (int r = 0; r < 16; ++r)
+          s[x][r] *= Lift<T>::kOn ? fmaf(dp[x][r], lift.power(), -delta * lift.power()) : dp[x][r] - delta;
         add_columns<T, D>(dq, k_tile, x * kRows, s[x], reader);
       }
     bad_dq = columns_not_finite(dq, !seen.empty()), own_delta = delta;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
-      dq[db] *= a.scale;
+      dq[db] *= a.scale * lift.back();
       if (empties != 0) {  // (p = 0 is not enough where a key that others see is not finite)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[db][r] = seen.empty() ? 0.f : dq[db][r];
@@ -534,16 +600,17 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
   wave_lds_sync();  // nobody reads the wave's rows of K any more
   store_packed<T, D>(k_tile + own * D, dq_kept, a.dim, to(g.dq, a.queries));
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  Lift<T> lift;
 #pragma unroll 1
   for (int qb = 0; qb < WAVES; ++qb) {
     const i32x4 reach = bounds[qb];
     if (__builtin_amdgcn_readfirstlane(reach[0]) >= own + kRows || __builtin_amdgcn_readfirstlane(reach[1]) <= own) continue;
     const bool whole = __builtin_amdgcn_readfirstlane(reach[2]) <= own && __builtin_amdgcn_readfirstlane(reach[3]) >= own + kRows;
-    add_by_key<true, T, D, MODE>(dk, dv, q_tile, g_tile, qb * kRows, rows, u, w, nullptr, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
+    add_by_key<true, T, D, MODE>(dk, dv, lift, q_tile, g_tile, qb * kRows, rows, u, w, nullptr, reader, scores, qb * kRows + a.keys - a.queries, mine, whole);
   }
   const uint32_t bad = columns_not_finite(dk, mine < a.keys) | columns_not_finite(dv, mine < a.keys);
   wave_lds_sync();
-  store_rows<T, D>(k_tile + own * D, dk, a.scale, false, a.dim, to(g.dk, a.keys));
+  store_rows<T, D>(k_tile + own * D, dk, a.scale * lift.back(), false, a.dim, to(g.dk, a.keys));
   store_rows<T, D>(v_tile + own * D, dv, 1.f / (1 << (int)kRaise<T>), false, a.dim, to(g.dv, a.keys));
   if (__builtin_expect(bad_dq != 0, 0)) mend_dq<T, MODE>(g, bad_dq, b, head, head, own, seen, lse_log2, own_delta, scores);
   if (__builtin_expect(bad != 0, 0))

@@ -390,3 +390,32 @@ def test_large_caps_that_scores_reach(dtype):
     for cap in (65.0, 200.0):
         _check(2, 100, 100, 2, 2, 64, dtype, "causal", cap, scale=3.0, seed=20)
         _check(1, 300, 300, 4, 2, 80, dtype, "documents", cap, True, scale=3.0, seed=21)
+
+
+@pytest.mark.parametrize("raised", ["q", "k"])
+@pytest.mark.parametrize("sizes", [(2000, 4, 2, 64), (2000, 2, 2, 128), (120, 2, 2, 64)])
+@pytest.mark.parametrize("exponent", [-16, 0, 8])
+def test_gradients_of_any_size_in_float16(exponent, sizes, raised):
+    """Gradients are linear in dout: with dout 2^e as large (exactly) they are 2^e as large, in float16 as far as the results
+    themselves can be held: a result's own step is 2^-25 at most.  q 32 times and k a 32nd as large, or the other way round,
+    so that the scores are the same and dk, or dq, is large enough to be held at 2^-16."""
+    from gear_amd import ops
+    T, H, HK, D = sizes
+    g = torch.Generator(device="cuda").manual_seed(18)
+    q, k, v = (_rows(g, 1, T, h, D, torch.float16) for h in (H, HK, HK))
+    q, k = (q * 32, k / 32) if raised == "q" else (q / 32, k * 32)
+    dout = (torch.randn(1, T, H, D, generator=g, device="cuda") * 8).round().clamp(-16, 16) / 8  # (exact at all three sizes)
+    lo, hi = _masks("all", 1, T, T, g)
+    announce("gradients of float16, 2^%d, T=%d D=%d, %s raised" % (exponent, T, D, raised))
+    ref = Attention(q, k, v, lo, hi, dout=dout.half())
+    out, lse = ops.range_attention(q, k, v, lo, hi)
+    grads = ops.range_attention_backward((dout * 2.0 ** exponent).half(), q, k, v, out, lse, lo, hi)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        bound = getattr(ref, name + "_bound") + 2.0 ** (-25 - exponent)
+        assert worst(got.double() * 2.0 ** -exponent, getattr(ref, name), bound) <= 1, name
+    # norm of the difference over the norm: a rounding of ds and one of the result, each 2^-11 / sqrt(3) at most
+    # (rounding is evenly spread), delta's from out of about as much: 2^-10 holds all; what a step of 2^-25 leaves on top
+    name, got = ("dk", grads[1]) if raised == "q" else ("dq", grads[0])
+    want = getattr(ref, name)
+    off = (got.double() * 2.0 ** -exponent - want).norm()
+    assert float(off) <= 2.0 ** -10 * float(want.norm()) + 2.0 ** (-25 - exponent) * want.numel() ** 0.5
