@@ -83,7 +83,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
   const TileReader<T, D> reader;
   const int place = i + a.keys - a.queries;
   f32x16 o[D / 32] = {};
-  float m = -INFINITY, sum = 0;  // m: of z
+  float m = -INFINITY;  // of z
+  Sum sums;
 
   const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
@@ -116,16 +117,18 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
       const float grown = fmaxf(m, top);
       const float rescale = grown == -INFINITY ? 1.f : exp2_fast((m - grown) * scores.factor);
       m = grown;
-      sum *= rescale;
+      sums.scale(rescale);
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
     }
     const float from = m == -INFINITY ? 0.f : -m * scores.factor;  // (no key seen yet)
+    float of_tile = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       s[r] = exp2_fast(fmaf(s[r], scores.factor, from));
-      sum += s[r];
+      of_tile += s[r];
     }
+    sums.add(of_tile);
     const vec8<T> p0 = packed<T, 0>(s), p1 = packed<T, 1>(s);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
@@ -147,7 +150,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
     tile(k0 + kTile, k_tile[1], v_tile[1]);
   }
 
-  sum = sum_of_halves(sum);
+  const float sum = sum_of_halves(sums.x);
   const bool empty = seen.empty();
   const float lse_log2 = m * scores.factor + scores.offset + __builtin_log2f(sum);
   if (lse != nullptr && half == 0 && row_there)

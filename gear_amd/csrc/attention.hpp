@@ -323,6 +323,19 @@ struct Scores {
   }
 };
 
+// The sum of p along a row: a tile's first, then with what the sum so far has no bits for carried on, so that a key with most of
+// the weight does not swallow thousands that have little.
+struct Sum {
+  float x = 0, over = 0;
+  __device__ __forceinline__ void add(float y) {
+    y -= over;
+    const float to = x + y;
+    over = (to - x) - y;
+    x = to;
+  }
+  __device__ __forceinline__ void scale(float by) { x *= by, over *= by; }
+};
+
 // Workgroups go round the 8 dies: neighbours in this numbering share a die, and its cache.
 __device__ __forceinline__ int same_die_index() {
   const int n = gridDim.x, per = n / 8, rest = n % 8, die = blockIdx.x % 8;

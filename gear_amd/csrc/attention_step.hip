@@ -84,7 +84,8 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
   const Scores<MODE> scores(a, row_there ? head : 0, std::false_type());
   const TileReader<T, D> reader;
   f32x16 o[D / 32] = {};
-  float m = -INFINITY, sum = 0;  // m: of z
+  float m = -INFINITY;  // of z
+  Sum sums;
   const Stage<T, D, kRows, true> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kRows, true> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
   constexpr int kStep = kWaves * kRows;
@@ -116,16 +117,18 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
       const float grown = fmaxf(m, top);
       const float rescale = grown == -INFINITY ? 1.f : exp2_fast((m - grown) * scores.factor);
       m = grown;
-      sum *= rescale;
+      sums.scale(rescale);
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
     }
     const float from = m == -INFINITY ? 0.f : -m * scores.factor;
+    float of_tile = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       s[r] = exp2_fast(fmaf(s[r], scores.factor, from));
-      sum += s[r];
+      of_tile += s[r];
     }
+    sums.add(of_tile);
     const vec8<T> p0 = packed<T, 0>(s), p1 = packed<T, 1>(s);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) {
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
     tile(k0, buffer);
     if (k0 + 2 * kStep < end) ask(k0 + 2 * kStep, buffer);
   }
-  sum = sum_of_halves(sum);
+  const float sum = sum_of_halves(sums.x);
 
   // join the waves (each reads and writes its own memory until here)
   m = m == -INFINITY ? m : m * scores.factor;

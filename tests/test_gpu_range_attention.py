@@ -1,5 +1,6 @@
 """Attention over ranges of keys, forward, backward and over caches, against 64 bits."""
 import itertools
+import math
 
 import pytest
 
@@ -419,3 +420,21 @@ def test_gradients_of_any_size_in_float16(exponent, sizes, raised):
     want = getattr(ref, name)
     off = (got.double() * 2.0 ** -exponent - want).norm()
     assert float(off) <= 2.0 ** -10 * float(want.norm()) + 2.0 ** (-25 - exponent) * want.numel() ** 0.5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_key_with_most_of_the_weight_does_not_swallow_the_others(dtype):
+    """One key with nearly all of the weight, first, in the middle or last, 50 000 with 2^-25.5 of it each: their thousandth is part of
+    the sum, in 32 bits.  (The bound of lse has no term for the number of keys.)"""
+    from gear_amd import ops
+    S, D = 50000, 32
+    announce("a key with most of the weight, %s" % dtype)
+    q, k, v = (torch.zeros(1, n, 1, D, dtype=dtype, device="cuda") for n in (1, S, S))
+    q[..., 0] = 1.0
+    lo, hi = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.full((1, 1), S, dtype=torch.int32, device="cuda")
+    for at in (0, 777, S - 1):
+        k.zero_()
+        k[:, at, :, 0] = 25.5 * math.log(2)
+        ref = Attention(q, k, v, lo, hi, scale=1.0)
+        _, lse = ops.range_attention(q, k, v, lo, hi, scale=1.0)
+        assert worst(lse, ref.lse, ref.lse_bound) <= 1
