@@ -121,7 +121,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
     }
-    const float from = m == -INFINITY ? 0.f : -m * scores.factor;  // (no key seen yet)
+    const float from = m == -INFINITY ? 0.f : kLevel<T> - m * scores.factor;  // (no key seen yet)
     float of_tile = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
 
   const float sum = sum_of_halves(sums.x);
   const bool empty = seen.empty();
-  const float lse_log2 = m * scores.factor + scores.offset + __builtin_log2f(sum);
+  const float lse_log2 = m * scores.factor + scores.offset + __builtin_log2f(sum * (1.f / (1 << (int)kLevel<T>)));
   if (lse != nullptr && half == 0 && row_there)
     lse[((int64_t)b * a.heads + head) * a.queries + i] = empty ? -INFINITY : lse_log2 * kLn2;
   uint32_t bad = columns_not_finite(o, !empty);

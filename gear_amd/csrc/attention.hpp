@@ -336,6 +336,12 @@ struct Sum {
   __device__ __forceinline__ void scale(float by) { x *= by, over *= by; }
 };
 
+// What p is times, in exponents of 2, where it is rounded for its product with V: a maximum that is up to 2^8 behind leaves fp16 room
+// for 2^7, and what is below 2^-25 of that, 2^-32 of the largest p, is lost, not 2^-25 of it: over 131071 keys 2^-15 of the weight
+// at most.  (It is taken off again by the sum, which has it too.)
+template <typename T>
+constexpr float kLevel = std::is_same<T, f16>::value ? 7.f : 0.f;
+
 // Workgroups go round the 8 dies: neighbours in this numbering share a die, and its cache.
 __device__ __forceinline__ int same_die_index() {
   const int n = gridDim.x, per = n / 8, rest = n % 8, die = blockIdx.x % 8;

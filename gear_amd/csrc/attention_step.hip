@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] *= rescale;
     }
-    const float from = m == -INFINITY ? 0.f : -m * scores.factor;
+    const float from = m == -INFINITY ? 0.f : kLevel<T> - m * scores.factor;
     float of_tile = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
   const float sum = sum_of_halves(sums.x);
 
   // join the waves (each reads and writes its own memory until here)
-  m = m == -INFINITY ? m : m * scores.factor;
+  m = m == -INFINITY ? m : m * scores.factor - kLevel<T>;
   float *own_sums = reinterpret_cast<float *>(memory[wave]);
   wave_lds_sync();
 #pragma unroll

@@ -438,3 +438,22 @@ def test_a_key_with_most_of_the_weight_does_not_swallow_the_others(dtype):
         ref = Attention(q, k, v, lo, hi, scale=1.0)
         _, lse = ops.range_attention(q, k, v, lo, hi, scale=1.0)
         assert worst(lse, ref.lse, ref.lse_bound) <= 1
+
+
+def test_many_small_probabilities_in_float16():
+    """One key with nearly all of the weight and v = 0, 50 000 with 2^-25.5 of it each and v = 1: together they are a thousandth.
+    A probability is held to half a step, 2^-32 of the largest at most (bound), whatever its own size."""
+    from gear_amd import ops
+    S, D = 50000, 32
+    announce("many small probabilities")
+    q, k, v = (torch.zeros(1, n, 1, D, dtype=torch.float16, device="cuda") for n in (1, S, S))
+    q[..., 0] = 1.0
+    k[:, 777, :, 0] = 25.5 * math.log(2)
+    v[...] = 1.0
+    v[:, 777] = 0.0
+    lo, hi = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.full((1, 1), S, dtype=torch.int32, device="cuda")
+    ref = Attention(q, k, v, lo, hi, scale=1.0)
+    bound = 2 * 2.0 ** -11 * ref.out + 2.0 ** -32 * S + 1e-5 * ref.out
+    out, lse = ops.range_attention(q, k, v, lo, hi, scale=1.0)
+    assert worst(out, ref.out, bound) <= 1 and worst(lse, ref.lse, ref.lse_bound) <= 1
+    assert worst(ops.range_attention_step(q, k, v, lo, hi, scale=1.0), ref.out, bound) <= 1
