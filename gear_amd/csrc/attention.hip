@@ -86,7 +86,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
   float m = -INFINITY;  // of z
   Sum sums;
 
-  const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+  const Stage<T, D, kTile, false, true> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
   auto load = [&](int k0, T *k_to, T *v_to) {
     k_rows.template ask<WAVES>(k_to, k0, wave);
@@ -137,6 +137,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_kernel(AttentionArg
     }
   };
   int k0 = first < end ? first / kTile * kTile : 0;
+  for (int x = wave; x < 2; x += WAVES) k_rows.clear_beyond(k_tile[x]);
   if (k0 < end) load(k0, k_tile[0], v_tile[0]);
   for (; k0 < end; k0 += 2 * kTile) {
     staged_wait();

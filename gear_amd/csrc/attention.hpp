@@ -137,9 +137,11 @@ __device__ __forceinline__ void own_row_frags(vec8<T> (&f)[D / 16], const T *row
 // beyond `dim` by the last: what a tile holds there is finite wherever the rows in range are, and multiplied
 // by zeros only.  A tile is complete after staged_wait() in every wave and a barrier.
 // ONCE: what nobody reads again is loaded past the caches.
+// KEYS: pieces beyond `dim` are left as clear_beyond() made them, once for all that the tile is asked for: a key's last piece may
+// be infinite, and that times the zeros of a query would be NaN where the score is -inf.
 // The instruction is written out because the compiler, which cannot tell the tile that is asked for from
 // the one that is read meanwhile, has every read of LDS behind its builtin wait for the memory.
-template <typename T, int D, int ROWS, bool ONCE = false>
+template <typename T, int D, int ROWS, bool ONCE = false, bool KEYS = false>
 struct Stage {
   static constexpr int kPieces = D / 8, kRowsEach = kWave / kPieces, kCount = ROWS / kRowsEach;
   const T *base;
@@ -153,17 +155,17 @@ struct Stage {
     for (int odd = 0; odd < 2; ++odd) offset[odd] = (lane / kPieces) * stride + piece(odd) * 8;
   }
   // (rows of an instruction differ from those of the next but one by a multiple of 8: the same swizzle)
-  __device__ __forceinline__ int piece(int x) const {
-    return min((lane % kPieces) ^ swizzle<D>(x * kRowsEach + lane / kPieces), dim / 8 - 1);
-  }
-  __device__ __forceinline__ void one(const T *from, uint32_t at) const {
+  __device__ __forceinline__ int own_piece(int x) const { return (lane % kPieces) ^ swizzle<D>(x * kRowsEach + lane / kPieces); }
+  __device__ __forceinline__ int piece(int x) const { return min(own_piece(x), dim / 8 - 1); }
+  __device__ __forceinline__ void one(const T *from, uint32_t at, int x) const {
+    if (KEYS && own_piece(x & 1) >= dim / 8) return;
     const uint32_t m0 = __builtin_amdgcn_readfirstlane(at);
     if (ONCE)
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(m0) : "memory", "m0");
     else
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
   }
-  // pieces beyond dim, which repeat the last, made zeros: for the operand that has to be (once complete)
+  // pieces beyond dim made zeros, by one wave: for the operand that has to be (once complete, or with KEYS before it is asked for)
   __device__ __forceinline__ void clear_beyond(T *tile) const {
     const int extra = kPieces - dim / 8;
     for (int x = lane_id(); x < ROWS * extra; x += kWave)
@@ -179,13 +181,13 @@ struct Stage {
       for (int y = 0; y < (kCount + WAVES - 1) / WAVES; ++y) {
         const int x = wave + y * WAVES;
         if ((y + 1) * WAVES > kCount && x >= kCount) break;
-        one(base + (int64_t)(row0 + x * kRowsEach) * stride + ((x & 1) ? offset[1] : offset[0]), at + y * kNext);
+        one(base + (int64_t)(row0 + x * kRowsEach) * stride + ((x & 1) ? offset[1] : offset[0]), at + y * kNext, x);
       }
     } else {
 #pragma unroll 1
       for (int x = wave, to = at; x < kCount; x += WAVES, to += kNext) {
         const int row = row0 + x * kRowsEach + lane / kPieces;
-        one(base + (int64_t)min(max(row, first), end - 1) * stride + piece(x) * 8, to);
+        one(base + (int64_t)min(max(row, first), end - 1) * stride + piece(x) * 8, to, x);
       }
     }
   }

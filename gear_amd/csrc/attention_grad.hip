@@ -322,13 +322,14 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   f32x16 dq[D / 32] = {};
   Lift<T> lift;
   float summed = 0;  // sum p dp: what delta is, without the rounding of out
-  const Stage<T, D, kTile> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+  const Stage<T, D, kTile, false, true> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kTile> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
   auto load = [&](int k0, int to) __attribute__((always_inline)) {
     k_rows.template ask<WAVES>(k_tile[to], k0, wave);
     v_rows.template ask<WAVES>(v_tile[to], k0, wave);
   };
   int k0 = first < end ? first / kTile * kTile : 0, buffer = 0;
+  for (int x = wave; x < 2; x += WAVES) k_rows.clear_beyond(k_tile[x]);
   if (k0 < end) load(k0, 0);
   for (; k0 < end; k0 += kTile, buffer ^= 1) {
     staged_wait();
@@ -525,8 +526,9 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_window_grad_kernel(
   for (int w = 0; w < WAVES; ++w) first = min(first, bounds[w][0]), end = max(end, bounds[w][1]);
   first = __builtin_amdgcn_readfirstlane(first), end = __builtin_amdgcn_readfirstlane(end);
   if (first < end) {
-    const Stage<T, D, kRows> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + head * a.ks.head, a.ks.token, first, end, a.dim);
+    const Stage<T, D, kRows, false, true> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + head * a.ks.head, a.ks.token, first, end, a.dim);
     const Stage<T, D, kRows> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + head * a.vs.head, a.vs.token, first, end, a.dim);
+    k_rows.clear_beyond(k_tile + own * D);
     k_rows.template ask<1>(k_tile + own * D, own, 0);
     v_rows.template ask<1>(v_tile + own * D, own, 0);
   }

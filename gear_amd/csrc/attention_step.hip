@@ -45,7 +45,9 @@ __device__ __forceinline__ void mend_row(const StepArgs &g, int64_t b, int r, in
     store_pair(static_cast<T *>(g.out) + (row * a.heads + head) * a.dim, x, a.dim);
 }
 
-template <typename T, int D, int MODE>
+// WHOLE: rows have D elements.  (Chosen inside the kernel, that costs a wave that is alone on its SIMD 5 %: 3 rollouts of up to 131071
+// keys 68 us for 64.)
+template <typename T, int D, int MODE, bool WHOLE>
 __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g) {
   constexpr int kAsks = D / 8;  // instructions that ask for a tile of K and V
   constexpr size_t kTileBytes = sizeof(T) * kRows * D, kJoinBytes = sizeof(float) * kRows * D;
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
   f32x16 o[D / 32] = {};
   float m = -INFINITY;  // of z
   Sum sums;
-  const Stage<T, D, kRows, true> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
+  const Stage<T, D, kRows, true, !WHOLE> k_rows(static_cast<const T *>(a.k) + b * a.ks.batch + kv_head * a.ks.head, a.ks.token, first, end, a.dim);
   const Stage<T, D, kRows, true> v_rows(static_cast<const T *>(a.v) + b * a.vs.batch + kv_head * a.vs.head, a.vs.token, first, end, a.dim);
   constexpr int kStep = kWaves * kRows;
   auto ask = [&](int k0, int to) __attribute__((always_inline)) {
@@ -137,6 +139,8 @@ __global__ __launch_bounds__(kThreads, 1) void attention_step_kernel(StepArgs g)
     }
   };
   int k0 = first + wave * kRows;
+  if (!WHOLE)
+    for (int x = 0; x < 2; ++x) k_rows.clear_beyond(k_tile[x]);
   if (k0 < end) ask(k0, 0);
   if (k0 + kStep < end) ask(k0 + kStep, 1);
   for (int buffer = 0; k0 < end; k0 += kStep, buffer ^= 1) {
@@ -298,8 +302,15 @@ extern "C" int gear_hip_attention_step(const gear_hip_attention_desc *desc, void
   g.out = out;
   by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
-    hipLaunchKernelGGL((attention_step_kernel<T, decltype(dim)::value, decltype(mode)::value>),
-                       dim3((unsigned)workgroups), dim3(kThreads), 0, as_stream(stream), g);
+    constexpr int D = decltype(dim)::value, kMode = decltype(mode)::value;
+    auto step = [&](auto whole) {
+      hipLaunchKernelGGL((attention_step_kernel<T, D, kMode, decltype(whole)::value>), dim3((unsigned)workgroups), dim3(kThreads), 0,
+                         as_stream(stream), g);
+    };
+    if (a.dim == D)
+      step(std::true_type());
+    else
+      step(std::false_type());
     if (g.splits > 1)
       hipLaunchKernelGGL((attention_join_kernel<T, decltype(mode)::value>), dim3((unsigned)(a.queries * a.heads * a.batch)), dim3(kThreads), 0,
                          as_stream(stream), g);

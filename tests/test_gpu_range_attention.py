@@ -5,7 +5,7 @@ import math
 import pytest
 
 from conftest import announce
-from sequence_reference import Attention, worst
+from sequence_reference import UNIT, Attention, worst
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -457,3 +457,45 @@ def test_many_small_probabilities_in_float16():
     out, lse = ops.range_attention(q, k, v, lo, hi, scale=1.0)
     assert worst(out, ref.out, bound) <= 1 and worst(lse, ref.lse, ref.lse_bound) <= 1
     assert worst(ops.range_attention_step(q, k, v, lo, hi, scale=1.0), ref.out, bound) <= 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 112, 128])
+def test_a_score_of_minus_infinity_is_a_probability_of_zero(D, dtype):
+    """Keys that hold -inf where every query is positive, in the first and in the last elements of a row: rows see them with
+    p = 0, as the formula says, and dv of such a key is 0."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(19)
+    for T, H, HK in ((70, 2, 2), (150, 4, 2)):
+        for at in (1, D - 2):
+            q, k, v, dout = (_rows(g, 1, T, h, D, dtype) for h in (H, HK, HK, H))
+            q[..., at] = q[..., at].abs() + 0.5
+            lo, hi = _masks("causal", 1, T, T, g)
+            lo[:] = 0
+            gone = torch.arange(T, device="cuda") % 3 == 1  # (not the first: every row keeps a key)
+            k[:, gone, :, at] = -float("inf")
+            without = k.clone()
+            without[:, gone, :, at] = 0
+            announce("scores of -inf, D=%d at %d, T=%d, %s" % (D, at, T, dtype))
+            # the definition: the same keys, not seen.  In 64 bits, with the scores of those keys at -inf
+            out, lse = ops.range_attention(q, k, v, lo, hi)
+            ref = Attention(q, without, v, lo, hi)
+            heads = lambda x: x.double().permute(0, 2, 1, 3).contiguous()  # noqa: E731
+            many = lambda x: heads(x).repeat_interleave(H // HK, 1)  # noqa: E731
+            s = heads(q) @ many(without).transpose(2, 3) * D ** -0.5
+            i = torch.arange(T, device="cuda")
+            s = s.masked_fill((i > i[:, None]) | gone, -float("inf"))
+            p = torch.softmax(s, -1)
+            want = (p @ many(v)).permute(0, 2, 1, 3)
+            # (weights of what is left are at most what they were times the share of what went: the bound by that of |v|)
+            most = float(v.abs().max())
+            unit = UNIT[dtype] + 2.0 ** -24 * (8 + math.sqrt(D)) * 40
+            assert worst(out, want, torch.full_like(want, 1.01 * unit * 2 * most + 2.0 ** -20)) <= 1
+            assert worst(lse, torch.logsumexp(s, -1), ref.lse_bound + 1e-5) <= 1
+            _, _, dv = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi)
+            assert not dv[:, gone].any()
+            want = (p.transpose(2, 3) @ heads(dout)).view(1, HK, H // HK, T, D).sum(2).permute(0, 2, 1, 3)
+            size = (p.transpose(2, 3) @ heads(dout).abs()).view(1, HK, H // HK, T, D).sum(2).permute(0, 2, 1, 3)
+            assert worst(dv, want, 1.01 * 2 * unit * size + 2.0 ** -20) <= 1
+            step = ops.range_attention_step(q[:, -2:], k, v, lo[:, -2:].contiguous(), hi[:, -2:].contiguous())
+            assert worst(step, (p @ many(v)).permute(0, 2, 1, 3)[:, -2:], torch.full_like(step, 1.01 * unit * 2 * most + 2.0 ** -20).double()) <= 1
