@@ -87,14 +87,22 @@ class _Block(nn.Module):
 
 
 class Rollouts:
-    """The caches of a batch of rollouts: per layer keys and values of up to `tokens` tokens, and how many are there."""
+    """The caches of a batch of rollouts: per layer keys and values of up to `tokens` tokens, and how many are there.
+    A step is two tokens, the first of a rollout one."""
 
     def __init__(self, model, batch, tokens):
+        self.tokens, self.taken = tokens, 0  # (known here as well: no step waits for the GPU to compare them)
         at = dict(dtype=model.dtype, device=model.freqs.device)
         shape = (len(model.blocks), 2, batch, tokens, model.blocks[0].kv_heads, model.blocks[0].dim)
         self.caches = torch.zeros(shape, **at)
         self.length = torch.zeros(batch, 1, dtype=torch.int32, device=at["device"])
         self.time = torch.zeros(batch, 1, dtype=torch.int32, device=at["device"])
+
+    def restart(self):
+        """All rollouts begin anew, in the same caches."""
+        self.taken = 0
+        self.length.zero_()
+        self.time.zero_()
 
 
 class WindowModel(nn.Module):
@@ -131,6 +139,10 @@ class WindowModel(nn.Module):
     def step(self, rollouts, observation, last_action=None):
         """The next action of every rollout, from its newest observation [batch, ...] and the action before it (None: the
         first step)."""
+        new = 1 if last_action is None else 2
+        if rollouts.taken + new > rollouts.tokens:
+            raise ValueError("the rollouts' caches of %d tokens hold %d: no room for %d more"
+                             % (rollouts.tokens, rollouts.taken, new))
         x = [self.embed[0](observation)]
         column = [torch.zeros_like(rollouts.time)]
         time = [rollouts.time]
@@ -145,6 +157,7 @@ class WindowModel(nn.Module):
             q = ops.norm_rotate_append(q, k, v, pos, self.freqs, self.sections, block.q_weight, block.k_weight,
                                        slots=slots, k_cache=keys, v_cache=values)
             x = block.rest(x, ops.range_attention_step(q, keys, values, lo, hi, cap=self.cap))
-        rollouts.length += x.shape[1]
+        rollouts.taken += new
+        rollouts.length += new
         rollouts.time += 1
         return self.head(x[:, -1])

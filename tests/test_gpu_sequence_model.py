@@ -129,3 +129,25 @@ def test_a_captured_step_replays():
         for a, b in zip(captured, work()):
             assert torch.equal(a, b), replay
         torch.cuda.synchronize()
+
+
+def test_rollouts_end_where_their_caches_end():
+    """A step that the caches have no room for is refused before anything of it is written."""
+    from gear_amd.sequence import Rollouts, WindowModel
+    torch.manual_seed(0)
+    announce("rollouts to the end of their caches")
+    model = WindowModel(5, 3, width=64, heads=2, kv_heads=1).cuda()
+    obs, act = torch.randn(4, 5, device="cuda"), torch.randn(4, 3, device="cuda")
+    for tokens, steps in ((5, 3), (6, 3), (1, 1)):  # the first step is one token, every other two
+        rollouts = Rollouts(model, 4, tokens)
+        for t in range(steps):
+            model.step(rollouts, obs, act if t else None)
+        before = (rollouts.caches.clone(), rollouts.length.clone(), rollouts.time.clone())
+        with pytest.raises(ValueError, match="caches of %d tokens" % tokens):
+            model.step(rollouts, obs, act)
+        assert all(torch.equal(a, b) for a, b in zip(before, (rollouts.caches, rollouts.length, rollouts.time)))
+        rollouts.restart()  # in the same caches, which hold what the last ones left
+        assert torch.equal(model.step(rollouts, obs), model.step(Rollouts(model, 4, tokens), obs))
+    rollouts = Rollouts(model, 4, 0)
+    with pytest.raises(ValueError, match="caches of 0 tokens"):
+        model.step(rollouts, obs)
