@@ -81,6 +81,10 @@ class _Block(nn.Module):
         qkv = self.qkv(self.before(x)).to(dtype).view(*x.shape[:2], -1, self.dim)
         return qkv.split([self.heads, self.kv_heads, self.kv_heads], 2)
 
+    def weights(self, dtype):
+        """Of the norm, in a type that it takes beside rows of `dtype`: theirs, or 32 bits."""
+        return [w if w.dtype in (dtype, torch.float32) else w.float() for w in (self.q_weight, self.k_weight)]
+
     def rest(self, x, attended):
         x = x + self.out(attended.flatten(2).to(x.dtype))
         return x + self.mlp(self.between(x))
@@ -110,7 +114,7 @@ class WindowModel(nn.Module):
 
     A step is two tokens, observation then action; a token sees its document (the window's valid steps up to the
     last end of an episode) up to itself.  Positions have the axes (time, row, column) of a grid of 1 x 2 tokens a step.
-    The projections run in the parameters' type, attention in `dtype`."""
+    The projections run in the parameters' type (any, and what comes in has it), attention in `dtype`."""
 
     TOKENS = 2
 
@@ -124,6 +128,14 @@ class WindowModel(nn.Module):
         self.sections = (pairs - pairs // 4, 0, pairs // 4)
         self.register_buffer("freqs", ops.rotation_freqs(self.sections, device="cpu"), persistent=False)
 
+    def _apply(self, *args, **kwargs):
+        """Casts are for the parameters: the frequencies stay in 64 bits, and go along to another device."""
+        freqs = self.freqs
+        super()._apply(*args, **kwargs)
+        device = self.freqs.device
+        self.freqs = ops.rotation_freqs(self.sections, device=device) if freqs.is_meta else freqs.to(device)
+        return self
+
     def forward(self, observations, actions, mask, done):
         """observations [batch, steps, ...], actions, the loader's mask, the done column -> actions [batch, steps, ...]."""
         batch, steps = mask.shape
@@ -131,7 +143,7 @@ class WindowModel(nn.Module):
         x = torch.stack([self.embed[0](observations.flatten(2)), self.embed[1](actions.flatten(2))], 2).flatten(1, 2)
         for block in self.blocks:
             q, k, v = block.split(x, self.dtype)
-            q, k = norm_rotate(q, k, pos, self.freqs, self.sections, block.q_weight, block.k_weight)
+            q, k = norm_rotate(q, k, pos, self.freqs, self.sections, *block.weights(self.dtype))
             x = block.rest(x, range_attention(q, k, v, lo, hi, cap=self.cap))
         return self.head(x.view(batch, steps, self.TOKENS, -1)[:, :, 0])
 
@@ -154,8 +166,8 @@ class WindowModel(nn.Module):
         lo, hi = torch.zeros_like(slots), slots + 1
         for block, (keys, values) in zip(self.blocks, rollouts.caches):
             q, k, v = block.split(x, self.dtype)
-            q = ops.norm_rotate_append(q, k, v, pos, self.freqs, self.sections, block.q_weight, block.k_weight,
-                                       slots=slots, k_cache=keys, v_cache=values)
+            q = ops.norm_rotate_append(q, k, v, pos, self.freqs, self.sections, *block.weights(self.dtype), slots=slots,
+                                       k_cache=keys, v_cache=values)
             x = block.rest(x, ops.range_attention_step(q, keys, values, lo, hi, cap=self.cap))
         rollouts.taken += new
         rollouts.length += new

@@ -151,3 +151,31 @@ def test_rollouts_end_where_their_caches_end():
     rollouts = Rollouts(model, 4, 0)
     with pytest.raises(ValueError, match="caches of 0 tokens"):
         model.step(rollouts, obs)
+
+
+@pytest.mark.parametrize("parameters", [torch.float16, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_parameters_of_any_type(parameters, dtype):
+    """The projections run in the parameters' type, attention in the model's: training and a rollout, the same numbers as with 32-bit
+    parameters up to the roundings of the types."""
+    from gear_amd.sequence import Rollouts, WindowModel
+    torch.manual_seed(0)
+    announce("parameters of %s, attention in %s" % (parameters, dtype))
+    model = WindowModel(5, 3, width=64, heads=2, kv_heads=1, dtype=dtype).cuda()
+    obs, act = torch.randn(3, 8, 5, device="cuda"), torch.randn(3, 8, 3, device="cuda")
+    mask, done = torch.ones(3, 8, dtype=torch.uint8, device="cuda"), torch.zeros(3, 8, dtype=torch.uint8, device="cuda")
+    want = model(obs, act, mask, done).detach()
+    freqs = model.freqs.clone()
+    model = model.to(parameters)
+    assert model.freqs.dtype == torch.float64 and torch.equal(model.freqs, freqs)
+    got = model(obs.to(parameters), act.to(parameters), mask, done)
+    assert got.dtype == parameters
+    # (2 layers of the coarser of both types, outputs and operands of O(1))
+    unit = max(torch.finfo(parameters).eps, torch.finfo(dtype).eps)
+    assert float((got.detach() - want).abs().max()) < 32 * unit
+    got.square().mean().backward()
+    assert all(p.grad is not None and p.grad.dtype == parameters and bool(torch.isfinite(p.grad).all()) for p in model.blocks.parameters())
+    rollouts = Rollouts(model, 3, 16)
+    for t in range(8):
+        last = model.step(rollouts, obs[:, t].to(parameters), act[:, t - 1].to(parameters) if t else None)
+        assert float((last - got[:, t]).detach().abs().max()) < 32 * unit
