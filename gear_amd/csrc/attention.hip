@@ -190,6 +190,7 @@ extern "C" int gear_hip_attention(const gear_hip_attention_desc *desc, void *out
   // as few workgroups as hold all rows, and in each no more waves than the rows need
   const int groups = (int)ceil_div64(a.queries, kRows), blocks = (groups + kMostWaves - 1) / kMostWaves;
   const int waves = (groups + blocks - 1) / blocks;
+  if (!launchable((int64_t)blocks * a.heads * a.batch, waves)) return GEAR_HIP_ERANGE;
   by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
     by_waves(waves, [&](auto w) {

@@ -432,6 +432,8 @@ void by_waves(int waves, const F &f) {
 
 // Checks of what every attention call takes.  0: go on; 1: no queries; else the error.
 int attention_args(const gear_hip_attention_desc *d, AttentionArgs &a);
+// Whether a launch of so many workgroups can be.
+inline bool launchable(int64_t workgroups, int waves) { return workgroups <= kMostItems / (waves * kWave); }
 // base and strides are multiples of 16 bytes
 bool rows_aligned(const void *p, const int64_t *stride, int element);
 

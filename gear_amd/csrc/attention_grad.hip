@@ -665,6 +665,7 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
   g.dq = dq, g.dk = dk, g.dv = dv;
   const int longest = a.queries > a.keys ? a.queries : a.keys;
   if (longest <= 4 * kRows && a.dim <= 64 && a.heads == a.kv_heads && a.queries > 0) {
+    if (!launchable((int64_t)a.heads * a.batch, (longest + kRows - 1) / kRows)) return GEAR_HIP_ERANGE;
     by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
       if constexpr (decltype(dim)::value <= 64)
         by_waves((longest + kRows - 1) / kRows, [&](auto w) {
@@ -675,20 +676,24 @@ extern "C" int gear_hip_attention_backward(const gear_hip_attention_desc *desc, 
     GEARHIP_RETURN_IF_LAUNCH_FAILED();
     return 0;
   }
+  const int groups = g.padded / kRows;  // (padding included: its statistics are written too)
+  const int query_blocks = (groups + kWaves - 1) / kWaves, waves = query_blocks > 0 ? (groups + query_blocks - 1) / query_blocks : 1;
+  const int key_blocks = (int)ceil_div64(a.keys, kWaves * kRows);
+  if (!launchable((int64_t)query_blocks * a.heads * a.batch, waves) || !launchable((int64_t)key_blocks * a.kv_heads * a.batch, kWaves))
+    return GEAR_HIP_ERANGE;
   by_attention_type(a, desc->dtype, [&](auto dim, auto type, auto mode) {
     typedef decltype(type) T;
     constexpr int D = decltype(dim)::value;
     constexpr int kMode = decltype(mode)::value;
-    if (a.queries > 0) {
-      const int groups = g.padded / kRows;  // (padding included: its statistics are written too)
-      g.blocks = (groups + kWaves - 1) / kWaves;
-      by_waves((groups + g.blocks - 1) / g.blocks, [&](auto w) {
+    if (query_blocks > 0) {
+      g.blocks = query_blocks;
+      by_waves(waves, [&](auto w) {
         hipLaunchKernelGGL((attention_dq_kernel<T, D, kMode, decltype(w)::value>),
                            dim3((unsigned)g.blocks * a.heads * a.batch), dim3(decltype(w)::value * kWave), 0,
                            as_stream(stream), g);
       });
     }
-    g.blocks = (int)ceil_div64(a.keys, kWaves * kRows);
+    g.blocks = key_blocks;
     if (g.blocks > 0)
       hipLaunchKernelGGL((attention_dkv_kernel<T, D, kMode>), dim3((unsigned)g.blocks * a.kv_heads * a.batch),
                          dim3(kThreads), 0, as_stream(stream), g);

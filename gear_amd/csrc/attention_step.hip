@@ -255,8 +255,8 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(StepArgs g) {
     mend_row<T, MODE>(g, b, r, kv_head, top + __builtin_log2f(total));
 }
 
-int row_blocks_of(int64_t queries, int64_t heads, int64_t kv_heads) {
-  return (int)ceil_div64(queries * (heads / kv_heads), kRows);
+int64_t row_blocks_of(int64_t queries, int64_t heads, int64_t kv_heads) {
+  return ceil_div64(queries * (heads / kv_heads), kRows);
 }
 
 // Parts of a rollout's keys: enough workgroups for the GPU, at least 256 keys each.
@@ -292,11 +292,11 @@ extern "C" int gear_hip_attention_step(const gear_hip_attention_desc *desc, void
   const size_t want = gear_hip_attention_step_workspace_bytes(a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim);
   if (want > 0 && (workspace == nullptr || workspace_bytes < want)) return GEAR_HIP_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(out) % 16 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return GEAR_HIP_EALIGN;
-  g.row_blocks = row_blocks_of(a.queries, a.heads, a.kv_heads);
+  g.row_blocks = (int)row_blocks_of(a.queries, a.heads, a.kv_heads);
   const int64_t units = (int64_t)a.batch * a.kv_heads * g.row_blocks;
   g.splits = splits_of(units, a.keys);
   const int64_t workgroups = ceil_div64((int64_t)a.batch * g.row_blocks * g.splits, 8) * 8 * a.kv_heads;
-  if (workgroups > INT_MAX) return GEAR_HIP_ERANGE;
+  if (!launchable(workgroups, kWaves)) return GEAR_HIP_ERANGE;  // (the join is for fewer than 1024 blocks of 32 rows)
   g.part_o = static_cast<float *>(workspace);
   g.part_ml = reinterpret_cast<float2 *>(g.part_o + units * g.splits * kRows * a.dim);
   g.out = out;

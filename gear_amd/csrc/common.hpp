@@ -43,6 +43,8 @@ __host__ __device__ inline int64_t ceil_div64(int64_t a, int64_t b) { return (a 
 // happens at set-up rather than inside the first hot-path call.
 int scan_static_init();
 
+constexpr int64_t kMostItems = ((int64_t)1 << 32) - 1;  // work items of a launch
+
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 }  // namespace gearhip

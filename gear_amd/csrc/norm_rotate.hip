@@ -43,6 +43,7 @@ struct NormArgs {
   int weight_f32;
   float eps;
   // forward
+  int64_t first;  // token of the launch
   void *q_out, *k_out, *v_out;
   const int32_t *slots;  // append: the row of the cache, else null
   int64_t cache_tokens;
@@ -171,7 +172,7 @@ template <typename T, int LPR>
 __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormArgs a, int per_block) {
   __shared__ __attribute__((aligned(16))) float2 cs[kTurns];  // [token][dim / 2]
   __shared__ Tokens tokens;
-  const int64_t all = a.batch * a.tokens, first = (int64_t)blockIdx.x * per_block;
+  const int64_t all = a.batch * a.tokens, first = a.first + (int64_t)blockIdx.x * per_block;
   const int count = (int)min((int64_t)per_block, all - first), half = a.dim / 2;
   const int at = (threadIdx.x % LPR) * kEach<T>;
   const bool active = at < half;
@@ -387,14 +388,18 @@ int tokens_per_block(int64_t tokens, int dim) {
   return n;
 }
 
-int forward(const NormArgs &a, int dtype, void *stream) {
+int forward(NormArgs &a, int dtype, void *stream) {
   const int64_t all = a.batch * a.tokens;
   const int n = tokens_per_block(all, a.dim);
-  by_type_and_lanes(dtype, a.dim, [&](auto type, auto lanes) {
-    hipLaunchKernelGGL((norm_rotate_kernel<decltype(type), decltype(lanes)::value>), dim3((unsigned)ceil_div64(all, n)),
-                       dim3(kBlock), 0, as_stream(stream), a, n);
-  });
-  GEARHIP_RETURN_IF_LAUNCH_FAILED();
+  const int64_t most = kMostItems / kBlock;  // workgroups of a launch
+  for (a.first = 0; a.first < all; a.first += most * n) {
+    const int64_t left = ceil_div64(all - a.first, n), blocks = left < most ? left : most;
+    by_type_and_lanes(dtype, a.dim, [&](auto type, auto lanes) {
+      hipLaunchKernelGGL((norm_rotate_kernel<decltype(type), decltype(lanes)::value>), dim3((unsigned)blocks), dim3(kBlock), 0,
+                         as_stream(stream), a, n);
+    });
+    GEARHIP_RETURN_IF_LAUNCH_FAILED();
+  }
   return 0;
 }
 

@@ -157,9 +157,17 @@ extern "C" int gear_hip_token_ranges(const uint8_t *mask, const uint8_t *done, i
   const int64_t longest = steps < kWave ? steps : kWave;
   RangesArgs a{mask, done, batch, steps, (uint32_t)ceil_div64(steps, kWave), (uint32_t)ceil_div64(longest * tokens_per_step, kWrite), (int)tokens_per_step, mode, (int)grid_cols,
                prefix < steps ? prefix : steps, lo, hi, pos};
-  if (batch > kMost / a.chunks / a.slices) return GEAR_HIP_ERANGE;
-  const int64_t blocks = ceil_div64(batch * a.chunks * a.slices, kWaves);
-  hipLaunchKernelGGL(token_ranges_kernel, dim3((unsigned)blocks), dim3(kWaves * kWave), 0, as_stream(stream), a);
-  GEARHIP_RETURN_IF_LAUNCH_FAILED();
+  // a launch has less than 2^32 work items; a window needs at most 2^25 waves
+  const int64_t waves = (int64_t)a.chunks * a.slices, most = (kMostItems / kWave - kWaves) / waves;
+  for (int64_t from = 0; from < batch; from += most) {
+    a.batch = batch - from < most ? batch - from : most;
+    hipLaunchKernelGGL(token_ranges_kernel, dim3((unsigned)ceil_div64(a.batch * waves, kWaves)), dim3(kWaves * kWave), 0,
+                       as_stream(stream), a);
+    GEARHIP_RETURN_IF_LAUNCH_FAILED();
+    const int64_t tokens = a.batch * steps * tokens_per_step;
+    if (a.mask != nullptr) a.mask += a.batch * steps;
+    if (a.done != nullptr) a.done += a.batch * steps;
+    a.lo += tokens, a.hi += tokens, a.pos += tokens * (grid_cols > 0 ? 3 : 1);
+  }
   return 0;
 }

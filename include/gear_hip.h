@@ -524,7 +524,9 @@ int gear_hip_norm_rotate_backward(const gear_hip_norm_rotate_desc *desc, const v
  *   dtype     GEAR_HIP_F16 or GEAR_HIP_BF16; head_dim a multiple of 16, at most 128
  *   q, k, v   batch x queries|keys x heads|kv_heads x head_dim, the innermost contiguous; strides
  *             of batch, token and head in elements; bases and strides multiples of 16 bytes
- *   queries, keys < 2^30;  0 < scale < 1e30;  cap 0 (none), or below 1e30 and above 1e-30 scale */
+ *   queries, keys < 2^30, and less than 2^32 work items a launch, else GEAR_HIP_ERANGE: batch * heads * (queries / 128, rounded
+ *   up) and batch * kv_heads * (keys / 128, rounded up) below 2^24, for steps batch * kv_heads *
+ *   (queries * heads / kv_heads / 32, rounded up) below 2^24;  0 < scale < 1e30;  cap 0 (none), or below 1e30 and above 1e-30 scale */
 typedef struct gear_hip_attention_desc {
   const void *q, *k, *v;
   int64_t q_stride[3], k_stride[3], v_stride[3];

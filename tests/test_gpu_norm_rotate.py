@@ -153,3 +153,26 @@ def test_zero_rows_nan_rows_and_empty_batches():
         assert a.shape == (*shape, 2, 32) and b.shape == (*shape, 1, 32)
         _, _, dwq, dwk = ops.norm_rotate_backward(e(2), e(1), e(2), e(1), p, freqs, sections, wq, wk)
         assert not dwq.any() and not dwk.any()
+
+
+def test_tokens_beyond_one_launch():
+    """A launch has less than 2^32 work items, 16 of them a token: 2^28 tokens and some are two."""
+    from gear_amd import ops
+    B, T, D = (1 << 18) + 3, 1024, 16
+    announce("norm_rotate of 2^28 + 3072 tokens")
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.ones(B, T, 1, D, dtype=torch.float16, device="cuda")
+    k = q[:, :, :0]
+    pos = torch.zeros(B, T, 1, dtype=torch.int32, device="cuda")
+    freqs = torch.full((8,), 0.5, dtype=torch.float64, device="cuda")
+    for b in (0, (1 << 18) - 1, 1 << 18, B - 1):  # the border lies 16 tokens before window 2^18
+        q[b] = torch.randn(T, 1, D, generator=g, device="cuda").half()
+        pos[b, :, 0] = torch.arange(T, dtype=torch.int32, device="cuda")
+    out, _ = ops.norm_rotate(q, k, pos, freqs, (8,))
+    for b in (0, (1 << 18) - 1, 1 << 18, B - 1):
+        want, _ = ops.norm_rotate(q[b:b + 1], k[b:b + 1], pos[b:b + 1].contiguous(), freqs, (8,))
+        assert torch.equal(out[b:b + 1], want)
+    ones = torch.ones(1, dtype=torch.float16, device="cuda")
+    for b in range(1, B, 8192):
+        if b not in (0, (1 << 18) - 1, 1 << 18, B - 1):
+            assert bool((out[b] - ones).abs().max() <= 2.0 ** -10)

@@ -80,3 +80,20 @@ def test_nothing_to_do_and_a_table_slice():
         assert lo.shape == hi.shape == (shape[0], shape[1] * 2) and pos.shape == (shape[0], shape[1] * 2, 1)
     lo, hi, _ = ops.token_ranges(torch.ones(2, 4, device="cuda") > 0)
     assert hi.tolist() == [[1, 2, 3, 4]] * 2 and not lo.any()
+
+
+def test_windows_beyond_one_launch():
+    """A launch has less than 2^32 work items, a wave a window: 2^26 windows and some are two."""
+    from gear_amd import ops
+    announce("2^26 + 5 windows of one step")
+    mask = (torch.arange((1 << 26) + 5, device="cuda") % 7 != 3).to(torch.uint8)[:, None].contiguous()
+    lo, hi, pos = ops.token_ranges(mask)
+    assert torch.equal(hi, mask.int()) and not lo.any() and not pos.any()
+    announce("2^25 + 3 windows of 65 steps")
+    mask = torch.ones((1 << 25) + 3, 65, dtype=torch.bool, device="cuda")
+    mask[-1, 40] = False
+    lo, hi, pos = ops.token_ranges(mask)
+    want = ops.token_ranges(mask[-2:].contiguous())
+    assert all(torch.equal(a[-2:], b) for a, b in zip((lo, hi, pos), want))
+    at = torch.arange(65, dtype=torch.int32, device="cuda")
+    assert bool((hi[:-1] == at + 1).all()) and not lo[:-1].any() and bool((pos[:-1, :, 0] == at).all())

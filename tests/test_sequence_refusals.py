@@ -172,3 +172,28 @@ def test_attention_refuses_caps_and_scales_by_name():
             call(q, q, q, lo, lo, scale=1e30)
         with pytest.raises(ValueError, match="scale must be"):
             call(q, q, q, lo, lo, scale=1e-300)
+
+
+def test_launches_that_cannot_be():
+    """2^32 work items and more are refused by code, before the device is touched (the pointers are no memory)."""
+    from gear_amd import _cabi
+    lib, none = _cabi.load(), ctypes.c_void_p(256)
+
+    def attention(**sizes):
+        return _cabi.AttentionDesc(**dict(dict(q=256, k=256, v=256, lo=256, hi=256, batch=1, queries=1, keys=1, heads=1, kv_heads=1,
+                                               head_dim=128, dtype=1, scale=1.0), **sizes))
+
+    strides = (ctypes.c_int64 * 3)(0, 0, 0)
+    forward = lambda d: lib.gear_hip_attention(ctypes.byref(d), none, none, None)  # noqa: E731
+    backward = lambda d: lib.gear_hip_attention_backward(  # noqa: E731
+        ctypes.byref(d), none, strides, none, none, none, none, none, none, 1 << 60, None)
+    step = lambda d: lib.gear_hip_attention_step(ctypes.byref(d), none, none, 1 << 60, None)  # noqa: E731
+    most = 1 << 20
+    assert forward(attention(batch=most, heads=64, kv_heads=64)) == -3  # one wave each
+    assert forward(attention(batch=most, heads=16, kv_heads=16, queries=128)) == -3  # four
+    assert forward(attention(batch=1, heads=2, kv_heads=1, queries=(1 << 30) - 1)) == -3
+    assert backward(attention(batch=most, heads=64, kv_heads=64, head_dim=64)) == -3  # in one launch
+    assert backward(attention(batch=most, heads=64, kv_heads=64, queries=200, keys=0)) == -3  # in two
+    assert backward(attention(batch=most, heads=16, kv_heads=16)) == -3  # the keys' side: four waves always
+    assert step(attention(batch=most, heads=16, kv_heads=16)) == -3
+    assert step(attention(batch=1, queries=1 << 20, heads=1 << 15, kv_heads=1 << 10)) == -3
