@@ -176,3 +176,34 @@ def test_tokens_beyond_one_launch():
     for b in range(1, B, 8192):
         if b not in (0, (1 << 18) - 1, 1 << 18, B - 1):
             assert bool((out[b] - ones).abs().max() <= 2.0 ** -10)
+
+
+def test_gradient_against_differences_in_64_bits():
+    """The gradients against central differences of the definition in 64 bits: h = 1e-4, the differences are off by h^2 / 6 of a third
+    derivative (rows of about 3 an element, weights of about 1: below 16 a unit of the gradient that comes in) and 1e-16 / h of
+    the value, the gradients by 64 units of 32 bits of what is summed.  Every element, and the largest are a hundred times the
+    bound and more."""
+    from gear_amd import ops
+    q, k, _, pos, freqs, sections, wq, wk, g = _inputs(2, 3, 2, 1, 32, torch.float32, 5)
+    gq, gk = torch.randn(2, 3, 2, 32, generator=g, device="cuda"), torch.randn(2, 3, 1, 32, generator=g, device="cuda")
+    announce("norm_rotate: differences in 64 bits")
+    grads = ops.norm_rotate_backward(gq, gk, q, k, pos, freqs, sections, wq, wk)
+    args = [x.double().contiguous() for x in (q, k, wq, wk)]
+
+    def value(q, k, wq, wk):
+        a, b = norm_rotate(q, wq, pos, freqs, sections, 1e-6), norm_rotate(k, wk, pos, freqs, sections, 1e-6)
+        return float((a * gq.double()).sum() + (b * gk.double()).sum())
+
+    h = 1e-4
+    size = float(gq.abs().sum() + gk.abs().sum())
+    tol = h * h / 6 * 16 * float(gq.abs().max()) * 32 + 1e-15 * size * 4 / h + 64 * 2.0 ** -24 * float(gq.abs().amax()) * 32
+    for i, grad in enumerate(grads):
+        slopes = []
+        for at in range(grad.numel()):
+            plus, minus = [x.clone() for x in args], [x.clone() for x in args]
+            plus[i].view(-1)[at] += h
+            minus[i].view(-1)[at] -= h
+            slopes.append((value(*plus) - value(*minus)) / (2 * h))
+        slopes = torch.tensor(slopes, dtype=torch.float64, device="cuda").view(grad.shape)
+        assert float(slopes.abs().max()) > 100 * tol
+        assert float((grad.double() - slopes).abs().max()) <= tol
