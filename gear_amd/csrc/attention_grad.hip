@@ -8,10 +8,13 @@
 //   2. by keys: a wave holds 32 keys and passes over all queries (of all heads that share them) whose ranges
 //      reach them; scores are not transposed here, a lane holds one key
 // dq's delta is dout . out, which starts from out as it was stored, rounded; on the way sum_j p_ij dp_ij is summed in 32 bits for the
-// second launch, which costs it next to nothing.  In bf16 dk is then within 0.0024 of the exact one (norm of the difference over
-// the norm; 0.0034 with dout . out), dq within 0.0025..0.0029, where the rounding of the results alone leaves 0.0017.  The exact
-// delta for dq too takes a third pass over the keys with two products, 2/7 more work.  Short windows, whose
-// probabilities stay in registers, have it for nothing: one launch (below).
+// second launch, which costs it next to nothing.  The difference matters where dp - delta is a small one, in rows of which one key has
+// most of the weight (dq off by 1.7 % in bf16 where all rows are such): tiles where some p is above 1/2 are gone through once more
+// at the end, with two products, for what they owe to it.  dq and dk are then within 0.0024 of the exact ones in bf16 (norm of the difference
+// over the norm; packed, dq 0.0029 without), where the rounding of the results alone leaves 0.0017.  us of the launch with / without:
+// 2 x 8193 with a bias, in half of whose heads nearly all rows are such, 450 / 413, without a bias 377 / 367, 32 x 1470 684 / 671; from 1/16 on
+// 483 and 945.  The exact delta for all tiles takes a third pass, 2/7 more work.  Short windows, whose probabilities stay in
+// registers, have it for nothing: one launch (below).
 // p and ds are rounded to the type for their products, the sums are held in 32 bits.
 // Bound by the matrix unit, the exponentials and LDS together: 2 x 8193, 16 heads of 128 over 8, packed, with a bias: 1. 411 us (three
 // products, 880 TFLOP/s), 2. 678 us (four products of twice the loads, 710); 32 x 1470, 16 over 4, frames, a cap: 674 and 950 us.
@@ -141,18 +144,25 @@ __device__ __forceinline__ float largest(const f32x16 &x) {
   return top;
 }
 
-// What by_query() does with the largest |dp| that a row sees of a tile: has the row's sums follow it, or keeps it.
+// A key that has this much of a row's weight: the launch by queries goes through its tile again.
+constexpr float kHeavy = 1.f / 2;
+
+// What by_query() does with what a row sees of a tile: its probabilities, and the largest |dp|, which the row's sums follow or
+// which is kept.
 template <typename T, int N>
 struct Follow {
   Lift<T> &lift;
   f32x16 (&sums)[N];
   float delta;  // its size
+  bool &heavy;  // whether a row of the wave has much of its weight in one key of the tile
+  __device__ __forceinline__ void weights(const f32x16 &p) const { heavy = wave_ballot(largest(p) > kHeavy) != 0; }
   __device__ __forceinline__ void saw(float top) const {
     if (__builtin_expect(lift.beyond(top + delta), 0)) lift.lower(top + delta, sums);
   }
 };
 struct Keep {
   float &most;
+  __device__ __forceinline__ void weights(const f32x16 &) const {}
   __device__ __forceinline__ void saw(float top) const { most = fmaxf(most, top); }
 };
 
@@ -186,6 +196,7 @@ __device__ __forceinline__ void by_query(f32x16 &s, f32x16 &dp, float &delta, co
     if (Lift<T>::kOn) top = largest(dp);
     asm volatile("");  // (keeps this a branch of its own: whole tiles pay nothing)
   }
+  of_row.weights(s);
   of_row.saw(top);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
@@ -275,6 +286,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
   __shared__ __attribute__((aligned(16))) T k_tile[2][kTile * D];  // (at the end: the rows of dq)
   __shared__ __attribute__((aligned(16))) T v_tile[2][kTile * D];
   __shared__ int ranges[WAVES][2];
+  __shared__ uint64_t heavy_of[WAVES];
   const AttentionArgs &a = g.a;
   const int tid = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), half = l >> 5;
   const int at = same_die_index(), block = g.blocks - 1 - at % g.blocks, bh = at / g.blocks, head = bh % a.heads, b = bh / a.heads;
@@ -328,7 +340,12 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
     k_rows.template ask<WAVES>(k_tile[to], k0, wave);
     v_rows.template ask<WAVES>(v_tile[to], k0, wave);
   };
-  int k0 = first < end ? first / kTile * kTile : 0, buffer = 0;
+  const int k_first = first < end ? first / kTile * kTile : 0;
+  int k0 = k_first, buffer = 0;
+  // the tiles in which a key has much of a row's weight, a bit for each of 64 (or 128, 256 .. keys, where there are more tiles)
+  uint64_t heavy_tiles = 0;
+  int keys_a_bit = 6;
+  while ((end - 1 - k_first) >> keys_a_bit >= 64) ++keys_a_bit;
   for (int x = wave; x < 2; x += WAVES) k_rows.clear_beyond(k_tile[x]);
   if (k0 < end) load(k0, 0);
   for (; k0 < end; k0 += kTile, buffer ^= 1) {
@@ -341,23 +358,66 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attention_dq_kernel(GradArgs 
       const int kk = k0 + kb * 32;
       if (!seen.touches(kk, kk + 32)) continue;
       f32x16 s, dp;
-      by_query<T, D, MODE>(s, dp, summed, Follow<T, D / 32>{lift, dq, fabsf(delta)}, k_here, v_here, kb * 32, kk, q, dout, reader, scores, seen, place, less);
+      bool heavy = false;
+      by_query<T, D, MODE>(s, dp, summed, Follow<T, D / 32>{lift, dq, fabsf(delta), heavy}, k_here, v_here, kb * 32, kk, q, dout, reader,
+                           scores, seen, place, less);
+      if (heavy) heavy_tiles |= 1ull << ((k0 - k_first) >> keys_a_bit);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= Lift<T>::kOn ? fmaf(dp[r], lift.power(), -delta * lift.power()) : dp[r] - delta;
       add_columns<T, D>(dq, k_here, kb * 32, s, reader);
     }
   }
-  summed = sum_of_halves(summed);
+  summed = seen.empty() ? 0.f : sum_of_halves(summed);
   if (half == 0 && i < g.padded) {
     const int64_t stats = ((int64_t)b * a.heads + head) * g.padded + i;
-    g.lse_log2[stats] = lse_log2, g.delta[stats] = seen.empty() ? 0.f : summed;
+    g.lse_log2[stats] = lse_log2, g.delta[stats] = summed;
+  }
+  if (l == 0) heavy_of[wave] = heavy_tiles;
+  __syncthreads();
+  // those tiles again, by what their sums owe to the difference of both deltas: p (dout . out - sum p dp) (1 - tanh^2) k
+  const float owed = seen.empty() ? 0.f : (delta - summed) * lift.power();
+  uint64_t any_heavy = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) any_heavy |= heavy_of[w];
+  any_heavy = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(any_heavy >> 32)) << 32 |
+              (uint32_t)__builtin_amdgcn_readfirstlane((int)any_heavy);
+  auto heavy_from = [&](int k) __attribute__((always_inline)) {
+    while (k < end && !((any_heavy >> ((k - k_first) >> keys_a_bit)) & 1)) k += kTile;
+    return k;
+  };
+  k0 = heavy_from(k_first), buffer = 0;
+  if (k0 < end) k_rows.template ask<WAVES>(k_tile[0], k0, wave);
+  while (k0 < end) {
+    staged_wait();
+    __syncthreads();
+    const int next = heavy_from(k0 + kTile);
+    if (next < end) k_rows.template ask<WAVES>(k_tile[buffer ^ 1], next, wave);
+#pragma unroll 1
+    for (int kb = 0; kb < 2; ++kb) {
+      const int kk = k0 + kb * 32;
+      if (!seen.touches(kk, kk + 32)) continue;
+      f32x16 s = {};
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) s = mfma(reader.rows(k_tile[buffer], kb * 32, x), q[x], s);
+      scores.cap_far(s);
+      const float ahead = (float)(place - kk - 4 * half);
+      const uint32_t from_lo = (uint32_t)(kk + 4 * half - seen.lo), count = (uint32_t)(seen.hi - seen.lo);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float c = scores.in_tile(s[r]), z = scores.z(c, ahead - (float)(8 * (r >> 2) + (r & 3)));
+        const float ds = exp2_fast(fmaf(z, scores.factor, less)) * scores.shrink(c) * owed;
+        s[r] = from_lo + (uint32_t)(8 * (r >> 2) + (r & 3)) < count ? ds : 0.f;
+      }
+      add_columns<T, D>(dq, k_tile[buffer], kb * 32, s, reader);
+    }
+    k0 = next, buffer ^= 1;
   }
   __syncthreads();
   const uint32_t bad = columns_not_finite(dq, !seen.empty());
   store_rows<T, D>(k_tile[0] + wave * kRows * D, dq, a.scale * lift.back(), seen.empty(), a.dim, [&](int r) {
     return i0 + r < a.queries ? static_cast<T *>(g.dq) + (((int64_t)b * a.queries + i0 + r) * a.heads + head) * a.dim : nullptr;
   });
-  if (__builtin_expect(bad != 0, 0)) mend_dq<T, MODE>(g, bad, b, head, kv_head, i0, seen, lse_log2, delta, scores);
+  if (__builtin_expect(bad != 0, 0)) mend_dq<T, MODE>(g, bad, b, head, kv_head, i0, seen, lse_log2, summed, scores);
 }
 
 // Rows of 128 elements leave no registers for V beside K, dk and dv at two waves a SIMD (spilled, they would be waited for

@@ -499,3 +499,24 @@ def test_a_score_of_minus_infinity_is_a_probability_of_zero(D, dtype):
             assert worst(dv, want, 1.01 * 2 * unit * size + 2.0 ** -20) <= 1
             step = ops.range_attention_step(q[:, -2:], k, v, lo[:, -2:].contiguous(), hi[:, -2:].contiguous())
             assert worst(step, (p @ many(v)).permute(0, 2, 1, 3)[:, -2:], torch.full_like(step, 1.01 * unit * 2 * most + 2.0 ** -20).double()) <= 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_dq_where_one_key_has_most_of_the_weight(cap, dtype):
+    """Steep slopes: a row's last key has 0.9 and more of its weight, dp - delta is a small difference there, and a delta that
+    begins from the rounded out is off by more than it.  dq is held to the roundings that it needs: of ds and of the result, each
+    u / sqrt(3) of the norm at most (a rounding is evenly spread over at most 2 u), a fifth more for what keys of small weight
+    and 32 bits leave.  In two launches (long rows, shared key heads, rows of 128) and in one."""
+    from gear_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(21)
+    for T, H, HK, D in ((300, 2, 2, 64), (90, 4, 2, 48), (1000, 2, 1, 128), (5000, 1, 1, 32), (100, 2, 2, 64)):
+        q, k, v, dout = (_rows(g, 1, T, h, D, dtype) for h in (H, HK, HK, H))
+        lo, hi = _masks("causal", 1, T, T, g)
+        form = dict(cap=cap, slopes=torch.linspace(4, 6, H, device="cuda"))
+        announce("dq of rows with one key, %s T=%d heads=%d/%d D=%d cap=%g" % (dtype, T, H, HK, D, cap))
+        out, lse = ops.range_attention(q, k, v, lo, hi, **form)
+        dq, dk, _ = ops.range_attention_backward(dout, q, k, v, out, lse, lo, hi, **form)
+        ref = Attention(q, k, v, lo, hi, dout=dout, **form)
+        for got, want in ((dq, ref.dq), (dk, ref.dk)):
+            assert float((got.double() - want).norm() / want.norm()) <= 1.2 * UNIT[dtype] * (2 / 3) ** 0.5
