@@ -6,8 +6,8 @@
 // and the sums of p v are rescaled when m grows.  Tiles outside a wave's ranges are passed over, tiles that all its rows
 // see in full need no comparison.  p is rounded to the type for its product (the matrix unit takes nothing wider at this
 // rate), its sum is of the values before that.
-// bf16: 2048 windows of 90, 8 heads of 64, causal: 133 us, bound by memory (755 MB, 5.7 TB/s).  2 x 8193, 16 heads of 128 over 8,
-// packed, a bias: 334 us, 720 TFLOP/s of the pairs that are seen; 32 x 1470, 16 over 4, frames, a cap: 429 us, 410 TFLOP/s.  There the
+// bf16: 2048 windows of 90, 8 heads of 64, causal: 134 us, bound by memory (755 MB, 5.7 TB/s).  2 x 8193, 16 heads of 128 over 8,
+// packed, a bias: 327 us; 32 x 1470, 16 over 4, frames, a cap: 439 us, 400 TFLOP/s of the pairs that are seen.  There the
 // exponentials (and the tanh of the cap) and the matrix unit take about the same time and do not overlap in full.
 #include <type_traits>
 

@@ -264,8 +264,8 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // most, which moves p by a thirtieth of its own rounding to fp16.  kFar, for larger caps, takes tanh up to |u| = kSmall
 // as u + u^3 P(u^2), with P fitted to be least off relative to tanh (0.7 units of 2^-24 at most): a score is within a few units of
 // itself whatever the cap.  A tile whose arguments are all that small, as they are where the cap is far above the scores, takes
-// only that.  At a cap of 30 kFar would take 457 / 684 / 1035 us in the three kernels of 32 x 1470 against 432 / 690 / 970, at
-// one of 5, whose tiles hold both kinds of arguments, 580 forward against 431.
+// only that.  32 x 1470: 478 + 690 + 1022 us in the three kernels at a cap of 100, 439 + 683 + 946 of the first form at 30; at a cap of 5,
+// whose tiles hold both kinds of arguments, kFar took 580 forward against 431.
 constexpr int kCap = 1, kBias = 2, kFar = 4;
 constexpr float kNearCap = 64.f;
 template <int MODE>

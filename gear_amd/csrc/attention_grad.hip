@@ -16,9 +16,9 @@
 // 483 and 945.  The exact delta for all tiles takes a third pass, 2/7 more work.  Short windows, whose probabilities stay in
 // registers, have it for nothing: one launch (below).
 // p and ds are rounded to the type for their products, the sums are held in 32 bits.
-// Bound by the matrix unit, the exponentials and LDS together: 2 x 8193, 16 heads of 128 over 8, packed, with a bias: 1. 411 us (three
-// products, 880 TFLOP/s), 2. 678 us (four products of twice the loads, 710); 32 x 1470, 16 over 4, frames, a cap: 674 and 950 us.
-// Tiles of 32 keys in 1., which the forward pass gains by, change nothing here: 404 against 407, 697 against 686 us.
+// Bound by the matrix unit, the exponentials and LDS together: 2 x 8193, 16 heads of 128 over 8, packed, with a bias: 1. 432 us (three
+// products), 2. 671 us (four products of twice the loads); 32 x 1470, 16 over 4, frames, a cap: 683 and 946 us.  Tiles of 32
+// keys in 1., which the forward pass gains by, changed nothing here: 404 against 407, 697 against 686 us.
 #include <type_traits>
 
 #include "attention_exact.hpp"
@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kThreads, D == 64 && MODE == kBias ? 3 : 2) void at
 // Where all queries and all keys of a window are at most 128 (and a row at most 64 elements, and no heads share keys),
 // a workgroup holds queries, keys, values and dout of a window and head in LDS: each is read once, out not at all, because delta
 // can be summed from the probabilities themselves -- in 32 bits, where dout . out begins from the rounded out.
-// us in one launch / two: 2048 x 90, 8 heads of 64, causal, bf16: 361 / 527; 64 x 60, 4 of 32, f16: 8.5 / 12.0.  The first is 1.3 GB at
+// us in one launch / two: 2048 x 90, 8 heads of 64, causal, bf16: 361 / 527; 64 x 60, 4 of 32, bf16: 8.7 / 12.0.  The first is 1.3 GB at
 // 3.7 TB/s: loads, products and stores of a workgroup follow each other, and 200 registers leave two waves a SIMD to
 // overlap them (three: 28 registers spilled, 490 us).
 // A wave is responsible for 32 queries (delta, dq) and for 32 keys (dk, dv) in turn.

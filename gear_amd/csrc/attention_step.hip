@@ -2,13 +2,14 @@
 //
 // Few queries, many keys: what counts is reading the caches once, at the rate of memory.  The queries of
 // all heads that share a key head are the rows of one matrix operand (32 at a time; most calls have fewer, the
-// unused rows cost nothing that memory would not), so every key is read once for all of them.  A rollout's
+// unused rows cost nothing that memory would not), so every key is read once for 32 of them; with more, each 32 read the keys
+// again, past the caches.  A rollout's
 // keys are split over `splits` workgroups and within one over its waves, 32 keys at a time.  A wave has two tiles of K and
 // V in a piece of LDS of its own, filled past the caches (nobody reads a key again) while the one before is worked on, so no
 // wave waits for another before the end.  What the parts of a split have -- maximum, sum, sums of p v -- is joined by a second
 // launch, in a fixed order.
 // Bound by memory.  bf16: 256 rollouts of up to 3000 keys, 8 heads of 64: 142 us, 5.3 TB/s of the keys that are seen; 3 of up to 131071,
-// 16 heads of 128 over 2: 64 us (3.1 TB/s; 49 at best) and 6 for the join.  There a workgroup fills a CU's LDS alone, and its start
+// 16 heads of 128 over 2: 66 us (3.1 TB/s; 49 at best) and 6 for the join.  There a workgroup fills a CU's LDS alone, and its start
 // and end are time in which the CU asks for little: two waves a workgroup 63 us, 64 parts 62, 256 parts 84, parts of
 // one size 75.
 #include <type_traits>

@@ -190,7 +190,7 @@ __global__ __launch_bounds__(kBlock) void norm_rotate_kernel(NormArgs a, int per
                                             : row_at<T>(a.v, a.vs, b, t, kh - a.k_heads),
                        at, half);
   };
-  // (a row is asked for before the one before it is worked on, the first before the sines)
+  // (the first row is asked for before the sines)
   RowWalk walk(threadIdx.x / LPR, heads), ahead = walk;
   Halves<T> next = load(ahead);
   Part<T> w[2][2] = {};
@@ -380,7 +380,8 @@ void by_type_and_lanes(int dtype, int dim, const F &f) {
 
 // Tokens a workgroup: the sines of a token serve all its heads, and what is done once a workgroup has to be spread over
 // its rows (forward, 94080 tokens of 20 heads of 128: 2 tokens 436 us, 4 296, 8 241, 16 216, 32 224), but few tokens are
-// spread over the GPU, two workgroups for each of 256 CUs.
+// spread over the GPU, two workgroups for each of 256 CUs.  (Few heads of short rows leave most of a workgroup idle, in the
+// gradient above all: 61440 tokens, 4 + 1 heads of 32 in bf16, 25 and 41 us where a copy of as much takes 20 for both.)
 int tokens_per_block(int64_t tokens, int dim) {
   int n = kTurns / (dim / 2);
   if (n > kTokens) n = kTokens;

@@ -450,7 +450,9 @@ def range_attention(q, k, v, lo, hi, *, scale=None, cap=0.0, slopes=None):
     token_ranges gives them): (out, lse float32 [batch, heads, queries]).
     scale: of the products (None: head_dim ** -0.5); cap > 0 (below 1e30): scores become cap * tanh(score / cap);
     slopes (float32 [heads]): scores lose slopes[head] * |i + keys - queries - j|.  Queries that see
-    nothing get out 0 and lse -inf.  k, v may have fewer heads than q.  float16, bfloat16."""
+    nothing get out 0 and lse -inf.  k, v may have fewer heads than q.  float16, bfloat16.
+    Scores, statistics and sums are held in 32 bits; the probabilities are rounded to the inputs' type for their
+    product with v (and in the gradients with dout, as their own gradients are with k and q)."""
     return _hostops.range_attention(q, k, v, lo, hi, scale, float(cap), slopes)
 
 
