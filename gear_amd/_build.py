@@ -11,7 +11,7 @@ INCLUDE = os.path.join(_ROOT, "include")
 
 HIP_SOURCES = ["runtime.hip", "gather.hip", "scan.hip", "search.hip", "sort.hip", "topk.hip",
                "scatter.hip", "ranges.hip", "norm_rotate.hip", "attention.hip", "attention_grad.hip",
-               "attention_step.hip"]
+               "attention_step.hip", "embed.hip", "layer_norm.hip", "logits.hip"]
 LIBGEARHIP = os.path.join(_PKG, "libgearhip.so")
 
 # -packed-fp32-ops is switched off on purpose: hipcc -O3 otherwise forms v_pk_*_f32 from plain
@@ -100,7 +100,7 @@ def build_hostops():
           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I", INCLUDE] + inc +
          ["-isystem", sysconfig.get_paths()["include"]] +
-         [os.path.join(CSRC, "torchops", f) for f in ("ops.cc", "sequence.cc")] +
+         [os.path.join(CSRC, "torchops", f) for f in ("ops.cc", "sequence.cc", "tokens.cc")] +
          ["-o", out, "-L", _PKG, "-lgearhip", "-Wl,-rpath,$ORIGIN"] + lib +
          ["-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lamdhip64"])
     return out

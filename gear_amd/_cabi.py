@@ -46,6 +46,19 @@ class AttentionDesc(ctypes.Structure):
                 ("cap", ctypes.c_float)]
 
 
+class LayerNormDesc(ctypes.Structure):
+    """struct gear_hip_layer_norm_desc"""
+    _fields_ = [("x", c_void_p), ("residual", c_void_p), ("x_stride", c_i64), ("residual_stride", c_i64),
+                ("rows", c_i64), ("width", c_i64), ("weight", c_void_p), ("bias", c_void_p),
+                ("weight_f32", ctypes.c_int32), ("dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class LogitsDesc(ctypes.Structure):
+    """struct gear_hip_logits_desc"""
+    _fields_ = [("logits", c_void_p), ("row_stride", c_i64), ("rows", c_i64), ("vocab", c_i64),
+                ("dtype", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); one entry per function of include/gear_hip.h
 SIGNATURES = {
     "gear_hip_abi_version": (c_int, []),
@@ -151,6 +164,25 @@ SIGNATURES = {
     "gear_hip_attention_step_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
     "gear_hip_attention_step": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_void_p, c_size_t,
                                         c_void_p]),
+    "gear_hip_embed": (c_int, [c_void_p, c_int, c_i64, c_void_p, c_i64, c_i64, c_i64, c_int, ctypes.c_float,
+                               c_void_p, c_void_p]),
+    "gear_hip_embed_backward_workspace_bytes": (c_size_t, [c_i64, c_i64]),
+    "gear_hip_embed_backward": (c_int, [c_void_p, c_i64, c_void_p, c_int, c_i64, c_i64, c_i64, c_int,
+                                        ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "gear_hip_layer_norm": (c_int, [ctypes.POINTER(LayerNormDesc), c_void_p, c_void_p, c_void_p]),
+    "gear_hip_layer_norm_backward_workspace_bytes": (c_size_t, [c_i64, c_i64]),
+    "gear_hip_layer_norm_backward": (c_int, [ctypes.POINTER(LayerNormDesc), c_void_p, c_i64, c_void_p, c_i64,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "gear_hip_token_log_probs_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64]),
+    "gear_hip_token_log_probs": (c_int, [ctypes.POINTER(LogitsDesc), c_void_p, c_int, c_i64, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "gear_hip_token_log_probs_backward": (c_int, [ctypes.POINTER(LogitsDesc), c_void_p, c_void_p, c_void_p, c_int,
+                                                  c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gear_hip_distill_workspace_bytes": (c_size_t, [c_i64, c_i64]),
+    "gear_hip_distill": (c_int, [ctypes.POINTER(LogitsDesc), c_void_p, c_int, c_void_p, c_i64, c_void_p, c_void_p,
+                                 c_void_p, c_size_t, c_void_p]),
+    "gear_hip_distill_backward": (c_int, [ctypes.POINTER(LogitsDesc), c_void_p, c_void_p, c_int, c_void_p, c_i64,
+                                          c_void_p, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,831 @@
+// What is asked of rows of logits: log probabilities of given tokens, entropies, the best tokens, the divergence from a
+// teacher's best tokens, and the gradients (gear_hip_token_log_probs, gear_hip_distill and the calls beside them).
+//
+// With x a row, m its maximum, d_j = scale (x_j - m), S = sum exp d, A = sum d exp d:
+//   lse = scale m + log S,  log p_t = d_t - log S,  entropy = log S - A / S
+// which leaves no difference of large numbers.  A logit of -inf is a probability of 0 and has no part in A.  The
+// gradient is p_j (alpha + beta log p_j), with p as exact as lse is in 32 bits, plus what the given token (+dlogp) or the teacher's entries (-dloss q) add:
+// after the row is written the few columns concerned are written again.
+//
+// All are bound by memory: a row is read once and held in registers as it came, its maximum is taken before any exponential.
+// Rows of up to 256 vectors of 16 bytes: a wave or a part of one.  Wider ones: a workgroup for every part of a row of at
+// most 20 vectors a thread; rows in several parts (wide ones, and few ones, to fill the GPU) are joined by a second launch.
+//
+// The best k: groups of lanes have a maximum each, 64 in all; the k-th largest of those is a bound below which none of
+// the best k lies, so that few elements are left to be put in order.  Where more are left than a list holds (rows of equal
+// logits), or a row holds NaN or infinity, they are taken one after the other.
+#include <algorithm>
+
+#include "rows.hpp"
+
+namespace gearhip {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / kWave;
+constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxTop = 64;     // best tokens, and a teacher's entries
+constexpr int kHeld = 20;       // vectors of a thread
+constexpr int kList = 256;      // candidates for the best
+constexpr int kJoined = 4096;   // entries that a join puts in order
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLow = -1e30f;  // below any exponent that counts, and any logit that is allowed
+
+struct LogitsArgs {
+  const void *logits;
+  int64_t stride, rows;
+  int vocab;
+  float scale, scale2;  // scale2: scale log2 e
+  // log probabilities
+  const void *tokens;  // or null
+  int wide;            // tokens (and entries) in 64 bits
+  int top;
+  float *log_probs, *entropy, *lse, *top_log_probs;
+  int64_t *top_tokens;
+  // distillation
+  const void *entries;
+  const float *teacher;
+  int count;
+  float *loss;
+  // rows in parts
+  int parts, part_vecs;
+  float *stats;     // [rows][parts][4]: m, S, A
+  uint64_t *lists;  // [rows][parts][top]
+  // gradients
+  const float *dlog_probs, *dentropy, *dloss, *lse_in, *entropy_in;
+  void *dlogits;
+};
+
+enum { kLogProbs, kDistill };
+
+// ---- order: larger first, the lower index first among equals, NaN before all --------------------------------------
+__device__ __forceinline__ uint64_t entry_of(float x, int column) {
+  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 is 0)
+  const uint32_t key = x != x ? ~1u : (int32_t)b < 0 ? ~b : b | 0x80000000u;
+  return (uint64_t)key << 32 | (uint32_t)~column;
+}
+__device__ __forceinline__ float entry_value(uint64_t e) {
+  const uint32_t key = (uint32_t)(e >> 32);
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ int entry_column(uint64_t e) { return (int)~(uint32_t)e; }
+
+template <int kLanes>
+__device__ __forceinline__ uint64_t lanes_max64(uint64_t x) {
+#pragma unroll
+  for (int by = 1; by < kLanes; by *= 2) {
+    const uint64_t y = __shfl_xor((unsigned long long)x, by);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
+// ---- the statistics of a row ------------------------------------------------------------------------------------
+struct Stats {
+  float m, s, a;  // maximum, S, A / ln 2 (or 0)
+};
+// (m less itself is NaN for an infinite m: a row without a finite logit has S = 0 that way round)
+__device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <typename T>
+__device__ __forceinline__ Raw<T> nothing() {
+  Raw<T> x;
+#pragma unroll
+  for (int e = 0; e < kPer<T>; ++e) x[e] = (T)-INFINITY;
+  return x;
+}
+// a vector of a row, -inf where it has no elements of its own
+template <bool kNarrow, typename T>
+__device__ __forceinline__ Raw<T> load_logits(const T *row, int v, int vocab) {
+  const Slot<T> s(v, vocab);
+  if (!s.any()) return nothing<T>();
+  Raw<T> x = load_slot<kNarrow>(row, s);
+  if (!s.whole()) {
+#pragma unroll
+    for (int e = 0; e < kPer<T>; ++e)
+      if (!s.own(e)) x[e] = (T)-INFINITY;
+  }
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ float max_of(const Raw<T> &x) {
+  float m = (float)x[0];
+#pragma unroll
+  for (int e = 1; e < kPer<T>; ++e) m = fmaxf(m, (float)x[e]);
+  return m;
+}
+template <bool kEntropy, typename T>
+__device__ __forceinline__ void add_to(Stats &t, const Raw<T> &x, float shift, float scale2) {
+#pragma unroll
+  for (int e = 0; e < kPer<T>; ++e) {
+    const float d = ((float)x[e] - shift) * scale2, p = __builtin_amdgcn_exp2f(d);
+    t.s += p;
+    if (kEntropy) t.a = fmaf(fmaxf(d, kLow), p, t.a);
+  }
+}
+__device__ __forceinline__ Stats joined(const Stats &x, const Stats &y, float scale2) {
+  const float m = fmaxf(x.m, y.m), dx = fmaxf((x.m - shift_of(m)) * scale2, kLow), dy = fmaxf((y.m - shift_of(m)) * scale2, kLow);
+  const float ex = __builtin_amdgcn_exp2f(dx), ey = __builtin_amdgcn_exp2f(dy);
+  return Stats{m, x.s * ex + y.s * ey, fmaf(dx, x.s, x.a) * ex + fmaf(dy, y.s, y.a) * ey};
+}
+
+// ---- what is made of them ---------------------------------------------------------------------------------------
+struct Result {
+  float shift, log_s;
+  bool none;  // nothing is allowed (the lowest numbers of a type are as good a mask as -inf)
+  __device__ __forceinline__ Result(const Stats &t) : shift(shift_of(t.m)), log_s(__builtin_amdgcn_logf(t.s) * kLn2), none(t.m < kLow) {}
+  __device__ __forceinline__ float log_p(float x, float scale) const {
+    return none || x == -INFINITY ? -INFINITY : (x - shift) * scale - log_s;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float logit_at(const LogitsArgs &a, int64_t row, int64_t column) {
+  return (float)static_cast<const T *>(a.logits)[row * a.stride + column];
+}
+
+// by one lane
+template <typename T>
+__device__ __forceinline__ void finish_log_probs(const LogitsArgs &a, int64_t row, int64_t token, const Stats &t) {
+  const Result r(t);
+  if (a.log_probs) a.log_probs[row] = r.log_p(logit_at<T>(a, row, token), a.scale);
+  a.lse[row] = r.none ? -INFINITY : fmaf(a.scale, t.m, r.log_s);
+  a.entropy[row] = r.none ? 0.f : r.log_s - t.a / t.s * kLn2;
+}
+__device__ __forceinline__ void pass_over(const LogitsArgs &a, int64_t row) {
+  if (a.log_probs) a.log_probs[row] = 0;
+  if (a.entropy) a.entropy[row] = 0;
+  if (a.loss) a.loss[row] = 0;
+  a.lse[row] = 0;
+}
+__device__ __forceinline__ void put_best(const LogitsArgs &a, int64_t row, int at, uint64_t e, const Stats &t) {
+  a.top_log_probs[row * a.top + at] = e == 0 ? -INFINITY : Result(t).log_p(entry_value(e), a.scale);
+  a.top_tokens[row * a.top + at] = e == 0 ? -1 : entry_column(e);
+}
+
+// The teacher's entries of a row, lane by lane: entry k is lane k's, k + kLanes the same lane's next.
+struct Teacher {
+  float top, sum;
+  bool some;
+};
+__device__ __forceinline__ float teacher_at(const LogitsArgs &a, int64_t row, int k, int64_t &column) {
+  column = token_at(a.entries, a.wide, row * a.count + k, a.vocab);
+  return column < 0 ? -INFINITY : a.teacher[row * a.count + k];
+}
+template <int kLanes>
+__device__ __forceinline__ Teacher teacher_of(const LogitsArgs &a, int64_t row, int count, int lane) {
+  Teacher q{-INFINITY, 0.f, false};
+  float any = 0;
+  int64_t column;
+  for (int k = lane; k < count; k += kLanes) {
+    const float t = teacher_at(a, row, k, column);
+    q.top = fmaxf(q.top, t);
+    if (!(t == -INFINITY)) any = 1;
+  }
+  q.top = lanes_max<kLanes>(q.top);
+  q.some = lanes_max<kLanes>(any) > 0;
+  for (int k = lane; k < count; k += kLanes)
+    q.sum += __builtin_amdgcn_exp2f((teacher_at(a, row, k, column) - shift_of(q.top)) * kLog2e);
+  q.sum = lanes_sum<kLanes>(q.sum);
+  return q;
+}
+template <typename T, int kLanes>
+__device__ __forceinline__ void finish_distill(const LogitsArgs &a, int64_t row, int count, int lane, const Teacher &q,
+                                               const Stats &t) {
+  const Result r(t);
+  const float log_sum = __builtin_amdgcn_logf(q.sum) * kLn2, over = 1.f / q.sum;
+  float loss = 0;
+  for (int k = lane; k < count; k += kLanes) {
+    int64_t column;
+    const float l = teacher_at(a, row, k, column) - shift_of(q.top), p = __builtin_amdgcn_exp2f(l * kLog2e) * over;
+    if (column >= 0 && !(p == 0)) loss += p * (l - log_sum - r.log_p(logit_at<T>(a, row, column), a.scale));
+  }
+  loss = lanes_sum<kLanes>(loss);
+  if (lane == 0 && count > 0) {
+    a.loss[row] = loss;
+    a.lse[row] = r.none ? -INFINITY : fmaf(a.scale, t.m, r.log_s);
+  }
+}
+
+// ---- rows of a wave or less -------------------------------------------------------------------------------------
+template <typename T, int kLanes, int kVecs, int kKind>
+__global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
+  constexpr int kRows = kBlock / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  // (the lanes of a wave go round alike: they exchange sums)
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
+    const int64_t row = base + threadIdx.x / kLanes;
+    int64_t token = -1;
+    bool here = row < a.rows;
+    Teacher q{};
+    if (kKind == kDistill) {
+      q = teacher_of<kLanes>(a, row, here ? a.count : 0, lane);
+      if (here && !q.some && lane == 0) pass_over(a, row);
+      here = here && q.some;
+    } else if (here && a.tokens) {
+      token = token_at(a.tokens, a.wide, row, a.vocab);
+      if (token < 0) {
+        if (lane == 0) pass_over(a, row);
+        for (int k = lane; k < a.top; k += kLanes) put_best(a, row, k, 0, Stats{});
+        here = false;
+      }
+    }
+    Raw<T> x[kVecs];
+    Stats t{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      x[i] = here ? load_logits<true>(static_cast<const T *>(a.logits) + row * a.stride, lane + i * kLanes, a.vocab) : nothing<T>();
+      t.m = fmaxf(t.m, max_of<T>(x[i]));
+    }
+    t.m = lanes_max<kLanes>(t.m);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) add_to<kKind == kLogProbs, T>(t, x[i], shift_of(t.m), a.scale2);
+    t.s = lanes_sum<kLanes>(t.s);
+    if (kKind == kDistill) {
+      finish_distill<T, kLanes>(a, row, here ? a.count : 0, lane, q, t);
+      continue;
+    }
+    t.a = lanes_sum<kLanes>(t.a);
+    if (here && lane == 0) finish_log_probs<T>(a, row, token, t);
+    uint64_t last = ~0ull;
+    for (int k = 0; k < a.top; ++k) {
+      uint64_t best = 0;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const Slot<T> s(lane + i * kLanes, a.vocab);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) {
+          const uint64_t w = entry_of((float)x[i][e], s.col + e);
+          if (s.own(e) && w < last && w > best) best = w;
+        }
+      }
+      last = lanes_max64<kLanes>(best);
+      if (here && lane == k % kLanes) put_best(a, row, k, last, t);
+    }
+  }
+}
+
+// ---- rows, or parts of them, of a workgroup ---------------------------------------------------------------------
+template <typename F>
+__device__ __forceinline__ float block_reduce(float x, float *part, const F &f) {  // (x: of the wave)
+  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
+  __syncthreads();
+  x = part[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) x = f(x, part[w]);
+  return x;
+}
+
+struct WideSmem {
+  float max[kWaves], sum[2][kWaves], groups[kWave];
+  uint64_t best[2][kWaves];
+  uint64_t list[kList];
+  int count;
+  int some;
+};
+
+// The best `top` of what a workgroup holds, put(place, entry) for each; entries that are not there are 0.
+template <typename T, int kVecs, typename Put>
+__device__ __forceinline__ void best_of(const Raw<T> (&x)[kVecs], float mine, bool finite, int first, int last, int vocab, int top,
+                                        WideSmem &sm, const Put &put) {
+  // (the k-th largest of 64 maxima)
+  float g = fmaxf(mine, dpp_f32<0xB1>(mine));
+  g = fmaxf(g, dpp_f32<0x4E>(g));
+  if (threadIdx.x % 4 == 0) sm.groups[threadIdx.x / 4] = g;
+  if (threadIdx.x == 0) sm.count = 0;
+  __syncthreads();
+  const int lane = threadIdx.x % kWave;
+  g = sm.groups[lane];
+  int before = 0;
+#pragma unroll 8
+  for (int j = 0; j < kWave; ++j) {
+    const float other = sm.groups[j];
+    before += other > g || (other == g && j < lane);
+  }
+  const uint64_t which = __ballot(before == top - 1);
+  const float bound = which == 0 ? -INFINITY : sm.groups[__builtin_ctzll(which)];
+  if (finite && mine >= bound) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = first + threadIdx.x + i * kBlock;
+      if (v < last) {
+        const Slot<T> s(v, vocab);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e)
+          if ((float)x[i][e] >= bound && s.own(e)) {
+            const int at = atomicAdd(&sm.count, 1);
+            if (at < kList) sm.list[at] = entry_of((float)x[i][e], s.col + e);
+          }
+      }
+    }
+  }
+  __syncthreads();
+  const int count = sm.count;
+  if (finite && count <= kList) {
+    if ((int)threadIdx.x < count) {
+      const uint64_t w = sm.list[threadIdx.x];
+      int place = 0;
+      for (int j = 0; j < count; ++j) place += sm.list[j] > w;
+      if (place < top) put(place, w);
+    }
+    if ((int)threadIdx.x >= count && (int)threadIdx.x < top) put(threadIdx.x, 0ull);
+    return;
+  }
+  uint64_t limit = ~0ull;
+#pragma unroll 1
+  for (int k = 0; k < top; ++k) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = first + threadIdx.x + i * kBlock;
+      if (v < last) {
+        const Slot<T> s(v, vocab);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) {
+          const uint64_t w = entry_of((float)x[i][e], s.col + e);
+          if (s.own(e) && w < limit && w > best) best = w;
+        }
+      }
+    }
+    best = lanes_max64<kWave>(best);
+    if (lane == 0) sm.best[k & 1][threadIdx.x / kWave] = best;
+    __syncthreads();
+    limit = sm.best[k & 1][0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) limit = sm.best[k & 1][w] > limit ? sm.best[k & 1][w] : limit;
+    if ((int)threadIdx.x == k) put(k, limit);
+  }
+}
+
+template <typename T, int kVecs, int kKind, bool kTop>
+__global__ __launch_bounds__(kBlock) void wide_kernel(LogitsArgs a) {
+  __shared__ WideSmem sm;
+  const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
+  for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
+    const int64_t row = unit / a.parts;
+    const int part = (int)(unit - row * a.parts), first = part * a.part_vecs, last = min(first + a.part_vecs, vecs);
+    int64_t token = -1;
+    if (kKind == kLogProbs && a.tokens) {
+      token = token_at(a.tokens, a.wide, row, a.vocab);
+      if (token < 0) {  // (with several parts the launch that joins them sees to the row)
+        if (a.parts == 1) {
+          if (threadIdx.x == 0) pass_over(a, row);
+          if (kTop && (int)threadIdx.x < a.top) put_best(a, row, threadIdx.x, 0, Stats{});
+        }
+        continue;
+      }
+    }
+    Teacher q{};
+    if (kKind == kDistill) {
+      q = teacher_of<kWave>(a, row, a.count, threadIdx.x % kWave);
+      if (!q.some) {
+        if (a.parts == 1 && threadIdx.x == 0) pass_over(a, row);
+        continue;
+      }
+    }
+    Raw<T> x[kVecs];
+    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
+    float mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = first + threadIdx.x + i * kBlock;
+      x[i] = v < last ? load_logits<false>(from, v, a.vocab) : nothing<T>();
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (first + i * kBlock < last) mine = fmaxf(mine, max_of<T>(x[i]));
+    __syncthreads();  // (of the unit before: its shared memory)
+    Stats t{block_reduce(lanes_max<kWave>(mine), sm.max, [](float p, float r) { return fmaxf(p, r); }), 0.f, 0.f};
+    const float shift = shift_of(t.m);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (first + i * kBlock < last) add_to<kKind == kLogProbs, T>(t, x[i], shift, a.scale2);
+    auto plus = [](float p, float r) { return p + r; };
+    t.s = block_reduce(lanes_sum<kWave>(t.s), sm.sum[0], plus);
+    if (kKind == kLogProbs) t.a = block_reduce(lanes_sum<kWave>(t.a), sm.sum[1], plus);
+    if (a.parts > 1) {
+      if (threadIdx.x == 0) *reinterpret_cast<f32x4 *>(a.stats + unit * 4) = f32x4{t.m, t.s, t.a, 0.f};
+      if constexpr (kTop)
+        best_of<T, kVecs>(x, mine, t.s == t.s, first, last, a.vocab, a.top, sm,
+                          [&](int place, uint64_t e) { a.lists[unit * a.top + place] = e; });
+      continue;
+    }
+    if (kKind == kLogProbs) {
+      if (threadIdx.x == 0) finish_log_probs<T>(a, row, token, t);
+      if constexpr (kTop)
+        best_of<T, kVecs>(x, mine, t.s == t.s, first, last, a.vocab, a.top, sm,
+                          [&](int place, uint64_t e) { put_best(a, row, place, e, t); });
+    } else if (threadIdx.x < kWave) {
+      finish_distill<T, kWave>(a, row, a.count, threadIdx.x, q, t);
+    }
+  }
+}
+
+// Rows in several parts: a workgroup each.
+template <typename T, int kKind>
+__global__ __launch_bounds__(kBlock) void join_kernel(LogitsArgs a) {
+  __shared__ uint64_t lists[kKind == kLogProbs ? kJoined : 1];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    int64_t token = -1;
+    Teacher q{};
+    bool over;
+    if (kKind == kLogProbs) {
+      if (a.tokens) token = token_at(a.tokens, a.wide, row, a.vocab);
+      over = a.tokens && token < 0;
+    } else {
+      q = teacher_of<kWave>(a, row, a.count, threadIdx.x % kWave);
+      over = !q.some;
+    }
+    if (over) {
+      if (threadIdx.x == 0) pass_over(a, row);
+      if (kKind == kLogProbs && (int)threadIdx.x < a.top) put_best(a, row, threadIdx.x, 0, Stats{});
+      continue;
+    }
+    Stats t{-INFINITY, 0.f, 0.f};
+    for (int p = 0; p < a.parts; ++p) {
+      const f32x4 s = *reinterpret_cast<const f32x4 *>(a.stats + (row * a.parts + p) * 4);
+      t = joined(t, Stats{s[0], s[1], s[2]}, a.scale2);
+    }
+    if (kKind == kDistill) {
+      if (threadIdx.x < kWave) finish_distill<T, kWave>(a, row, a.count, threadIdx.x, q, t);
+      continue;
+    }
+    if (threadIdx.x == 0) finish_log_probs<T>(a, row, token, t);
+    if (a.top == 0) continue;
+    const int all = a.parts * a.top;
+    __syncthreads();  // (of the row before)
+    for (int i = threadIdx.x; i < all; i += kBlock) lists[i] = a.lists[row * all + i];
+    __syncthreads();
+    // an entry's place: how many of every part's, each in order, come before it
+    for (int i = threadIdx.x; i < all; i += kBlock) {
+      const uint64_t w = lists[i];
+      if (w == 0) continue;
+      int place = 0;
+      for (int p = 0; p < a.parts && place < a.top; ++p) {
+        int lo = 0, hi = a.top;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (lists[p * a.top + mid] > w)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        place += lo;
+      }
+      if (place < a.top) put_best(a, row, place, w, t);
+    }
+  }
+}
+
+// ---- gradients --------------------------------------------------------------------------------------------------
+// p (alpha + beta log p) of a logit, times the scale
+struct Slope {
+  float lse, scale, alpha, beta;
+  __device__ __forceinline__ float at(float x) const {
+    // (above 0 only by what lse lost when it was rounded, where logits are huge)
+    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale, -lse), kLow, 0.f), p = __builtin_amdgcn_exp2f(l * kLog2e);
+    return p * fmaf(beta, l, alpha);
+  }
+};
+
+// Of a row: whether it has a gradient at all, its slope, and what is added at the given token.
+template <int kKind>
+__device__ __forceinline__ bool slope_of(const LogitsArgs &a, int64_t row, bool some, int64_t token, Slope &s, float &more) {
+  if (kKind == kLogProbs ? a.tokens && token < 0 : !some) return false;
+  s.lse = a.lse_in[row];
+  if (s.lse == -INFINITY) return false;  // nothing was allowed
+  s.scale = a.scale;
+  const float nan = s.lse - s.lse;       // 0, or NaN for a row of NaN
+  if (kKind == kLogProbs) {
+    const float dl = a.dlog_probs ? a.dlog_probs[row] : 0.f, de = a.dentropy ? a.dentropy[row] : 0.f;
+    s.alpha = -a.scale * (dl + (a.dentropy ? de * a.entropy_in[row] : 0.f)) + nan;
+    s.beta = -a.scale * de;
+    more = a.scale * dl;
+  } else {
+    s.alpha = a.scale * a.dloss[row] + nan, s.beta = 0;
+    more = -s.alpha;
+  }
+  return true;
+}
+
+struct Fix {
+  int column;  // or -1
+  float q;
+};
+// The entries of a teacher that stand for columns of their own, with the weights of those that name the same.
+template <int kLanes>
+__device__ __forceinline__ Teacher teacher_fixes(const LogitsArgs &a, int64_t row, int count, int lane, bool write, Fix *fix) {
+  const Teacher q = teacher_of<kLanes>(a, row, count, lane);
+  const float over = 1.f / q.sum;
+  for (int k = lane; k < count && write; k += kLanes) {
+    int64_t column;
+    const float t = teacher_at(a, row, k, column);
+    fix[k] = Fix{(int)column, column < 0 ? 0.f : __builtin_amdgcn_exp2f((t - shift_of(q.top)) * kLog2e) * over};
+  }
+  return q;
+}
+__device__ __forceinline__ Fix fix_of(const Fix *fix, int k, int count) {
+  Fix f = fix[k];
+  for (int j = 0; j < count && f.column >= 0; ++j) {
+    if (j == k || fix[j].column != f.column) continue;
+    if (j < k) f.column = -1;
+    f.q += fix[j].q;
+  }
+  return f;
+}
+
+template <typename T, int kLanes, int kKind>
+__global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
+  constexpr int kRows = kBlock / kLanes;
+  __shared__ Fix fixes[kKind == kDistill ? kRows : 1][kMaxTop];
+  const int lane = threadIdx.x % kLanes;
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
+    const int64_t row = base + threadIdx.x / kLanes;
+    const bool here = row < a.rows;
+    Fix *fix = fixes[kKind == kDistill ? threadIdx.x / kLanes : 0];
+    int64_t token = -1;
+    bool some = false;
+    if (kKind == kDistill) {
+      __syncthreads();
+      some = teacher_fixes<kLanes>(a, row, here ? a.count : 0, lane, true, fix).some;
+    } else if (here && a.tokens) {
+      token = token_at(a.tokens, a.wide, row, a.vocab);
+    }
+    Slope slope{};
+    float more = 0;
+    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
+    T *to = static_cast<T *>(a.dlogits) + row * a.vocab;
+    const bool live = here && slope_of<kKind>(a, row, some, token, slope, more);
+    if (here) {
+      for (int v = lane; v * kPer<T> < a.vocab; v += kLanes) {
+        const Slot<T> s(v, a.vocab);
+        Vals<T> y = {};
+        if (live) {
+          y = __builtin_convertvector(load_slot<true>(from, s), Vals<T>);
+#pragma unroll
+          for (int e = 0; e < kPer<T>; ++e) {
+            y[e] = slope.at(y[e]);
+            if (kKind == kLogProbs && s.col + e == token) y[e] += more;
+          }
+        }
+        store_slot(to, s, y);
+      }
+    }
+    if (kKind == kDistill) {
+      __syncthreads();  // the entries are there, and the row is written
+      if (live)
+        for (int k = lane; k < a.count; k += kLanes) {
+          const Fix f = fix_of(fix, k, a.count);
+          if (f.column >= 0) to[f.column] = (T)fmaf(more, f.q, slope.at((float)from[f.column]));
+        }
+    }
+  }
+}
+
+constexpr int kGradVecs = 8;  // vectors of a thread
+template <typename T, int kKind>
+__global__ __launch_bounds__(kBlock) void wide_grad_kernel(LogitsArgs a) {
+  __shared__ Fix fix[kMaxTop];
+  const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
+  for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
+    const int64_t row = unit / a.parts;
+    const int part = (int)(unit - row * a.parts), first = part * kGradVecs * kBlock, last = min(first + kGradVecs * kBlock, vecs);
+    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
+    T *to = static_cast<T *>(a.dlogits) + row * a.vocab;
+    int64_t token = -1;
+    bool some = false;
+    if (kKind == kDistill) {
+      __syncthreads();
+      some = teacher_fixes<kWave>(a, row, a.count, threadIdx.x % kWave, threadIdx.x < kWave, fix).some;
+    } else if (a.tokens) {
+      token = token_at(a.tokens, a.wide, row, a.vocab);
+    }
+    Slope slope{};
+    float more = 0;
+    const bool live = slope_of<kKind>(a, row, some, token, slope, more);
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i) {
+      const int v = first + threadIdx.x + i * kBlock;
+      if (v >= last) continue;
+      const Slot<T> s(v, a.vocab);
+      Vals<T> y = {};
+      if (live) {
+        y = __builtin_convertvector(load_slot<false>(from, s), Vals<T>);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) {
+          y[e] = slope.at(y[e]);
+          if (kKind == kLogProbs && s.col + e == token) y[e] += more;
+        }
+      }
+      store_slot(to, s, y);
+    }
+    if (kKind == kDistill) {
+      __syncthreads();  // the entries are there, and the part is written
+      if (live && (int)threadIdx.x < a.count) {
+        const Fix f = fix_of(fix, threadIdx.x, a.count);
+        if (f.column >= first * kPer<T> && f.column < last * kPer<T>)
+          to[f.column] = (T)fmaf(more, f.q, slope.at((float)from[f.column]));
+      }
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------
+constexpr int kWaveVecs = 256;  // widest row of a wave
+// Parts of a row: what a workgroup holds at most, and more where rows are few, down to two vectors a thread.
+void split(int64_t rows, int vecs, int &parts, int &part_vecs) {
+  int n = (vecs + kHeld * kBlock - 1) / (kHeld * kBlock);
+  if (rows < 1024) {
+    const int64_t fill = 1024 / rows, most = vecs / (2 * kBlock);
+    n = (int)std::max<int64_t>(n, std::min(std::min(fill, most), (int64_t)kJoined / kMaxTop));
+  }
+  part_vecs = (vecs + n - 1) / n;
+  parts = (vecs + part_vecs - 1) / part_vecs;
+}
+// (of the type with most vectors: the workspace does not go by the type)
+size_t split_bytes(int64_t rows, int64_t vocab, int64_t top) {
+  if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab || top < 0 || top > kMaxTop) return 0;
+  size_t most = 0;
+  for (const int per : {4, 8}) {
+    int parts, each;
+    split(rows, (int)((vocab + per - 1) / per), parts, each);
+    if (parts > 1) most = std::max(most, align_up((size_t)rows * parts * 16, 256) + (size_t)rows * parts * (size_t)top * 8);
+  }
+  return most;
+}
+
+// f(lanes of a row, vectors of a lane) for rows of a wave or less
+template <typename F>
+void by_lanes(int vecs, const F &f) {
+  if (vecs <= 4)
+    f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+  else if (vecs <= 16)
+    f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+  else if (vecs <= 64)
+    f(std::integral_constant<int, 32>(), std::integral_constant<int, 2>());
+  else
+    f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+}
+
+int64_t grid_of(int64_t blocks) { return std::min(blocks, kMostItems / kBlock); }
+
+template <int kKind>
+int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
+  by_type(dtype, [&](auto type) {
+    using T = decltype(type);
+    const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
+    if (vecs <= kWaveVecs) {
+      by_lanes(vecs, [&](auto lanes, auto held) {
+        constexpr int kLanes = decltype(lanes)::value;
+        hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind>),
+                           dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))), dim3(kBlock), 0, st, a);
+      });
+      return;
+    }
+    split(a.rows, vecs, a.parts, a.part_vecs);
+    a.stats = reinterpret_cast<float *>(ws);
+    a.lists = reinterpret_cast<uint64_t *>(ws + align_up((size_t)a.rows * a.parts * 16, 256));
+    const dim3 grid((unsigned)grid_of(a.rows * a.parts)), block(kBlock);
+    auto launch = [&](auto held) {
+      constexpr int kVecs = decltype(held)::value;
+      if (kKind == kLogProbs && a.top > 0)
+        hipLaunchKernelGGL((wide_kernel<T, kVecs, kKind, kKind == kLogProbs>), grid, block, 0, st, a);
+      else
+        hipLaunchKernelGGL((wide_kernel<T, kVecs, kKind, false>), grid, block, 0, st, a);
+    };
+    if (a.part_vecs <= 4 * kBlock)
+      launch(std::integral_constant<int, 4>());
+    else if (a.part_vecs <= 8 * kBlock)
+      launch(std::integral_constant<int, 8>());
+    else
+      launch(std::integral_constant<int, kHeld>());
+    if (a.parts > 1)
+      hipLaunchKernelGGL((join_kernel<T, kKind>), dim3((unsigned)grid_of(a.rows)), block, 0, st, a);
+  });
+  GEARHIP_RETURN_IF_LAUNCH_FAILED();
+  return 0;
+}
+
+template <int kKind>
+int backward(LogitsArgs &a, int dtype, hipStream_t st) {
+  by_type(dtype, [&](auto type) {
+    using T = decltype(type);
+    const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
+    if (vecs <= kWaveVecs) {
+      by_lanes(vecs, [&](auto lanes, auto) {
+        constexpr int kLanes = decltype(lanes)::value;
+        hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, kKind>), dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))),
+                           dim3(kBlock), 0, st, a);
+      });
+      return;
+    }
+    a.parts = (vecs + kGradVecs * kBlock - 1) / (kGradVecs * kBlock);
+    hipLaunchKernelGGL((wide_grad_kernel<T, kKind>), dim3((unsigned)grid_of(a.rows * a.parts)), dim3(kBlock), 0, st, a);
+  });
+  GEARHIP_RETURN_IF_LAUNCH_FAILED();
+  return 0;
+}
+
+// 0: go on; 1: nothing to do; else the error
+int prepare(const gear_hip_logits_desc *d, LogitsArgs &a) {
+  if (d == nullptr || d->rows < 0 || d->vocab < 1 || element_bytes(d->dtype) == 0 || !(d->scale > 0) || !(d->scale < 1e30f))
+    return GEAR_HIP_EINVAL;
+  if (d->vocab > kMaxVocab || d->rows >= (int64_t)1 << 31) return GEAR_HIP_ERANGE;
+  if (d->rows == 0) return 1;
+  if (d->logits == nullptr) return GEAR_HIP_EINVAL;
+  if (!aligned_to(d->logits, element_bytes(d->dtype))) return GEAR_HIP_EALIGN;
+  a.logits = d->logits, a.stride = d->row_stride, a.rows = d->rows, a.vocab = (int)d->vocab;
+  a.scale = d->scale, a.scale2 = d->scale * kLog2e;
+  return 0;
+}
+int enough(void *workspace, size_t bytes, size_t need) {
+  if (need > 0 && (workspace == nullptr || bytes < need)) return GEAR_HIP_EWORKSPACE;
+  if (need > 0 && !aligned_to(workspace, 256)) return GEAR_HIP_EALIGN;
+  return 0;
+}
+
+}  // namespace
+}  // namespace gearhip
+
+using namespace gearhip;
+
+extern "C" size_t gear_hip_token_log_probs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
+  return split_bytes(rows, vocab, top);
+}
+
+extern "C" int gear_hip_token_log_probs(const gear_hip_logits_desc *desc, const void *tokens, int tokens_i64, int64_t top,
+                                        float *log_probs, float *entropy, float *lse, float *top_log_probs, int64_t *top_tokens,
+                                        void *workspace, size_t workspace_bytes, void *stream) {
+  LogitsArgs a = {};
+  const int rc = prepare(desc, a);
+  if (rc < 0) return rc;
+  if (top < 0 || top > desc->vocab) return GEAR_HIP_EINVAL;
+  if (top > kMaxTop) return GEAR_HIP_ERANGE;
+  if (rc == 1) return 0;
+  if ((tokens == nullptr) != (log_probs == nullptr)) return GEAR_HIP_EINVAL;
+  if (entropy == nullptr || lse == nullptr || (top > 0 && (top_log_probs == nullptr || top_tokens == nullptr))) return GEAR_HIP_EINVAL;
+  if (!aligned_to(tokens, tokens_i64 ? 8 : 4) || !aligned_to(log_probs, 4) || !aligned_to(entropy, 4) || !aligned_to(lse, 4) ||
+      !aligned_to(top_log_probs, 4) || !aligned_to(top_tokens, 8))
+    return GEAR_HIP_EALIGN;
+  const int ws = enough(workspace, workspace_bytes, split_bytes(a.rows, a.vocab, top));
+  if (ws != 0) return ws;
+  a.tokens = tokens, a.wide = tokens_i64 != 0, a.top = (int)top;
+  a.log_probs = log_probs, a.entropy = entropy, a.lse = lse, a.top_log_probs = top_log_probs, a.top_tokens = top_tokens;
+  return forward<kLogProbs>(a, desc->dtype, static_cast<char *>(workspace), as_stream(stream));
+}
+
+extern "C" int gear_hip_token_log_probs_backward(const gear_hip_logits_desc *desc, const float *dlog_probs, const float *dentropy,
+                                                 const void *tokens, int tokens_i64, const float *lse, const float *entropy,
+                                                 void *dlogits, void *stream) {
+  LogitsArgs a = {};
+  const int rc = prepare(desc, a);
+  if (rc != 0) return rc < 0 ? rc : 0;
+  if (lse == nullptr || dlogits == nullptr || (dlog_probs != nullptr && tokens == nullptr) || (dentropy != nullptr && entropy == nullptr))
+    return GEAR_HIP_EINVAL;
+  if (!aligned_to(tokens, tokens_i64 ? 8 : 4) || !aligned_to(dlogits, element_bytes(desc->dtype)) || !aligned_to(dlog_probs, 4) ||
+      !aligned_to(dentropy, 4) || !aligned_to(lse, 4) || !aligned_to(entropy, 4))
+    return GEAR_HIP_EALIGN;
+  a.tokens = tokens, a.wide = tokens_i64 != 0;
+  a.dlog_probs = dlog_probs, a.dentropy = dentropy, a.lse_in = lse, a.entropy_in = entropy, a.dlogits = dlogits;
+  return backward<kLogProbs>(a, desc->dtype, as_stream(stream));
+}
+
+extern "C" size_t gear_hip_distill_workspace_bytes(int64_t rows, int64_t vocab) { return split_bytes(rows, vocab, 0); }
+
+namespace {
+int entries(LogitsArgs &a, const void *top_tokens, int tokens_i64, const float *top_logits, int64_t count) {
+  if (count < 1 || top_tokens == nullptr || top_logits == nullptr) return GEAR_HIP_EINVAL;
+  if (count > kMaxTop) return GEAR_HIP_ERANGE;
+  if (!aligned_to(top_tokens, tokens_i64 ? 8 : 4) || !aligned_to(top_logits, 4)) return GEAR_HIP_EALIGN;
+  a.entries = top_tokens, a.wide = tokens_i64 != 0, a.teacher = top_logits, a.count = (int)count;
+  return 0;
+}
+}  // namespace
+
+extern "C" int gear_hip_distill(const gear_hip_logits_desc *desc, const void *top_tokens, int tokens_i64, const float *top_logits,
+                                int64_t count, float *loss, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+  LogitsArgs a = {};
+  int rc = prepare(desc, a);
+  if (rc != 0) return rc < 0 ? rc : 0;
+  rc = entries(a, top_tokens, tokens_i64, top_logits, count);
+  if (rc != 0) return rc;
+  if (loss == nullptr || lse == nullptr) return GEAR_HIP_EINVAL;
+  if (!aligned_to(loss, 4) || !aligned_to(lse, 4)) return GEAR_HIP_EALIGN;
+  rc = enough(workspace, workspace_bytes, split_bytes(a.rows, a.vocab, 0));
+  if (rc != 0) return rc;
+  a.loss = loss, a.lse = lse;
+  return forward<kDistill>(a, desc->dtype, static_cast<char *>(workspace), as_stream(stream));
+}
+
+extern "C" int gear_hip_distill_backward(const gear_hip_logits_desc *desc, const float *dloss, const void *top_tokens, int tokens_i64,
+                                         const float *top_logits, int64_t count, const float *lse, void *dlogits, void *stream) {
+  LogitsArgs a = {};
+  int rc = prepare(desc, a);
+  if (rc != 0) return rc < 0 ? rc : 0;
+  rc = entries(a, top_tokens, tokens_i64, top_logits, count);
+  if (rc != 0) return rc;
+  if (dloss == nullptr || lse == nullptr || dlogits == nullptr) return GEAR_HIP_EINVAL;
+  if (!aligned_to(dloss, 4) || !aligned_to(lse, 4) || !aligned_to(dlogits, element_bytes(desc->dtype))) return GEAR_HIP_EALIGN;
+  a.dloss = dloss, a.lse_in = lse, a.dlogits = dlogits;
+  return backward<kDistill>(a, desc->dtype, as_stream(stream));
+}

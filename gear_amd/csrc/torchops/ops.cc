@@ -13,6 +13,7 @@
 using namespace gear_hostops;
 
 void bind_sequence(py::module_ &m);  // sequence.cc
+void bind_tokens(py::module_ &m);    // tokens.cc
 
 namespace {
 
@@ -618,4 +619,5 @@ PYBIND11_MODULE(_hostops, m) {
            py::arg("index_offset"), py::arg("timesteps"), py::arg("host_timesteps"), py::arg("ws"),
            py::arg("to_draw") = -1);
   bind_sequence(m);
+  bind_tokens(m);
 }

@@ -465,3 +465,59 @@ def range_attention_step(q, k_cache, v_cache, lo, hi, *, scale=None, cap=0.0, sl
     """range_attention for the newest tokens of rollouts over their caches: out.  The distance that
     slopes count is the one from the last key a query sees, |hi - 1 - j|."""
     return _hostops.range_attention_step(q, k_cache, v_cache, lo, hi, scale, float(cap), slopes, _ws)
+
+
+# ---- tokens: into a sequence model and out of it -----------------------------------------------
+# Tokens are int64 or int32; one outside the vocabulary (-1) stands for none, as padding does.  Rows are the last
+# dimension of a tensor, contiguous and at one stride (a slice of a projection's output is).  float32, float16,
+# bfloat16; sums and statistics are held in 32 bits, and results are the same bits on every run.
+
+def embed_tokens(tokens, table, *, scale=1.0):
+    """scale * table[tokens] ([..., width] of the table's type); rows of zeros where there is no token."""
+    return _hostops.embed_tokens(tokens, table, float(scale))
+
+
+def embed_tokens_backward(dout, tokens, vocab, *, scale=1.0):
+    """Gradient [vocab, width] of embed_tokens' table, in the type of dout: every token's rows summed in 32 bits, in
+    the order in which they lie; zeros for tokens that do not occur."""
+    return _hostops.embed_tokens_backward(dout, tokens, int(vocab), float(scale), _ws)
+
+
+def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
+    """Rows of x (at most 16384 wide) less their mean over their deviation, times a weight, plus a bias (of the rows'
+    type or float32).  With a residual (y, sum): sum = x + residual, of which the norm is taken, is returned as well."""
+    return _hostops.layer_norm(x, weight, bias, residual, float(eps))
+
+
+def layer_norm_backward(dy, x, weight=None, bias=None, *, dsum=None, eps=1e-5):
+    """Gradients of layer_norm: (dx, dweight, dbias); None where there is no weight or bias.  After a norm with a
+    residual x is its sum, dsum the gradient of the sum (None: none), and dx is the gradient of both inputs."""
+    return _hostops.layer_norm_backward(dy, x, weight, bias, dsum, float(eps), _ws)
+
+
+def token_log_probs(logits, tokens=None, *, scale=1.0, top=0):
+    """What softmax(scale * logits) says, all float32 [...]: (log_probs of the given tokens, entropy, lse,
+    top_log_probs [..., top], top_tokens int64 [..., top]); None for what was not asked for.
+    lse: the logarithm of the sum of exponentials, for the gradient.  top (at most 64): the largest logits, the lower
+    token first among equals, NaN before all.  A logit of -inf is a token that is not allowed; a row that allows none (no logit of -1e30 or
+    more) has lse -inf, log probabilities of -inf and entropy 0.  With tokens, a row whose token is none is passed over: 0, 0, 0, top -inf and -1."""
+    return _hostops.token_log_probs(logits, tokens, float(scale), int(top), _ws)
+
+
+def token_log_probs_backward(dlog_probs, dentropy, logits, tokens, lse, entropy, *, scale=1.0):
+    """Gradient of token_log_probs' logits, in their type, from its lse and entropy; dlog_probs, or dentropy, may be
+    None.  Zeros for rows that are passed over and rows that allow nothing."""
+    return _hostops.token_log_probs_backward(dlog_probs, dentropy, logits, tokens, lse, entropy, float(scale))
+
+
+def distill(logits, top_tokens, top_logits, *, scale=1.0):
+    """Divergence of softmax(scale * logits) from a teacher's best tokens: (loss, lse), float32 [...].
+    top_tokens, top_logits (float32) [..., count], count at most 64: as token_log_probs' top gives them (logarithms of
+    probabilities, or logits times the teacher's own scale: q is their softmax over the row's entries).  loss =
+    sum of q (log q - log p[top_tokens]).  Entries whose token is none have no part, rows without any are passed over: 0."""
+    return _hostops.distill(logits, top_tokens, top_logits, float(scale), _ws)
+
+
+def distill_backward(dloss, logits, top_tokens, top_logits, lse, *, scale=1.0):
+    """Gradient of distill's logits, in their type, from its lse (the teacher has none)."""
+    return _hostops.distill_backward(dloss, logits, top_tokens, top_logits, lse, float(scale))

@@ -5,6 +5,12 @@ small causal model of observations and actions that uses them as they are meant 
     queries, keys      --norm_rotate--->  range_attention          (a batch of windows, with gradients)
                        --norm_rotate_append--> range_attention_step  (the next step of rollouts, from caches)
 
+and the same for windows whose observations and actions are tokens:
+
+    tokens --embed_tokens--> [layer_norm, attention, layer_norm with the sum]... --> logits
+    logits --token_log_probs--> log probabilities of actions, entropies, the best few (acting; a teacher's say)
+           --distill----------> the divergence from a teacher's best few
+
 No counterpart in the reference, whose loader hands its batches to models outside of it
 (gear/loader/offline_loader.py:155-204)."""
 import torch
@@ -67,6 +73,120 @@ def range_attention(q, k, v, lo, hi, *, scale=None, cap=0.0, slopes=None):
     return _RangeAttention.apply(q, k, v, lo, hi, scale, cap, slopes)
 
 
+def _matrix(t):
+    """A gradient as it comes, with rows at one stride."""
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    fits = t.stride(-1) == 1 and all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:]))
+    return t if fits else t.contiguous()
+
+
+class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, table, scale):
+        ctx.save_for_backward(tokens)
+        ctx.form = (table.shape[0], scale)
+        return ops.embed_tokens(tokens, table, scale=scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        vocab, scale = ctx.form
+        return None, ops.embed_tokens_backward(_matrix(dout), ctx.saved_tensors[0], vocab, scale=scale), None
+
+
+def embed_tokens(tokens, table, *, scale=1.0):
+    """gear_amd.ops.embed_tokens with the gradient of the table."""
+    return _EmbedTokens.apply(tokens, table, scale)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        ctx.save_for_backward(x, weight, bias)
+        ctx.eps = eps
+        return ops.layer_norm(x, weight, bias, eps=eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias = ctx.saved_tensors
+        return ops.layer_norm_backward(_matrix(dy), x, weight, bias, eps=ctx.eps) + (None,)
+
+
+class _SumNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        y, total = ops.layer_norm(x, weight, bias, residual=residual, eps=eps)
+        ctx.save_for_backward(total, weight, bias)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return y, total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dsum):
+        total, weight, bias = ctx.saved_tensors
+        if dy is None:
+            return dsum, dsum, None, None, None
+        dx, dweight, dbias = ops.layer_norm_backward(_matrix(dy), total, weight, bias,
+                                                     dsum=None if dsum is None else _matrix(dsum), eps=ctx.eps)
+        return dx, dx, dweight, dbias, None
+
+
+def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
+    """gear_amd.ops.layer_norm with gradients of x, the residual, the weight and the bias."""
+    if residual is None:
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _SumNorm.apply(x, residual, weight, bias, eps)
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, scale, top):
+        outs = ops.token_log_probs(logits, tokens, scale=scale, top=top)
+        ctx.save_for_backward(logits, tokens, outs[2], outs[1])
+        ctx.scale = scale
+        ctx.mark_non_differentiable(*(t for t in outs[2:] if t is not None))
+        ctx.set_materialize_grads(False)
+        return outs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlog_probs, dentropy, *_):
+        if dlog_probs is None and dentropy is None:
+            return None, None, None, None
+        logits, tokens, lse, entropy = ctx.saved_tensors
+        dlog_probs, dentropy = (None if t is None else t.contiguous() for t in (dlog_probs, dentropy))
+        return ops.token_log_probs_backward(dlog_probs, dentropy, logits, tokens, lse, entropy, scale=ctx.scale), None, None, None
+
+
+def token_log_probs(logits, tokens=None, *, scale=1.0, top=0):
+    """gear_amd.ops.token_log_probs with the gradient of the logits through the log probabilities and the entropy (lse
+    and the best tokens are constants)."""
+    return _TokenLogProbs.apply(logits, tokens, scale, top)
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_tokens, top_logits, scale):
+        loss, lse = ops.distill(logits, top_tokens, top_logits, scale=scale)
+        ctx.save_for_backward(logits, top_tokens, top_logits, lse)
+        ctx.scale = scale
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        return ops.distill_backward(dloss.contiguous(), *ctx.saved_tensors, scale=ctx.scale), None, None, None
+
+
+def distill(logits, top_tokens, top_logits, *, scale=1.0):
+    """The loss of gear_amd.ops.distill with the gradient of the logits (the teacher is a constant)."""
+    if top_logits.requires_grad:
+        raise ValueError("top_logits have no gradient: pass them detached")
+    return _Distill.apply(logits, top_tokens, top_logits, scale)
+
+
 class _Block(nn.Module):
     def __init__(self, width, heads, kv_heads):
         super().__init__()
@@ -78,7 +198,10 @@ class _Block(nn.Module):
         self.mlp = nn.Sequential(nn.Linear(width, 4 * width), nn.GELU(), nn.Linear(4 * width, width))
 
     def split(self, x, dtype):
-        qkv = self.qkv(self.before(x)).to(dtype).view(*x.shape[:2], -1, self.dim)
+        return self.project(self.before(x), dtype)
+
+    def project(self, y, dtype):
+        qkv = self.qkv(y).to(dtype).view(*y.shape[:2], -1, self.dim)
         return qkv.split([self.heads, self.kv_heads, self.kv_heads], 2)
 
     def weights(self, dtype):
@@ -92,7 +215,7 @@ class _Block(nn.Module):
 
 class Rollouts:
     """The caches of a batch of rollouts: per layer keys and values of up to `tokens` tokens, and how many are there.
-    A step is two tokens, the first of a rollout one."""
+    A step is as many tokens as the model has a step, the first of a rollout one less."""
 
     def __init__(self, model, batch, tokens):
         self.tokens, self.taken = tokens, 0  # (known here as well: no step waits for the GPU to compare them)
@@ -109,7 +232,24 @@ class Rollouts:
         self.time.zero_()
 
 
-class WindowModel(nn.Module):
+class _Positions(nn.Module):
+    """A model whose heads are rotated by their tokens' positions."""
+
+    def positions(self, dim):
+        pairs = dim // 2
+        self.sections = (pairs - pairs // 4, 0, pairs // 4)
+        self.register_buffer("freqs", ops.rotation_freqs(self.sections, device="cpu"), persistent=False)
+
+    def _apply(self, *args, **kwargs):
+        """Casts are for the parameters: the frequencies stay in 64 bits, and go along to another device."""
+        freqs = self.freqs
+        super()._apply(*args, **kwargs)
+        device = self.freqs.device
+        self.freqs = ops.rotation_freqs(self.sections, device=device) if freqs.is_meta else freqs.to(device)
+        return self
+
+
+class WindowModel(_Positions):
     """Predicts each step's action from the window's observations and actions up to it.
 
     A step is two tokens, observation then action; a token sees its document (the window's valid steps up to the
@@ -124,17 +264,7 @@ class WindowModel(nn.Module):
         self.embed = nn.ModuleList([nn.Linear(observation, width), nn.Linear(action, width)])
         self.blocks = nn.ModuleList(_Block(width, heads, kv_heads) for _ in range(layers))
         self.head = nn.Sequential(nn.LayerNorm(width), nn.Linear(width, action))
-        pairs = width // heads // 2
-        self.sections = (pairs - pairs // 4, 0, pairs // 4)
-        self.register_buffer("freqs", ops.rotation_freqs(self.sections, device="cpu"), persistent=False)
-
-    def _apply(self, *args, **kwargs):
-        """Casts are for the parameters: the frequencies stay in 64 bits, and go along to another device."""
-        freqs = self.freqs
-        super()._apply(*args, **kwargs)
-        device = self.freqs.device
-        self.freqs = ops.rotation_freqs(self.sections, device=device) if freqs.is_meta else freqs.to(device)
-        return self
+        self.positions(width // heads)
 
     def forward(self, observations, actions, mask, done):
         """observations [batch, steps, ...], actions, the loader's mask, the done column -> actions [batch, steps, ...]."""
@@ -173,3 +303,96 @@ class WindowModel(nn.Module):
         rollouts.length += new
         rollouts.time += 1
         return self.head(x[:, -1])
+
+
+class TokenModel(_Positions):
+    """A causal policy over tokens: a step is `step` of them, its observation's (in bins, patches, words) and its action
+    last; from the tokens up to an action comes the distribution of that action.  Ends of episodes and padding are
+    those of WindowModel.  Everything runs in the parameters' type (32, 16 bits or bfloat16), attention in `dtype`."""
+
+    def __init__(self, vocab, step, width=128, heads=4, kv_heads=2, layers=2, cap=30.0, dtype=torch.bfloat16):
+        super().__init__()
+        if step < 2:
+            raise ValueError("a step needs two tokens at least, an observation's and its action")
+        self.step_tokens, self.width, self.dtype, self.cap = step, width, dtype, cap
+        self.table = nn.Parameter(torch.randn(vocab, width) * width ** -0.5)
+        self.blocks = nn.ModuleList(_Block(width, heads, kv_heads) for _ in range(layers))
+        self.norm = nn.LayerNorm(width)
+        self.head = nn.Linear(width, vocab, bias=False)
+        self.positions(width // heads)
+
+    @staticmethod
+    def _norm(norm, x, residual=None):
+        return layer_norm(x, norm.weight, norm.bias, residual=residual, eps=norm.eps)
+
+    def _logits(self, tokens, attend, actions):
+        """tokens [batch, tokens]; attend(layer, block, q, k, v) -> [batch, tokens, heads, dim]; actions(x) picks the rows
+        that an action is read from."""
+        x = embed_tokens(tokens, self.table, scale=self.width ** 0.5)
+        y = self._norm(self.blocks[0].before, x)
+        for i, block in enumerate(self.blocks):
+            attended = attend(i, block, *block.project(y, self.dtype)).flatten(2).to(x.dtype)
+            y, x = self._norm(block.between, block.out(attended), x)
+            more = block.mlp(y)
+            if i + 1 < len(self.blocks):
+                y, x = self._norm(self.blocks[i + 1].before, more, x)
+        return self.head(self._norm(self.norm, actions(more), actions(x))[0])
+
+    def forward(self, tokens, mask, done):
+        """tokens [batch, steps, step], the loader's mask, the done column -> logits [batch, steps, vocab] of every
+        step's action."""
+        batch, steps, n = tokens.shape
+        lo, hi, pos = ops.token_ranges(mask, done, tokens_per_step=n, mode="causal", grid=(1, n))
+
+        def attend(_, block, q, k, v):
+            q, k = norm_rotate(q, k, pos, self.freqs, self.sections, *block.weights(self.dtype))
+            return range_attention(q, k, v, lo, hi, cap=self.cap)
+
+        return self._logits(tokens.flatten(1).contiguous(), attend, lambda x: x.view(batch, steps, n, -1)[:, :, n - 2])
+
+    @staticmethod
+    def taken(tokens, mask):
+        """The actions of windows, none (-1) in their padding."""
+        return tokens[:, :, -1].masked_fill(mask == 0, -1)
+
+    def log_probs(self, tokens, mask, done, *, scale=1.0, top=0):
+        """token_log_probs of the windows' actions."""
+        return token_log_probs(self(tokens, mask, done), self.taken(tokens, mask), scale=scale, top=top)
+
+    def distilled(self, teacher, tokens, mask, done, *, count=8, scale=1.0):
+        """distill [batch, steps] from the best `count` actions of a teacher (a TokenModel too) on the same windows."""
+        with torch.no_grad():
+            best = teacher.log_probs(tokens, mask, done, scale=scale, top=count)
+        return distill(self(tokens, mask, done), best[4], best[3], scale=scale)
+
+    @torch.no_grad()
+    def step(self, rollouts, observation, last_action=None, *, top=1, scale=1.0):
+        """The next action of every rollout, from the tokens of its newest observation [batch, step - 1] and the action
+        before it [batch] (None: the first step): (entropy [batch], top_log_probs, top_tokens [batch, top])."""
+        n = self.step_tokens
+        tokens, column, time = observation, torch.arange(n - 1, device=observation.device), rollouts.time.expand(-1, n - 1)
+        if last_action is not None:  # its token comes first: it belongs to the step before
+            tokens = torch.cat([last_action[:, None].to(tokens.dtype), tokens], 1)
+            column = torch.cat([column.new_full((1,), n - 1), column])
+            time = torch.cat([rollouts.time - 1, time], 1)
+        new = tokens.shape[1]
+        if rollouts.taken + new > rollouts.tokens:
+            raise ValueError("the rollouts' caches of %d tokens hold %d: no room for %d more"
+                             % (rollouts.tokens, rollouts.taken, new))
+        column = column.to(torch.int32).expand_as(time)
+        pos = torch.stack([time, torch.zeros_like(time), column], 2)
+        slots = rollouts.length + torch.arange(new, dtype=torch.int32, device=tokens.device)
+        lo, hi = torch.zeros_like(slots), slots + 1
+
+        def attend(i, block, q, k, v):
+            keys, values = rollouts.caches[i]
+            q = ops.norm_rotate_append(q, k, v, pos, self.freqs, self.sections, *block.weights(self.dtype), slots=slots,
+                                       k_cache=keys, v_cache=values)
+            return ops.range_attention_step(q, keys, values, lo, hi, cap=self.cap)
+
+        logits = self._logits(tokens.contiguous(), attend, lambda x: x[:, -1])
+        rollouts.taken += new
+        rollouts.length += new
+        rollouts.time += 1
+        _, entropy, _, value, best = ops.token_log_probs(logits, scale=scale, top=top)
+        return entropy, value, best

@@ -556,6 +556,82 @@ size_t gear_hip_attention_step_workspace_bytes(int64_t batch, int64_t queries, i
 int gear_hip_attention_step(const gear_hip_attention_desc *desc, void *out, void *workspace,
                             size_t workspace_bytes, void *stream);
 
+/* ---- tokens: into a sequence model and out of it ---------------------------------------------- */
+
+/* These have no counterpart in the reference either: they are what stands at both ends of a sequence model whose
+ * observations and actions are tokens, and between its blocks.  Tokens are int64 (tokens_i64 != 0) or int32; a token
+ * outside [0, vocab) stands for none (padding).  Rows are `width` or `vocab` contiguous elements of one of the types
+ * above, at any stride (in elements) and any element's address; results are contiguous.  Sums and statistics are held
+ * in 32 bits, results are rounded once, and no call uses atomics on results: the same bits on every run. */
+
+/* out[i] = scale * table[tokens[i]], zeros where there is no token.  n, vocab < 2^31 - 1, width <= 2^20. */
+int gear_hip_embed(const void *tokens, int tokens_i64, int64_t n, const void *table, int64_t table_stride,
+                   int64_t vocab, int64_t width, int dtype, float scale, void *out, void *stream);
+/* dtable[v] = scale * (sum over i with tokens[i] = v of dout[i]), all of [vocab][width] written, in the type of dout.
+ * workspace: gear_hip_embed_backward_workspace_bytes(n, width) bytes on the device, 16-byte aligned. */
+size_t gear_hip_embed_backward_workspace_bytes(int64_t n, int64_t width);
+int gear_hip_embed_backward(const void *dout, int64_t dout_stride, const void *tokens, int tokens_i64, int64_t n,
+                            int64_t vocab, int64_t width, int dtype, float scale, void *dtable,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
+/* Layer norm of rows: u = x + residual, rounded to the type (residual NULL: u = x),
+ * y = (u - mean u) / sqrt(mean (u - mean u)^2 + eps) * weight + bias (NULL: ones, zeros; both of type f32 if
+ * weight_f32 != 0, else of the rows' type).  width <= 16384. */
+typedef struct gear_hip_layer_norm_desc {
+  const void *x, *residual;
+  int64_t x_stride, residual_stride;
+  int64_t rows, width;
+  const void *weight, *bias;
+  int32_t weight_f32, dtype;
+  float eps;
+} gear_hip_layer_norm_desc;
+/* sum: u, with a residual; else NULL */
+int gear_hip_layer_norm(const gear_hip_layer_norm_desc *desc, void *y, void *sum, void *stream);
+/* Gradients from dy and (NULL: none) dsum, that of the sum: dx, which is the residual's as well, and of the weights
+ * (of their type; NULL: not wanted).  desc->x is u, desc->residual is not looked at.
+ * workspace, where a weight's gradient is wanted: gear_hip_layer_norm_backward_workspace_bytes(rows, width) bytes on
+ * the device, 16-byte aligned. */
+size_t gear_hip_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int gear_hip_layer_norm_backward(const gear_hip_layer_norm_desc *desc, const void *dy, int64_t dy_stride,
+                                 const void *dsum, int64_t dsum_stride, void *dx, void *dweight, void *dbias,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+
+/* Rows of logits; 0 < scale < 1e30, vocab <= 2^20.  z = scale * logits, lse = log sum_j exp z_j, p = exp(z - lse).
+ * A logit of -inf is a token that is not allowed; rows that allow none (no logit of -1e30 or more) have lse = -inf,
+ * log probabilities of -inf, entropy 0 and no gradient.
+ * NaN or +inf makes its row's results NaN. */
+typedef struct gear_hip_logits_desc {
+  const void *logits;
+  int64_t row_stride, rows, vocab;
+  int32_t dtype;
+  float scale;
+} gear_hip_logits_desc;
+/* log_probs[i] = z[i][tokens[i]] - lse[i];  entropy[i] = -sum_j p_j log p_j;  the `top` (<= 64, <= vocab) largest logits
+ * of a row, the lower token first among equals and NaN before all, as top_tokens and their log probabilities.  A row
+ * whose token is none is not looked at: 0, 0, 0, and -1 with -inf.  tokens and log_probs may both be NULL.
+ * workspace: gear_hip_token_log_probs_workspace_bytes(rows, vocab, top) bytes on the device, 256-byte aligned. */
+size_t gear_hip_token_log_probs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top);
+int gear_hip_token_log_probs(const gear_hip_logits_desc *desc, const void *tokens, int tokens_i64, int64_t top,
+                             float *log_probs, float *entropy, float *lse, float *top_log_probs,
+                             int64_t *top_tokens, void *workspace, size_t workspace_bytes, void *stream);
+/* dlogits = scale * (dlog_probs (1[j = token] - p_j) - dentropy p_j (log p_j + entropy)), in the logits' type, from the
+ * forward call's lse and entropy.  dlog_probs, or dentropy and entropy, may be NULL. */
+int gear_hip_token_log_probs_backward(const gear_hip_logits_desc *desc, const float *dlog_probs,
+                                      const float *dentropy, const void *tokens, int tokens_i64, const float *lse,
+                                      const float *entropy, void *dlogits, void *stream);
+/* Divergence of rows from a teacher's `count` (<= 64) best tokens: q = softmax of top_logits over a row's entries
+ * [rows][count] (entries without a token have no part), loss = sum_k q_k (log q_k - log p[top_tokens_k]).  Rows without
+ * an entry are not looked at: 0.  A token that is named twice counts with both.
+ * workspace: gear_hip_distill_workspace_bytes(rows, vocab) bytes on the device, 256-byte aligned. */
+size_t gear_hip_distill_workspace_bytes(int64_t rows, int64_t vocab);
+int gear_hip_distill(const gear_hip_logits_desc *desc, const void *top_tokens, int tokens_i64,
+                     const float *top_logits, int64_t count, float *loss, float *lse, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* dlogits = scale * dloss (p_j - the q_k of entries that name j), from the forward call's lse. */
+int gear_hip_distill_backward(const gear_hip_logits_desc *desc, const float *dloss, const void *top_tokens,
+                              int tokens_i64, const float *top_logits, int64_t count, const float *lse,
+                              void *dlogits, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
