@@ -62,19 +62,29 @@ struct RowSums {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ Vals<T> weights_at(const void *w, int f32, const Slot<T> &s, float none) {
+template <typename T, typename P>
+__device__ __forceinline__ Vals<T> weights_at(const void *w, int f32, const P &s, float none) {
   Vals<T> x;
 #pragma unroll
-  for (int e = 0; e < kPer<T>; ++e)
-    x[e] = w == nullptr || !s.own(e) ? none
-           : f32                     ? static_cast<const float *>(w)[s.col + e]
-                                     : (float)static_cast<const T *>(w)[s.col + e];
+  for (int e = 0; e < kPer<T>; ++e) x[e] = none;
+  if (w == nullptr || !s.any()) return x;
+  if (s.whole()) {
+    if (f32) {
+#pragma unroll
+      for (int e = 0; e < kPer<T>; ++e) x[e] = static_cast<const float *>(w)[s.col + e];
+    } else {
+      x = __builtin_convertvector(reinterpret_cast<const AnyRaw<T> *>(static_cast<const T *>(w) + s.col)->v, Vals<T>);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer<T>; ++e)
+      if (s.own(e)) x[e] = f32 ? static_cast<const float *>(w)[s.col + e] : (float)static_cast<const T *>(w)[s.col + e];
+  }
   return x;
 }
 
-template <typename T>
-__device__ __forceinline__ Vals<T> own_only(Vals<T> x, const Slot<T> &s) {
+template <typename T, typename P>
+__device__ __forceinline__ Vals<T> own_only(Vals<T> x, const P &s) {
   if (!s.whole()) {
 #pragma unroll
     for (int e = 0; e < kPer<T>; ++e)
@@ -88,31 +98,46 @@ __device__ __forceinline__ float inverse(float squares, float off, const LayerAr
   return __builtin_amdgcn_rsqf(fmaxf(fmaf(squares, a.over_width, -off * off), 0.f) + a.eps);
 }
 
-template <typename T, int kLanes, int kVecs, bool kResidual>
+template <typename T, int kLanes, int kVecs, bool kWhole, bool kResidual>
 __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArgs a) {
   constexpr int kThreads = kThreadsOf<kLanes>, kRows = kThreads / kLanes;
+  using At = Place<kWhole, T>;
   __shared__ float part[2][kThreads / kWave][4];
   const int lane = threadIdx.x % kLanes;
   int turn = 0;
+  Vals<T> w[kVecs], b[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const At s(lane + i * kLanes, a.width);
+    w[i] = weights_at<T>(a.weight, a.weight_f32, s, 1.f), b[i] = weights_at<T>(a.bias, a.weight_f32, s, 0.f);
+  }
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / kLanes;
     const bool here = row < a.rows;
     Vals<T> u[kVecs];
     float total[1] = {0.f};
+    const T *x = static_cast<const T *>(a.x) + row * a.xs, *r = static_cast<const T *>(a.residual) + row * a.rs;
+    T *y = static_cast<T *>(a.y) + row * a.width, *sum = static_cast<T *>(a.sum) + row * a.width;
+    Raw<T> xs[kVecs], rs[kVecs];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
-      u[i] = Vals<T>{};
+      const At s(lane + i * kLanes, a.width);
+      xs[i] = rs[i] = Raw<T>{};
       if (here && s.any()) {
-        const Raw<T> x = load_slot<true>(static_cast<const T *>(a.x) + row * a.xs, s);
-        u[i] = __builtin_convertvector(x, Vals<T>);
-        if constexpr (kResidual) {
-          u[i] += __builtin_convertvector(load_slot<true>(static_cast<const T *>(a.residual) + row * a.rs, s), Vals<T>);
-          store_slot(static_cast<T *>(a.sum) + row * a.width, s, u[i]);
-          u[i] = __builtin_convertvector(__builtin_convertvector(u[i], Raw<T>), Vals<T>);
-        }
-        u[i] = own_only<T>(u[i], s);
+        xs[i] = load_slot<true>(x, s);
+        if constexpr (kResidual) rs[i] = load_slot<true>(r, s);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const At s(lane + i * kLanes, a.width);
+      u[i] = __builtin_convertvector(xs[i], Vals<T>);
+      if constexpr (kResidual) {
+        u[i] += __builtin_convertvector(rs[i], Vals<T>);
+        if (here && s.any()) store_slot(sum, s, u[i]);
+        u[i] = __builtin_convertvector(__builtin_convertvector(u[i], Raw<T>), Vals<T>);
+      }
+      u[i] = own_only<T>(u[i], s);
       total[0] += sum_of(u[i]);
     }
     RowSums<kLanes, 1>::run(total, part, turn);
@@ -120,49 +145,56 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArg
     float sums[2] = {0.f, 0.f};  // of c, c^2
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
-      u[i] = own_only<T>(u[i] - mean, s);
+      const At s(lane + i * kLanes, a.width);
+      u[i] = s.any() ? own_only<T>(u[i] - mean, s) : Vals<T>{};
       sums[0] += sum_of(u[i]), sums[1] += sum_of(u[i] * u[i]);
     }
     RowSums<kLanes, 2>::run(sums, part, turn);
-    const float off = sums[0] * a.over_width, r = inverse(sums[1], off, a);
+    const float off = sums[0] * a.over_width, inv = inverse(sums[1], off, a);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
-      if (here && s.any())
-        store_slot(static_cast<T *>(a.y) + row * a.width, s,
-                   (u[i] - off) * r * weights_at<T>(a.weight, a.weight_f32, s, 1.f) + weights_at<T>(a.bias, a.weight_f32, s, 0.f));
+      const At s(lane + i * kLanes, a.width);
+      if (here && s.any()) store_slot(y, s, (u[i] - off) * inv * w[i] + b[i]);
     }
   }
 }
 
-template <typename T, int kLanes, int kVecs, bool kSum>
+template <typename T, int kLanes, int kVecs, bool kWhole, bool kSum>
 __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(LayerArgs a) {
   constexpr int kThreads = kThreadsOf<kLanes>, kRows = kThreads / kLanes;
+  constexpr bool kHoldWeights = kLanes < 512;
+  using At = Place<kWhole, T>;
   __shared__ float part[2][kThreads / kWave][4];
   const int lane = threadIdx.x % kLanes;
   int turn = 0;
   Vals<T> w[kVecs], dw[kVecs], db[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    w[i] = weights_at<T>(a.weight, a.weight_f32, Slot<T>(lane + i * kLanes, a.width), 1.f);
+    if (kHoldWeights) w[i] = weights_at<T>(a.weight, a.weight_f32, At(lane + i * kLanes, a.width), 1.f);
     dw[i] = db[i] = Vals<T>{};
   }
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / kLanes;
     const bool here = row < a.rows;
-    Vals<T> u[kVecs], g[kVecs], plus[kVecs];
+    const T *x = static_cast<const T *>(a.x) + row * a.xs, *dy = static_cast<const T *>(a.dy) + row * a.dys,
+            *ds = static_cast<const T *>(a.dsum) + row * a.dss;
+    T *dx = static_cast<T *>(a.dx) + row * a.width;
+    Raw<T> us[kVecs], g[kVecs], plus[kVecs];
+    Vals<T> u[kVecs];
     float mean[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
-      u[i] = g[i] = plus[i] = Vals<T>{};
+      const At s(lane + i * kLanes, a.width);
+      us[i] = g[i] = plus[i] = Raw<T>{};
       if (here && s.any()) {
-        u[i] = own_only<T>(__builtin_convertvector(load_slot<true>(static_cast<const T *>(a.x) + row * a.xs, s), Vals<T>), s);
-        g[i] = own_only<T>(__builtin_convertvector(load_slot<true>(static_cast<const T *>(a.dy) + row * a.dys, s), Vals<T>), s);
-        if constexpr (kSum)
-          plus[i] = __builtin_convertvector(load_slot<true>(static_cast<const T *>(a.dsum) + row * a.dss, s), Vals<T>);
+        us[i] = load_slot<true>(x, s), g[i] = load_slot<true>(dy, s);
+        if constexpr (kSum) plus[i] = load_slot<true>(ds, s);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const At s(lane + i * kLanes, a.width);
+      u[i] = own_only<T>(__builtin_convertvector(us[i], Vals<T>), s);
       mean[0] += sum_of(u[i]);
     }
     RowSums<kLanes, 1>::run(mean, part, turn);
@@ -170,21 +202,25 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
     float sums[4] = {0.f, 0.f, 0.f, 0.f};  // of c, c^2, h, h c
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
-      u[i] = own_only<T>(u[i] - mean[0], s);
-      const Vals<T> h = g[i] * w[i];
+      const At s(lane + i * kLanes, a.width);
+      u[i] = s.any() && here ? own_only<T>(u[i] - mean[0], s) : Vals<T>{};
+      if (!kHoldWeights) w[i] = weights_at<T>(a.weight, a.weight_f32, s, 1.f);
+      const Vals<T> h = own_only<T>(__builtin_convertvector(g[i], Vals<T>), s) * w[i];
       sums[0] += sum_of(u[i]), sums[1] += sum_of(u[i] * u[i]), sums[2] += sum_of(h), sums[3] += sum_of(h * u[i]);
+      as_it_came<T>(g[i]);
     }
     RowSums<kLanes, 4>::run(sums, part, turn);
-    const float off = sums[0] * a.over_width, r = inverse(sums[1], off, a);
-    const float mean_h = sums[2] * a.over_width, mean_hn = (sums[3] * a.over_width - off * mean_h) * r;
+    const float off = sums[0] * a.over_width, inv = inverse(sums[1], off, a);
+    const float mean_h = sums[2] * a.over_width, mean_hn = (sums[3] * a.over_width - off * mean_h) * inv;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
-      const Vals<T> n = (u[i] - off) * r;
-      dw[i] += here ? g[i] * n : Vals<T>{}, db[i] += g[i];
-      if (here && s.any())
-        store_slot(static_cast<T *>(a.dx) + row * a.width, s, r * (g[i] * w[i] - mean_h - n * mean_hn) + plus[i]);
+      const At s(lane + i * kLanes, a.width);
+      if (!kHoldWeights) w[i] = weights_at<T>(a.weight, a.weight_f32, s, 1.f);
+      if (here && s.any()) {
+        const Vals<T> n = (u[i] - off) * inv, gv = own_only<T>(__builtin_convertvector(g[i], Vals<T>), s);
+        dw[i] += gv * n, db[i] += gv;
+        store_slot(dx, s, inv * (gv * w[i] - mean_h - n * mean_hn) + __builtin_convertvector(plus[i], Vals<T>));
+      }
     }
   }
   if (a.sums == nullptr) return;
@@ -192,7 +228,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
   if constexpr (kRows == 1) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
+      const At s(lane + i * kLanes, a.width);
 #pragma unroll
       for (int e = 0; e < kPer<T>; ++e)
         if (s.own(e)) to[s.col + e] = dw[i][e], to[a.width + s.col + e] = db[i][e];
@@ -202,7 +238,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
     __shared__ Vals<T> pile[kThreads];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s(lane + i * kLanes, a.width);
+      const At s(lane + i * kLanes, a.width);
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
         __syncthreads();
@@ -244,10 +280,16 @@ __global__ __launch_bounds__(kBlock) void layer_norm_weights_kernel(const float 
     static_cast<T *>(to)[i] = (T)s;
 }
 
-// f(T(), lanes of a row, vectors of a lane)
+// f(T(), lanes of a row, vectors of a lane, whether vectors are whole)
 template <typename F>
-void by_type_and_lanes(int dtype, int width, const F &f) {
+void by_type_and_lanes(int dtype, int width, const F &given) {
   by_type(dtype, [&](auto type) {
+    auto f = [&](auto, auto lanes, auto vecs) {
+      if (width % kPer<decltype(type)> == 0)
+        given(type, lanes, vecs, std::true_type());
+      else
+        given(type, lanes, vecs, std::false_type());
+    };
     const int vecs = (width + kPer<decltype(type)> - 1) / kPer<decltype(type)>;
     using two = std::integral_constant<int, 2>;
     if (vecs <= 8)
@@ -309,13 +351,13 @@ extern "C" int gear_hip_layer_norm(const gear_hip_layer_norm_desc *desc, void *y
   const int element = element_bytes(desc->dtype);
   if (!aligned_to(y, element) || !aligned_to(sum, element)) return GEAR_HIP_EALIGN;
   a.y = y, a.sum = sum;
-  by_type_and_lanes(desc->dtype, a.width, [&](auto type, auto lanes, auto vecs) {
+  by_type_and_lanes(desc->dtype, a.width, [&](auto type, auto lanes, auto vecs, auto whole) {
     constexpr int kLanes = decltype(lanes)::value, kThreads = kThreadsOf<kLanes>;
     const dim3 grid((unsigned)blocks_of(a.rows, kThreads / kLanes, (1 << 24) / kThreads)), block(kThreads);
     if (a.residual)
-      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, true>), grid, block, 0, as_stream(stream), a);
+      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, true>), grid, block, 0, as_stream(stream), a);
     else
-      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, false>), grid, block, 0, as_stream(stream), a);
+      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, false>), grid, block, 0, as_stream(stream), a);
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
   return 0;
@@ -344,14 +386,14 @@ extern "C" int gear_hip_layer_norm_backward(const gear_hip_layer_norm_desc *desc
       return GEAR_HIP_EALIGN;
     a.dy = dy, a.dys = dy_stride, a.dsum = dsum, a.dss = dsum_stride, a.dx = dx;
     a.sums = want ? static_cast<float *>(workspace) : nullptr;
-    by_type_and_lanes(desc->dtype, a.width, [&](auto type, auto lanes, auto vecs) {
+    by_type_and_lanes(desc->dtype, a.width, [&](auto type, auto lanes, auto vecs, auto whole) {
       constexpr int kLanes = decltype(lanes)::value, kThreads = kThreadsOf<kLanes>;
       blocks = blocks_of(a.rows, kThreads / kLanes, grad_blocks(kThreads));
       const dim3 grid((unsigned)blocks), block(kThreads);
       if (dsum)
-        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, true>), grid, block, 0, as_stream(stream), a);
+        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, true>), grid, block, 0, as_stream(stream), a);
       else
-        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, false>), grid, block, 0, as_stream(stream), a);
+        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, false>), grid, block, 0, as_stream(stream), a);
     });
     GEARHIP_RETURN_IF_LAUNCH_FAILED();
   }

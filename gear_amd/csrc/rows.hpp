@@ -60,6 +60,38 @@ __device__ __forceinline__ void store_slot(T *row, const Slot<T> &s, const Vals<
   }
 }
 
+// The same for rows whose width is a multiple of a vector (kWhole): nothing of theirs is partial.
+template <bool kWhole, typename T>
+struct Place : Slot<T> {
+  __device__ __forceinline__ Place(int v, int width) : Slot<T>(v, width) {}
+};
+template <typename T>
+struct Place<true, T> {
+  int col;
+  bool here;
+  __device__ __forceinline__ Place(int v, int width) : col(v * kPer<T>), here(v * kPer<T> < width) {}
+  __device__ __forceinline__ bool any() const { return here; }
+  __device__ __forceinline__ bool whole() const { return true; }
+  __device__ __forceinline__ bool own(int) const { return here; }
+};
+template <bool kNarrow, typename T>
+__device__ __forceinline__ Raw<T> load_slot(const T *row, const Place<true, T> &s) {
+  return reinterpret_cast<const AnyRaw<T> *>(row + s.col)->v;
+}
+template <typename T>
+__device__ __forceinline__ void store_slot(T *row, const Place<true, T> &s, const Vals<T> &x) {
+  reinterpret_cast<AnyRaw<T> *>(row + s.col)->v = __builtin_convertvector(x, Raw<T>);
+}
+
+// A vector as it came, from here on: the compiler may not keep what it made of it earlier in its place (which takes two to
+// four times the registers).
+template <typename T>
+__device__ __forceinline__ void as_it_came(Raw<T> &x) {
+  u32x4 y = __builtin_bit_cast(u32x4, x);
+  asm volatile("" : "+v"(y));
+  x = __builtin_bit_cast(Raw<T>, y);
+}
+
 // ---- over the kLanes lanes of a row (a power of two, at most 64), the result in all of them ----------------------
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float x) {
