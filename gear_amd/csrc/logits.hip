@@ -9,7 +9,7 @@
 //
 // All are bound by memory: a row is read once and held in registers as it came, its maximum is taken before any exponential.
 // Rows of up to 256 vectors of 16 bytes: a wave or a part of one.  Wider ones: a workgroup for every part of a row of at
-// most 20 vectors a thread; rows in several parts (wide ones, and few ones, to fill the GPU) are joined by a second launch.
+// most 17 vectors a thread; rows in several parts (wide ones, and few ones, to fill the GPU) are joined by a second launch.
 //
 // The best k: groups of lanes have a maximum each, 64 in all; the k-th largest of those is a bound below which none of
 // the best k lies, so that few elements are left to be put in order.  Where more are left than a list holds (rows of equal
@@ -22,11 +22,10 @@ namespace gearhip {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / kWave;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxTop = 64;     // best tokens, and a teacher's entries
-constexpr int kHeld = 20;       // vectors of a thread
-constexpr int kList = 256;      // candidates for the best
+constexpr int kHeld = 17;       // vectors of a thread
+constexpr int kHeldFew = 16;    // ... of a workgroup of 1024
 constexpr int kJoined = 4096;   // entries that a join puts in order
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kLow = -1e30f;  // below any exponent that counts, and any logit that is allowed
@@ -84,7 +83,7 @@ __device__ __forceinline__ uint64_t lanes_max64(uint64_t x) {
 struct Stats {
   float m, s, a;  // maximum, S, A / ln 2 (or 0)
 };
-// (m less itself is NaN for an infinite m: a row without a finite logit has S = 0 that way round)
+// (a row without a finite logit has S = 0 that way round, not NaN)
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <typename T>
@@ -98,7 +97,7 @@ __device__ __forceinline__ Raw<T> nothing() {
 template <bool kNarrow, typename T>
 __device__ __forceinline__ Raw<T> load_logits(const T *row, int v, int vocab) {
   const Slot<T> s(v, vocab);
-  if (!s.any()) return nothing<T>();
+  if (kNarrow && !s.any()) return nothing<T>();
   Raw<T> x = load_slot<kNarrow>(row, s);
   if (!s.whole()) {
 #pragma unroll
@@ -114,19 +113,26 @@ __device__ __forceinline__ float max_of(const Raw<T> &x) {
   for (int e = 1; e < kPer<T>; ++e) m = fmaxf(m, (float)x[e]);
   return m;
 }
-template <bool kEntropy, typename T>
-__device__ __forceinline__ void add_to(Stats &t, const Raw<T> &x, float shift, float scale2) {
+// Exponents are in base 2.  Those of x scale2 - m2, with m2 = m scale2 as it is rounded, take one operation an element;
+// what m2 is off by is the same for all of them and taken out of the sums.  Where m2 is so large that this would not
+// do, x less m comes first.
+struct Shift {
+  float m, m2, rest;
+  __device__ __forceinline__ Shift(float maximum, float scale2) : m(shift_of(maximum)), m2(m * scale2), rest(fmaf(m, scale2, -m2)) {}
+  __device__ __forceinline__ bool huge() const { return !(fabsf(m2) < 0x1p29f); }
+  __device__ __forceinline__ void settle(Stats &t) const {
+    const float by = __builtin_amdgcn_exp2f(-rest);
+    t.a = fmaf(-rest, t.s, t.a) * by, t.s *= by;
+  }
+};
+template <bool kEntropy, bool kHuge, typename T>
+__device__ __forceinline__ void add_to(Stats &t, const Raw<T> &x, const Shift &m, float scale2) {
 #pragma unroll
   for (int e = 0; e < kPer<T>; ++e) {
-    const float d = ((float)x[e] - shift) * scale2, p = __builtin_amdgcn_exp2f(d);
+    const float d = kHuge ? ((float)x[e] - m.m) * scale2 : fmaf((float)x[e], scale2, -m.m2), p = __builtin_amdgcn_exp2f(d);
     t.s += p;
     if (kEntropy) t.a = fmaf(fmaxf(d, kLow), p, t.a);
   }
-}
-__device__ __forceinline__ Stats joined(const Stats &x, const Stats &y, float scale2) {
-  const float m = fmaxf(x.m, y.m), dx = fmaxf((x.m - shift_of(m)) * scale2, kLow), dy = fmaxf((y.m - shift_of(m)) * scale2, kLow);
-  const float ex = __builtin_amdgcn_exp2f(dx), ey = __builtin_amdgcn_exp2f(dy);
-  return Stats{m, x.s * ex + y.s * ey, fmaf(dx, x.s, x.a) * ex + fmaf(dy, y.s, y.a) * ey};
 }
 
 // ---- what is made of them ---------------------------------------------------------------------------------------
@@ -137,6 +143,7 @@ struct Result {
   __device__ __forceinline__ float log_p(float x, float scale) const {
     return none || x == -INFINITY ? -INFINITY : (x - shift) * scale - log_s;
   }
+  __device__ __forceinline__ float lse(const Stats &t, float scale) const { return none ? -INFINITY : fmaf(scale, t.m, log_s); }
 };
 
 template <typename T>
@@ -144,12 +151,11 @@ __device__ __forceinline__ float logit_at(const LogitsArgs &a, int64_t row, int6
   return (float)static_cast<const T *>(a.logits)[row * a.stride + column];
 }
 
-// by one lane
-template <typename T>
-__device__ __forceinline__ void finish_log_probs(const LogitsArgs &a, int64_t row, int64_t token, const Stats &t) {
+// by one lane; x: the token's logit
+__device__ __forceinline__ void finish_log_probs(const LogitsArgs &a, int64_t row, float x, const Stats &t) {
   const Result r(t);
-  if (a.log_probs) a.log_probs[row] = r.log_p(logit_at<T>(a, row, token), a.scale);
-  a.lse[row] = r.none ? -INFINITY : fmaf(a.scale, t.m, r.log_s);
+  if (a.log_probs) a.log_probs[row] = r.log_p(x, a.scale);
+  a.lse[row] = r.lse(t, a.scale);
   a.entropy[row] = r.none ? 0.f : r.log_s - t.a / t.s * kLn2;
 }
 __device__ __forceinline__ void pass_over(const LogitsArgs &a, int64_t row) {
@@ -163,210 +169,268 @@ __device__ __forceinline__ void put_best(const LogitsArgs &a, int64_t row, int a
   a.top_tokens[row * a.top + at] = e == 0 ? -1 : entry_column(e);
 }
 
-// The teacher's entries of a row, lane by lane: entry k is lane k's, k + kLanes the same lane's next.
-struct Teacher {
-  float top, sum;
-  bool some;
-};
-__device__ __forceinline__ float teacher_at(const LogitsArgs &a, int64_t row, int k, int64_t &column) {
-  column = token_at(a.entries, a.wide, row * a.count + k, a.vocab);
-  return column < 0 ? -INFINITY : a.teacher[row * a.count + k];
-}
+// The teacher's entries of a row: entry k is held by lane k % kLanes.  `count` 0: the lanes have no row.
 template <int kLanes>
-__device__ __forceinline__ Teacher teacher_of(const LogitsArgs &a, int64_t row, int count, int lane) {
-  Teacher q{-INFINITY, 0.f, false};
-  float any = 0;
-  int64_t column;
-  for (int k = lane; k < count; k += kLanes) {
-    const float t = teacher_at(a, row, k, column);
-    q.top = fmaxf(q.top, t);
-    if (!(t == -INFINITY)) any = 1;
+struct Teacher {
+  static constexpr int kHeldEntries = kMaxTop / kLanes;
+  int column[kHeldEntries];                       // -1: none
+  float l[kHeldEntries], q[kHeldEntries], log_sum;  // logits less their maximum, weights
+  bool some;
+  __device__ __forceinline__ Teacher(const LogitsArgs &a, int64_t row, int count, int lane) {
+    float top = -INFINITY, any = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+      column[i] = -1, l[i] = -INFINITY, q[i] = 0;
+      const int k = lane + i * kLanes;
+      if (k < count) {
+        column[i] = (int)token_at(a.entries, a.wide, row * a.count + k, a.vocab);
+        if (column[i] >= 0) l[i] = a.teacher[row * a.count + k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+      top = fmaxf(top, l[i]);
+      if (!(l[i] == -INFINITY)) any = 1;
+    }
+    top = shift_of(lanes_max<kLanes>(top));
+    some = lanes_max<kLanes>(any) > 0;
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+      l[i] -= top;
+      q[i] = __builtin_amdgcn_exp2f(l[i] * kLog2e);
+      sum += q[i];
+    }
+    sum = lanes_sum<kLanes>(sum);
+    log_sum = __builtin_amdgcn_logf(sum) * kLn2;
+    const float over = 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) q[i] *= over;
   }
-  q.top = lanes_max<kLanes>(q.top);
-  q.some = lanes_max<kLanes>(any) > 0;
-  for (int k = lane; k < count; k += kLanes)
-    q.sum += __builtin_amdgcn_exp2f((teacher_at(a, row, k, column) - shift_of(q.top)) * kLog2e);
-  q.sum = lanes_sum<kLanes>(q.sum);
-  return q;
-}
+};
 template <typename T, int kLanes>
-__device__ __forceinline__ void finish_distill(const LogitsArgs &a, int64_t row, int count, int lane, const Teacher &q,
+__device__ __forceinline__ void finish_distill(const LogitsArgs &a, int64_t row, bool here, int lane, const Teacher<kLanes> &q,
                                                const Stats &t) {
   const Result r(t);
-  const float log_sum = __builtin_amdgcn_logf(q.sum) * kLn2, over = 1.f / q.sum;
-  float loss = 0;
-  for (int k = lane; k < count; k += kLanes) {
-    int64_t column;
-    const float l = teacher_at(a, row, k, column) - shift_of(q.top), p = __builtin_amdgcn_exp2f(l * kLog2e) * over;
-    if (column >= 0 && !(p == 0)) loss += p * (l - log_sum - r.log_p(logit_at<T>(a, row, column), a.scale));
-  }
+  float x[Teacher<kLanes>::kHeldEntries], loss = 0;
+#pragma unroll
+  for (int i = 0; i < Teacher<kLanes>::kHeldEntries; ++i) x[i] = here && q.column[i] >= 0 ? logit_at<T>(a, row, q.column[i]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < Teacher<kLanes>::kHeldEntries; ++i)
+    if (here && q.column[i] >= 0 && !(q.q[i] == 0)) loss += q.q[i] * (q.l[i] - q.log_sum - r.log_p(x[i], a.scale));
   loss = lanes_sum<kLanes>(loss);
-  if (lane == 0 && count > 0) {
+  if (here && lane == 0) {
     a.loss[row] = loss;
-    a.lse[row] = r.none ? -INFINITY : fmaf(a.scale, t.m, r.log_s);
+    a.lse[row] = r.lse(t, a.scale);
   }
 }
 
-// ---- rows of a wave or less -------------------------------------------------------------------------------------
-template <typename T, int kLanes, int kVecs, int kKind>
-__global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
-  constexpr int kRows = kBlock / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  // (the lanes of a wave go round alike: they exchange sums)
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = base + threadIdx.x / kLanes;
-    int64_t token = -1;
-    bool here = row < a.rows;
-    Teacher q{};
-    if (kKind == kDistill) {
-      q = teacher_of<kLanes>(a, row, here ? a.count : 0, lane);
-      if (here && !q.some && lane == 0) pass_over(a, row);
-      here = here && q.some;
-    } else if (here && a.tokens) {
-      token = token_at(a.tokens, a.wide, row, a.vocab);
-      if (token < 0) {
-        if (lane == 0) pass_over(a, row);
-        for (int k = lane; k < a.top; k += kLanes) put_best(a, row, k, 0, Stats{});
-        here = false;
-      }
-    }
-    Raw<T> x[kVecs];
-    Stats t{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      x[i] = here ? load_logits<true>(static_cast<const T *>(a.logits) + row * a.stride, lane + i * kLanes, a.vocab) : nothing<T>();
-      t.m = fmaxf(t.m, max_of<T>(x[i]));
-    }
-    t.m = lanes_max<kLanes>(t.m);
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) add_to<kKind == kLogProbs, T>(t, x[i], shift_of(t.m), a.scale2);
-    t.s = lanes_sum<kLanes>(t.s);
-    if (kKind == kDistill) {
-      finish_distill<T, kLanes>(a, row, here ? a.count : 0, lane, q, t);
-      continue;
-    }
-    t.a = lanes_sum<kLanes>(t.a);
-    if (here && lane == 0) finish_log_probs<T>(a, row, token, t);
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const Slot<T> s(lane + i * kLanes, a.vocab);
-#pragma unroll
-        for (int e = 0; e < kPer<T>; ++e) {
-          const uint64_t w = entry_of((float)x[i][e], s.col + e);
-          if (s.own(e) && w < last && w > best) best = w;
-        }
-      }
-      last = lanes_max64<kLanes>(best);
-      if (here && lane == k % kLanes) put_best(a, row, k, last, t);
-    }
-  }
+// ---- the best tokens ----------------------------------------------------------------------------------------------
+template <int kThreads>
+__device__ __forceinline__ void group_sync() {
+  if (kThreads == kWave)
+    wave_lds_sync();
+  else
+    __syncthreads();
 }
 
-// ---- rows, or parts of them, of a workgroup ---------------------------------------------------------------------
-template <typename F>
-__device__ __forceinline__ float block_reduce(float x, float *part, const F &f) {  // (x: of the wave)
-  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
-  __syncthreads();
-  x = part[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) x = f(x, part[w]);
-  return x;
-}
-
-struct WideSmem {
-  float max[kWaves], sum[2][kWaves], groups[kWave];
-  uint64_t best[2][kWaves];
+template <int kThreads>
+struct BestSmem {
+  static constexpr int kList = kThreads < 256 ? 128 : 256;  // candidates
+  uint32_t groups[kWave];
+  uint64_t best[2][kThreads / kWave];
   uint64_t list[kList];
   int count;
-  int some;
 };
 
-// The best `top` of what a workgroup holds, put(place, entry) for each; entries that are not there are 0.
-template <typename T, int kVecs, typename Put>
-__device__ __forceinline__ void best_of(const Raw<T> (&x)[kVecs], float mine, bool finite, int first, int last, int vocab, int top,
-                                        WideSmem &sm, const Put &put) {
-  // (the k-th largest of 64 maxima)
-  float g = fmaxf(mine, dpp_f32<0xB1>(mine));
-  g = fmaxf(g, dpp_f32<0x4E>(g));
-  if (threadIdx.x % 4 == 0) sm.groups[threadIdx.x / 4] = g;
-  if (threadIdx.x == 0) sm.count = 0;
-  __syncthreads();
-  const int lane = threadIdx.x % kWave;
-  g = sm.groups[lane];
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return (int32_t)b < 0 ? ~b : b | 0x80000000u;
+}
+
+// The best `top` of what kThreads threads hold of the vectors [first, last), put(place, entry) for each; entries that are
+// not there are 0.  mine: the largest of a thread's elements; finite: whether the row holds no NaN or infinity.
+template <typename T, int kThreads, int kVecs, typename Put>
+__device__ __forceinline__ void best_of(const T *row, Raw<T> (&x)[kVecs], float mine, bool finite, int first, int last, int vocab,
+                                        int top, BestSmem<kThreads> &sm, const Put &put) {
+  constexpr int kGroup = kThreads / kWave;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) as_it_came<T>(x[i]);
+  const int lane = threadIdx.x % kWave, id = threadIdx.x % kThreads;
+  // 64 maxima; the lowest bits make them differ, and leave the bound a little low
+  const float g = lanes_max<(kGroup > 1 ? kGroup : 1)>(mine);
+  if (id % kGroup == 0) sm.groups[id / kGroup] = (order_of(g) & ~63u) | (id / kGroup);
+  if (id == 0) sm.count = 0;
+  group_sync<kThreads>();
+  const uint32_t key = sm.groups[lane];
   int before = 0;
-#pragma unroll 8
-  for (int j = 0; j < kWave; ++j) {
-    const float other = sm.groups[j];
-    before += other > g || (other == g && j < lane);
+#pragma unroll
+  for (int j = 0; j < kWave; j += 4) {
+    const u32x4 other = *reinterpret_cast<const u32x4 *>(&sm.groups[j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) before += other[i] > key;
   }
-  const uint64_t which = __ballot(before == top - 1);
-  const float bound = which == 0 ? -INFINITY : sm.groups[__builtin_ctzll(which)];
+  const uint32_t kth = __builtin_amdgcn_readlane(key, __builtin_ctzll(__ballot(before == top - 1))) & ~63u;
+  const float bound = kth <= 0x007fffffu ? -INFINITY : __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
   if (finite && mine >= bound) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int v = first + threadIdx.x + i * kBlock;
-      if (v < last) {
+      if (first + i * kThreads < last && max_of<T>(x[i]) >= bound) {
+        const int v = first + id + i * kThreads;
         const Slot<T> s(v, vocab);
 #pragma unroll
         for (int e = 0; e < kPer<T>; ++e)
-          if ((float)x[i][e] >= bound && s.own(e)) {
+          if ((float)x[i][e] >= bound && v < last && s.own(e)) {
             const int at = atomicAdd(&sm.count, 1);
-            if (at < kList) sm.list[at] = entry_of((float)x[i][e], s.col + e);
+            if (at < sm.kList) sm.list[at] = entry_of((float)x[i][e], s.col + e);
           }
       }
     }
   }
-  __syncthreads();
+  group_sync<kThreads>();
   const int count = sm.count;
-  if (finite && count <= kList) {
-    if ((int)threadIdx.x < count) {
-      const uint64_t w = sm.list[threadIdx.x];
-      int place = 0;
-      for (int j = 0; j < count; ++j) place += sm.list[j] > w;
-      if (place < top) put(place, w);
+  if (finite && count <= sm.kList) {
+    for (int c = id; c < count || c < top; c += kThreads) {
+      if (c < count) {
+        const uint64_t w = sm.list[c];
+        int place = 0;
+#pragma unroll 4
+        for (int j = 0; j < count; ++j) place += sm.list[j] > w;
+        if (place < top) put(place, w);
+      } else {
+        put(c, 0ull);
+      }
     }
-    if ((int)threadIdx.x >= count && (int)threadIdx.x < top) put(threadIdx.x, 0ull);
+    group_sync<kThreads>();
     return;
   }
   uint64_t limit = ~0ull;
 #pragma unroll 1
   for (int k = 0; k < top; ++k) {
     uint64_t best = 0;
+#pragma unroll 1
+    for (int v = first + id; v < last; v += kThreads) {
+      const Slot<T> s(v, vocab);
+      const Raw<T> y = load_slot<kThreads == kWave>(row, s);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int v = first + threadIdx.x + i * kBlock;
-      if (v < last) {
-        const Slot<T> s(v, vocab);
-#pragma unroll
-        for (int e = 0; e < kPer<T>; ++e) {
-          const uint64_t w = entry_of((float)x[i][e], s.col + e);
-          if (s.own(e) && w < limit && w > best) best = w;
-        }
+      for (int e = 0; e < kPer<T>; ++e) {
+        const uint64_t w = entry_of((float)y[e], s.col + e);
+        if (s.own(e) && w < limit && w > best) best = w;
       }
     }
-    best = lanes_max64<kWave>(best);
-    if (lane == 0) sm.best[k & 1][threadIdx.x / kWave] = best;
-    __syncthreads();
-    limit = sm.best[k & 1][0];
+    limit = lanes_max64<kWave>(best);
+    if (kThreads > kWave) {
+      if (lane == 0) sm.best[k & 1][id / kWave] = limit;
+      __syncthreads();
+      limit = sm.best[k & 1][0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) limit = sm.best[k & 1][w] > limit ? sm.best[k & 1][w] : limit;
-    if ((int)threadIdx.x == k) put(k, limit);
+      for (int w = 1; w < kThreads / kWave; ++w) limit = sm.best[k & 1][w] > limit ? sm.best[k & 1][w] : limit;
+    }
+    if (id == 0) put(k, limit);
   }
 }
 
-template <typename T, int kVecs, int kKind, bool kTop>
-__global__ __launch_bounds__(kBlock) void wide_kernel(LogitsArgs a) {
-  __shared__ WideSmem sm;
+// ---- rows of a wave or less -------------------------------------------------------------------------------------
+template <typename T, int kLanes, int kVecs, int kKind, bool kTop>
+__global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
+  constexpr int kRows = kBlock / kLanes;
+  __shared__ BestSmem<kWave> best[kTop && kLanes == kWave ? kRows : 1];
+  const int lane = threadIdx.x % kLanes;
+  // (the lanes of a wave go round alike: they exchange sums)
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
+    const int64_t row = base + threadIdx.x / kLanes;
+    bool here = row < a.rows;
+    float at_token = 0;
+    if (kKind == kLogProbs && a.tokens) {
+      const int64_t token = here ? token_at(a.tokens, a.wide, row, a.vocab) : -1;
+      if (here && token < 0) {
+        if (lane == 0) pass_over(a, row);
+        if (kTop)
+          for (int k = lane; k < a.top; k += kLanes) put_best(a, row, k, 0, Stats{});
+      }
+      here = token >= 0;
+      if (here) at_token = logit_at<T>(a, row, token);
+    }
+    Raw<T> x[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      x[i] = here ? load_logits<true>(static_cast<const T *>(a.logits) + row * a.stride, lane + i * kLanes, a.vocab) : nothing<T>();
+    auto stats = [&](Stats &t) __attribute__((always_inline)) {
+      const float mine = t.m;
+      t.m = lanes_max<kLanes>(mine);
+      const Shift m(t.m, a.scale2);
+      if (m.huge()) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) add_to<kKind == kLogProbs, true, T>(t, x[i], m, a.scale2);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) add_to<kKind == kLogProbs, false, T>(t, x[i], m, a.scale2);
+      }
+      t.s = lanes_sum<kLanes>(t.s);
+      if (kKind == kLogProbs) t.a = lanes_sum<kLanes>(t.a);
+      if (!m.huge()) m.settle(t);
+    };
+    Stats t{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) t.m = fmaxf(t.m, max_of<T>(x[i]));
+    const float mine = t.m;
+    if constexpr (kKind == kDistill) {
+      const Teacher<kLanes> q(a, row, here ? a.count : 0, lane);
+      if (here && !q.some && lane == 0) pass_over(a, row);
+      stats(t);
+      finish_distill<T, kLanes>(a, row, here && q.some, lane, q, t);
+    } else {
+      stats(t);
+      if (here && lane == 0) finish_log_probs(a, row, at_token, t);
+      if constexpr (kTop && kLanes == kWave) {
+        if (here)
+          best_of<T, kWave, kVecs>(static_cast<const T *>(a.logits) + row * a.stride, x, mine, t.s == t.s, 0,
+                                   (a.vocab + kPer<T> - 1) / kPer<T>, a.vocab, a.top, best[threadIdx.x / kWave],
+                                   [&](int place, uint64_t e) { put_best(a, row, place, e, t); });
+      } else if constexpr (kTop) {
+        uint64_t entry[kVecs * kPer<T>], last = 0;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          const Slot<T> s(lane + i * kLanes, a.vocab);
+#pragma unroll
+          for (int e = 0; e < kPer<T>; ++e) entry[i * kPer<T> + e] = s.own(e) ? entry_of((float)x[i][e], s.col + e) : 0;
+        }
+        for (int k = 0; k < a.top; ++k) {
+          uint64_t best = 0;
+#pragma unroll
+          for (int e = 0; e < kVecs * kPer<T>; ++e) {
+            if (entry[e] == last) entry[e] = 0;  // (it was the last one's)
+            best = entry[e] > best ? entry[e] : best;
+          }
+          last = lanes_max64<kLanes>(best);
+          if (here && lane == k % kLanes) put_best(a, row, k, last, t);
+        }
+      }
+    }
+  }
+}
+
+// ---- rows, or parts of them, of a workgroup ---------------------------------------------------------------------
+template <int kThreads, typename F>
+__device__ __forceinline__ float block_reduce(float x, float *part, const F &f) {  // (x: of the wave)
+  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
+  __syncthreads();
+  x = part[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / kWave; ++w) x = f(x, part[w]);
+  return x;
+}
+
+template <typename T, int kThreads, int kVecs, int kKind, bool kTop>
+__global__ __launch_bounds__(kThreads) void wide_kernel(LogitsArgs a) {
+  __shared__ float part_max[kThreads / kWave], part_sum[2][kThreads / kWave];
+  __shared__ BestSmem<kTop ? kThreads : kWave> best;
   const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
   for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
     const int64_t row = unit / a.parts;
     const int part = (int)(unit - row * a.parts), first = part * a.part_vecs, last = min(first + a.part_vecs, vecs);
-    int64_t token = -1;
+    float at_token = 0;
     if (kKind == kLogProbs && a.tokens) {
-      token = token_at(a.tokens, a.wide, row, a.vocab);
+      const int64_t token = token_at(a.tokens, a.wide, row, a.vocab);
       if (token < 0) {  // (with several parts the launch that joins them sees to the row)
         if (a.parts == 1) {
           if (threadIdx.x == 0) pass_over(a, row);
@@ -374,105 +438,146 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(LogitsArgs a) {
         }
         continue;
       }
+      at_token = logit_at<T>(a, row, token);
     }
-    Teacher q{};
-    if (kKind == kDistill) {
-      q = teacher_of<kWave>(a, row, a.count, threadIdx.x % kWave);
+    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
+    Raw<T> x[kVecs];
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int v = first + threadIdx.x + i * kThreads;
+        x[i] = nothing<T>();
+        if (v < last) x[i] = load_logits<false>(from, v, a.vocab);
+      }
+    };
+    auto stats = [&](float &mine) __attribute__((always_inline)) {
+      mine = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        if (first + i * kThreads < last) mine = fmaxf(mine, max_of<T>(x[i]));
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) as_it_came<T>(x[i]);
+      __syncthreads();  // (of the unit before: its shared memory)
+      Stats t{block_reduce<kThreads>(lanes_max<kWave>(mine), part_max, [](float p, float r) { return fmaxf(p, r); }), 0.f, 0.f};
+      const Shift m(t.m, a.scale2);
+      if (__builtin_expect(m.huge(), 0)) {
+#pragma unroll 1
+        for (int v = first + threadIdx.x; v < last; v += kThreads)
+          add_to<kKind == kLogProbs, true, T>(t, load_logits<false>(from, v, a.vocab), m, a.scale2);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          if (first + i * kThreads < last) add_to<kKind == kLogProbs, false, T>(t, x[i], m, a.scale2);
+        }
+      }
+      auto plus = [](float p, float r) { return p + r; };
+      const float s = lanes_sum<kWave>(t.s);
+      if (kKind == kLogProbs) {
+        const float a2 = lanes_sum<kWave>(t.a);
+        if (threadIdx.x % kWave == 0) part_sum[1][threadIdx.x / kWave] = a2;
+      }
+      t.s = block_reduce<kThreads>(s, part_sum[0], plus);
+      if (kKind == kLogProbs) {
+        t.a = part_sum[1][0];
+#pragma unroll
+        for (int w = 1; w < kThreads / kWave; ++w) t.a += part_sum[1][w];
+      }
+      if (!m.huge()) m.settle(t);
+      return t;
+    };
+    float mine;
+    if constexpr (kKind == kDistill) {
+      const Teacher<kWave> q(a, row, a.count, threadIdx.x % kWave);
       if (!q.some) {
         if (a.parts == 1 && threadIdx.x == 0) pass_over(a, row);
         continue;
       }
-    }
-    Raw<T> x[kVecs];
-    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
-    float mine = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int v = first + threadIdx.x + i * kBlock;
-      x[i] = v < last ? load_logits<false>(from, v, a.vocab) : nothing<T>();
-    }
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (first + i * kBlock < last) mine = fmaxf(mine, max_of<T>(x[i]));
-    __syncthreads();  // (of the unit before: its shared memory)
-    Stats t{block_reduce(lanes_max<kWave>(mine), sm.max, [](float p, float r) { return fmaxf(p, r); }), 0.f, 0.f};
-    const float shift = shift_of(t.m);
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (first + i * kBlock < last) add_to<kKind == kLogProbs, T>(t, x[i], shift, a.scale2);
-    auto plus = [](float p, float r) { return p + r; };
-    t.s = block_reduce(lanes_sum<kWave>(t.s), sm.sum[0], plus);
-    if (kKind == kLogProbs) t.a = block_reduce(lanes_sum<kWave>(t.a), sm.sum[1], plus);
-    if (a.parts > 1) {
-      if (threadIdx.x == 0) *reinterpret_cast<f32x4 *>(a.stats + unit * 4) = f32x4{t.m, t.s, t.a, 0.f};
+      load();
+      const Stats t = stats(mine);
+      if (a.parts > 1) {
+        if (threadIdx.x == 0) *reinterpret_cast<f32x4 *>(a.stats + unit * 4) = f32x4{t.m, t.s, t.a, 0.f};
+      } else if (threadIdx.x < kWave) {
+        finish_distill<T, kWave>(a, row, true, threadIdx.x, q, t);
+      }
+    } else {
+      load();
+      const Stats t = stats(mine);
+      const bool alone = a.parts == 1;
+      if (threadIdx.x == 0) {
+        if (alone)
+          finish_log_probs(a, row, at_token, t);
+        else
+          *reinterpret_cast<f32x4 *>(a.stats + unit * 4) = f32x4{t.m, t.s, t.a, 0.f};
+      }
       if constexpr (kTop)
-        best_of<T, kVecs>(x, mine, t.s == t.s, first, last, a.vocab, a.top, sm,
-                          [&](int place, uint64_t e) { a.lists[unit * a.top + place] = e; });
-      continue;
-    }
-    if (kKind == kLogProbs) {
-      if (threadIdx.x == 0) finish_log_probs<T>(a, row, token, t);
-      if constexpr (kTop)
-        best_of<T, kVecs>(x, mine, t.s == t.s, first, last, a.vocab, a.top, sm,
-                          [&](int place, uint64_t e) { put_best(a, row, place, e, t); });
-    } else if (threadIdx.x < kWave) {
-      finish_distill<T, kWave>(a, row, a.count, threadIdx.x, q, t);
+        best_of<T, kThreads, kVecs>(from, x, mine, t.s == t.s, first, last, a.vocab, a.top, best, [&](int place, uint64_t e) {
+          if (alone)
+            put_best(a, row, place, e, t);
+          else
+            a.lists[unit * a.top + place] = e;
+        });
     }
   }
 }
 
-// Rows in several parts: a workgroup each.
+// Rows in several parts: a workgroup each, a part a lane.
 template <typename T, int kKind>
 __global__ __launch_bounds__(kBlock) void join_kernel(LogitsArgs a) {
   __shared__ uint64_t lists[kKind == kLogProbs ? kJoined : 1];
+  const int lane = threadIdx.x % kWave;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    int64_t token = -1;
-    Teacher q{};
-    bool over;
-    if (kKind == kLogProbs) {
-      if (a.tokens) token = token_at(a.tokens, a.wide, row, a.vocab);
-      over = a.tokens && token < 0;
-    } else {
-      q = teacher_of<kWave>(a, row, a.count, threadIdx.x % kWave);
-      over = !q.some;
-    }
-    if (over) {
-      if (threadIdx.x == 0) pass_over(a, row);
-      if (kKind == kLogProbs && (int)threadIdx.x < a.top) put_best(a, row, threadIdx.x, 0, Stats{});
-      continue;
-    }
-    Stats t{-INFINITY, 0.f, 0.f};
-    for (int p = 0; p < a.parts; ++p) {
-      const f32x4 s = *reinterpret_cast<const f32x4 *>(a.stats + (row * a.parts + p) * 4);
-      t = joined(t, Stats{s[0], s[1], s[2]}, a.scale2);
-    }
-    if (kKind == kDistill) {
-      if (threadIdx.x < kWave) finish_distill<T, kWave>(a, row, a.count, threadIdx.x, q, t);
-      continue;
-    }
-    if (threadIdx.x == 0) finish_log_probs<T>(a, row, token, t);
-    if (a.top == 0) continue;
-    const int all = a.parts * a.top;
-    __syncthreads();  // (of the row before)
-    for (int i = threadIdx.x; i < all; i += kBlock) lists[i] = a.lists[row * all + i];
-    __syncthreads();
-    // an entry's place: how many of every part's, each in order, come before it
-    for (int i = threadIdx.x; i < all; i += kBlock) {
-      const uint64_t w = lists[i];
-      if (w == 0) continue;
-      int place = 0;
-      for (int p = 0; p < a.parts && place < a.top; ++p) {
-        int lo = 0, hi = a.top;
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (lists[p * a.top + mid] > w)
-            lo = mid + 1;
-          else
-            hi = mid;
-        }
-        place += lo;
+    auto stats = [&]() __attribute__((always_inline)) {
+      f32x4 p = {-INFINITY, 0.f, 0.f, 0.f};
+      if (lane < a.parts) p = *reinterpret_cast<const f32x4 *>(a.stats + (row * a.parts + lane) * 4);
+      Stats t{lanes_max<kWave>(p[0]), 0.f, 0.f};
+      const float d = fmaxf((p[0] - shift_of(t.m)) * a.scale2, kLow), e = __builtin_amdgcn_exp2f(d);
+      t.s = lanes_sum<kWave>(p[1] * e), t.a = lanes_sum<kWave>(fmaf(d, p[1], p[2]) * e);
+      return t;
+    };
+    if constexpr (kKind == kDistill) {
+      const Teacher<kWave> q(a, row, a.count, lane);
+      if (threadIdx.x < kWave) {
+        if (q.some)
+          finish_distill<T, kWave>(a, row, true, lane, q, stats());
+        else if (lane == 0)
+          pass_over(a, row);
       }
-      if (place < a.top) put_best(a, row, place, w, t);
+    } else {
+      const int all = a.parts * a.top;
+      __syncthreads();  // (of the row before)
+      for (int i = threadIdx.x; i < all; i += kBlock) lists[i] = a.lists[row * all + i];
+      float at_token = 0;
+      if (a.tokens) {
+        const int64_t token = token_at(a.tokens, a.wide, row, a.vocab);
+        if (token < 0) {
+          if (threadIdx.x == 0) pass_over(a, row);
+          if ((int)threadIdx.x < a.top) put_best(a, row, threadIdx.x, 0, Stats{});
+          continue;
+        }
+        at_token = logit_at<T>(a, row, token);
+      }
+      const Stats t = stats();
+      if (threadIdx.x == 0) finish_log_probs(a, row, at_token, t);
+      if (a.top == 0) continue;
+      __syncthreads();
+      // an entry's place: how many of every part's, each in order, come before it
+      for (int i = threadIdx.x; i < all; i += kBlock) {
+        const uint64_t w = lists[i];
+        if (w == 0) continue;
+        int place = 0;
+        for (int p = 0; p < a.parts && place < a.top; ++p) {
+          int lo = 0, hi = a.top;
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (lists[p * a.top + mid] > w)
+              lo = mid + 1;
+            else
+              hi = mid;
+          }
+          place += lo;
+        }
+        if (place < a.top) put_best(a, row, place, w, t);
+      }
     }
   }
 }
@@ -512,18 +617,16 @@ struct Fix {
   int column;  // or -1
   float q;
 };
-// The entries of a teacher that stand for columns of their own, with the weights of those that name the same.
+// The teacher's entries with their weights, where the lanes of a row find them all.
 template <int kLanes>
-__device__ __forceinline__ Teacher teacher_fixes(const LogitsArgs &a, int64_t row, int count, int lane, bool write, Fix *fix) {
-  const Teacher q = teacher_of<kLanes>(a, row, count, lane);
-  const float over = 1.f / q.sum;
-  for (int k = lane; k < count && write; k += kLanes) {
-    int64_t column;
-    const float t = teacher_at(a, row, k, column);
-    fix[k] = Fix{(int)column, column < 0 ? 0.f : __builtin_amdgcn_exp2f((t - shift_of(q.top)) * kLog2e) * over};
-  }
-  return q;
+__device__ __forceinline__ bool put_entries(const LogitsArgs &a, int64_t row, int count, int lane, bool write, Fix *fix) {
+  const Teacher<kLanes> q(a, row, count, lane);
+#pragma unroll
+  for (int i = 0; i < Teacher<kLanes>::kHeldEntries; ++i)
+    if (write && lane + i * kLanes < count) fix[lane + i * kLanes] = Fix{q.column[i], q.column[i] < 0 ? 0.f : q.q[i]};
+  return q.some;
 }
+// An entry that stands for its column, with the weights of all that name it.
 __device__ __forceinline__ Fix fix_of(const Fix *fix, int k, int count) {
   Fix f = fix[k];
   for (int j = 0; j < count && f.column >= 0; ++j) {
@@ -547,7 +650,7 @@ __global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
     bool some = false;
     if (kKind == kDistill) {
       __syncthreads();
-      some = teacher_fixes<kLanes>(a, row, here ? a.count : 0, lane, true, fix).some;
+      some = put_entries<kLanes>(a, row, here ? a.count : 0, lane, true, fix);
     } else if (here && a.tokens) {
       token = token_at(a.tokens, a.wide, row, a.vocab);
     }
@@ -596,7 +699,7 @@ __global__ __launch_bounds__(kBlock) void wide_grad_kernel(LogitsArgs a) {
     bool some = false;
     if (kKind == kDistill) {
       __syncthreads();
-      some = teacher_fixes<kWave>(a, row, a.count, threadIdx.x % kWave, threadIdx.x < kWave, fix).some;
+      some = put_entries<kWave>(a, row, a.count, threadIdx.x % kWave, threadIdx.x < kWave, fix);
     } else if (a.tokens) {
       token = token_at(a.tokens, a.wide, row, a.vocab);
     }
@@ -632,16 +735,16 @@ __global__ __launch_bounds__(kBlock) void wide_grad_kernel(LogitsArgs a) {
 
 // ---- host -------------------------------------------------------------------------------------------------------
 constexpr int kWaveVecs = 256;  // widest row of a wave
-// Parts of a row: what a workgroup holds at most, and more where rows are few, down to two vectors a thread.
+constexpr int kLarge = 1024;    // threads of a workgroup where rows are few
+constexpr int kFewRows = 512;
+// Parts of a row: what a workgroup holds at most.
 void split(int64_t rows, int vecs, int &parts, int &part_vecs) {
-  int n = (vecs + kHeld * kBlock - 1) / (kHeld * kBlock);
-  if (rows < 1024) {
-    const int64_t fill = 1024 / rows, most = vecs / (2 * kBlock);
-    n = (int)std::max<int64_t>(n, std::min(std::min(fill, most), (int64_t)kJoined / kMaxTop));
-  }
+  const int most = rows < kFewRows ? kHeldFew * kLarge : kHeld * kBlock, n = (vecs + most - 1) / most;
   part_vecs = (vecs + n - 1) / n;
   parts = (vecs + part_vecs - 1) / part_vecs;
 }
+static_assert(kMaxVocab / 4 / (kHeld * kBlock) < kWave && (kMaxVocab / 4 / (kHeld * kBlock) + 1) * kMaxTop <= kJoined,
+              "a part a lane, and all their best tokens in shared memory");
 // (of the type with most vectors: the workspace does not go by the type)
 size_t split_bytes(int64_t rows, int64_t vocab, int64_t top) {
   if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab || top < 0 || top > kMaxTop) return 0;
@@ -657,12 +760,20 @@ size_t split_bytes(int64_t rows, int64_t vocab, int64_t top) {
 // f(lanes of a row, vectors of a lane) for rows of a wave or less
 template <typename F>
 void by_lanes(int vecs, const F &f) {
+  using one = std::integral_constant<int, 1>;
+  using two = std::integral_constant<int, 2>;
   if (vecs <= 4)
-    f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 4>(), one());
+  else if (vecs <= 8)
+    f(std::integral_constant<int, 4>(), two());
   else if (vecs <= 16)
-    f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 8>(), two());
+  else if (vecs <= 32)
+    f(std::integral_constant<int, 16>(), two());
   else if (vecs <= 64)
-    f(std::integral_constant<int, 32>(), std::integral_constant<int, 2>());
+    f(std::integral_constant<int, 32>(), two());
+  else if (vecs <= 128)
+    f(std::integral_constant<int, 64>(), two());
   else
     f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
 }
@@ -677,30 +788,40 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
     if (vecs <= kWaveVecs) {
       by_lanes(vecs, [&](auto lanes, auto held) {
         constexpr int kLanes = decltype(lanes)::value;
-        hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind>),
-                           dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))), dim3(kBlock), 0, st, a);
+        const dim3 grid((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes)));
+        if (kKind == kLogProbs && a.top > 0)
+          hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind, kKind == kLogProbs>), grid, dim3(kBlock), 0, st, a);
+        else
+          hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind, false>), grid, dim3(kBlock), 0, st, a);
       });
       return;
     }
     split(a.rows, vecs, a.parts, a.part_vecs);
     a.stats = reinterpret_cast<float *>(ws);
     a.lists = reinterpret_cast<uint64_t *>(ws + align_up((size_t)a.rows * a.parts * 16, 256));
-    const dim3 grid((unsigned)grid_of(a.rows * a.parts)), block(kBlock);
-    auto launch = [&](auto held) {
-      constexpr int kVecs = decltype(held)::value;
+    auto launch = [&](auto size, auto held) {
+      constexpr int kThreads = decltype(size)::value, kVecs = decltype(held)::value;
+      const dim3 grid((unsigned)std::min(a.rows * a.parts, kMostItems / kThreads)), block(kThreads);
       if (kKind == kLogProbs && a.top > 0)
-        hipLaunchKernelGGL((wide_kernel<T, kVecs, kKind, kKind == kLogProbs>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, kKind == kLogProbs>), grid, block, 0, st, a);
       else
-        hipLaunchKernelGGL((wide_kernel<T, kVecs, kKind, false>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, false>), grid, block, 0, st, a);
     };
-    if (a.part_vecs <= 4 * kBlock)
-      launch(std::integral_constant<int, 4>());
+    using small = std::integral_constant<int, kBlock>;
+    using large = std::integral_constant<int, kLarge>;
+    const bool few = a.rows < kFewRows && vecs > 4 * kBlock;
+    if (few && a.part_vecs <= 4 * kLarge)
+      launch(large(), std::integral_constant<int, 4>());
+    else if (few)
+      launch(large(), std::integral_constant<int, kHeldFew>());
+    else if (a.part_vecs <= 4 * kBlock)
+      launch(small(), std::integral_constant<int, 4>());
     else if (a.part_vecs <= 8 * kBlock)
-      launch(std::integral_constant<int, 8>());
+      launch(small(), std::integral_constant<int, 8>());
     else
-      launch(std::integral_constant<int, kHeld>());
+      launch(small(), std::integral_constant<int, kHeld>());
     if (a.parts > 1)
-      hipLaunchKernelGGL((join_kernel<T, kKind>), dim3((unsigned)grid_of(a.rows)), block, 0, st, a);
+      hipLaunchKernelGGL((join_kernel<T, kKind>), dim3((unsigned)grid_of(a.rows)), dim3(kBlock), 0, st, a);
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
   return 0;
