@@ -42,7 +42,7 @@ __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
     for (int v = lane; v * kPer<T> < a.width; v += kLanes) {
       const Slot<T> s(v, a.width);
       Vals<T> x = {};
-      if (token >= 0) x = __builtin_convertvector(load_slot<true>(from, s), Vals<T>) * a.scale;
+      if (token >= 0) x = __builtin_convertvector(load_slot<T>(from, s, a.width < kPer<T>), Vals<T>) * a.scale;
       store_slot(to, s, x);
     }
   }
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kBlock) void embed_sums_kernel(SumArgs a) {
       key[i] = at + i < end ? a.keys[at + i] : none;
       row[i] = Raw<T>{};
       if (key[i] != none && s.any())
-        row[i] = load_slot<true>(static_cast<const T *>(a.e.rows) + (int64_t)a.places[at + i] * a.e.stride, s);
+        row[i] = load_slot<T>(static_cast<const T *>(a.e.rows) + (int64_t)a.places[at + i] * a.e.stride, s, a.e.width < kPer<T>);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {

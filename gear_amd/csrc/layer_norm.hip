@@ -104,6 +104,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArg
   using At = Place<kWhole, T>;
   __shared__ float part[2][kThreads / kWave][4];
   const int lane = threadIdx.x % kLanes;
+  const bool tiny = a.width < kPer<T>;
   int turn = 0;
   Vals<T> w[kVecs], b[kVecs];
 #pragma unroll
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArg
       const At s(lane + i * kLanes, a.width);
       xs[i] = rs[i] = Raw<T>{};
       if (here && s.any()) {
-        xs[i] = load_slot<true>(x, s);
-        if constexpr (kResidual) rs[i] = load_slot<true>(r, s);
+        xs[i] = load_slot<T>(x, s, tiny);
+        if constexpr (kResidual) rs[i] = load_slot<T>(r, s, tiny);
       }
     }
 #pragma unroll
@@ -166,6 +167,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
   using At = Place<kWhole, T>;
   __shared__ float part[2][kThreads / kWave][4];
   const int lane = threadIdx.x % kLanes;
+  const bool tiny = a.width < kPer<T>;
   int turn = 0;
   Vals<T> w[kVecs], dw[kVecs], db[kVecs];
 #pragma unroll
@@ -187,8 +189,8 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
       const At s(lane + i * kLanes, a.width);
       us[i] = g[i] = plus[i] = Raw<T>{};
       if (here && s.any()) {
-        us[i] = load_slot<true>(x, s), g[i] = load_slot<true>(dy, s);
-        if constexpr (kSum) plus[i] = load_slot<true>(ds, s);
+        us[i] = load_slot<T>(x, s, tiny), g[i] = load_slot<T>(dy, s, tiny);
+        if constexpr (kSum) plus[i] = load_slot<T>(ds, s, tiny);
       }
     }
 #pragma unroll

@@ -25,7 +25,7 @@ constexpr int kBlock = 256;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxTop = 64;     // best tokens, and a teacher's entries
 constexpr int kHeld = 17;       // vectors of a thread
-constexpr int kHeldFew = 16;    // ... of a workgroup of 1024
+constexpr int kHeldFew = 12;    // ... of a workgroup of 1024
 constexpr int kJoined = 4096;   // entries that a join puts in order
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kLow = -1e30f;  // below any exponent that counts, and any logit that is allowed
@@ -94,11 +94,10 @@ __device__ __forceinline__ Raw<T> nothing() {
   return x;
 }
 // a vector of a row, -inf where it has no elements of its own
-template <bool kNarrow, typename T>
-__device__ __forceinline__ Raw<T> load_logits(const T *row, int v, int vocab) {
-  const Slot<T> s(v, vocab);
-  if (kNarrow && !s.any()) return nothing<T>();
-  Raw<T> x = load_slot<kNarrow>(row, s);
+template <typename T>
+__device__ __forceinline__ Raw<T> load_logits(const T *row, const Slot<T> &s, bool tiny) {
+  if (!s.any()) return nothing<T>();
+  Raw<T> x = load_slot<T>(row, s, tiny);
   if (!s.whole()) {
 #pragma unroll
     for (int e = 0; e < kPer<T>; ++e)
@@ -106,11 +105,30 @@ __device__ __forceinline__ Raw<T> load_logits(const T *row, int v, int vocab) {
   }
   return x;
 }
+// A row of more than a vector, cut where addresses are multiples of 16 bytes: elements before the first such place, whole
+// vectors, elements behind the last.  (16384 odd rows of 66 KB, read at any address 213 us, cut so 170.)
+template <typename T>
+struct Cut {
+  int head, vecs, tail;
+  __device__ __forceinline__ Cut(const T *row, int width) {
+    head = (kPer<T> - misaligned(row)) & (kPer<T> - 1);
+    vecs = (width - head) / kPer<T>;
+    tail = width - head - vecs * kPer<T>;
+  }
+  __device__ __forceinline__ Slot<T> whole(int v) const { return Slot<T>(head + v * kPer<T>, 0, kPer<T>); }
+  // both ends, of lanes 0 and 1 of a workgroup that has them
+  __device__ __forceinline__ Slot<T> edge(int id, int width, bool first, bool last) const {
+    if (id == 0 && first && head > 0) return Slot<T>(0, 0, head);
+    if (id == 1 && last && tail > 0) return Slot<T>(width - kPer<T>, kPer<T> - tail, kPer<T>);
+    return Slot<T>::none();
+  }
+};
 template <typename T>
 __device__ __forceinline__ float max_of(const Raw<T> &x) {
-  float m = (float)x[0];
+  const Vals<T> v = values_of<T>(x);
+  float m = v[0];
 #pragma unroll
-  for (int e = 1; e < kPer<T>; ++e) m = fmaxf(m, (float)x[e]);
+  for (int e = 1; e < kPer<T>; ++e) m = fmaxf(m, v[e]);
   return m;
 }
 // Exponents are in base 2.  Those of x scale2 - m2, with m2 = m scale2 as it is rounded, take one operation an element;
@@ -127,9 +145,10 @@ struct Shift {
 };
 template <bool kEntropy, bool kHuge, typename T>
 __device__ __forceinline__ void add_to(Stats &t, const Raw<T> &x, const Shift &m, float scale2) {
+  const Vals<T> v = values_of<T>(x);
 #pragma unroll
   for (int e = 0; e < kPer<T>; ++e) {
-    const float d = kHuge ? ((float)x[e] - m.m) * scale2 : fmaf((float)x[e], scale2, -m.m2), p = __builtin_amdgcn_exp2f(d);
+    const float d = kHuge ? (v[e] - m.m) * scale2 : fmaf(v[e], scale2, -m.m2), p = __builtin_amdgcn_exp2f(d);
     t.s += p;
     if (kEntropy) t.a = fmaf(fmaxf(d, kLow), p, t.a);
   }
@@ -247,11 +266,12 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return (int32_t)b < 0 ? ~b : b | 0x80000000u;
 }
 
-// The best `top` of what kThreads threads hold of the vectors [first, last), put(place, entry) for each; entries that are
-// not there are 0.  mine: the largest of a thread's elements; finite: whether the row holds no NaN or infinity.
-template <typename T, int kThreads, int kVecs, typename Put>
-__device__ __forceinline__ void best_of(const T *row, Raw<T> (&x)[kVecs], float mine, bool finite, int first, int last, int vocab,
-                                        int top, BestSmem<kThreads> &sm, const Put &put) {
+// The best `top` of what kThreads threads hold, put(place, entry) for each; entries that are not there are 0.  slot(i): where
+// a thread's vector i lies; rounds: how many there are; mine: the largest of a thread's elements; finite: whether the row
+// holds no NaN or infinity.
+template <typename T, int kThreads, int kVecs, typename At, typename Put>
+__device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVecs], const At &slot, float mine, bool finite, int top,
+                                        BestSmem<kThreads> &sm, const Put &put) {
   constexpr int kGroup = kThreads / kWave;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) as_it_came<T>(x[i]);
@@ -274,14 +294,14 @@ __device__ __forceinline__ void best_of(const T *row, Raw<T> (&x)[kVecs], float 
   if (finite && mine >= bound) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      if (first + i * kThreads < last && max_of<T>(x[i]) >= bound) {
-        const int v = first + id + i * kThreads;
-        const Slot<T> s(v, vocab);
+      if (max_of<T>(x[i]) >= bound) {
+        const Slot<T> s = slot(i);
+        const Vals<T> value = values_of<T>(x[i]);
 #pragma unroll
         for (int e = 0; e < kPer<T>; ++e)
-          if ((float)x[i][e] >= bound && v < last && s.own(e)) {
+          if (value[e] >= bound && s.own(e)) {
             const int at = atomicAdd(&sm.count, 1);
-            if (at < sm.kList) sm.list[at] = entry_of((float)x[i][e], s.col + e);
+            if (at < sm.kList) sm.list[at] = entry_of(value[e], s.col + e);
           }
       }
     }
@@ -308,12 +328,13 @@ __device__ __forceinline__ void best_of(const T *row, Raw<T> (&x)[kVecs], float 
   for (int k = 0; k < top; ++k) {
     uint64_t best = 0;
 #pragma unroll 1
-    for (int v = first + id; v < last; v += kThreads) {
-      const Slot<T> s(v, vocab);
-      const Raw<T> y = load_slot<kThreads == kWave>(row, s);
+    for (int i = 0; i < kVecs; ++i) {
+      const Slot<T> s = slot(i);
+      if (!s.any()) continue;
+      const Vals<T> y = values_of<T>(load_slot<T>(row, s, tiny));
 #pragma unroll
       for (int e = 0; e < kPer<T>; ++e) {
-        const uint64_t w = entry_of((float)y[e], s.col + e);
+        const uint64_t w = entry_of(y[e], s.col + e);
         if (s.own(e) && w < limit && w > best) best = w;
       }
     }
@@ -335,6 +356,7 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
   constexpr int kRows = kBlock / kLanes;
   __shared__ BestSmem<kWave> best[kTop && kLanes == kWave ? kRows : 1];
   const int lane = threadIdx.x % kLanes;
+  const bool tiny = a.vocab < kPer<T>;
   // (the lanes of a wave go round alike: they exchange sums)
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / kLanes;
@@ -351,9 +373,11 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
       if (here) at_token = logit_at<T>(a, row, token);
     }
     Raw<T> x[kVecs];
+    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
+    const int shift = kLanes < 32 || tiny ? 0 : misaligned(from);  // (short rows share their lines anyway)
+    auto slot = [&](int i) { return Slot<T>::shifted(lane + i * kLanes, a.vocab, shift); };
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      x[i] = here ? load_logits<true>(static_cast<const T *>(a.logits) + row * a.stride, lane + i * kLanes, a.vocab) : nothing<T>();
+    for (int i = 0; i < kVecs; ++i) x[i] = here ? load_logits<T>(from, slot(i), tiny) : nothing<T>();
     auto stats = [&](Stats &t) __attribute__((always_inline)) {
       const float mine = t.m;
       t.m = lanes_max<kLanes>(mine);
@@ -383,14 +407,13 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
       if (here && lane == 0) finish_log_probs(a, row, at_token, t);
       if constexpr (kTop && kLanes == kWave) {
         if (here)
-          best_of<T, kWave, kVecs>(static_cast<const T *>(a.logits) + row * a.stride, x, mine, t.s == t.s, 0,
-                                   (a.vocab + kPer<T> - 1) / kPer<T>, a.vocab, a.top, best[threadIdx.x / kWave],
+          best_of<T, kWave, kVecs>(from, tiny, x, slot, mine, t.s == t.s, a.top, best[threadIdx.x / kWave],
                                    [&](int place, uint64_t e) { put_best(a, row, place, e, t); });
       } else if constexpr (kTop) {
         uint64_t entry[kVecs * kPer<T>], last = 0;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-          const Slot<T> s(lane + i * kLanes, a.vocab);
+          const Slot<T> s = slot(i);
 #pragma unroll
           for (int e = 0; e < kPer<T>; ++e) entry[i * kPer<T> + e] = s.own(e) ? entry_of((float)x[i][e], s.col + e) : 0;
         }
@@ -424,10 +447,16 @@ template <typename T, int kThreads, int kVecs, int kKind, bool kTop>
 __global__ __launch_bounds__(kThreads) void wide_kernel(LogitsArgs a) {
   __shared__ float part_max[kThreads / kWave], part_sum[2][kThreads / kWave];
   __shared__ BestSmem<kTop ? kThreads : kWave> best;
-  const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
   for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
     const int64_t row = unit / a.parts;
-    const int part = (int)(unit - row * a.parts), first = part * a.part_vecs, last = min(first + a.part_vecs, vecs);
+    const int part = (int)(unit - row * a.parts);
+    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
+    const Cut<T> cut(from, a.vocab);
+    const int first = part * a.part_vecs, last = min(first + a.part_vecs, cut.vecs);
+    auto slot = [&](int i) {  // (the last one is an end of the row)
+      const int v = first + (int)threadIdx.x + i * kThreads;
+      return i == kVecs ? cut.edge(threadIdx.x, a.vocab, part == 0, part == a.parts - 1) : v < last ? cut.whole(v) : Slot<T>::none();
+    };
     float at_token = 0;
     if (kKind == kLogProbs && a.tokens) {
       const int64_t token = token_at(a.tokens, a.wide, row, a.vocab);
@@ -440,35 +469,37 @@ __global__ __launch_bounds__(kThreads) void wide_kernel(LogitsArgs a) {
       }
       at_token = logit_at<T>(a, row, token);
     }
-    const T *from = static_cast<const T *>(a.logits) + row * a.stride;
-    Raw<T> x[kVecs];
+    Raw<T> x[kVecs + 1];
     auto load = [&]() __attribute__((always_inline)) {
+      const T *at = from + cut.head + (int64_t)(first + threadIdx.x) * kPer<T>;
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
-        const int v = first + threadIdx.x + i * kThreads;
         x[i] = nothing<T>();
-        if (v < last) x[i] = load_logits<false>(from, v, a.vocab);
+        if (first + (int)threadIdx.x + i * kThreads < last) x[i] = reinterpret_cast<const AnyRaw<T> *>(at + i * kThreads * kPer<T>)->v;
       }
+      x[kVecs] = nothing<T>();
+      if (threadIdx.x < 2) x[kVecs] = load_logits<T>(from, slot(kVecs), false);
     };
+    // (whether a wave has anything of round i)
+    auto some = [&](int i) __attribute__((always_inline)) { return i < kVecs ? first + i * kThreads < last : threadIdx.x < kWave; };
     auto stats = [&](float &mine) __attribute__((always_inline)) {
       mine = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-        if (first + i * kThreads < last) mine = fmaxf(mine, max_of<T>(x[i]));
+      for (int i = 0; i <= kVecs; ++i)
+        if (some(i)) mine = fmaxf(mine, max_of<T>(x[i]));
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) as_it_came<T>(x[i]);
+      for (int i = 0; i <= kVecs; ++i) as_it_came<T>(x[i]);
       __syncthreads();  // (of the unit before: its shared memory)
       Stats t{block_reduce<kThreads>(lanes_max<kWave>(mine), part_max, [](float p, float r) { return fmaxf(p, r); }), 0.f, 0.f};
       const Shift m(t.m, a.scale2);
       if (__builtin_expect(m.huge(), 0)) {
 #pragma unroll 1
-        for (int v = first + threadIdx.x; v < last; v += kThreads)
-          add_to<kKind == kLogProbs, true, T>(t, load_logits<false>(from, v, a.vocab), m, a.scale2);
+        for (int i = 0; i <= kVecs; ++i)
+          add_to<kKind == kLogProbs, true, T>(t, load_logits<T>(from, slot(i), false), m, a.scale2);
       } else {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-          if (first + i * kThreads < last) add_to<kKind == kLogProbs, false, T>(t, x[i], m, a.scale2);
-        }
+        for (int i = 0; i <= kVecs; ++i)
+          if (some(i)) add_to<kKind == kLogProbs, false, T>(t, x[i], m, a.scale2);
       }
       auto plus = [](float p, float r) { return p + r; };
       const float s = lanes_sum<kWave>(t.s);
@@ -510,7 +541,7 @@ __global__ __launch_bounds__(kThreads) void wide_kernel(LogitsArgs a) {
           *reinterpret_cast<f32x4 *>(a.stats + unit * 4) = f32x4{t.m, t.s, t.a, 0.f};
       }
       if constexpr (kTop)
-        best_of<T, kThreads, kVecs>(from, x, mine, t.s == t.s, first, last, a.vocab, a.top, best, [&](int place, uint64_t e) {
+        best_of<T, kThreads, kVecs + 1>(from, false, x, slot, mine, t.s == t.s, a.top, best, [&](int place, uint64_t e) {
           if (alone)
             put_best(a, row, place, e, t);
           else
@@ -583,34 +614,53 @@ __global__ __launch_bounds__(kBlock) void join_kernel(LogitsArgs a) {
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------
-// p (alpha + beta log p) of a logit, times the scale
+// p (alpha + beta log2 p) of a logit, times the scale; kBeta: beta is not 0
 struct Slope {
-  float lse, scale, alpha, beta;
+  float lse2, scale2, alpha, beta;
+  template <bool kBeta>
   __device__ __forceinline__ float at(float x) const {
     // (above 0 only by what lse lost when it was rounded, where logits are huge)
-    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale, -lse), kLow, 0.f), p = __builtin_amdgcn_exp2f(l * kLog2e);
-    return p * fmaf(beta, l, alpha);
+    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale2, -lse2), kLow, 0.f), p = __builtin_amdgcn_exp2f(l);
+    return p * (kBeta ? fmaf(beta, l, alpha) : alpha);
   }
 };
 
 // Of a row: whether it has a gradient at all, its slope, and what is added at the given token.
 template <int kKind>
-__device__ __forceinline__ bool slope_of(const LogitsArgs &a, int64_t row, bool some, int64_t token, Slope &s, float &more) {
-  if (kKind == kLogProbs ? a.tokens && token < 0 : !some) return false;
-  s.lse = a.lse_in[row];
-  if (s.lse == -INFINITY) return false;  // nothing was allowed
-  s.scale = a.scale;
-  const float nan = s.lse - s.lse;       // 0, or NaN for a row of NaN
+__device__ __forceinline__ bool slope_of(const LogitsArgs &a, int64_t row, bool some, Slope &s, float &more) {
+  if (!some) return false;
+  const float lse = a.lse_in[row];
+  if (lse == -INFINITY) return false;  // nothing was allowed
+  s.lse2 = lse * kLog2e, s.scale2 = a.scale2;
+  const float nan = lse - lse;         // 0, or NaN for a row of NaN
   if (kKind == kLogProbs) {
     const float dl = a.dlog_probs ? a.dlog_probs[row] : 0.f, de = a.dentropy ? a.dentropy[row] : 0.f;
     s.alpha = -a.scale * (dl + (a.dentropy ? de * a.entropy_in[row] : 0.f)) + nan;
-    s.beta = -a.scale * de;
+    s.beta = -a.scale * de * kLn2;
     more = a.scale * dl;
   } else {
     s.alpha = a.scale * a.dloss[row] + nan, s.beta = 0;
     more = -s.alpha;
   }
   return true;
+}
+
+// The gradient of a vector; token: a column of the row, or -1
+template <bool kBeta, bool kToken, typename T>
+__device__ __forceinline__ void grad_vector(const T *from, T *to, const Slot<T> &s, bool tiny, bool live, const Slope &slope, int token,
+                                            float more) {
+  Vals<T> y = {};
+  if (live) {
+    y = values_of<T>(load_slot<T>(from, s, tiny));
+#pragma unroll
+    for (int e = 0; e < kPer<T>; ++e) y[e] = slope.template at<kBeta>(y[e]);
+    if (kToken && (unsigned)(token - s.col) < (unsigned)kPer<T>) {
+#pragma unroll
+      for (int e = 0; e < kPer<T>; ++e)
+        if (s.col + e == token) y[e] += more;
+    }
+  }
+  store_slot(to, s, y);
 }
 
 struct Fix {
@@ -637,97 +687,85 @@ __device__ __forceinline__ Fix fix_of(const Fix *fix, int k, int count) {
   return f;
 }
 
-template <typename T, int kLanes, int kKind>
+template <typename T, int kLanes, int kKind, bool kBeta>
 __global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
   constexpr int kRows = kBlock / kLanes;
   __shared__ Fix fixes[kKind == kDistill ? kRows : 1][kMaxTop];
   const int lane = threadIdx.x % kLanes;
+  const bool tiny = a.vocab < kPer<T>;
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / kLanes;
     const bool here = row < a.rows;
     Fix *fix = fixes[kKind == kDistill ? threadIdx.x / kLanes : 0];
-    int64_t token = -1;
-    bool some = false;
+    int token = -1;
+    bool some = here;
     if (kKind == kDistill) {
-      __syncthreads();
-      some = put_entries<kLanes>(a, row, here ? a.count : 0, lane, true, fix);
+      __syncthreads();  // (of the rows before)
+      some = put_entries<kLanes>(a, row, here ? a.count : 0, lane, true, fix) && here;
     } else if (here && a.tokens) {
-      token = token_at(a.tokens, a.wide, row, a.vocab);
+      token = (int)token_at(a.tokens, a.wide, row, a.vocab);
+      some = token >= 0;
     }
     Slope slope{};
     float more = 0;
     const T *from = static_cast<const T *>(a.logits) + row * a.stride;
     T *to = static_cast<T *>(a.dlogits) + row * a.vocab;
-    const bool live = here && slope_of<kKind>(a, row, some, token, slope, more);
+    const bool live = slope_of<kKind>(a, row, some, slope, more);
     if (here) {
-      for (int v = lane; v * kPer<T> < a.vocab; v += kLanes) {
-        const Slot<T> s(v, a.vocab);
-        Vals<T> y = {};
-        if (live) {
-          y = __builtin_convertvector(load_slot<true>(from, s), Vals<T>);
-#pragma unroll
-          for (int e = 0; e < kPer<T>; ++e) {
-            y[e] = slope.at(y[e]);
-            if (kKind == kLogProbs && s.col + e == token) y[e] += more;
-          }
-        }
-        store_slot(to, s, y);
-      }
+      const int shift = kLanes < 32 || tiny ? 0 : misaligned(to);
+      for (int v = lane; v * kPer<T> < a.vocab + shift; v += kLanes)
+        grad_vector<kBeta, kKind == kLogProbs>(from, to, Slot<T>::shifted(v, a.vocab, shift), tiny, live, slope, token, more);
     }
     if (kKind == kDistill) {
       __syncthreads();  // the entries are there, and the row is written
       if (live)
         for (int k = lane; k < a.count; k += kLanes) {
           const Fix f = fix_of(fix, k, a.count);
-          if (f.column >= 0) to[f.column] = (T)fmaf(more, f.q, slope.at((float)from[f.column]));
+          if (f.column >= 0) to[f.column] = (T)fmaf(more, f.q, slope.at<false>((float)from[f.column]));
         }
     }
   }
 }
 
-constexpr int kGradVecs = 8;  // vectors of a thread
-template <typename T, int kKind>
+constexpr int kGradVecs = 8;  // vectors of a thread, at most
+template <typename T, int kKind, bool kBeta>
 __global__ __launch_bounds__(kBlock) void wide_grad_kernel(LogitsArgs a) {
   __shared__ Fix fix[kMaxTop];
-  const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
   for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
     const int64_t row = unit / a.parts;
-    const int part = (int)(unit - row * a.parts), first = part * kGradVecs * kBlock, last = min(first + kGradVecs * kBlock, vecs);
+    const int part = (int)(unit - row * a.parts);
     const T *from = static_cast<const T *>(a.logits) + row * a.stride;
     T *to = static_cast<T *>(a.dlogits) + row * a.vocab;
-    int64_t token = -1;
-    bool some = false;
+    const Cut<T> cut(to, a.vocab);  // (where logits and gradients lie differently, it is for the stores)
+    const int first = part * a.part_vecs, last = min(first + a.part_vecs, cut.vecs);
+    int token = -1;
+    bool some = true;
     if (kKind == kDistill) {
-      __syncthreads();
+      __syncthreads();  // (of the unit before)
       some = put_entries<kWave>(a, row, a.count, threadIdx.x % kWave, threadIdx.x < kWave, fix);
     } else if (a.tokens) {
-      token = token_at(a.tokens, a.wide, row, a.vocab);
+      token = (int)token_at(a.tokens, a.wide, row, a.vocab);
+      some = token >= 0;
     }
     Slope slope{};
     float more = 0;
-    const bool live = slope_of<kKind>(a, row, some, token, slope, more);
+    const bool live = slope_of<kKind>(a, row, some, slope, more);
 #pragma unroll
     for (int i = 0; i < kGradVecs; ++i) {
       const int v = first + threadIdx.x + i * kBlock;
-      if (v >= last) continue;
-      const Slot<T> s(v, a.vocab);
-      Vals<T> y = {};
-      if (live) {
-        y = __builtin_convertvector(load_slot<false>(from, s), Vals<T>);
-#pragma unroll
-        for (int e = 0; e < kPer<T>; ++e) {
-          y[e] = slope.at(y[e]);
-          if (kKind == kLogProbs && s.col + e == token) y[e] += more;
-        }
-      }
-      store_slot(to, s, y);
+      if (v < last) grad_vector<kBeta, kKind == kLogProbs>(from, to, cut.whole(v), false, live, slope, token, more);
+    }
+    if (threadIdx.x < 2) {
+      const Slot<T> edge = cut.edge(threadIdx.x, a.vocab, part == 0, part == a.parts - 1);
+      if (edge.any()) grad_vector<kBeta, kKind == kLogProbs>(from, to, edge, false, live, slope, token, more);
     }
     if (kKind == kDistill) {
       __syncthreads();  // the entries are there, and the part is written
       if (live && (int)threadIdx.x < a.count) {
         const Fix f = fix_of(fix, threadIdx.x, a.count);
-        if (f.column >= first * kPer<T> && f.column < last * kPer<T>)
-          to[f.column] = (T)fmaf(more, f.q, slope.at((float)from[f.column]));
+        const int begin = part == 0 ? 0 : cut.head + first * kPer<T>, end = part == a.parts - 1 ? a.vocab : cut.head + last * kPer<T>;
+        if (f.column >= begin && f.column < end)
+          to[f.column] = (T)fmaf(more, f.q, slope.at<false>((float)from[f.column]));
       }
     }
   }
@@ -778,13 +816,21 @@ void by_lanes(int vecs, const F &f) {
     f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
 }
 
+// vectors of a row at most (one that is partial at both ends has one more)
+template <typename T>
+int vecs_of(const LogitsArgs &a) {
+  const bool same = aligned_to(a.logits, 16) && (a.rows == 1 || a.stride % kPer<T> == 0) &&
+                    aligned_to(a.dlogits, 16) && (a.dlogits == nullptr || a.rows == 1 || a.vocab % kPer<T> == 0);
+  return a.vocab < kPer<T> ? 1 : (a.vocab + (same ? 0 : kPer<T> - 1) + kPer<T> - 1) / kPer<T>;
+}
+
 int64_t grid_of(int64_t blocks) { return std::min(blocks, kMostItems / kBlock); }
 
 template <int kKind>
 int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
   by_type(dtype, [&](auto type) {
     using T = decltype(type);
-    const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
+    const int vecs = vecs_of<T>(a);
     if (vecs <= kWaveVecs) {
       by_lanes(vecs, [&](auto lanes, auto held) {
         constexpr int kLanes = decltype(lanes)::value;
@@ -796,7 +842,7 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
       });
       return;
     }
-    split(a.rows, vecs, a.parts, a.part_vecs);
+    split(a.rows, (a.vocab + kPer<T> - 1) / kPer<T>, a.parts, a.part_vecs);
     a.stats = reinterpret_cast<float *>(ws);
     a.lists = reinterpret_cast<uint64_t *>(ws + align_up((size_t)a.rows * a.parts * 16, 256));
     auto launch = [&](auto size, auto held) {
@@ -831,17 +877,29 @@ template <int kKind>
 int backward(LogitsArgs &a, int dtype, hipStream_t st) {
   by_type(dtype, [&](auto type) {
     using T = decltype(type);
-    const int vecs = (a.vocab + kPer<T> - 1) / kPer<T>;
-    if (vecs <= kWaveVecs) {
-      by_lanes(vecs, [&](auto lanes, auto) {
-        constexpr int kLanes = decltype(lanes)::value;
-        hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, kKind>), dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))),
-                           dim3(kBlock), 0, st, a);
-      });
-      return;
+    const int vecs = vecs_of<T>(a);
+    auto launch = [&](auto beta) {
+      constexpr bool kBeta = decltype(beta)::value;
+      if (vecs <= kWaveVecs) {
+        by_lanes(vecs, [&](auto lanes, auto) {
+          constexpr int kLanes = decltype(lanes)::value;
+          hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, kKind, kBeta>), dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))),
+                             dim3(kBlock), 0, st, a);
+        });
+      } else {
+        // (parts of as many rounds each)
+        const int rounds = (vecs + kBlock - 1) / kBlock, parts = (rounds + kGradVecs - 1) / kGradVecs;
+        a.part_vecs = (rounds + parts - 1) / parts * kBlock, a.parts = (vecs + a.part_vecs - 1) / a.part_vecs;
+        hipLaunchKernelGGL((wide_grad_kernel<T, kKind, kBeta>), dim3((unsigned)grid_of(a.rows * a.parts)), dim3(kBlock), 0, st, a);
+      }
+    };
+    if constexpr (kKind == kLogProbs) {
+      if (a.dentropy) {
+        launch(std::true_type());
+        return;
+      }
     }
-    a.parts = (vecs + kGradVecs * kBlock - 1) / (kGradVecs * kBlock);
-    hipLaunchKernelGGL((wide_grad_kernel<T, kKind>), dim3((unsigned)grid_of(a.rows * a.parts)), dim3(kBlock), 0, st, a);
+    launch(std::false_type());
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
   return 0;

@@ -19,11 +19,14 @@ struct __attribute__((packed, aligned(alignof(T)))) AnyRaw {
   Raw<T> v;
 };
 
-// Where vector v of a row lies.  The last one of a row whose width is no multiple is moved back to the row's end, so that
-// it is one load as well: its elements [skip, end) are its own, those before are the vector's before.
+// Where vector v of a row lies, if the row begins `shift` elements behind a multiple of 16 bytes and vectors lie at such
+// multiples.  Those at both ends, partial in general, are moved inside the row, so that each is one load: the elements
+// [skip, end) are a vector's own, the others another one's.
 template <typename T>
 struct Slot {
   int col, skip, end;
+  Slot() = default;
+  __device__ __forceinline__ Slot(int c, int s, int e) : col(c), skip(s), end(e) {}
   __device__ __forceinline__ Slot(int v, int width) {
     const int at = v * kPer<T>;
     col = at + kPer<T> <= width ? at : width - kPer<T> < 0 ? 0 : width - kPer<T>;
@@ -31,15 +34,26 @@ struct Slot {
     end = width - col < kPer<T> ? width - col : kPer<T>;
     if (at >= width) col = 0;
   }
+  static __device__ __forceinline__ Slot shifted(int v, int width, int shift) {
+    const int at = v * kPer<T> - shift, lo = max(at, 0), hi = min(at + kPer<T>, width);
+    const int c = max(min(at, width - kPer<T>), 0);
+    return lo < hi ? Slot(c, lo - c, hi - c) : none();
+  }
+  static __device__ __forceinline__ Slot none() { return Slot(0, kPer<T>, 0); }
   __device__ __forceinline__ bool any() const { return skip < kPer<T>; }
   __device__ __forceinline__ bool whole() const { return skip == 0 && end == kPer<T>; }
   __device__ __forceinline__ bool own(int e) const { return e >= skip && e < end; }
 };
+// elements from the multiple of 16 bytes before
+template <typename T>
+__device__ __forceinline__ int misaligned(const T *p) {
+  return (int)(reinterpret_cast<uintptr_t>(p) / sizeof(T)) & (kPer<T> - 1);
+}
 
-// kNarrow: a row may be narrower than a vector
-template <bool kNarrow, typename T>
-__device__ __forceinline__ Raw<T> load_slot(const T *row, const Slot<T> &s) {
-  if (kNarrow && s.end < kPer<T>) {
+// tiny: the row is narrower than a vector
+template <typename T>
+__device__ __forceinline__ Raw<T> load_slot(const T *row, const Slot<T> &s, bool tiny) {
+  if (tiny) {
     Raw<T> x = {};
 #pragma unroll
     for (int e = 0; e < kPer<T>; ++e)
@@ -74,8 +88,8 @@ struct Place<true, T> {
   __device__ __forceinline__ bool whole() const { return true; }
   __device__ __forceinline__ bool own(int) const { return here; }
 };
-template <bool kNarrow, typename T>
-__device__ __forceinline__ Raw<T> load_slot(const T *row, const Place<true, T> &s) {
+template <typename T>
+__device__ __forceinline__ Raw<T> load_slot(const T *row, const Place<true, T> &s, bool) {
   return reinterpret_cast<const AnyRaw<T> *>(row + s.col)->v;
 }
 template <typename T>
@@ -90,6 +104,21 @@ __device__ __forceinline__ void as_it_came(Raw<T> &x) {
   u32x4 y = __builtin_bit_cast(u32x4, x);
   asm volatile("" : "+v"(y));
   x = __builtin_bit_cast(Raw<T>, y);
+}
+
+// Its elements in 32 bits.  (bfloat16 by its bits: a maximum of two numbers that the compiler knows to have been bfloat16 is
+// taken in that type, which gfx950 has no instruction for, and costs a conversion back and forth.)
+template <typename T>
+__device__ __forceinline__ Vals<T> values_of(const Raw<T> &x) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    const u32x4 y = __builtin_bit_cast(u32x4, x);
+    Vals<T> v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(y[i] << 16), v[2 * i + 1] = __uint_as_float(y[i] & 0xffff0000u);
+    return v;
+  } else {
+    return __builtin_convertvector(x, Vals<T>);
+  }
 }
 
 // ---- over the kLanes lanes of a row (a power of two, at most 64), the result in all of them ----------------------
