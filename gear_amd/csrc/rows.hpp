@@ -106,6 +106,20 @@ __device__ __forceinline__ void as_it_came(Raw<T> &x) {
   x = __builtin_bit_cast(Raw<T>, y);
 }
 
+// kOnce: data that nobody reads again soon, passed by the caches (a load or store of 16 bytes at any element's address).
+template <bool kOnce, typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T *p) {
+  if (kOnce) return __builtin_bit_cast(Raw<T>, __builtin_nontemporal_load(reinterpret_cast<const u32x4_a1 *>(p)));
+  return reinterpret_cast<const AnyRaw<T> *>(p)->v;
+}
+template <bool kOnce, typename T>
+__device__ __forceinline__ void store_raw(T *p, const Raw<T> &x) {
+  if (kOnce)
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, x), reinterpret_cast<u32x4_a1 *>(p));
+  else
+    reinterpret_cast<AnyRaw<T> *>(p)->v = x;
+}
+
 // Its elements in 32 bits.  (bfloat16 by its bits: a maximum of two numbers that the compiler knows to have been bfloat16 is
 // taken in that type, which gfx950 has no instruction for, and costs a conversion back and forth.)
 template <typename T>
