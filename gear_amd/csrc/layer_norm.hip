@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArg
   using At = Place<kWhole, T>;
   __shared__ float part[2][kThreads / kWave][4];
   const int lane = threadIdx.x % kLanes;
-  const bool tiny = a.width < kPer<T>;
+  const bool tiny = kLanes == 4 && a.width < kPer<T>;
   int turn = 0;
   Vals<T> w[kVecs], b[kVecs];
 #pragma unroll
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
   using At = Place<kWhole, T>;
   __shared__ float part[2][kThreads / kWave][4];
   const int lane = threadIdx.x % kLanes;
-  const bool tiny = a.width < kPer<T>;
+  const bool tiny = kLanes == 4 && a.width < kPer<T>;
   int turn = 0;
   Vals<T> w[kVecs], dw[kVecs], db[kVecs];
 #pragma unroll

@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
   constexpr int kRows = kBlock / kLanes;
   __shared__ BestSmem<kWave> best[kTop && kLanes == kWave ? kRows : 1];
   const int lane = threadIdx.x % kLanes;
-  const bool tiny = a.vocab < kPer<T>;
+  const bool tiny = kLanes == 4 && a.vocab < kPer<T>;
   // (the lanes of a wave go round alike: they exchange sums)
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / kLanes;
@@ -711,7 +711,7 @@ __global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
   constexpr int kRows = kBlock / kLanes;
   __shared__ Fix fixes[kKind == kDistill ? kRows : 1][kMaxTop];
   const int lane = threadIdx.x % kLanes;
-  const bool tiny = a.vocab < kPer<T>;
+  const bool tiny = kLanes == 4 && a.vocab < kPer<T>;
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / kLanes;
     const bool here = row < a.rows;
