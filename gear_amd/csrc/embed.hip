@@ -32,7 +32,13 @@ struct EmbedArgs {
   int64_t stride;
   void *to;          // out, or dtable: contiguous
   float scale;
+  bool once;
 };
+
+// Two rows a group of lanes (184320 x 512 bf16 from 1025 rows: 1, 2, 4, 8 rows 52, 29, 30, 34 us).  Rows of more than the L2
+// caches hold are written past them (300000 x 512 from 33025 rows: 91 -> 57 us).
+constexpr int kRowsEach = 2;
+constexpr int64_t kOnceBytes = 32 << 20;
 
 // kRows rows a group of lanes
 template <typename T, int kLanes, int kRows>
@@ -55,7 +61,14 @@ __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
       }
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
-        if (base + r < a.n) store_slot(static_cast<T *>(a.to) + (base + r) * a.width, s, values_of<T>(x[r]) * a.scale);
+        if (base + r < a.n) {
+          T *to = static_cast<T *>(a.to) + (base + r) * a.width;
+          const Vals<T> y = values_of<T>(x[r]) * a.scale;
+          if (a.once && s.whole())
+            store_raw<true>(to + s.col, __builtin_convertvector(y, Raw<T>));
+          else
+            store_slot(to, s, y);
+        }
     }
   }
 }
@@ -195,13 +208,13 @@ __global__ __launch_bounds__(kBlock) void embed_place_kernel(CountArgs a) {
   uint32_t carry = 0;
   for (int w = 0; w < wave; ++w) carry += sums[w];
 #pragma unroll
-  for (int i = 0; i < kMostLoads; ++i) {
-    if (i >= loads) break;
-    const int b = bin0 + i * kWave + lane;
-    const uint32_t upto = (uint32_t)wave_inclusive_sum((int)total[i]);
-    if (b < a.bins) next[b] = carry + upto - total[i] + before[i];
-    carry += (uint32_t)wave_read_lane((int)upto, kWave - 1);
-  }
+  for (int i = 0; i < kMostLoads; ++i)
+    if (i < loads) {
+      const int b = bin0 + i * kWave + lane;
+      const uint32_t upto = (uint32_t)wave_inclusive_sum((int)total[i]);
+      if (b < a.bins) next[b] = carry + upto - total[i] + before[i];
+      carry += (uint32_t)wave_read_lane((int)upto, kWave - 1);
+    }
   const int bits = 32 - __builtin_clz((uint32_t)a.bins);
   const uint64_t lower = lane == 0 ? 0ull : ~0ull >> (64 - lane);
   uint32_t rank[kRounds];
@@ -287,8 +300,10 @@ __global__ __launch_bounds__(kBlock) void embed_sums_kernel(SumArgs a) {
         key[i] = kHeld > 1 ? of_lane<kLanes>(keys[i / kLanes], i % kLanes) : of_lane<kLanes>(keys[0], b + i);
         const uint32_t place = kHeld > 1 ? of_lane<kLanes>(places[i / kLanes], i % kLanes) : of_lane<kLanes>(places[0], b + i);
         row[i] = Raw<T>{};
-        if (key[i] < none)  // (lanes without columns read the first ones)
-          row[i] = load_slot<T>(static_cast<const T *>(a.e.rows) + (int64_t)place * a.e.stride, s, tiny);
+        if (key[i] < none) {  // (lanes without columns read the first ones)
+          const T *from = static_cast<const T *>(a.e.rows) + (int64_t)place * a.e.stride;
+          row[i] = tiny ? load_slot<T>(from, s, true) : load_raw<true>(from + s.col);  // (read once)
+        }
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -438,10 +453,10 @@ extern "C" int gear_hip_embed(const void *tokens, int tokens_i64, int64_t n, con
   if (tokens == nullptr || out == nullptr || (vocab > 0 && table == nullptr)) return GEAR_HIP_EINVAL;
   const int element = element_bytes(dtype);
   if (!aligned_to(tokens, tokens_i64 ? 8 : 4) || !aligned_to(table, element) || !aligned_to(out, element)) return GEAR_HIP_EALIGN;
-  const EmbedArgs a{tokens, tokens_i64 != 0, n, vocab, (int)width, table, table_stride, out, scale};
+  const EmbedArgs a{tokens, tokens_i64 != 0, n, vocab, (int)width, table, table_stride, out, scale, n * width * element >= kOnceBytes};
   by_type_and_lanes(dtype, (int)width, [&](auto type, auto lanes) {
     constexpr int kLanes = decltype(lanes)::value;
-    constexpr int kRows = 4;
+    constexpr int kRows = kRowsEach;
     const int64_t blocks = ceil_div64(n, kBlock / kLanes * kRows), most = kMostItems / kBlock;
     hipLaunchKernelGGL((embed_kernel<decltype(type), kLanes, kRows>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(kBlock), 0,
                        as_stream(stream), a);
@@ -471,7 +486,7 @@ extern "C" int gear_hip_embed_backward(const void *dout, int64_t dout_stride, co
   hipStream_t st = as_stream(stream);
   char *ws = static_cast<char *>(workspace);
   auto list = [&](size_t at) { return reinterpret_cast<uint32_t *>(ws + at); };
-  EmbedArgs e{tokens, tokens_i64 != 0, n, vocab, (int)width, dout, dout_stride, dtable, scale};
+  EmbedArgs e{tokens, tokens_i64 != 0, n, vocab, (int)width, dout, dout_stride, dtable, scale, false};
   const int64_t bytes = vocab * width * element;
   const int bits = 64 - __builtin_clzll((uint64_t)vocab);
   const int64_t fill = std::min<int64_t>(ceil_div64(bytes / 16 + 1, kBlock), 8192);

@@ -16,7 +16,12 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kMaxWidth = 16384;
-constexpr int kGradBlocks = 1024;  // workgroups of 256 of the backward pass, fewer larger ones
+// Workgroups of the backward pass, each of which leaves a row of sums.  47040 x 2048 bf16, 256 / 512 / 768 / 1024 of them: 206 / 152 /
+// 146 / 150 us, and the sums of all 5 / 5 / 6 / 7; of 512 threads (8192 x 8192) 128 / 256 / 384 / 512: 217 / 134 / 142 / 130 and 5 / 7 / 9 / 12.
+constexpr int kGradBlocks = 768, kGradBlocksWide = 256;
+// Results of more than the L2 caches hold are written past them, for what else they hold (122880 x 128 in 32 bits: 21 + 31 -> 19 + 30 us,
+// 47040 x 2048 bf16 with a residual 134 + 165 -> 136 + 146).
+constexpr int64_t kOnceBytes = 32 << 20;
 
 struct LayerArgs {
   const void *x, *residual, *weight, *bias;
@@ -24,6 +29,7 @@ struct LayerArgs {
   int64_t rows;
   int width, weight_f32;
   float eps, over_width;
+  bool once;
   void *y, *sum;
   // backward
   const void *dy, *dsum;
@@ -61,6 +67,14 @@ struct RowSums {
     }
   }
 };
+
+template <typename T, typename P>
+__device__ __forceinline__ void store(const LayerArgs &a, T *row, const P &s, const Vals<T> &x) {
+  if (a.once && s.whole())
+    store_raw<true>(row + s.col, __builtin_convertvector(x, Raw<T>));
+  else
+    store_slot(row, s, x);
+}
 
 template <typename T, typename P>
 __device__ __forceinline__ Vals<T> weights_at(const void *w, int f32, const P &s, float none) {
@@ -135,7 +149,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArg
       u[i] = __builtin_convertvector(xs[i], Vals<T>);
       if constexpr (kResidual) {
         u[i] += __builtin_convertvector(rs[i], Vals<T>);
-        if (here && s.any()) store_slot(sum, s, u[i]);
+        if (here && s.any()) store<T>(a, sum, s, u[i]);
         u[i] = __builtin_convertvector(__builtin_convertvector(u[i], Raw<T>), Vals<T>);
       }
       u[i] = own_only<T>(u[i], s);
@@ -155,7 +169,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_kernel(LayerArg
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const At s(lane + i * kLanes, a.width);
-      if (here && s.any()) store_slot(y, s, (u[i] - off) * inv * w[i] + b[i]);
+      if (here && s.any()) store<T>(a, y, s, (u[i] - off) * inv * w[i] + b[i]);
     }
   }
 }
@@ -221,7 +235,7 @@ __global__ __launch_bounds__(kThreadsOf<kLanes>) void layer_norm_grad_kernel(Lay
       if (here && s.any()) {
         const Vals<T> n = (u[i] - off) * inv, gv = own_only<T>(__builtin_convertvector(g[i], Vals<T>), s);
         dw[i] += gv * n, db[i] += gv;
-        store_slot(dx, s, inv * (gv * w[i] - mean_h - n * mean_hn) + __builtin_convertvector(plus[i], Vals<T>));
+        store<T>(a, dx, s, inv * (gv * w[i] - mean_h - n * mean_hn) + __builtin_convertvector(plus[i], Vals<T>));
       }
     }
   }
@@ -329,6 +343,7 @@ int prepare(const gear_hip_layer_norm_desc *d, LayerArgs &a) {
   a.x = d->x, a.xs = d->x_stride, a.residual = d->residual, a.rs = d->residual_stride;
   a.weight = d->weight, a.bias = d->bias, a.weight_f32 = d->weight_f32 != 0;
   a.rows = d->rows, a.width = (int)d->width;
+  a.once = d->rows * d->width * element >= kOnceBytes;
   a.eps = d->eps, a.over_width = (float)(1.0 / (double)d->width);
   return 0;
 }
@@ -338,7 +353,7 @@ int64_t blocks_of(int64_t rows, int each, int64_t most) {
   const int64_t n = ceil_div64(rows, each);
   return n < most ? n : most;
 }
-int64_t grad_blocks(int threads) { return kGradBlocks * kBlock / threads; }
+int64_t grad_blocks(int threads) { return threads > kBlock ? kGradBlocksWide : kGradBlocks; }
 
 }  // namespace
 }  // namespace gearhip
