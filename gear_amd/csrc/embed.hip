@@ -9,9 +9,14 @@
 // A run inside its chunk goes straight to the table; a run that a border cuts leaves a partial sum on each side of it,
 // and a last launch adds those up.  So a token that is half of the batch costs no more than one that is rare.
 //
-// The sort: a batch of 4096 positions or less is ranked in one launch, up to 20 000 sorted in one (range_sort.hpp).  More
-// of them, in a vocabulary of less than 4096: one pass by counting, tiles' counts, their prefixes, and a wave a tile that
-// ranks its positions in order.  Else digits of 8 bits (radix_sort.hpp).
+// The sort: a batch of 4096 positions or less is ranked in one launch.  More of them, in a vocabulary of less than 4096:
+// one pass by counting, tiles' counts, their prefixes, and a workgroup a tile that ranks its positions in order (184320
+// positions, 1025 tokens: 5 + 6 + 10 us, where two digits of 8 bits take 30).  Else digits of 8 bits (radix_sort.hpp), or, for
+// three of them and up to 32768 positions, one launch (range_sort.hpp; two digits of 16016 words take 18 us, one launch 23,
+// because some words are everywhere).
+//
+// Measured, us: 184320 x 512 bf16 of 1025 rows: look-up 31 (6.1 TB/s), gradient 68, of which 39 for the rows (4.8 TB/s: 1 KB each, in
+// no order); 16016 x 768 in 32 bits of 33025 rows: 13 and 54, of which 14 to clear the table (7.2 TB/s) and 18 for the sort.
 #include <algorithm>
 
 #include "range_sort.hpp"
@@ -491,7 +496,7 @@ extern "C" int gear_hip_embed_backward(const void *dout, int64_t dout_stride, co
   const int bits = 64 - __builtin_clzll((uint64_t)vocab);
   const int64_t fill = std::min<int64_t>(ceil_div64(bytes / 16 + 1, kBlock), 8192);
   char *table = static_cast<char *>(dtable);
-  if (n > radix::kRankMax && vocab < kMostBins && n > ranges::worth(bits) && ceil_div64(n, kTile) <= kMostTiles) {
+  if (n > radix::kRankMax && vocab < kMostBins && ceil_div64(n, kTile) <= kMostTiles) {
     const int tiles = (int)ceil_div64(n, kTile), bins = (int)vocab + 1;
     const CountArgs c{e, tiles, bins, list(p.hist) + kMostBins, list(p.hist), list(p.sorted_keys), list(p.sorted_places)};
     embed_count_kernel<<<dim3((unsigned)(tiles + fill)), dim3(kBlock), 0, st>>>(c, table, bytes);
@@ -499,7 +504,7 @@ extern "C" int gear_hip_embed_backward(const void *dout, int64_t dout_stride, co
     embed_place_kernel<<<dim3((unsigned)tiles), dim3(kBlock), 0, st>>>(c);
     GEARHIP_RETURN_IF_LAUNCH_FAILED();
   } else {
-    const bool one = n > radix::kRankMax && ranges::fits(n) && n <= ranges::worth(bits);
+    const bool one = bits > 16 && n > radix::kRankMax && ranges::fits(n) && n <= ranges::worth(bits);
     const bool lists = n > 0 && !one;
     const int64_t blocks = std::max(fill, lists ? std::min<int64_t>(ceil_div64(n, kBlock), 8192) : 0);
     embed_keys_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(e, lists ? list(p.keys) : nullptr,

@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
     // (asked for before it is known whether the row is passed over)
     Raw<T> x[kVecs];
     const T *from = static_cast<const T *>(a.logits) + row * a.stride;
-    const int shift = kLanes < 32 || tiny ? 0 : misaligned(from);  // (short rows share their lines anyway)
+    const int shift = kLanes * kVecs < 64 || tiny ? 0 : misaligned(from);  // (short rows share their lines anyway)
     auto slot = [&](int i) { return Slot<T>::shifted(lane + i * kLanes, a.vocab, shift); };
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) x[i] = here ? load_logits<T>(from, slot(i), tiny) : nothing<T>();
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
           for (int k = lane; k < a.top; k += kLanes) put_best(a, row, k, 0, Stats{});
       }
       here = token >= 0;
-      if constexpr (kLanes <= 16) {  // (from where it is: another load would wait for the token)
+      if constexpr (kLanes * kVecs <= 32) {  // (from where it is: another load would wait for the token)
         float found = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
@@ -718,7 +718,7 @@ __global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
     Fix *fix = fixes[kKind == kDistill ? threadIdx.x / kLanes : 0];
     const T *from = static_cast<const T *>(a.logits) + row * a.stride;
     T *to = static_cast<T *>(a.dlogits) + row * a.vocab;
-    const int shift = kLanes < 32 || tiny ? 0 : misaligned(to);
+    const int shift = kLanes * kVecs < 64 || tiny ? 0 : misaligned(to);
     auto slot = [&](int i) { return Slot<T>::shifted(lane + i * kLanes, a.vocab, shift); };
     // (asked for before it is known whether the row is passed over)
     Raw<T> x[kVecs];
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
       for (int i = 0; i < kVecs; ++i) {
         const Slot<T> s = slot(i);
         Vals<T> y = grad_of<kBeta, T>(x[i], live, slope);
-        if (kKind == kLogProbs && kLanes <= 16 && live) {
+        if (kKind == kLogProbs && kLanes * kVecs <= 32 && live) {
 #pragma unroll
           for (int e = 0; e < kPer<T>; ++e)
             if (s.col + e == token) y[e] += more;
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(kBlock) void narrow_grad_kernel(LogitsArgs a) {
         if (s.any()) store_slot(to, s, y);
       }
       // (the lane that wrote the token's column writes it again)
-      if (kKind == kLogProbs && kLanes > 16 && live && token >= 0 && (token + shift) / kPer<T> % kLanes == lane)
+      if (kKind == kLogProbs && kLanes * kVecs > 32 && live && token >= 0 && (token + shift) / kPer<T> % kLanes == lane)
         to[token] = (T)(slope.at<kBeta>((float)from[token]) + more);
     }
     if (kKind == kDistill) {
@@ -849,25 +849,30 @@ size_t split_bytes(int64_t rows, int64_t vocab, int64_t top) {
   return most;
 }
 
-// f(lanes of a row, vectors of a lane) for rows of a wave or less
-template <typename F>
+// f(lanes of a row, vectors of a lane) for rows of a wave or less.  With few lanes and many vectors each, more rows of a wave
+// share what is done once a row: 184320 rows of 50 vectors, 16 lanes with four against 32 with two, 44 + 51 us against 52 + 53; of 128,
+// 32 with four against 64 with two (16 with eight), 94 + 117 against 101 + 118 (98 + 127), but against a teacher's 16 entries 110 +
+// 188 against 105 + 175.  The best tokens are looked for by whole waves.
+template <int kKind, bool kTop, typename F>
 void by_lanes(int vecs, const F &f) {
-  using one = std::integral_constant<int, 1>;
   using two = std::integral_constant<int, 2>;
+  using four = std::integral_constant<int, 4>;
   if (vecs <= 4)
-    f(std::integral_constant<int, 4>(), one());
+    f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
   else if (vecs <= 8)
     f(std::integral_constant<int, 4>(), two());
   else if (vecs <= 16)
     f(std::integral_constant<int, 8>(), two());
   else if (vecs <= 32)
     f(std::integral_constant<int, 16>(), two());
-  else if (vecs <= 64)
-    f(std::integral_constant<int, 32>(), two());
+  else if (vecs <= 64 && !kTop)
+    f(std::integral_constant<int, 16>(), four());
+  else if (vecs <= 128 && !kTop && kKind == kLogProbs)
+    f(std::integral_constant<int, 32>(), four());
   else if (vecs <= 128)
     f(std::integral_constant<int, 64>(), two());
   else
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    f(std::integral_constant<int, 64>(), four());
 }
 
 // vectors of a row at most (one that is partial at both ends has one more)
@@ -895,14 +900,21 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
     using T = decltype(type);
     const int vecs = vecs_of<T>(a);
     if (vecs <= kWaveVecs) {
-      by_lanes(vecs, [&](auto lanes, auto held) {
-        constexpr int kLanes = decltype(lanes)::value;
-        const dim3 grid((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes)));
-        if (kKind == kLogProbs && a.top > 0)
-          hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind, kKind == kLogProbs>), grid, dim3(kBlock), 0, st, a);
-        else
-          hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind, false>), grid, dim3(kBlock), 0, st, a);
-      });
+      auto narrow = [&](auto top) {
+        constexpr bool kTop = decltype(top)::value;
+        by_lanes<kKind, kTop>(vecs, [&](auto lanes, auto held) {
+          constexpr int kLanes = decltype(lanes)::value;
+          const dim3 grid((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes)));
+          hipLaunchKernelGGL((narrow_kernel<T, kLanes, decltype(held)::value, kKind, kTop>), grid, dim3(kBlock), 0, st, a);
+        });
+      };
+      if constexpr (kKind == kLogProbs) {
+        if (a.top > 0) {
+          narrow(std::true_type());
+          return;
+        }
+      }
+      narrow(std::false_type());
       return;
     }
     split(a.rows, (a.vocab + kPer<T> - 1) / kPer<T>, a.parts, a.part_vecs);
@@ -945,7 +957,7 @@ int backward(LogitsArgs &a, int dtype, hipStream_t st) {
     auto launch = [&](auto beta) {
       constexpr bool kBeta = decltype(beta)::value;
       if (vecs <= kWaveVecs) {
-        by_lanes(vecs, [&](auto lanes, auto held) {
+        by_lanes<kKind, false>(vecs, [&](auto lanes, auto held) {
           constexpr int kLanes = decltype(lanes)::value;
           hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, decltype(held)::value, kKind, kBeta>), dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))),
                              dim3(kBlock), 0, st, a);
