@@ -253,13 +253,16 @@ __device__ __forceinline__ void group_sync() {
     __syncthreads();
 }
 
-template <int kThreads>
+template <typename T, int kThreads, int kVecs>
 struct BestSmem {
-  static constexpr int kList = kThreads < 256 ? 128 : 256;  // candidates
+  static constexpr int kList = kThreads < 256 ? 512 : 1024;  // candidates: for 64 of the best there are about 300
+  static constexpr int kOwners = kThreads < 256 ? 64 : 96;   // threads that have some: for 32 of the best about 50
   uint32_t groups[kWave];
   uint64_t best[2][kThreads / kWave];
   uint64_t list[kList];
-  int count;
+  u32x4 held[kOwners][kVecs];
+  uint16_t owner[kOwners];
+  int owners, listed;
 };
 
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -267,12 +270,11 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return (int32_t)b < 0 ? ~b : b | 0x80000000u;
 }
 
-// The best `top` of what kThreads threads hold, put(place, entry) for each; entries that are not there are 0.  slot(i): where
-// a thread's vector i lies; rounds: how many there are; mine: the largest of a thread's elements; finite: whether the row
-// holds no NaN or infinity.
+// The best `top` of what kThreads threads hold, put(place, entry) for each; entries that are not there are 0.  slot(id, i): where
+// vector i of a thread lies; mine: the largest of a thread's elements; finite: whether the row holds no NaN or infinity.
 template <typename T, int kThreads, int kVecs, typename At, typename Put>
 __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVecs], const At &slot, float mine, bool finite, int top,
-                                        BestSmem<kThreads> &sm, const Put &put) {
+                                        BestSmem<T, kThreads, kVecs> &sm, const Put &put) {
   constexpr int kGroup = kThreads / kWave;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) as_it_came<T>(x[i]);
@@ -280,7 +282,7 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
   // 64 maxima; the lowest bits make them differ, and leave the bound a little low
   const float g = lanes_max<(kGroup > 1 ? kGroup : 1)>(mine);
   if (id % kGroup == 0) sm.groups[id / kGroup] = (order_of(g) & ~63u) | (id / kGroup);
-  if (id == 0) sm.count = 0;
+  if (id == 0) sm.owners = sm.listed = 0;
   group_sync<kThreads>();
   const uint32_t key = sm.groups[lane];
   int before = 0;
@@ -291,25 +293,43 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
     for (int i = 0; i < 4; ++i) before += other[i] > key;
   }
   const uint32_t kth = __builtin_amdgcn_readlane(key, __builtin_ctzll(__ballot(before == top - 1))) & ~63u;
-  const float bound = kth <= 0x007fffffu ? -INFINITY : __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
-  if (finite && mine >= bound) {
+  const float bound = __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
+  const bool listing = finite && kth > 0x007fffffu;  // (-inf is no bound)
+  // What the few threads hold that have some goes where all threads look at it.
+  if (listing && mine >= bound) {
+    const int at = atomicAdd(&sm.owners, 1);
+    if (at < sm.kOwners) {
+      sm.owner[at] = (uint16_t)id;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      if (max_of<T>(x[i]) >= bound) {
-        const Slot<T> s = slot(i);
-        const Vals<T> value = values_of<T>(x[i]);
-#pragma unroll
-        for (int e = 0; e < kPer<T>; ++e)
-          if (value[e] >= bound && s.own(e)) {
-            const int at = atomicAdd(&sm.count, 1);
-            if (at < sm.kList) sm.list[at] = entry_of(value[e], s.col + e);
-          }
-      }
+      for (int i = 0; i < kVecs; ++i) sm.held[at][i] = __builtin_bit_cast(u32x4, x[i]);
     }
   }
   group_sync<kThreads>();
-  const int count = sm.count;
-  if (finite && count <= sm.kList) {
+  auto add = [&](float value, int column) __attribute__((always_inline)) {
+    const int at = atomicAdd(&sm.listed, 1);
+    if (at < sm.kList) sm.list[at] = entry_of(value, column);
+  };
+  const int owners = sm.owners;
+  if (listing && owners <= sm.kOwners) {
+    constexpr int kEach = kVecs * kPer<T>;
+    for (int c = id; c < owners * kEach; c += kThreads) {
+      const int o = c / kEach, e = c - o * kEach;
+      const float value = (float)reinterpret_cast<const T *>(&sm.held[o][0])[e];
+      if (value >= bound) add(value, slot(sm.owner[o], e / kPer<T>).col + e % kPer<T>);
+    }
+  } else if (listing && mine >= bound) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (max_of<T>(x[i]) >= bound) {
+        const Vals<T> value = values_of<T>(x[i]);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e)
+          if (value[e] >= bound) add(value[e], slot(id, i).col + e);
+      }
+  }
+  group_sync<kThreads>();
+  const int count = sm.listed;
+  if (listing && count <= sm.kList) {
     for (int c = id; c < count || c < top; c += kThreads) {
       if (c < count) {
         const uint64_t w = sm.list[c];
@@ -330,7 +350,7 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
     uint64_t best = 0;
 #pragma unroll 1
     for (int i = 0; i < kVecs; ++i) {
-      const Slot<T> s = slot(i);
+      const Slot<T> s = slot(id, i);
       if (!s.any()) continue;
       const Vals<T> y = values_of<T>(load_slot<T>(row, s, tiny));
 #pragma unroll
@@ -355,7 +375,7 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
 template <typename T, int kLanes, int kVecs, int kKind, bool kTop>
 __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
   constexpr int kRows = kBlock / kLanes;
-  __shared__ BestSmem<kWave> best[kTop && kLanes == kWave ? kRows : 1];
+  __shared__ BestSmem<T, kWave, kTop && kLanes == kWave ? kVecs : 1> best[kTop && kLanes == kWave ? kRows : 1];
   const int lane = threadIdx.x % kLanes;
   const bool tiny = kLanes == 4 && a.vocab < kPer<T>;
   // (the lanes of a wave go round alike: they exchange sums)
@@ -366,9 +386,9 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
     Raw<T> x[kVecs];
     const T *from = static_cast<const T *>(a.logits) + row * a.stride;
     const int shift = kLanes * kVecs < 64 || tiny ? 0 : misaligned(from);  // (short rows share their lines anyway)
-    auto slot = [&](int i) { return Slot<T>::shifted(lane + i * kLanes, a.vocab, shift); };
+    auto slot = [&](int id, int i) { return Slot<T>::shifted(id + i * kLanes, a.vocab, shift); };
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) x[i] = here ? load_logits<T>(from, slot(i), tiny) : nothing<T>();
+    for (int i = 0; i < kVecs; ++i) x[i] = here ? load_logits<T>(from, slot(lane, i), tiny) : nothing<T>();
     float at_token = 0;
     if (kKind == kLogProbs && a.tokens) {
       const int64_t token = here ? token_at(a.tokens, a.wide, row, a.vocab) : -1;
@@ -382,7 +402,7 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
         float found = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-          const Slot<T> s = slot(i);
+          const Slot<T> s = slot(lane, i);
           const Vals<T> value = values_of<T>(x[i]);
 #pragma unroll
           for (int e = 0; e < kPer<T>; ++e)
@@ -428,7 +448,7 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
         uint64_t entry[kVecs * kPer<T>], last = 0;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-          const Slot<T> s = slot(i);
+          const Slot<T> s = slot(lane, i);
 #pragma unroll
           for (int e = 0; e < kPer<T>; ++e) entry[i * kPer<T> + e] = s.own(e) ? entry_of((float)x[i][e], s.col + e) : 0;
         }
@@ -461,16 +481,16 @@ __device__ __forceinline__ float block_reduce(float x, float *part, const F &f) 
 template <typename T, int kThreads, int kVecs, int kKind, bool kTop>
 __global__ __launch_bounds__(kThreads, kThreads == kBlock && kVecs == kHeld ? (kTop ? 4 : 5) : 1) void wide_kernel(LogitsArgs a) {
   __shared__ float part_max[kThreads / kWave], part_sum[2][kThreads / kWave];
-  __shared__ BestSmem<kTop ? kThreads : kWave> best;
+  __shared__ BestSmem<T, kTop ? kThreads : kWave, kTop ? kVecs + 1 : 1> best;
   for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
     const int64_t row = unit / a.parts;
     const int part = (int)(unit - row * a.parts);
     const T *from = static_cast<const T *>(a.logits) + row * a.stride;
     const Cut<T> cut(from, a.vocab);
     const int first = part * a.part_vecs, last = min(first + a.part_vecs, cut.vecs);
-    auto slot = [&](int i) {  // (the last one is an end of the row)
-      const int v = first + (int)threadIdx.x + i * kThreads;
-      return i == kVecs ? cut.edge(threadIdx.x, a.vocab, part == 0, part == a.parts - 1) : v < last ? cut.whole(v) : Slot<T>::none();
+    auto slot = [&](int id, int i) {  // (the last one is an end of the row)
+      const int v = first + id + i * kThreads;
+      return i == kVecs ? cut.edge(id, a.vocab, part == 0, part == a.parts - 1) : v < last ? cut.whole(v) : Slot<T>::none();
     };
     float at_token = 0;
     if (kKind == kLogProbs && a.tokens) {
@@ -499,7 +519,7 @@ __global__ __launch_bounds__(kThreads, kThreads == kBlock && kVecs == kHeld ? (k
       else
         vectors(std::false_type());
       x[kVecs] = nothing<T>();
-      if (threadIdx.x < 2) x[kVecs] = load_logits<T>(from, slot(kVecs), false);
+      if (threadIdx.x < 2) x[kVecs] = load_logits<T>(from, slot(threadIdx.x, kVecs), false);
     };
     if (kKind == kLogProbs) load();
     // (whether a wave has anything of round i)
@@ -517,7 +537,7 @@ __global__ __launch_bounds__(kThreads, kThreads == kBlock && kVecs == kHeld ? (k
       if (__builtin_expect(m.huge(), 0)) {
 #pragma unroll 1
         for (int i = 0; i <= kVecs; ++i)
-          add_to<kKind == kLogProbs, true, T>(t, load_logits<T>(from, slot(i), false), m, a.scale2);
+          add_to<kKind == kLogProbs, true, T>(t, load_logits<T>(from, slot(threadIdx.x, i), false), m, a.scale2);
       } else {
 #pragma unroll
         for (int i = 0; i <= kVecs; ++i)
@@ -827,11 +847,14 @@ __global__ __launch_bounds__(kBlock) void wide_grad_kernel(LogitsArgs a) {
 
 // ---- host -------------------------------------------------------------------------------------------------------
 constexpr int kWaveVecs = 256;  // widest row of a wave
-constexpr int kLarge = 1024;    // threads of a workgroup where rows are few
-constexpr int kFewRows = 512;
+constexpr int kLarge = 1024;    // threads of a workgroup where rows are few and one of 256 would not hold them
+// Rows for which there is a CU each, in workgroups of 1024 threads, and the rest in parts that are joined: 64 rows of 65537 fp16
+// 7.4 us and 8.6, 128 of 33024 in 32 bits 5.9 and 8.2, 400 of them 12.9 and 13.9; rows of 33024 bf16 fit 256 threads, 6.3 and 6.2.
+constexpr int kFewRows = 256;
+bool few(int64_t rows, int vecs) { return rows <= kFewRows && vecs > kHeld * kBlock && vecs <= kHeldFew * kLarge; }
 // Parts of a row: what a workgroup holds at most.
 void split(int64_t rows, int vecs, int &parts, int &part_vecs) {
-  const int most = rows < kFewRows ? kHeldFew * kLarge : kHeld * kBlock, n = (vecs + most - 1) / most;
+  const int most = few(rows, vecs) ? vecs : kHeld * kBlock, n = (vecs + most - 1) / most;
   part_vecs = (vecs + n - 1) / n;
   parts = (vecs + part_vecs - 1) / part_vecs;
 }
@@ -931,10 +954,7 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
     };
     using small = std::integral_constant<int, kBlock>;
     using large = std::integral_constant<int, kLarge>;
-    const bool few = a.rows < kFewRows && vecs > 4 * kBlock;
-    if (few && a.part_vecs <= 4 * kLarge)
-      launch(large(), std::integral_constant<int, 4>());
-    else if (few)
+    if (few(a.rows, (a.vocab + kPer<T> - 1) / kPer<T>))
       launch(large(), std::integral_constant<int, kHeldFew>());
     else if (a.part_vecs <= 4 * kBlock)
       launch(small(), std::integral_constant<int, 4>());

@@ -163,7 +163,7 @@ def test_codes_without_a_gpu():
     assert backward(norm(rows=0), None, 0, None, 0, None, None, None, None, 0, None) == 0
 
     def rows(**over):
-        d = _cabi.LogitsDesc(logits=some, row_stride=9000, rows=3, vocab=9000, dtype=0, scale=1.0)
+        d = _cabi.LogitsDesc(logits=some, row_stride=99000, rows=3, vocab=99000, dtype=0, scale=1.0)
         for k, v in over.items():
             setattr(d, k, v)
         return ctypes.byref(d)
@@ -171,8 +171,8 @@ def test_codes_without_a_gpu():
     log_probs = lib.gear_hip_token_log_probs
     need = lib.gear_hip_token_log_probs_workspace_bytes
     outs = (some, some, some)
-    assert need(3, 9000, 0) > 0 and need(3, 9000, 64) > need(3, 9000, 0) and need(100000, 9000, 64) == 0
-    assert need(3, 1 << 21, 0) == 0 and need(3, 9000, 65) == 0 and need(0, 9000, 0) == 0
+    assert need(3, 99000, 0) > 0 and need(3, 99000, 64) > need(3, 99000, 0) and need(100000, 9000, 64) == 0
+    assert need(3, 1 << 21, 0) == 0 and need(3, 99000, 65) == 0 and need(0, 9000, 0) == 0
     assert log_probs(None, None, 1, 0, None, some, some, None, None, None, 0, None) == -1
     assert log_probs(rows(rows=0), None, 1, 0, None, None, None, None, None, None, 0, None) == 0
     assert log_probs(rows(vocab=0), None, 1, 0, None, some, some, None, None, None, 0, None) == -1
@@ -182,10 +182,10 @@ def test_codes_without_a_gpu():
     assert log_probs(rows(), some, 1, 0, None, some, some, None, None, some, 1 << 30, None) == -1
     assert log_probs(rows(), None, 1, 0, *outs, None, None, some, 1 << 30, None) == -1
     assert log_probs(rows(), some, 1, 2, *outs, None, None, some, 1 << 30, None) == -1
-    assert log_probs(rows(), some, 1, 9001, *outs, some, some, some, 1 << 30, None) == -1
+    assert log_probs(rows(), some, 1, 99001, *outs, some, some, some, 1 << 30, None) == -1
     assert log_probs(rows(), some, 1, 65, *outs, some, some, some, 1 << 30, None) == -3
     assert log_probs(rows(), some, 1, 2, *outs, some, some, None, 0, None) == -2
-    assert log_probs(rows(), some, 1, 2, *outs, some, some, some, need(3, 9000, 2) - 1, None) == -2
+    assert log_probs(rows(), some, 1, 2, *outs, some, some, some, need(3, 99000, 2) - 1, None) == -2
     assert log_probs(rows(), some, 1, 2, *outs, some, some, some + 128, 1 << 30, None) == -4
     assert log_probs(rows(logits=some + 2), some, 1, 0, *outs, None, None, some, 1 << 30, None) == -4
     grad = lib.gear_hip_token_log_probs_backward
