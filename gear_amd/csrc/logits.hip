@@ -256,7 +256,7 @@ __device__ __forceinline__ void group_sync() {
 template <typename T, int kThreads, int kVecs>
 struct BestSmem {
   static constexpr int kList = kThreads < 256 ? 512 : 1024;  // candidates: for 64 of the best there are about 300
-  static constexpr int kOwners = kThreads < 256 ? 64 : 96;   // threads that have some: for 32 of the best about 50
+  static constexpr int kOwners = 40;                         // threads that have some: for 16 of the best about 25
   uint32_t groups[kWave];
   uint64_t best[2][kThreads / kWave];
   uint64_t list[kList];
@@ -295,8 +295,10 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
   const uint32_t kth = __builtin_amdgcn_readlane(key, __builtin_ctzll(__ballot(before == top - 1))) & ~63u;
   const float bound = __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
   const bool listing = finite && kth > 0x007fffffu;  // (-inf is no bound)
-  // What the few threads hold that have some goes where all threads look at it.
-  if (listing && mine >= bound) {
+  // What the few threads hold that have some goes where all threads look at it; where they are not few, each looks at its own
+  // (4096 x 33024, the best 8: 59 us so, 60 each its own; the best 32: 73 and 69; 64 rows, the best 8: 9.5 and 15.7).
+  const bool few = listing && top <= 16;
+  if (few && mine >= bound) {
     const int at = atomicAdd(&sm.owners, 1);
     if (at < sm.kOwners) {
       sm.owner[at] = (uint16_t)id;
@@ -304,13 +306,13 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
       for (int i = 0; i < kVecs; ++i) sm.held[at][i] = __builtin_bit_cast(u32x4, x[i]);
     }
   }
-  group_sync<kThreads>();
+  if (few) group_sync<kThreads>();
   auto add = [&](float value, int column) __attribute__((always_inline)) {
     const int at = atomicAdd(&sm.listed, 1);
     if (at < sm.kList) sm.list[at] = entry_of(value, column);
   };
   const int owners = sm.owners;
-  if (listing && owners <= sm.kOwners) {
+  if (few && owners <= sm.kOwners) {
     constexpr int kEach = kVecs * kPer<T>;
     for (int c = id; c < owners * kEach; c += kThreads) {
       const int o = c / kEach, e = c - o * kEach;
