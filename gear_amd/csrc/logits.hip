@@ -28,7 +28,8 @@ constexpr int kHeld = 17;       // vectors of a thread
 constexpr int kHeldFew = 12;    // ... of a workgroup of 1024
 constexpr int kJoined = 4096;   // entries that a join puts in order
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kLow = -1e30f;  // below any exponent that counts, and any logit that is allowed
+constexpr float kLow = -1e30f;   // below any logit that is allowed
+constexpr float kLeast = -1e4f;  // below any exponent that counts
 
 struct LogitsArgs {
   const void *logits;
@@ -151,7 +152,7 @@ __device__ __forceinline__ void add_to(Stats &t, const Raw<T> &x, const Shift &m
   for (int e = 0; e < kPer<T>; ++e) {
     const float d = kHuge ? (v[e] - m.m) * scale2 : fmaf(v[e], scale2, -m.m2), p = __builtin_amdgcn_exp2f(d);
     t.s += p;
-    if (kEntropy) t.a = fmaf(fmaxf(d, kLow), p, t.a);
+    if (kEntropy) t.a = fmaf(fmaxf(d, kLeast), p, t.a);
   }
 }
 
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(LogitsArgs a) {
       f32x4 p = {-INFINITY, 0.f, 0.f, 0.f};
       if (lane < a.parts) p = *reinterpret_cast<const f32x4 *>(a.stats + (row * a.parts + lane) * 4);
       Stats t{lanes_max<kWave>(p[0]), 0.f, 0.f};
-      const float d = fmaxf((p[0] - shift_of(t.m)) * a.scale2, kLow), e = __builtin_amdgcn_exp2f(d);
+      const float d = fmaxf((p[0] - shift_of(t.m)) * a.scale2, kLeast), e = __builtin_amdgcn_exp2f(d);
       t.s = lanes_sum<kWave>(p[1] * e), t.a = lanes_sum<kWave>(fmaf(d, p[1], p[2]) * e);
       return t;
     };
@@ -663,7 +664,7 @@ struct Slope {
   template <bool kBeta>
   __device__ __forceinline__ float at(float x) const {
     // (above 0 only by what lse lost when it was rounded, where logits are huge)
-    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale2, -lse2), kLow, 0.f), p = __builtin_amdgcn_exp2f(l);
+    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale2, -lse2), kLeast, 0.f), p = __builtin_amdgcn_exp2f(l);
     return p * (kBeta ? fmaf(beta, l, alpha) : alpha);
   }
 };
@@ -973,6 +974,7 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
 
 template <int kKind>
 int backward(LogitsArgs &a, int dtype, hipStream_t st) {
+  if (a.rows > (((int64_t)1 << 32) - 1) / ceil_div64(a.vocab, 1024)) return GEAR_HIP_ERANGE;  // (parts are numbered in 32 bits)
   by_type(dtype, [&](auto type) {
     using T = decltype(type);
     const int vecs = vecs_of<T>(a);

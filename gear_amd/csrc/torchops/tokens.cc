@@ -136,6 +136,20 @@ float number(double x, const char *name) {
   return (float)x;
 }
 
+// A call that is being captured gets scratch of its own, out of the graph's memory: graphs that were captured on one stream may
+// be replayed on several.
+Scratch scratch(py::handle ws, const char *tag, size_t bytes, const at::Device &device) {
+  if (bytes == 0) return Scratch();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(current_stream()), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return Scratch(ws, tag, bytes, device);
+  Scratch s;
+  s.keep = empty((int64_t)std::max<size_t>(bytes, 256), at::kByte, device);
+  s.ptr = s.keep.data_ptr(), s.bytes = (size_t)s.keep.numel();
+  return s;
+}
+
 // ---- rows of a table by token --------------------------------------------------------------------
 constexpr int64_t kMostTokens = ((int64_t)1 << 31) - 1;
 
@@ -162,7 +176,7 @@ py::object embed_tokens_backward(py::handle dout_, py::handle tokens_, int64_t v
   const float scale = number(scale_, "scale");
   const c10::DeviceGuard guard(device);
   const at::Tensor dtable = make({vocab, dout.width}, dout.t.scalar_type(), device);
-  const Scratch s(ws, "embed_backward", gear_hip_embed_backward_workspace_bytes(dout.rows, dout.width), device);
+  const Scratch s = scratch(ws, "embed_backward", gear_hip_embed_backward_workspace_bytes(dout.rows, dout.width), device);
   call("gear_hip_embed_backward", s, gear_hip_embed_backward, dout.ptr(), dout.stride, tokens.ptr(), tokens.wide, dout.rows, vocab,
        dout.width, dout.dtype, scale, dtable.data_ptr(), s.ptr, s.bytes, current_stream());
   return wrap(dtable);
@@ -234,7 +248,7 @@ py::object layer_norm_backward(py::handle dy_, py::handle x, py::handle weight, 
   if (n.weight.defined()) dweight = make({n.x.width}, n.weight_dtype, device);
   if (n.bias.defined()) dbias = make({n.x.width}, n.weight_dtype, device);
   const Scratch s = n.weight.defined() || n.bias.defined()
-                        ? Scratch(ws, "layer_norm", gear_hip_layer_norm_backward_workspace_bytes(n.x.rows, n.x.width), device)
+                        ? scratch(ws, "layer_norm", gear_hip_layer_norm_backward_workspace_bytes(n.x.rows, n.x.width), device)
                         : Scratch();
   call("gear_hip_layer_norm_backward", s, gear_hip_layer_norm_backward, &n.d, dy.ptr(), dy.stride,
        dsum.t.defined() ? dsum.ptr() : nullptr, dsum.stride, dx.data_ptr(), dweight.defined() ? dweight.data_ptr() : nullptr,
@@ -268,7 +282,7 @@ py::object token_log_probs(py::handle logits, py::handle tokens_, double scale, 
   if (tokens.t.defined()) log_probs = make(lead, at::kFloat, device);
   const at::Tensor entropy = make(lead, at::kFloat, device), lse = make(lead, at::kFloat, device);
   if (top > 0) value = make(with(lead, top), at::kFloat, device), best = make(with(lead, top), at::kLong, device);
-  const Scratch s(ws, "token_log_probs", gear_hip_token_log_probs_workspace_bytes(l.x.rows, l.x.width, top), device);
+  const Scratch s = scratch(ws, "token_log_probs", gear_hip_token_log_probs_workspace_bytes(l.x.rows, l.x.width, top), device);
   call("gear_hip_token_log_probs", s, gear_hip_token_log_probs, &l.d, tokens.ptr(), tokens.wide, top, float_ptr(log_probs),
        ptr<float>(entropy), ptr<float>(lse), float_ptr(value), best.defined() ? ptr<int64_t>(best) : nullptr, s.ptr, s.bytes,
        current_stream());
@@ -316,7 +330,7 @@ py::object distill(py::handle logits, py::handle top_tokens, py::handle top_logi
   const at::Device device = l.device();
   const c10::DeviceGuard guard(device);
   const at::Tensor loss = make(l.x.lead(), at::kFloat, device), lse = make(l.x.lead(), at::kFloat, device);
-  const Scratch s(ws, "distill", gear_hip_distill_workspace_bytes(l.x.rows, l.x.width), device);
+  const Scratch s = scratch(ws, "distill", gear_hip_distill_workspace_bytes(l.x.rows, l.x.width), device);
   call("gear_hip_distill", s, gear_hip_distill, &l.d, q.tokens.ptr(), q.tokens.wide, ptr<float>(q.logits), q.count,
        ptr<float>(loss), ptr<float>(lse), s.ptr, s.bytes, current_stream());
   return py::make_tuple(wrap(loss), wrap(lse));

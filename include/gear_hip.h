@@ -596,7 +596,7 @@ int gear_hip_layer_norm_backward(const gear_hip_layer_norm_desc *desc, const voi
                                  const void *dsum, int64_t dsum_stride, void *dx, void *dweight, void *dbias,
                                  void *workspace, size_t workspace_bytes, void *stream);
 
-/* Rows of logits; 0 < scale < 1e30, vocab <= 2^20.  z = scale * logits, lse = log sum_j exp z_j, p = exp(z - lse).
+/* Rows of logits; 0 < scale < 1e30, vocab <= 2^20, rows < 2^31 (gradients: rows * (vocab / 1024, rounded up) < 2^32).  z = scale * logits, lse = log sum_j exp z_j, p = exp(z - lse).
  * A logit of -inf is a token that is not allowed; rows that allow none (no logit of -1e30 or more) have lse = -inf,
  * log probabilities of -inf, entropy 0 and no gradient.
  * NaN or +inf makes its row's results NaN. */

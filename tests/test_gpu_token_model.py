@@ -63,6 +63,38 @@ def test_a_captured_run_replays():
         torch.cuda.synchronize()
 
 
+def test_graphs_of_one_stream_replay_on_several():
+    """Two graphs captured on one stream have nothing in common: replayed at once, each gives its own results."""
+    from gear_amd import ops
+    announce("two graphs of token operators at once")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    runs = []
+    for n in (60000, 50000):
+        tokens = torch.randint(0, 300, (n,), generator=g, device="cuda")
+        dout, w = torch.randn(n, 256, generator=g, device="cuda"), torch.ones(256, device="cuda")
+        logits = torch.randn(40, 150000, generator=g, device="cuda")
+        runs.append(lambda tokens=tokens, dout=dout, w=w, logits=logits: (
+            ops.embed_tokens_backward(dout, tokens, 300),) + ops.layer_norm_backward(dout, dout, w, w) + ops.token_log_probs(logits, top=6)[1:])
+    want = [run() for run in runs]
+    side, others = torch.cuda.Stream(), [torch.cuda.Stream() for _ in runs]
+    with torch.cuda.stream(side):
+        runs[0]()  # (scratch of this stream is there already)
+    torch.cuda.synchronize()
+    graphs, captured = [], []
+    for run in runs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured.append(run())
+        graphs.append(graph)
+    for replay in range(6):
+        for graph, stream in zip(graphs, others):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, captured):
+            assert all(torch.equal(x, y) for x, y in zip(a, b)), replay
+
+
 def test_streams_and_threads():
     """Calls at once from several threads, each on a stream of its own and two on the same: the results of one alone."""
     announce("token operators on streams and threads")

@@ -193,6 +193,7 @@ def test_codes_without_a_gpu():
     assert grad(rows(), None, some, None, 1, some, None, some, None) == -1
     assert grad(rows(), some, some, some, 1, None, some, some, None) == -1
     assert grad(rows(rows=0), None, None, None, 1, None, None, None, None) == 0
+    assert grad(rows(rows=(1 << 31) - 1), None, some, None, 1, some, some, some, None) == -3
     assert lib.gear_hip_distill(rows(), some, 1, some, 0, some, some, some, 1 << 30, None) == -1
     assert lib.gear_hip_distill(rows(), some, 1, some, 65, some, some, some, 1 << 30, None) == -3
     assert lib.gear_hip_distill(rows(), some, 1, some, 8, some, some, None, 0, None) == -2
