@@ -6,9 +6,13 @@
 // difference of two sums, which would leave nothing of a small deviation around a large mean; and what the first mean is
 // off by (the sum of u less it) is taken off again, so that such a row keeps its digits.
 //
-// Bound by memory.  kLanes lanes hold a row in registers (two vectors of 16 bytes each where it is wide enough), so that a row is
-// read once; rows of more than 64 lanes exchange sums through LDS.  A workgroup goes on to further rows with the sums of
-// dw and db in registers, leaves them in the workspace, and a second launch adds those up in a fixed order.
+// Bound by memory.  kLanes lanes hold a row in registers, two vectors of 16 bytes each (a row of 16384 in 32 bits four), so that
+// it is read once; rows of more than 64 lanes exchange sums through LDS.  A workgroup of the gradients goes on to further rows with
+// the sums of dw and db in registers, leaves them in the workspace, and a second launch adds those up in a fixed order.
+// One vector a lane with twice the lanes is as fast; a row asked for ahead slower (47040 x 2048 bf16: 184 us against 165).
+//
+// Measured, forward and gradients, us: 47040 x 2048 bf16 with a residual 136 and 145 + 6 (5.7 and 5.3 TB/s), 184320 x 512 of the same 123 and
+// 138 + 5 (6.1 and 5.5), 8192 x 8192 92 and 133 + 7; 122880 x 128 in 32 bits 19 and 30 + 5 (6.7 and 6.4, the caches help).
 #include "rows.hpp"
 
 namespace gearhip {
