@@ -376,9 +376,11 @@ extern "C" int gear_hip_layer_norm(const gear_hip_layer_norm_desc *desc, void *y
     constexpr int kLanes = decltype(lanes)::value, kThreads = kThreadsOf<kLanes>;
     const dim3 grid((unsigned)blocks_of(a.rows, kThreads / kLanes, (1 << 24) / kThreads)), block(kThreads);
     if (a.residual)
-      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, true>), grid, block, 0, as_stream(stream), a);
+      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, true>), grid, block, 0,
+                         as_stream(stream), a);
     else
-      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, false>), grid, block, 0, as_stream(stream), a);
+      hipLaunchKernelGGL((layer_norm_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, false>), grid, block, 0,
+                         as_stream(stream), a);
   });
   GEARHIP_RETURN_IF_LAUNCH_FAILED();
   return 0;
@@ -412,9 +414,11 @@ extern "C" int gear_hip_layer_norm_backward(const gear_hip_layer_norm_desc *desc
       blocks = blocks_of(a.rows, kThreads / kLanes, grad_blocks(kThreads));
       const dim3 grid((unsigned)blocks), block(kThreads);
       if (dsum)
-        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, true>), grid, block, 0, as_stream(stream), a);
+        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, true>), grid, block, 0,
+                           as_stream(stream), a);
       else
-        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, false>), grid, block, 0, as_stream(stream), a);
+        hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(type), kLanes, decltype(vecs)::value, decltype(whole)::value, false>), grid, block, 0,
+                           as_stream(stream), a);
     });
     GEARHIP_RETURN_IF_LAUNCH_FAILED();
   }

@@ -14,11 +14,14 @@
 //
 // The best k: groups of lanes have a maximum each, 64 in all; the k-th largest of those is a bound below which none of
 // the best k lies, so that few elements are left to be put in order.  Where more are left than a list holds (rows of equal
-// logits), or a row holds NaN or infinity, they are taken one after the other.
+// logits, or of fewer that are allowed than are asked for), or a row holds NaN or infinity, the bound is taken once more of
+// pairs of logit and column, which all differ; where that leaves too many as well, they are taken one after the other.
 //
 // Measured: 16384 x 33025 bf16 155-190 us forward (with how memory lies; 5.6-6.8 TB/s), 361 backward (5.9 TB/s); 8191 x 33025 against 32
 // entries 100 and 191; 184320 x 1024 bf16 95 and 117 (4.0 and 6.5 TB/s); 184320 x 18 in 32 bits 8 and 8; 64 x 65537 fp16 with the best
-// eight 11; 4096 x 33024 bf16 43, with the best 32 74 (64: 170).
+// eight 11; 4096 x 33024 bf16 43, with the best 32 74 (64: 180; of equal logits 264 and 323, one after the other 2230 and 4350).
+// The wide rows' forward with 128, 512 or 1024 threads of 34, 9 or 5 vectors in place of 256 of 17: 16384 x 33025 220, 219 and 394 for
+// 185, 4096 x 33024 with the best 32 106, 107 and 165 for 75-84.
 #include <algorithm>
 
 #include "rows.hpp"
@@ -336,8 +339,7 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
       }
   }
   group_sync<kThreads>();
-  const int count = sm.listed;
-  if (listing && count <= sm.kList) {
+  auto listed = [&](int count) __attribute__((always_inline)) {
     for (int c = id; c < count || c < top; c += kThreads) {
       if (c < count) {
         const uint64_t w = sm.list[c];
@@ -350,23 +352,54 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
       }
     }
     group_sync<kThreads>();
-    return;
-  }
-  uint64_t limit = ~0ull;
-#pragma unroll 1
-  for (int k = 0; k < top; ++k) {
-    uint64_t best = 0;
+  };
+  // what is given for each element of a thread, from where it lies (nothing of this is kept in registers for it)
+  auto each = [&](const auto &f) __attribute__((always_inline)) {
 #pragma unroll 1
     for (int i = 0; i < kVecs; ++i) {
       const Slot<T> s = slot(id, i);
       if (!s.any()) continue;
       const Vals<T> y = values_of<T>(load_slot<T>(row, s, tiny));
 #pragma unroll
-      for (int e = 0; e < kPer<T>; ++e) {
-        const uint64_t w = entry_of(y[e], s.col + e);
-        if (s.own(e) && w < limit && w > best) best = w;
-      }
+      for (int e = 0; e < kPer<T>; ++e)
+        if (s.own(e)) f(entry_of(y[e], s.col + e));
     }
+  };
+  int count = sm.listed;
+  if (listing && count <= sm.kList) return listed(count);
+  // Once more with entries in place of values, so that equal logits differ; now the groups are of threads 64 apart: of equal
+  // logits the lowest columns are asked for, which then lie in as many groups as can be.
+  uint64_t own = 0;
+  each([&](uint64_t w) { own = w > own ? w : own; });
+  group_sync<kThreads>();
+  sm.list[id] = own;
+  if (id == 0) sm.listed = 0;
+  group_sync<kThreads>();
+#pragma unroll
+  for (int w = 0; w < kGroup; ++w) own = w == 0 || sm.list[lane + w * kWave] > own ? sm.list[lane + w * kWave] : own;
+  uint64_t least = 0;
+  int above = 0;
+#pragma unroll 4
+  for (int j = 0; j < kWave; ++j) above += __shfl((unsigned long long)own, j) > own;
+  const uint64_t kth_lane = __ballot(above == top - 1);  // (none where fewer groups than that have elements)
+  if (kth_lane) least = __shfl((unsigned long long)own, __builtin_ctzll(kth_lane));
+  group_sync<kThreads>();
+  each([&](uint64_t w) {
+    if (w >= least) {
+      const int at = atomicAdd(&sm.listed, 1);
+      if (at < sm.kList) sm.list[at] = w;
+    }
+  });
+  group_sync<kThreads>();
+  count = sm.listed;
+  if (count <= sm.kList) return listed(count);
+  uint64_t limit = ~0ull;
+#pragma unroll 1
+  for (int k = 0; k < top; ++k) {
+    uint64_t best = 0;
+    each([&](uint64_t w) {
+      if (w < limit && w > best) best = w;
+    });
     limit = lanes_max64<kWave>(best);
     if (kThreads > kWave) {
       if (lane == 0) sm.best[k & 1][id / kWave] = limit;
@@ -989,8 +1022,8 @@ int backward(LogitsArgs &a, int dtype, hipStream_t st) {
       if (vecs <= kWaveVecs) {
         by_lanes<kKind, false>(vecs, [&](auto lanes, auto held) {
           constexpr int kLanes = decltype(lanes)::value;
-          hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, decltype(held)::value, kKind, kBeta>), dim3((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes))),
-                             dim3(kBlock), 0, st, a);
+          const dim3 grid((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes)));
+          hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, decltype(held)::value, kKind, kBeta>), grid, dim3(kBlock), 0, st, a);
         });
       } else {
         // Few vectors a thread, so that what is read and written lies close together at any time (a plain copy of rows of

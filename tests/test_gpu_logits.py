@@ -179,6 +179,28 @@ def test_ties_and_signs(vocab):
             assert torch.equal(best, order(x, min(64, vocab)))
 
 
+@pytest.mark.parametrize("vocab", [64, 513, 2000, 2560, 9000, 33025, 70000])
+def test_best_of_few_allowed(vocab):
+    """Fewer allowed tokens than are asked for, in few places, and none in a part of every vector's columns; NaN and infinity
+    among them: as sorted, the tokens that are not allowed last."""
+    from gear_amd import ops
+    announce("best of few %d" % vocab)
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    at = torch.arange(vocab, device="cuda")
+    for rows in (3, 270):
+        x = torch.randn(rows, vocab, generator=g, device="cuda")
+        few = torch.rand(rows, vocab, generator=g, device="cuda") < 20 / vocab
+        for dtype in TYPES:
+            per = 4 if dtype == torch.float32 else 8
+            for name, y in (("few", x.masked_fill(~few, -INF)), ("one place", x.masked_fill(at // per % 64 == 63, -INF)),
+                            ("not finite", x.masked_fill(few, float("nan")).masked_fill(few.roll(5, 1), INF)),
+                            ("steps", (x * 2).round() / 2)):
+                y = y.to(dtype)
+                for top in (1, 16, 64):
+                    announce("%s %s rows=%d top=%d" % (name, dtype, rows, top))
+                    assert torch.equal(ops.token_log_probs(y, top=top)[4], order(y, top)), (name, dtype, rows, top)
+
+
 def test_shapes():
     from gear_amd import ops
     announce("logits: shapes")
