@@ -141,9 +141,11 @@ float number(double x, const char *name) {
 Scratch scratch(py::handle ws, const char *tag, size_t bytes, const at::Device &device) {
   if (bytes == 0) return Scratch();
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(static_cast<hipStream_t>(current_stream()), &status) != hipSuccess ||
-      status == hipStreamCaptureStatusNone)
-    return Scratch(ws, tag, bytes, device);
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(current_stream()), &status) != hipSuccess) {
+    (void)hipGetLastError();  // (or the next launch would be taken for failed)
+    status = hipStreamCaptureStatusNone;
+  }
+  if (status == hipStreamCaptureStatusNone) return Scratch(ws, tag, bytes, device);
   Scratch s;
   s.keep = empty((int64_t)std::max<size_t>(bytes, 256), at::kByte, device);
   s.ptr = s.keep.data_ptr(), s.bytes = (size_t)s.keep.numel();
