@@ -16,6 +16,7 @@
 // the best k lies, so that few elements are left to be put in order.  Where more are left than a list holds (rows of equal
 // logits, or of fewer that are allowed than are asked for), or a row holds NaN or infinity, the bound is taken once more of
 // pairs of logit and column, which all differ; where that leaves too many as well, they are taken one after the other.
+// The best one alone is the row's maximum, of which only the column is looked for.
 //
 // Measured: 16384 x 33025 bf16 155-190 us forward (with how memory lies; 5.6-6.8 TB/s), 361 backward (5.9 TB/s); 8191 x 33025 against 32
 // entries 100 and 191; 184320 x 1024 bf16 95 and 117 (4.0 and 6.5 TB/s); 184320 x 18 in 32 bits 8 and 8; 64 x 65537 fp16 with the best
@@ -66,6 +67,7 @@ struct LogitsArgs {
 };
 
 enum { kLogProbs, kDistill };
+enum { kNoBest, kOneBest, kSomeBest };
 
 // ---- order: larger first, the lower index first among equals, NaN before all --------------------------------------
 __device__ __forceinline__ uint64_t entry_of(float x, int column) {
@@ -412,11 +414,58 @@ __device__ __forceinline__ void best_of(const T *row, bool tiny, Raw<T> (&x)[kVe
   }
 }
 
+// The best one alone, as an entry in the lanes of its row (all threads of a workgroup come here): where the largest logit is known,
+// and finite, its lowest column is looked for, in the few vectors that hold it (184320 x 1024 92 us, as one of many 140; 4096 x 33024
+// 50 and 55; 64 x 65537 8.5 and 9.9).
+template <typename T, int kThreads, int kLanes, int kVecs, typename At>
+__device__ __forceinline__ uint64_t best_one(const T *row, bool tiny, Raw<T> (&x)[kVecs], const At &slot, bool here, float mine, float most,
+                                             bool finite, uint64_t *share) {
+  const int id = threadIdx.x % (kThreads > kWave ? kThreads : kLanes);
+  const bool known = finite && most > -INFINITY;
+  float column = -INFINITY;  // less than 0
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) as_it_came<T>(x[i]);
+  if (known && mine == most) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (max_of<T>(x[i]) == most) {
+        const Vals<T> value = values_of<T>(x[i]);
+        const int first = slot(id, i).col;
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e)
+          if (value[e] == most) column = fmaxf(column, -(float)(first + e));
+      }
+  }
+  column = lanes_max<kLanes>(column);
+  uint64_t best = column > -INFINITY ? entry_of(most, (int)-column) : 0ull;
+  if (__ballot(here && !known)) {
+    if (here && !known) {
+#pragma unroll 1
+      for (int i = 0; i < kVecs; ++i) {
+        const Slot<T> s = slot(id, i);
+        if (!s.any()) continue;
+        const Vals<T> y = values_of<T>(load_slot<T>(row, s, tiny));
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e)
+          if (s.own(e) && entry_of(y[e], s.col + e) > best) best = entry_of(y[e], s.col + e);
+      }
+    }
+    best = lanes_max64<kLanes>(best);
+  }
+  if (kThreads > kWave) {
+    if (threadIdx.x % kWave == 0) share[threadIdx.x / kWave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) best = share[w] > best ? share[w] : best;
+  }
+  return best;
+}
+
 // ---- rows of a wave or less -------------------------------------------------------------------------------------
-template <typename T, int kLanes, int kVecs, int kKind, bool kTop>
+template <typename T, int kLanes, int kVecs, int kKind, int kTop>
 __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
   constexpr int kRows = kBlock / kLanes;
-  __shared__ BestSmem<T, kWave, kTop && kLanes == kWave ? kVecs : 1> best[kTop && kLanes == kWave ? kRows : 1];
+  __shared__ BestSmem<T, kWave, kTop == kSomeBest && kLanes == kWave ? kVecs : 1> best[kTop == kSomeBest && kLanes == kWave ? kRows : 1];
   const int lane = threadIdx.x % kLanes;
   const bool tiny = kLanes == 4 && a.vocab < kPer<T>;
   // (the lanes of a wave go round alike: they exchange sums)
@@ -481,11 +530,14 @@ __global__ __launch_bounds__(kBlock) void narrow_kernel(LogitsArgs a) {
     } else {
       stats(t);
       if (here && lane == 0) finish_log_probs(a, row, at_token, t);
-      if constexpr (kTop && kLanes == kWave) {
+      if constexpr (kTop == kOneBest) {
+        const uint64_t e = best_one<T, kWave, kLanes, kVecs>(from, tiny, x, slot, here, mine, t.m, t.s == t.s, nullptr);
+        if (here && lane == 0) put_best(a, row, 0, e, t);
+      } else if constexpr (kTop == kSomeBest && kLanes == kWave) {
         if (here)
           best_of<T, kWave, kVecs>(from, tiny, x, slot, mine, t.s == t.s, a.top, best[threadIdx.x / kWave],
                                    [&](int place, uint64_t e) { put_best(a, row, place, e, t); });
-      } else if constexpr (kTop) {
+      } else if constexpr (kTop == kSomeBest) {
         uint64_t entry[kVecs * kPer<T>], last = 0;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
@@ -519,10 +571,11 @@ __device__ __forceinline__ float block_reduce(float x, float *part, const F &f) 
   return x;
 }
 
-template <typename T, int kThreads, int kVecs, int kKind, bool kTop>
+template <typename T, int kThreads, int kVecs, int kKind, int kTop>
 __global__ __launch_bounds__(kThreads, kThreads == kBlock && kVecs == kHeld ? (kTop ? 4 : 5) : 1) void wide_kernel(LogitsArgs a) {
   __shared__ float part_max[kThreads / kWave], part_sum[2][kThreads / kWave];
-  __shared__ BestSmem<T, kTop ? kThreads : kWave, kTop ? kVecs + 1 : 1> best;
+  __shared__ BestSmem<T, kTop == kSomeBest ? kThreads : kWave, kTop == kSomeBest ? kVecs + 1 : 1> best;
+  __shared__ uint64_t share[kTop == kOneBest ? kThreads / kWave : 1];
   for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
     const int64_t row = unit / a.parts;
     const int part = (int)(unit - row * a.parts);
@@ -622,13 +675,18 @@ __global__ __launch_bounds__(kThreads, kThreads == kBlock && kVecs == kHeld ? (k
         else
           *reinterpret_cast<f32x4 *>(a.stats + unit * 4) = f32x4{t.m, t.s, t.a, 0.f};
       }
-      if constexpr (kTop)
-        best_of<T, kThreads, kVecs + 1>(from, false, x, slot, mine, t.s == t.s, a.top, best, [&](int place, uint64_t e) {
-          if (alone)
-            put_best(a, row, place, e, t);
-          else
-            a.lists[unit * a.top + place] = e;
-        });
+      auto put = [&](int place, uint64_t e) __attribute__((always_inline)) {
+        if (alone)
+          put_best(a, row, place, e, t);
+        else
+          a.lists[unit * a.top + place] = e;
+      };
+      if constexpr (kTop == kOneBest) {
+        const uint64_t e = best_one<T, kThreads, kWave, kVecs + 1>(from, false, x, slot, true, mine, t.m, t.s == t.s, share);
+        if (threadIdx.x == 0) put(0, e);
+      } else if constexpr (kTop == kSomeBest) {
+        best_of<T, kThreads, kVecs + 1>(from, false, x, slot, mine, t.s == t.s, a.top, best, put);
+      }
     }
   }
 }
@@ -916,11 +974,12 @@ size_t split_bytes(int64_t rows, int64_t vocab, int64_t top) {
 // f(lanes of a row, vectors of a lane) for rows of a wave or less.  With few lanes and many vectors each, more rows of a wave
 // share what is done once a row: 184320 rows of 50 vectors, 16 lanes with four against 32 with two, 44 + 51 us against 52 + 53; of 128,
 // 32 with four against 64 with two (16 with eight), 94 + 117 against 101 + 118 (98 + 127), but against a teacher's 16 entries 110 +
-// 188 against 105 + 175.  The best tokens are looked for by whole waves.
-template <int kKind, bool kTop, typename F>
+// 188 against 105 + 175.  The best tokens, if more than one, are looked for by whole waves.
+template <int kKind, int kTop, typename F>
 void by_lanes(int vecs, const F &f) {
   using two = std::integral_constant<int, 2>;
   using four = std::integral_constant<int, 4>;
+  constexpr bool kWaves64 = kTop == kSomeBest, kWaves128 = kWaves64 || kKind != kLogProbs;
   if (vecs <= 4)
     f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
   else if (vecs <= 8)
@@ -929,12 +988,10 @@ void by_lanes(int vecs, const F &f) {
     f(std::integral_constant<int, 8>(), two());
   else if (vecs <= 32)
     f(std::integral_constant<int, 16>(), two());
-  else if (vecs <= 64 && !kTop)
-    f(std::integral_constant<int, 16>(), four());
-  else if (vecs <= 128 && !kTop && kKind == kLogProbs)
-    f(std::integral_constant<int, 32>(), four());
+  else if (vecs <= 64)
+    f(std::integral_constant<int, kWaves64 ? 64 : 16>(), std::integral_constant<int, kWaves64 ? 2 : 4>());
   else if (vecs <= 128)
-    f(std::integral_constant<int, 64>(), two());
+    f(std::integral_constant<int, kWaves128 ? 64 : 32>(), std::integral_constant<int, kWaves128 ? 2 : 4>());
   else
     f(std::integral_constant<int, 64>(), four());
 }
@@ -966,7 +1023,7 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
     const int vecs = vecs_of<T>(a);
     if (vecs <= kWaveVecs) {
       auto narrow = [&](auto top) {
-        constexpr bool kTop = decltype(top)::value;
+        constexpr int kTop = decltype(top)::value;
         by_lanes<kKind, kTop>(vecs, [&](auto lanes, auto held) {
           constexpr int kLanes = decltype(lanes)::value;
           const dim3 grid((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes)));
@@ -975,11 +1032,14 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
       };
       if constexpr (kKind == kLogProbs) {
         if (a.top > 0) {
-          narrow(std::true_type());
+          if (a.top == 1)
+            narrow(std::integral_constant<int, kOneBest>());
+          else
+            narrow(std::integral_constant<int, kSomeBest>());
           return;
         }
       }
-      narrow(std::false_type());
+      narrow(std::integral_constant<int, kNoBest>());
       return;
     }
     split(a.rows, (a.vocab + kPer<T> - 1) / kPer<T>, a.parts, a.part_vecs);
@@ -989,10 +1049,12 @@ int forward(LogitsArgs &a, int dtype, char *ws, hipStream_t st) {
     auto launch = [&](auto size, auto held) {
       constexpr int kThreads = decltype(size)::value, kVecs = decltype(held)::value;
       const dim3 grid((unsigned)std::min(a.rows * a.parts, kMostItems / kThreads)), block(kThreads);
-      if (kKind == kLogProbs && a.top > 0)
-        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, kKind == kLogProbs>), grid, block, 0, st, a);
+      if (kKind == kLogProbs && a.top == 1)
+        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, kKind == kLogProbs ? kOneBest : kNoBest>), grid, block, 0, st, a);
+      else if (kKind == kLogProbs && a.top > 0)
+        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, kKind == kLogProbs ? kSomeBest : kNoBest>), grid, block, 0, st, a);
       else
-        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, false>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((wide_kernel<T, kThreads, kVecs, kKind, kNoBest>), grid, block, 0, st, a);
     };
     using small = std::integral_constant<int, kBlock>;
     using large = std::integral_constant<int, kLarge>;
@@ -1020,7 +1082,7 @@ int backward(LogitsArgs &a, int dtype, hipStream_t st) {
     auto launch = [&](auto beta) {
       constexpr bool kBeta = decltype(beta)::value;
       if (vecs <= kWaveVecs) {
-        by_lanes<kKind, false>(vecs, [&](auto lanes, auto held) {
+        by_lanes<kKind, kNoBest>(vecs, [&](auto lanes, auto held) {
           constexpr int kLanes = decltype(lanes)::value;
           const dim3 grid((unsigned)grid_of(ceil_div64(a.rows, kBlock / kLanes)));
           hipLaunchKernelGGL((narrow_grad_kernel<T, kLanes, decltype(held)::value, kKind, kBeta>), grid, dim3(kBlock), 0, st, a);
