@@ -936,7 +936,8 @@ __global__ __launch_bounds__(kBlock) void wide_grad_kernel(LogitsArgs a) {
       __syncthreads();  // the entries are there, and the part is written
       if (live && (int)threadIdx.x < a.count) {
         const Fix f = fix_of(fix, threadIdx.x, a.count);
-        const int begin = part == 0 ? 0 : cut.head + first * kPer<T>, end = part == a.parts - 1 ? a.vocab : cut.head + last * kPer<T>;
+        // (parts are cut from as many vectors as a row can have, so that the last one may begin behind this row's and have only its end)
+        const int begin = part == 0 ? 0 : cut.head + min(first, cut.vecs) * kPer<T>, end = part == a.parts - 1 ? a.vocab : cut.head + last * kPer<T>;
         if (f.column >= begin && f.column < end)
           to[f.column] = (T)fmaf(more, f.q, slope.at<false>((float)from[f.column]));
       }

@@ -1,0 +1,63 @@
+"""Rows of logits where parts of rows meet and where rows end."""
+import pytest
+
+from conftest import announce
+from sequence_reference import worst
+from tokens_reference import TYPES, LogProbs, teacher
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def _borders(vocab):
+    """Both ends of a row and both sides of whatever a part may end at: parts are whole rounds of 256 vectors of 4 or 8
+    elements, counted from the first multiple of 16 bytes, which is up to 7 elements from the row's begin."""
+    at = set(range(8)) | set(range(vocab - 16, vocab))
+    for border in range(1024, vocab, 1024):
+        at |= set(range(border - 1, border + 8))
+    return torch.tensor(sorted(c for c in at if c < vocab), device="cuda")
+
+
+# 16 bits: a little beside multiples of 8192, 32 bits: of 4096, where a part has the row's end and nothing else
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [12287, 12289, 20481, 24571, 24577, 32767, 32769, 40963, 49153, 65535, 65537])
+def test_entries_at_the_borders(vocab, dtype):
+    """A teacher that names the columns at the borders of parts, in rows of every misalignment: each has its term."""
+    from gear_amd import ops
+    announce("distill at borders %s %d" % (dtype, vocab))
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    wide = (torch.randn(9, vocab + 3, generator=g, device="cuda") * 2).to(dtype)
+    for x in (wide[:, 1:1 + vocab], wide[:, :vocab].contiguous()):
+        ref = LogProbs(x, 1.0)
+        for best in _borders(vocab).split(64):
+            best = best.expand(9, -1).contiguous()
+            t = torch.randn(best.shape, generator=g, device="cuda")
+            dloss = 1 + torch.rand(9, generator=g, device="cuda")
+            _, lse = ops.distill(x, best, t)
+            got = ops.distill_backward(dloss, x, best, t, lse)
+            q, q_error, _ = teacher(best, t, vocab)
+            weight, error = (torch.zeros_like(ref.p).scatter_(1, best, v) for v in (q, q_error))
+            a = dloss.double()[:, None]
+            want, bound = ref.gradient(a, torch.zeros_like(a), -a * weight, dtype, ref.lse, a)
+            assert worst(got, want, bound + a * (error + 2.0 ** -24 * 66 * weight)) <= 1, (x.is_contiguous(), best[0, 0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [2049, 12289, 24577, 32767, 32769, 65537])
+def test_tokens_at_the_ends(vocab, dtype):
+    """The given token's term in the first and last columns, in rows of every misalignment."""
+    from gear_amd import ops
+    announce("log_probs_backward at the ends %s %d" % (dtype, vocab))
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    tokens = torch.cat([torch.arange(8), torch.arange(vocab - 16, vocab)]).cuda().repeat_interleave(8)
+    x = (torch.randn(len(tokens), vocab, generator=g, device="cuda") * 2).to(dtype)
+    ref = LogProbs(x, 1.0)
+    dl = 1 + torch.rand(len(tokens), generator=g, device="cuda")
+    outs = ops.token_log_probs(x, tokens)
+    got = ops.token_log_probs_backward(dl, None, x, tokens, outs[2], None)
+    a = dl.double()[:, None]
+    at = torch.zeros_like(ref.p).scatter_(1, tokens[:, None], 1.0)
+    want, bound = ref.gradient(-a, torch.zeros_like(a), a * at, dtype, ref.lse, a)
+    assert worst(got, want, bound) <= 1
