@@ -61,3 +61,49 @@ def test_tokens_at_the_ends(vocab, dtype):
     at = torch.zeros_like(ref.p).scatter_(1, tokens[:, None], 1.0)
     want, bound = ref.gradient(-a, torch.zeros_like(a), a * at, dtype, ref.lse, a)
     assert worst(got, want, bound) <= 1
+
+
+def _all_nan(*tensors):
+    return all(bool(torch.isnan(t).all()) for t in tensors)
+
+
+# rows of lane groups, of a wave, of a workgroup, of one of 1024 threads, of several parts that are joined
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1, 5, 70, 600, 2000, 3000, 9001, 33025, 70001, 150001])
+def test_nothing_but_nan(vocab, dtype):
+    """NaN is its row's whatever else the row holds: alone, among tokens that are not allowed, among the lowest numbers.  A
+    row that allows nothing and holds no NaN is one that allows nothing, and a row that is passed over is not looked at."""
+    from gear_amd import ops
+    announce("rows of nothing but NaN %s %d" % (dtype, vocab))
+    nan, low = float("nan"), torch.finfo(dtype).min
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(9, vocab, generator=g, device="cuda").to(dtype)
+    x[0] = nan
+    x[1:4] = -INF
+    x[1, 0], x[2, vocab - 1], x[3, vocab // 2] = nan, nan, nan
+    x[4] = low
+    x[4, vocab // 3] = nan
+    x[5] = -INF  # nothing is allowed
+    x[6] = nan   # passed over
+    tokens = torch.tensor([0, vocab - 1, 0, vocab - 1, 0, 0, -1, 0, vocab - 1], device="cuda")
+    first = [0, 0, vocab - 1, vocab // 2, vocab // 3]
+    for top in sorted({0, 1, min(5, vocab), min(64, vocab)}):
+        logp, entropy, lse, value, best = ops.token_log_probs(x, tokens, top=top)
+        assert _all_nan(logp[:5], entropy[:5], lse[:5])
+        assert float(logp[5]) == float(lse[5]) == -INF and float(entropy[5]) == 0
+        assert float(logp[6]) == float(lse[6]) == float(entropy[6]) == 0
+        assert bool(torch.isfinite(torch.stack([logp[7:], lse[7:], entropy[7:]])).all())
+        if top:
+            assert _all_nan(value[:5]) and best[:5, 0].tolist() == first
+            assert bool((value[5:7] == -INF).all()) and bool((best[6] == -1).all()) and best[5].tolist() == list(range(top))
+    one = torch.ones(9, device="cuda")
+    for a, b in ((one, None), (None, one), (one, one)):
+        grad = ops.token_log_probs_backward(a, b, x, tokens, lse, entropy)
+        assert _all_nan(grad[:5]) and float(grad[5:7].abs().sum()) == 0 and bool(torch.isfinite(grad[7:]).all())
+    best = tokens[:, None].clone()
+    t = torch.zeros(9, 1, device="cuda")
+    loss, lse = ops.distill(x, best, t)
+    assert _all_nan(loss[:5], lse[:5]) and float(loss[5]) == INF and float(lse[5]) == -INF
+    assert float(loss[6]) == float(lse[6]) == 0 and bool(torch.isfinite(torch.stack([loss[7:], lse[7:]])).all())
+    grad = ops.distill_backward(one, x, best, t, lse)
+    assert _all_nan(grad[:5]) and float(grad[5:7].abs().sum()) == 0 and bool(torch.isfinite(grad[7:]).all())
