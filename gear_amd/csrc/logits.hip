@@ -169,7 +169,9 @@ __device__ __forceinline__ void add_to(Stats &t, const Raw<T> &x, const Shift &m
 // ---- what is made of them ---------------------------------------------------------------------------------------
 struct Result {
   float shift, log_s;
-  bool none;  // nothing is allowed (the lowest numbers of a type are as good a mask as -inf), and nothing is NaN: maxima pass NaN by, S does not
+  // Nothing is allowed, and nothing is NaN: maxima pass NaN by, S does not.  (The lowest numbers of 32 bits and of bfloat16 are as good a
+  // mask as -inf; -65504, fp16's, is a logit like any other.)
+  bool none;
   __device__ __forceinline__ Result(const Stats &t)
       : shift(shift_of(t.m)), log_s(__builtin_amdgcn_logf(t.s) * kLn2), none(t.m < kLow && t.s == t.s) {}
   __device__ __forceinline__ float log_p(float x, float scale) const {

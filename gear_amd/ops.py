@@ -500,7 +500,8 @@ def token_log_probs(logits, tokens=None, *, scale=1.0, top=0):
     top_log_probs [..., top], top_tokens int64 [..., top]); None for what was not asked for.
     lse: the logarithm of the sum of exponentials, for the gradient.  top (at most 64): the largest logits, the lower
     token first among equals, NaN before all.  A logit of -inf is a token that is not allowed; a row that allows none (no logit of -1e30 or
-    more) has lse -inf, log probabilities of -inf and entropy 0.  With tokens, a row whose token is none is passed over: 0, 0, 0, top -inf and -1."""
+    more, and no NaN) has lse -inf, log probabilities of -inf and entropy 0 (mask float16 with -inf: its lowest number, -65504, is a logit
+    like any other).  NaN or infinity makes its row NaN.  With tokens, a row whose token is none is passed over: 0, 0, 0, top -inf and -1."""
     return _hostops.token_log_probs(logits, tokens, float(scale), int(top), _ws)
 
 

@@ -597,8 +597,9 @@ int gear_hip_layer_norm_backward(const gear_hip_layer_norm_desc *desc, const voi
                                  void *workspace, size_t workspace_bytes, void *stream);
 
 /* Rows of logits; 0 < scale < 1e30, vocab <= 2^20, rows < 2^31 (gradients: rows * (vocab / 1024, rounded up) < 2^32).  z = scale * logits, lse = log sum_j exp z_j, p = exp(z - lse).
- * A logit of -inf is a token that is not allowed; rows that allow none (no logit of -1e30 or more) have lse = -inf,
- * log probabilities of -inf, entropy 0 and no gradient.
+ * A logit of -inf is a token that is not allowed; rows that allow none (no logit of -1e30 or more, and no NaN) have lse = -inf,
+ * log probabilities of -inf, entropy 0 and no gradient.  So the lowest numbers of f32 and bf16 are as good a mask; f16's, -65504, is a
+ * logit like any other: a row of nothing else is a uniform distribution, and is masked with -inf instead.
  * NaN or +inf makes its row's results NaN. */
 typedef struct gear_hip_logits_desc {
   const void *logits;

@@ -1,4 +1,6 @@
-"""Rows of logits where parts of rows meet and where rows end."""
+"""Rows of logits where parts of rows meet, where rows end, and of what is not a number or not allowed."""
+import math
+
 import pytest
 
 from conftest import announce
@@ -107,3 +109,29 @@ def test_nothing_but_nan(vocab, dtype):
     assert float(loss[6]) == float(lse[6]) == 0 and bool(torch.isfinite(torch.stack([loss[7:], lse[7:]])).all())
     grad = ops.distill_backward(one, x, best, t, lse)
     assert _all_nan(grad[:5]) and float(grad[5:7].abs().sum()) == 0 and bool(torch.isfinite(grad[7:]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [2, 9, 700, 3000, 70001])
+def test_nothing_but_the_lowest(vocab, dtype):
+    """Rows of a type's lowest number allow nothing in 32 bits and in bfloat16; in fp16 it is a logit like any other, and all of
+    them are as probable as each other."""
+    from gear_amd import ops
+    announce("rows of the lowest number %s %d" % (dtype, vocab))
+    x = torch.full((3, vocab), torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    tokens, one = torch.tensor([0, vocab - 1, -1], device="cuda"), torch.ones(3, device="cuda")
+    logp, entropy, lse, value, best = ops.token_log_probs(x, tokens, top=2)
+    grad = ops.token_log_probs_backward(one, None, x, tokens, lse, None)
+    loss, _ = ops.distill(x, tokens[:, None], 0 * one[:, None])
+    assert best.tolist() == [[0, 1], [0, 1], [-1, -1]]
+    if dtype == torch.float16:
+        # S is a sum of equal numbers in 32 bits (200 roundings, LogProbs), its logarithm has a few more; lse is rounded once as -65504 is
+        logs = math.log(vocab)
+        bound = 2.0 ** -24 * (220 + 8 * logs)
+        for got in (-logp[:2], entropy[:2], -value[:2, 0], loss[:2]):
+            assert float((got.double() - logs).abs().max()) <= 2 * bound
+        assert float((lse[:2].double() + 65504 - logs).abs().max()) <= bound + 2.0 ** -9
+        assert float(grad[0, 0]) > 0 and float(grad[0, 1]) < 0
+    else:
+        assert bool((logp[:2] == -INF).all()) and bool((lse[:2] == -INF).all()) and bool((value[:2] == -INF).all())
+        assert float(entropy.abs().sum()) == 0 and float(grad.abs().sum()) == 0 and bool((loss[:2] == INF).all())
