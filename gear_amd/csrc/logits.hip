@@ -757,13 +757,14 @@ __global__ __launch_bounds__(kBlock) void join_kernel(LogitsArgs a) {
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------
-// p (alpha + beta log2 p) of a logit, times the scale; kBeta: beta is not 0
+// p (alpha + beta log2 p) of a logit, times the scale; kBeta: beta is not 0.  The difference from lse is taken before anything is
+// rounded: with scale2 and lse2 in its place, one operation less, p at logits of 500 was off by 1e-5 and at 70000 by 3e-3.
 struct Slope {
-  float lse2, scale2, alpha, beta;
+  float lse, scale, alpha, beta;
   template <bool kBeta>
   __device__ __forceinline__ float at(float x) const {
     // (above 0 only by what lse lost when it was rounded, where logits are huge)
-    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale2, -lse2), kLeast, 0.f), p = __builtin_amdgcn_exp2f(l);
+    const float l = __builtin_amdgcn_fmed3f(fmaf(x, scale, -lse) * kLog2e, kLeast, 0.f), p = __builtin_amdgcn_exp2f(l);
     return p * (kBeta ? fmaf(beta, l, alpha) : alpha);
   }
 };
@@ -784,7 +785,7 @@ struct Given {
   // whether there is anything to write but zeros; more: what is added at the given token, or taken at an entry
   __device__ __forceinline__ bool slope(const LogitsArgs &a, bool some, Slope &s, float &more) const {
     if (!some || lse == -INFINITY) return false;  // (nothing was allowed)
-    s.lse2 = lse * kLog2e, s.scale2 = a.scale2;
+    s.lse = lse, s.scale = a.scale;
     const float nan = lse - lse;  // 0, or NaN for a row of NaN
     s.alpha = (kKind == kDistill ? a.scale * by : -a.scale * (by + de * entropy)) + nan;
     s.beta = -a.scale * de * kLn2;

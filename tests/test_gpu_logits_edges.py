@@ -135,3 +135,29 @@ def test_nothing_but_the_lowest(vocab, dtype):
     else:
         assert bool((logp[:2] == -INF).all()) and bool((lse[:2] == -INF).all()) and bool((value[:2] == -INF).all())
         assert float(entropy.abs().sum()) == 0 and float(grad.abs().sum()) == 0 and bool((loss[:2] == INF).all())
+
+
+@pytest.mark.parametrize("vocab", [6, 900, 9001])
+@pytest.mark.parametrize("far", [-3000.0, 500.0, 70000.0])
+def test_gradients_far_from_zero(far, vocab):
+    """p is exp(z - lse) of the lse that is given: one rounding of a difference near 0, however large both are."""
+    from gear_amd import ops
+    announce("gradients of far logits %g %d" % (far, vocab))
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(5, vocab, generator=g, device="cuda") + far
+    scale = float(torch.tensor(0.7))
+    tokens, one = torch.zeros(5, dtype=torch.int64, device="cuda"), torch.ones(5, device="cuda")
+    _, entropy, lse, _, _ = ops.token_log_probs(x, tokens, scale=scale)
+    d = x.double() * scale - lse.double()[:, None]
+    p, h = torch.exp(d.clamp(max=0)), entropy.double()[:, None]  # (above 0 by no more than lse is off)
+    # d and log2 e are rounded, their product is, the power and two products are: each a unit of d or of the result
+    off = 2.0 ** -24 * (4 * d.abs() + 12)
+    token = torch.nn.functional.one_hot(tokens, vocab)
+    got = ops.token_log_probs_backward(one, None, x, tokens, lse, entropy, scale=scale)
+    assert worst(got, scale * (token - p), scale * (p * off + 2.0 ** -24 * 4 * token)) <= 1
+    got = ops.token_log_probs_backward(None, one, x, tokens, lse, entropy, scale=scale)
+    slope = d.clamp(max=0) + h
+    assert worst(got, -scale * p * slope, scale * p * (off * (slope.abs() + 1) + 2.0 ** -24 * 8 * (d.abs() + h))) <= 1
+    t = torch.zeros(5, 1, device="cuda")
+    got = ops.distill_backward(one, x, tokens[:, None], t, lse, scale=scale)
+    assert worst(got, scale * (p - token), scale * (p * off + 2.0 ** -24 * 4 * token)) <= 1
