@@ -308,7 +308,8 @@ class WindowModel(_Positions):
 class TokenModel(_Positions):
     """A causal policy over tokens: a step is `step` of them, its observation's (in bins, patches, words) and its action
     last; from the tokens up to an action comes the distribution of that action.  Ends of episodes and padding are
-    those of WindowModel.  Everything runs in the parameters' type (32, 16 bits or bfloat16), attention in `dtype`."""
+    those of WindowModel.  Everything runs in the parameters' type (32, 16 bits or bfloat16), attention in `dtype`; under
+    autocast the projections and the logits in its type."""
 
     def __init__(self, vocab, step, width=128, heads=4, kv_heads=2, layers=2, cap=30.0, dtype=torch.bfloat16):
         super().__init__()
@@ -332,8 +333,9 @@ class TokenModel(_Positions):
         y = self._norm(self.blocks[0].before, x)
         for i, block in enumerate(self.blocks):
             attended = attend(i, block, *block.project(y, self.dtype)).flatten(2).to(x.dtype)
-            y, x = self._norm(block.between, block.out(attended), x)
-            more = block.mlp(y)
+            # (autocast's results in 16 bits are added to in the table's type, as its sums are)
+            y, x = self._norm(block.between, block.out(attended).to(x.dtype), x)
+            more = block.mlp(y).to(x.dtype)
             if i + 1 < len(self.blocks):
                 y, x = self._norm(self.blocks[i + 1].before, more, x)
         return self.head(self._norm(self.norm, actions(more), actions(x))[0])

@@ -1,0 +1,54 @@
+"""The model of tokens as other programs use it."""
+import pytest
+
+from conftest import announce
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def _windows(vocab, step, batch=6, steps=7, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    tokens = torch.randint(0, vocab, (batch, steps, step), generator=g, device="cuda")
+    mask, done = torch.ones(batch, steps, dtype=torch.uint8, device="cuda"), torch.zeros(batch, steps, dtype=torch.uint8, device="cuda")
+    mask[0, :3], mask[1, 5:], done[2, 4] = 0, 0, 1
+    return tokens, mask, done
+
+
+@pytest.mark.parametrize("parameters", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16])
+def test_autocast(cast, parameters):
+    """Under autocast: the model's own numbers but for roundings, gradients in the parameters' type, and steps of rollouts."""
+    from gear_amd.sequence import Rollouts, TokenModel, distill
+    announce("token model under autocast %s %s" % (cast, parameters))
+    torch.manual_seed(4)
+    model = TokenModel(300, 4, width=64, heads=2, kv_heads=1, dtype=torch.float16).cuda().to(parameters)
+    tokens, mask, done = _windows(300, 4)
+    # (one teacher's say for both: which tokens are its best five jumps where two are nearly as probable)
+    with torch.no_grad():
+        best = model.log_probs(tokens, mask, done, top=5)
+
+    def grads():
+        model.zero_grad()
+        logp, entropy = model.log_probs(tokens, mask, done)[:2]
+        loss = distill(model(tokens, mask, done), best[4], best[3])
+        (-(logp.sum() + 0.1 * entropy.sum()) / 42 + loss.sum() / 42).backward()
+        return logp.detach(), entropy.detach(), [p.grad for p in model.parameters()]
+
+    want = grads()
+    with torch.autocast("cuda", dtype=cast):
+        assert model(tokens, mask, done).dtype == cast
+        got = grads()
+        assert bool(torch.isfinite(model.distilled(model, tokens, mask, done, count=5)).all())
+    # two layers of operands of O(1): the roundings of the coarsest type there is (as test_model_against_torch has it)
+    unit = max(torch.finfo(cast).eps, torch.finfo(parameters).eps)
+    assert float((got[0] - want[0]).abs().max()) < 32 * unit and float((got[1] - want[1]).abs().max()) < 32 * unit
+    for (n, p), a, b in zip(model.named_parameters(), got[2], want[2]):
+        assert a.dtype == parameters and float((a.float() - b.float()).norm()) <= 32 * unit * float(b.float().norm()) + 1e-6, n
+    steps, outs = tokens[3:, 0], []
+    for enabled in (False, True):
+        with torch.autocast("cuda", dtype=cast, enabled=enabled):
+            outs.append(model.step(Rollouts(model, 3, 8), steps[:, :3], top=64))
+    assert float((outs[0][0] - outs[1][0]).abs().max()) < 32 * unit
+    # (the k-th largest of numbers that are off by no more than that is off by no more)
+    assert float((outs[0][1] - outs[1][1]).abs().max()) < 32 * unit
