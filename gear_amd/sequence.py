@@ -187,11 +187,18 @@ def distill(logits, top_tokens, top_logits, *, scale=1.0):
     return _Distill.apply(logits, top_tokens, top_logits, scale)
 
 
+class _Norm(nn.LayerNorm):
+    """nn.LayerNorm by layer_norm; with a residual: (y, the sum)."""
+
+    def forward(self, x, residual=None):
+        return layer_norm(x, self.weight, self.bias, residual=residual, eps=self.eps)
+
+
 class _Block(nn.Module):
-    def __init__(self, width, heads, kv_heads):
+    def __init__(self, width, heads, kv_heads, norm=nn.LayerNorm):
         super().__init__()
         self.heads, self.kv_heads, self.dim = heads, kv_heads, width // heads
-        self.before, self.between = nn.LayerNorm(width), nn.LayerNorm(width)
+        self.before, self.between = norm(width), norm(width)
         self.qkv = nn.Linear(width, (heads + 2 * kv_heads) * self.dim, bias=False)
         self.q_weight, self.k_weight = nn.Parameter(torch.ones(self.dim)), nn.Parameter(torch.ones(self.dim))
         self.out = nn.Linear(width, width, bias=False)
@@ -317,14 +324,17 @@ class TokenModel(_Positions):
             raise ValueError("a step needs two tokens at least, an observation's and its action")
         self.step_tokens, self.width, self.dtype, self.cap = step, width, dtype, cap
         self.table = nn.Parameter(torch.randn(vocab, width) * width ** -0.5)
-        self.blocks = nn.ModuleList(_Block(width, heads, kv_heads) for _ in range(layers))
-        self.norm = nn.LayerNorm(width)
+        self.blocks = nn.ModuleList(_Block(width, heads, kv_heads, _Norm) for _ in range(layers))
+        self.norm = _Norm(width)
         self.head = nn.Linear(width, vocab, bias=False)
         self.positions(width // heads)
 
     @staticmethod
     def _norm(norm, x, residual=None):
-        return layer_norm(x, norm.weight, norm.bias, residual=residual, eps=norm.eps)
+        if isinstance(norm, _Norm) or residual is None:
+            return norm(x) if residual is None else norm(x, residual)
+        total = x + residual  # another module in a norm's place
+        return norm(total), total
 
     def _logits(self, tokens, attend, actions):
         """tokens [batch, tokens]; attend(layer, block, q, k, v) -> [batch, tokens, heads, dim]; actions(x) picks the rows

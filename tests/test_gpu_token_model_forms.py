@@ -52,3 +52,36 @@ def test_autocast(cast, parameters):
     assert float((outs[0][0] - outs[1][0]).abs().max()) < 32 * unit
     # (the k-th largest of numbers that are off by no more than that is off by no more)
     assert float((outs[0][1] - outs[1][1]).abs().max()) < 32 * unit
+
+
+def test_norms_are_modules():
+    """Hooks of the norms run, as those of any module, in windows and in steps; their names and states are nn.LayerNorm's."""
+    from gear_amd.sequence import Rollouts, TokenModel
+    announce("token model: hooks of norms")
+    model = TokenModel(50, 3, width=64, heads=2, kv_heads=1, layers=2).cuda()
+    norms = {n: m for n, m in model.named_modules() if isinstance(m, torch.nn.LayerNorm)}
+    assert sorted(norms) == ["blocks.0.before", "blocks.0.between", "blocks.1.before", "blocks.1.between", "norm"]
+    tokens, mask, done = _windows(50, 3)
+    want = model.log_probs(tokens, mask, done)
+    before, after = [], []
+    for n, m in norms.items():
+        m.register_forward_pre_hook(lambda module, args, n=n: before.append(n))
+        m.register_forward_hook(lambda module, args, out, n=n: after.append(n))
+    got = model.log_probs(tokens, mask, done)
+    order = ["blocks.0.before", "blocks.0.between", "blocks.1.before", "blocks.1.between", "norm"]
+    assert before == after == order and torch.equal(got[0], want[0])
+    model.step(Rollouts(model, 6, 4), tokens[:, 0, :2])
+    assert before == after == order * 2
+    # a hook's result takes the place of the norm's
+    model.norm.register_forward_hook(lambda module, args, out: (out[0] * 0, out[1]))
+    assert float(model(tokens, mask, done).detach().abs().max()) == 0
+    # the states that were saved before are those of today
+    other = TokenModel(50, 3, width=64, heads=2, kv_heads=1, layers=2).cuda()
+    other.load_state_dict(model.state_dict())
+    assert torch.equal(other.log_probs(tokens, mask, done)[0], want[0])
+    # other modules in their places: sums and norms of torch, in 32 bits a few roundings away
+    for block in other.blocks:
+        block.before, block.between = torch.nn.LayerNorm(64).cuda(), torch.nn.LayerNorm(64).cuda()
+    other.norm = torch.nn.LayerNorm(64).cuda()
+    # (attention in bfloat16: a rounding of its operands that falls the other way is 2^-8 of one)
+    assert float((other.log_probs(tokens, mask, done)[0] - want[0]).detach().abs().max()) < 32 * 2.0 ** -8
