@@ -18,9 +18,11 @@
 // pairs of logit and column, which all differ; where that leaves too many as well, they are taken one after the other.
 // The best one alone is the row's maximum, of which only the column is looked for.
 //
-// Measured: 16384 x 33025 bf16 155-190 us forward (with how memory lies; 5.6-6.8 TB/s), 361 backward (5.9 TB/s); 8191 x 33025 against 32
+// Measured: 16384 x 33025 bf16 155-190 us forward (with how memory lies; 5.6-6.8 TB/s), 366 backward (5.8 TB/s), rows of 20001 and
+// 50001 of as much memory 187 and 179 + 20, 377 and 375; 8191 x 33025 against 32
 // entries 100 and 191; 184320 x 1024 bf16 95 and 117 (4.0 and 6.5 TB/s); 184320 x 18 in 32 bits 8 and 8; 64 x 65537 fp16 with the best
-// eight 11; 4096 x 33024 bf16 43, with the best 32 74 (64: 180; of equal logits 264 and 323, one after the other 2230 and 4350).
+// eight 11; 4096 x 33024 bf16 46, 54 where no cache has any of it, with the best 32 76 and 79 (64: 180; of equal logits 283 and 345,
+// one after the other 2230 and 4350).
 // The wide rows' forward with 128, 512 or 1024 threads of 34, 9 or 5 vectors in place of 256 of 17: 16384 x 33025 220, 219 and 394 for
 // 185, 4096 x 33024 with the best 32 106, 107 and 165 for 75-84.
 #include <algorithm>
